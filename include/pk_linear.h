@@ -631,6 +631,122 @@ int32_t pk_quantize_fp8_fixed_transpose(const uint16_t* input, uint8_t* output, 
  * every attention kernel reads. */
 int32_t pk_pack_position_heads(const uint16_t* input, uint16_t* output, void* stream);
 
+/* ---- a decoder layer's serving step --------------------------------------------
+ * No reference counterpart: the operators of one step of a decoder (or of an
+ * encoder that is fed in chunks) whose keys and values live in a paged cache:
+ * page_plan, rms_norm_quantize, gemv_int4g128 (or a linear), paged_cache_write,
+ * paged_attention.  Inference only.
+ *
+ * The cache of a layer is a pool of `pages` pages of page_size (16, 32, 64, 128
+ * or 256) tokens.  Page p holds, per kv head, keys [page_size x head_dim] and
+ * values [head_dim x page_size] (transposed): key_cache is [pages x kv_heads x
+ * page_size x head_dim], value_cache [pages x kv_heads x head_dim x page_size],
+ * as fp16 or as e4m3 bytes of value * inverse_scale.  Slot p * page_size + i is
+ * token i of page p.  A request's block_table row lists its pages in order;
+ * requests may share pages. */
+
+#define PK_NORM_FP8 0
+#define PK_NORM_INT8 1
+#define PK_CACHE_FP16 0
+#define PK_CACHE_FP8 1
+
+/* Residual addition, root-mean-square norm and per-row 8-bit rows in one pass:
+ * h = input + residual, residual_out = fp16(h), y = h / sqrt(mean(h^2) +
+ * epsilon) * weight, scales[row] = max|y| / 448 (INT8: / 127), output =
+ * e4m3(y / scale) (INT8: round to nearest even).  h and y are not rounded in
+ * between.  residual may be NULL (h = input), residual_out may be NULL, input
+ * or residual.  [rows x width], width % 8 == 0 up to 16384, 0 <= epsilon <= 1.
+ * A row of zeros has scale 1 (also with epsilon 0); a row whose y holds an
+ * infinity or a NaN has scale NaN and codes 0x7f (INT8: 0).  The rows feed
+ * pk_linear_fp8_dyn, pk_linear_int8_dyn, pk_linear_int4g128_a8 and
+ * pk_gemv_int4g128_a8.  Rows and weight 16-byte, output 8-byte aligned. */
+int32_t pk_rms_norm_quantize(int32_t kind, const uint16_t* input, const uint16_t* residual, const uint16_t* weight,
+                             uint16_t* residual_out, void* output, float* scales, int32_t rows, int32_t width,
+                             float epsilon, void* stream);
+
+/* pk_linear_int4g128 and pk_linear_int4g128_a8 for 1..16 rows (single tokens of
+ * as many streams), bound by reading the weights once: output[m, n] = sum over
+ * groups of weight_scales * (sum of input * (q - z)) (* input_scales[m]) + bias.
+ * The levels q - z (weight_zeros whole numbers 0..15) multiply exactly and the
+ * scale is applied to the group's sum in fp32, where pk_linear_int4g128 rounds
+ * each dequantized weight to fp16 first.  The INT8 form's group sums are exact.
+ * n free, k % 128 == 0 up to 65536; input and weight_q 16-byte aligned, bias may
+ * be NULL; fp16 or fp32 output [m x n]. */
+int32_t pk_gemv_int4g128(const uint16_t* input, const uint32_t* weight_q, const uint16_t* weight_scales,
+                         const uint16_t* weight_zeros, const float* bias, void* output, int32_t output_fp32, int32_t m,
+                         int32_t n, int32_t k, void* stream);
+int32_t pk_gemv_int4g128_a8(const int8_t* input, const float* input_scales, const uint32_t* weight_q,
+                            const uint16_t* weight_scales, const uint16_t* weight_zeros, const float* bias, void* output,
+                            int32_t output_fp32, int32_t m, int32_t n, int32_t k, void* stream);
+
+/* Pages, block tables and slots of one step, on the GPU from the requests'
+ * lengths: request r has held[r] tokens in the cache and adds added[r] (0 is
+ * allowed).  With pages(t) = ceil(t / page_size) it takes pages(held + added) -
+ * pages(held) pages from free_pages[free_range[0] .. free_range[1]) in request
+ * order and writes them behind its pages in block_table [requests x max_pages];
+ * other table entries stay as they are.  Written are
+ *   query_starts [requests + 1]  exclusive sums of added,
+ *   key_lengths [requests]       held + added,
+ *   slots [token_capacity]       the slot of each new token, requests in order,
+ *                                -1 behind the last (and for a negative page id),
+ *   positions [token_capacity]   its position in its request, 0 behind the last;
+ *                                may be NULL,
+ *   info [4]                     {new tokens, pages taken, status, 0}.
+ * All or nothing: status is a sum of 1 (too few free pages), 2 (a request needs
+ * more than max_pages), 4 (more new tokens than token_capacity) and 8 (a
+ * negative length or free_range[0]); if it is not 0, key_lengths = held, the
+ * starts are 0, the slots -1, and the table is not touched.  free_range is not
+ * advanced: the caller adds info[1] to free_range[0] once it keeps the step.
+ * held, added, free_range [2] and free_pages [free_capacity] are device arrays;
+ * an output must not overlap any other array.  requests <= 4096, max_pages *
+ * page_size <= 2^30. */
+int32_t pk_page_plan(const int32_t* held, const int32_t* added, const int32_t* free_pages, const int32_t* free_range,
+                     int32_t free_capacity, int32_t* block_table, int32_t* query_starts, int32_t* key_lengths,
+                     int32_t* slots, int32_t* positions, int32_t* info, int32_t requests, int32_t max_pages,
+                     int32_t page_size, int32_t token_capacity, void* stream);
+
+/* New keys and values [tokens x kv_heads x head_dim] (fp16; token t starts
+ * key_stride * t / value_stride * t elements in, so both may be slices of one
+ * projection's rows) into their slots.  kind PK_CACHE_FP8 stores e4m3(x *
+ * inverse_scale) (saturating; NaN stays NaN), PK_CACHE_FP16 the value itself.
+ * A slot outside [0, pages * page_size) is skipped (-1: padding).  The slots of
+ * one call must differ.  head_dim 64 or 128; keys, values and caches 16-byte
+ * aligned, strides multiples of 8. */
+int32_t pk_paged_cache_write(int32_t kind, const uint16_t* key, int64_t key_stride, const uint16_t* value,
+                             int64_t value_stride, const int32_t* slots, void* key_cache, void* value_cache,
+                             int32_t tokens, int32_t kv_heads, int32_t head_dim, int32_t page_size, int32_t pages,
+                             float key_inverse_scale, float value_inverse_scale, void* stream);
+
+/* Attention of a chunk of new tokens over the paged cache (single tokens are
+ * chunks of one).  Sequence r's new tokens are the rows query_starts[r] ..
+ * query_starts[r + 1] of query [tokens x heads x head_dim] (row stride
+ * query_stride elements); with n of them and L = key_lengths[r] keys (the new
+ * ones among them, written before this call), token i stands at p = L - n + i
+ * and sees keys j with p - left <= j <= p + right, 0 <= j < L; a negative left
+ * or right is unlimited, so (-1, 0) is causal.  output = softmax(scale *
+ * key_scale * q.k) * value_scale * v over the seen keys; heads / kv_heads query
+ * heads in order share a kv head.  The scales of the cache apply to PK_CACHE_FP8
+ * only.  A query that sees no key gives zeros; infinities and NaN in keys and
+ * values that a query does not see do not reach it.  Keys of a page id outside
+ * [0, pages) count as not there; lengths beyond max_pages * page_size are cut.
+ * Rows of output outside the sequences' ranges stay as they were.  max_queries
+ * (<= tokens) is at least the largest n, tokens <= 2^20, sequences <= 65535.
+ * Scores, the running maximum and sum and the output's sum are fp32; scores
+ * multiply fp16 queries with fp16 or e4m3 keys exactly, probabilities are
+ * rounded to fp16 for the second product (their sum is not).
+ * workspace: pk_paged_attention_workspace_bytes of device memory (16-byte
+ * aligned), used by one call at a time; its content need not be kept or cleared
+ * between calls. */
+int64_t pk_paged_attention_workspace_bytes(int32_t tokens, int32_t max_queries, int32_t sequences, int32_t heads,
+                                           int32_t kv_heads, int32_t head_dim, int32_t page_size, int32_t max_pages);
+int32_t pk_paged_attention(int32_t kind, const uint16_t* query, int64_t query_stride, const void* key_cache,
+                           const void* value_cache, const int32_t* block_table, const int32_t* query_starts,
+                           const int32_t* key_lengths, uint16_t* output, int64_t output_stride, int32_t tokens,
+                           int32_t max_queries, int32_t sequences, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                           int32_t page_size, int32_t pages, int32_t max_pages, int32_t left, int32_t right,
+                           float scale, float key_scale, float value_scale, void* workspace,
+                           uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -869,4 +869,230 @@ int32_t pk_pack_position_heads(const uint16_t* input, uint16_t* output, void* st
     return check_launch("pack_position_heads");
 }
 
+// ---- a decoder layer's serving step -------------------------------------------------
+
+static bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    return a && b && (const char*)a < (const char*)b + b_bytes && (const char*)b < (const char*)a + a_bytes;
+}
+
+static int page_shift(int32_t page_size) {  // log2 of 16, 32, ..., 256; -1 otherwise
+    for (int s = 4; s <= 8; ++s)
+        if (page_size == 1 << s) return s;
+    return -1;
+}
+
+int32_t pk_rms_norm_quantize(int32_t kind, const uint16_t* input, const uint16_t* residual, const uint16_t* weight,
+                             uint16_t* residual_out, void* output, float* scales, int32_t rows, int32_t width, float epsilon,
+                             void* stream) {
+    if (kind != PK_NORM_FP8 && kind != PK_NORM_INT8) { set_error("norm kind must be 0 (fp8) or 1 (int8), got %d", kind); return PK_E_ARG; }
+    if (rows < 0 || width <= 0 || width % 8 || width > 16384) {
+        set_error("rms_norm_quantize needs rows >= 0 and width %% 8 == 0 up to 16384 (rows=%d width=%d)", rows, width);
+        return PK_E_SHAPE;
+    }
+    if (!(epsilon >= 0.0f) || epsilon > 1.0f) { set_error("epsilon must lie in [0, 1], got %g", (double)epsilon); return PK_E_ARG; }
+    if (rows == 0) return PK_OK;
+    if (!need(input, "input") || !need(weight, "weight") || !need(output, "output") || !need(scales, "scales")) return PK_E_ARG;
+    if (misaligned(input, 16) || misaligned(residual, 16) || misaligned(weight, 16) || misaligned(residual_out, 16) ||
+        misaligned(output, 8) || misaligned(scales, 4)) {
+        set_error("norm rows and weight must be 16-byte, output 8-byte, scales 4-byte aligned");
+        return PK_E_ALIGN;
+    }
+    const size_t n = (size_t)rows * width;
+    if ((residual_out != input && overlap(residual_out, 2 * n, input, 2 * n)) ||
+        (residual_out != residual && overlap(residual_out, 2 * n, residual, 2 * n)) || overlap(output, n, input, 2 * n) ||
+        overlap(output, n, residual, 2 * n) || overlap(output, n, residual_out, 2 * n)) {
+        set_error("residual_out may be input or residual itself; other overlaps of the norm's rows are refused");
+        return PK_E_ARG;
+    }
+    launch_rms_norm_quantize(kind, input, residual, weight, residual_out, output, scales, rows, width, epsilon, STREAM);
+    return check_launch("rms_norm_quantize");
+}
+
+static int32_t gemv(const void* input, const float* input_scales, const uint32_t* q, const uint16_t* scales, const uint16_t* zeros,
+                    const float* bias, void* output, int32_t output_fp32, int32_t m, int32_t n, int32_t k, void* stream) {
+    if (m < 0 || m > 16 || n < 0 || k <= 0 || k % 128 || k > 65536) {
+        set_error("int4g128 gemv needs m <= 16 and k %% 128 == 0 up to 65536 (m=%d n=%d k=%d); pk_linear_int4g128 takes more rows", m, n, k);
+        return PK_E_SHAPE;
+    }
+    if (m == 0 || n == 0) return PK_OK;
+    if (!need(input, "input") || !need(q, "weight_q") || !need(scales, "weight_scales") || !need(zeros, "weight_zeros") ||
+        !need(output, "output"))
+        return PK_E_ARG;
+    if (misaligned(input, 16) || misaligned(q, 16) || misaligned(scales, 2) || misaligned(zeros, 2) || misaligned(bias, 4) ||
+        misaligned(input_scales, 4) || misaligned(output, output_fp32 ? 4 : 2)) {
+        set_error("gemv input and weight_q must be 16-byte aligned, the others as their types");
+        return PK_E_ALIGN;
+    }
+    launch_gemv_g128(input, input_scales, q, scales, zeros, bias, output, output_fp32 != 0, m, n, k, STREAM);
+    return check_launch("gemv_int4g128");
+}
+
+int32_t pk_gemv_int4g128(const uint16_t* input, const uint32_t* weight_q, const uint16_t* weight_scales, const uint16_t* weight_zeros,
+                         const float* bias, void* output, int32_t output_fp32, int32_t m, int32_t n, int32_t k, void* stream) {
+    return gemv(input, nullptr, weight_q, weight_scales, weight_zeros, bias, output, output_fp32, m, n, k, stream);
+}
+
+int32_t pk_gemv_int4g128_a8(const int8_t* input, const float* input_scales, const uint32_t* weight_q, const uint16_t* weight_scales,
+                            const uint16_t* weight_zeros, const float* bias, void* output, int32_t output_fp32, int32_t m, int32_t n,
+                            int32_t k, void* stream) {
+    if (!need(input_scales, "input_scales")) return PK_E_ARG;
+    return gemv(input, input_scales, weight_q, weight_scales, weight_zeros, bias, output, output_fp32, m, n, k, stream);
+}
+
+int32_t pk_page_plan(const int32_t* held, const int32_t* added, const int32_t* free_pages, const int32_t* free_range,
+                     int32_t free_capacity, int32_t* block_table, int32_t* query_starts, int32_t* key_lengths, int32_t* slots,
+                     int32_t* positions, int32_t* info, int32_t requests, int32_t max_pages, int32_t page_size, int32_t token_capacity,
+                     void* stream) {
+    const int shift = page_shift(page_size);
+    if (shift < 0) { set_error("page_size must be 16, 32, 64, 128 or 256, got %d", page_size); return PK_E_SHAPE; }
+    if (requests <= 0 || requests > kMostPlanRequests || max_pages <= 0 || max_pages > (1 << 30) >> shift || token_capacity < 0 ||
+        free_capacity < 0) {
+        set_error("page_plan needs 1..%d requests, max_pages * page_size <= 2^30 and capacities >= 0 (requests=%d max_pages=%d "
+                  "token_capacity=%d free_capacity=%d)", kMostPlanRequests, requests, max_pages, token_capacity, free_capacity);
+        return PK_E_SHAPE;
+    }
+    if (!need(held, "held") || !need(added, "added") || !need(free_range, "free_range") || !need(block_table, "block_table") ||
+        !need(query_starts, "query_starts") || !need(key_lengths, "key_lengths") || !need(info, "info") ||
+        (free_capacity && !need(free_pages, "free_pages")) || (token_capacity && !need(slots, "slots")))
+        return PK_E_ARG;
+    const void* all[] = {held, added, free_pages, free_range, block_table, query_starts, key_lengths, slots, positions, info};
+    for (const void* p : all)
+        if (misaligned(p, 4)) { set_error("page_plan arrays must be 4-byte aligned"); return PK_E_ALIGN; }
+    // what is written overlaps nothing else: workgroups read while others write
+    const size_t r = (size_t)requests * 4, t = (size_t)token_capacity * 4;
+    const size_t bytes[] = {r, r, (size_t)free_capacity * 4, 8, r * max_pages, r + 4, r, t, t, 16};
+    for (int i = 4; i < 10; ++i)
+        for (int j = 0; j < i; ++j)
+            if (overlap(all[i], bytes[i], all[j], bytes[j])) {
+                set_error("page_plan: an output overlaps another array");
+                return PK_E_ARG;
+            }
+    launch_page_plan(held, added, free_pages, free_range, free_capacity, block_table, query_starts, key_lengths, slots, positions, info,
+                     requests, max_pages, shift, token_capacity, STREAM);
+    return check_launch("page_plan");
+}
+
+// Shape checks that the cache's writer and reader share; the shift or a status.
+static int32_t cache_shape(int32_t kind, int32_t kv_heads, int32_t head_dim, int32_t page_size, int32_t pages) {
+    if (kind != PK_CACHE_FP16 && kind != PK_CACHE_FP8) { set_error("cache kind must be 0 (fp16) or 1 (fp8), got %d", kind); return PK_E_ARG; }
+    const int shift = page_shift(page_size);
+    if (shift < 0) { set_error("page_size must be 16, 32, 64, 128 or 256, got %d", page_size); return PK_E_SHAPE; }
+    if (kv_heads <= 0 || kv_heads > 256 || (head_dim != 64 && head_dim != 128)) {
+        set_error("the paged cache holds 1..256 kv heads of 64 or 128 features, got %d of %d", kv_heads, head_dim);
+        return PK_E_SHAPE;
+    }
+    if (pages <= 0 || (int64_t)pages << shift > 0x7fffffffll) {
+        set_error("the paged cache needs 1 <= pages and pages * page_size < 2^31 (pages=%d page_size=%d)", pages, page_size);
+        return PK_E_SHAPE;
+    }
+    return shift;
+}
+
+int32_t pk_paged_cache_write(int32_t kind, const uint16_t* key, int64_t key_stride, const uint16_t* value, int64_t value_stride,
+                             const int32_t* slots, void* key_cache, void* value_cache, int32_t tokens, int32_t kv_heads,
+                             int32_t head_dim, int32_t page_size, int32_t pages, float key_inverse_scale, float value_inverse_scale,
+                             void* stream) {
+    const int32_t shift = cache_shape(kind, kv_heads, head_dim, page_size, pages);
+    if (shift < 0) return shift;
+    const int64_t width = (int64_t)kv_heads * head_dim;
+    if (tokens < 0 || key_stride < width || value_stride < width || key_stride >= 1ll << 31 || value_stride >= 1ll << 31) {
+        set_error("cache write needs tokens >= 0 and strides of at least kv_heads * head_dim = %lld (tokens=%d strides %lld, %lld)",
+                  (long long)width, tokens, (long long)key_stride, (long long)value_stride);
+        return PK_E_SHAPE;
+    }
+    if (tokens == 0) return PK_OK;
+    if (!need(key, "key") || !need(value, "value") || !need(slots, "slots") || !need(key_cache, "key_cache") ||
+        !need(value_cache, "value_cache"))
+        return PK_E_ARG;
+    if (misaligned(key, 16) || misaligned(value, 16) || key_stride % 8 || value_stride % 8 || misaligned(key_cache, 16) ||
+        misaligned(value_cache, 16) || misaligned(slots, 4)) {
+        set_error("keys, values and caches must be 16-byte aligned, strides multiples of 8, slots 4-byte aligned");
+        return PK_E_ALIGN;
+    }
+    launch_paged_cache_write(kind, key, value, key_stride, value_stride, slots, key_cache, value_cache, tokens, kv_heads, head_dim, shift,
+                             pages, key_inverse_scale, value_inverse_scale, STREAM);
+    return check_launch("paged_cache_write");
+}
+
+// Shape checks of the attention and its workspace; the shift or a status.
+static int32_t paged_shape(int32_t tokens, int32_t max_queries, int32_t sequences, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                           int32_t page_size, int32_t max_pages) {
+    const int32_t shift = cache_shape(0, kv_heads, head_dim, page_size, 1);
+    if (shift < 0) return shift;
+    if (heads <= 0 || heads % kv_heads || heads > 1024) {
+        set_error("heads must be a multiple of kv_heads up to 1024, got %d for %d", heads, kv_heads);
+        return PK_E_SHAPE;
+    }
+    if (tokens < 0 || tokens > 1 << 20 || max_queries < 0 || max_queries > tokens || sequences < 0 || sequences > 65535 || max_pages <= 0 ||
+        max_pages > (1 << 30) >> shift) {
+        set_error("paged attention needs tokens <= 2^20, max_queries <= tokens, sequences <= 65535 and max_pages * page_size <= 2^30 "
+                  "(tokens=%d max_queries=%d sequences=%d max_pages=%d)", tokens, max_queries, sequences, max_pages);
+        return PK_E_SHAPE;
+    }
+    return shift;
+}
+
+int64_t pk_paged_attention_workspace_bytes(int32_t tokens, int32_t max_queries, int32_t sequences, int32_t heads, int32_t kv_heads,
+                                           int32_t head_dim, int32_t page_size, int32_t max_pages) {
+    const int32_t shift = paged_shape(tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, max_pages);
+    if (shift < 0) return shift;
+    return 0;
+}
+
+int32_t pk_paged_attention(int32_t kind, const uint16_t* query, int64_t query_stride, const void* key_cache, const void* value_cache,
+                           const int32_t* block_table, const int32_t* query_starts, const int32_t* key_lengths, uint16_t* output,
+                           int64_t output_stride, int32_t tokens, int32_t max_queries, int32_t sequences, int32_t heads,
+                           int32_t kv_heads, int32_t head_dim, int32_t page_size, int32_t pages, int32_t max_pages, int32_t left,
+                           int32_t right, float scale, float key_scale, float value_scale, void* workspace, uint64_t workspace_bytes,
+                           void* stream) {
+    const int32_t shift = paged_shape(tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, max_pages);
+    if (shift < 0) return shift;
+    const int32_t cache = cache_shape(kind, kv_heads, head_dim, page_size, pages);
+    if (cache < 0) return cache;
+    const int64_t width = (int64_t)heads * head_dim;
+    if (query_stride < width || output_stride < width || query_stride >= 1ll << 31 || output_stride >= 1ll << 31) {
+        set_error("paged attention needs strides of at least heads * head_dim = %lld, got %lld and %lld", (long long)width,
+                  (long long)query_stride, (long long)output_stride);
+        return PK_E_SHAPE;
+    }
+    if (tokens == 0 || max_queries == 0 || sequences == 0) return PK_OK;
+    if (!need(query, "query") || !need(key_cache, "key_cache") || !need(value_cache, "value_cache") || !need(block_table, "block_table") ||
+        !need(query_starts, "query_starts") || !need(key_lengths, "key_lengths") || !need(output, "output"))
+        return PK_E_ARG;
+    if (misaligned(query, 16) || misaligned(output, 16) || query_stride % 8 || output_stride % 8 || misaligned(key_cache, 16) ||
+        misaligned(value_cache, 16) || misaligned(block_table, 4) || misaligned(query_starts, 4) || misaligned(key_lengths, 4) ||
+        misaligned(workspace, 16)) {
+        set_error("query, output, caches and workspace must be 16-byte aligned, strides multiples of 8, index arrays 4-byte aligned");
+        return PK_E_ALIGN;
+    }
+    const int64_t wanted = pk_paged_attention_workspace_bytes(tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, max_pages);
+    if (wanted > 0 && (!need(workspace, "workspace") || workspace_bytes < (uint64_t)wanted)) {
+        if (workspace) set_error("paged attention needs %lld bytes of workspace, got %llu", (long long)wanted, (unsigned long long)workspace_bytes);
+        return PK_E_ARG;
+    }
+    PagedArgs a{};
+    a.query = query;
+    a.key = (const uint8_t*)key_cache;
+    a.value = (const uint8_t*)value_cache;
+    a.table = block_table;
+    a.starts = query_starts;
+    a.lengths = key_lengths;
+    a.out = output;
+    a.query_stride = query_stride;
+    a.out_stride = output_stride;
+    a.tokens = tokens;
+    a.sequences = sequences;
+    a.kv_heads = kv_heads;
+    a.group = heads / kv_heads;
+    a.shift = shift;
+    a.pages = pages;
+    a.max_pages = max_pages;
+    a.left = left < 0 ? -1 : left;
+    a.right = right < 0 || right > 1 << 30 ? -1 : right;
+    a.scale_log2 = scale * (kind == PK_CACHE_FP8 ? key_scale : 1.0f) * 1.4426950408889634f;
+    a.value_scale = kind == PK_CACHE_FP8 ? value_scale : 1.0f;
+    launch_paged_attention(kind, a, head_dim, max_queries, STREAM);
+    return check_launch("paged_attention");
+}
+
 }  // extern "C"

@@ -74,6 +74,34 @@ int launch_sparse24_i8_contract(const uint8_t* data, const uint8_t* meta, const 
                                 const uint32_t* ovf, const uint8_t* data2, const uint8_t* meta2, const int8_t* w, const int8_t* wt,
                                 const float* w_scales, float* out, int m, int n, int k, hipStream_t s);
 int launch_transpose_i8(const int8_t* w, int8_t* wt, int n, int k, hipStream_t s);
+
+// kind: 0 e4m3 codes, 1 INT8 codes
+void launch_rms_norm_quantize(int kind, const uint16_t* in, const uint16_t* residual, const uint16_t* w, uint16_t* r_out, void* out,
+                              float* scales, int rows, int width, float eps, hipStream_t s);
+// xs set: INT8 rows with their scales; else fp16 rows.
+void launch_gemv_g128(const void* x, const float* xs, const uint32_t* q, const uint16_t* scales, const uint16_t* zeros, const float* bias,
+                      void* out, int out_f32, int m, int n, int k, hipStream_t s);
+constexpr int kMostPlanRequests = 4096;  // their ends lie in LDS
+void launch_page_plan(const int* held, const int* added, const int* free_pages, const int* free_range, int free_capacity, int* table,
+                      int* starts, int* lengths, int* slots, int* positions, int* info, int requests, int max_pages, int page_shift,
+                      int capacity, hipStream_t s);
+// cache kind: 0 fp16, 1 e4m3 bytes; strides in elements
+void launch_paged_cache_write(int kind, const uint16_t* key, const uint16_t* value, long long key_stride, long long value_stride,
+                              const int* slots, void* key_cache, void* value_cache, int tokens, int kv_heads, int head_dim, int page_shift,
+                              int pages, float k_inv, float v_inv, hipStream_t s);
+struct PagedArgs {
+    const uint16_t* query;
+    const uint8_t* key;
+    const uint8_t* value;
+    const int* table;
+    const int* starts;
+    const int* lengths;
+    uint16_t* out;
+    long long query_stride, out_stride;
+    int tokens, sequences, kv_heads, group, shift, pages, max_pages, left, right;
+    float scale_log2, value_scale;
+};
+void launch_paged_attention(int kind, const PagedArgs& args, int head_dim, int max_queries, hipStream_t s);
 void set_error(const char* fmt, ...);
 int cu_count();
 int launch_sparse24_contract(const uint8_t* data, const uint8_t* meta, const uint8_t* w, const float* w_scales, float in_scale,

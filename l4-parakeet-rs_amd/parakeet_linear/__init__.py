@@ -22,6 +22,7 @@ F = ctypes.c_float
 S = ctypes.c_size_t
 
 U64 = ctypes.c_uint64
+I64 = ctypes.c_int64
 
 
 class TensorInfo(ctypes.Structure):
@@ -119,6 +120,13 @@ SIGNATURES = {
     "pk_quantize_value_int4_register": (I, [P, P, I, F, I, P]),
     "pk_local_relpos_attention_tc_scores": (I, [P, P, P, P, P, P, P, P, I, I, I, I, I, I, P]),
     "pk_local_relpos_attention_packed": (I, [P, P, P, P, P, P, P, P, I, I, I, I, I, I, P, P, P, P, P]),
+    "pk_rms_norm_quantize": (I, [I, P, P, P, P, P, P, I, I, F, P]),
+    "pk_gemv_int4g128": (I, [P, P, P, P, P, P, I, I, I, I, P]),
+    "pk_gemv_int4g128_a8": (I, [P, P, P, P, P, P, P, I, I, I, I, P]),
+    "pk_page_plan": (I, [P, P, P, P, I, P, P, P, P, P, P, I, I, I, I, P]),
+    "pk_paged_cache_write": (I, [I, P, I64, P, I64, P, P, P, I, I, I, I, I, F, F, P]),
+    "pk_paged_attention_workspace_bytes": (I64, [I, I, I, I, I, I, I, I]),
+    "pk_paged_attention": (I, [I, P, I64, P, P, P, P, P, P, I64, I, I, I, I, I, I, I, I, I, I, I, F, F, F, P, U64, P]),
 }
 
 
@@ -395,3 +403,156 @@ def launch_decode(encoder_projection, frames, lstm, projection, joint, tokens, r
          b_hh1, projection[0], projection[1], joint[0], int(joint_int8), joint_scales, joint[1], hidden, token_outputs,
          durations, max_symbols, tokens, capacity, result, workspace, wbytes, stream=stream)
     return "fp16"
+
+
+# ---- a decoder layer's serving step (no reference counterpart) -----------------------
+
+NORM_FP8, NORM_INT8 = 0, 1
+CACHE_FP16, CACHE_FP8 = 0, 1
+
+
+def _check(what, *tensors):
+    """(name, tensor, dtypes, shape) each: the types and shapes that a call takes its sizes from, and the
+    current device, whose stream the call goes to."""
+    import torch
+
+    device = torch.cuda.current_device()
+    for name, t, dtypes, shape in tensors:
+        if t is None:
+            continue
+        if t.dtype not in dtypes:
+            raise ValueError(f"{what}: {name} is {t.dtype}, expected {' or '.join(map(str, dtypes))}")
+        if t.device.type != "cuda" or t.device.index != device:
+            raise ValueError(f"{what}: {name} is on {t.device}, not on the current device cuda:{device}")
+        if shape is not None and tuple(t.shape) != shape:
+            raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
+
+
+def _dense(what, *tensors):
+    for name, t in tensors:
+        if t is not None and not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be contiguous")
+
+
+def rms_norm_quantize(kind, input, residual, weight, residual_out, output, scales, epsilon, stream=None):
+    """h = input + residual (residual None: input), residual_out = fp16(h) (None: not kept), output = the 8-bit rows
+    of h's root-mean-square norm times weight with their scales: e4m3 bytes (kind NORM_FP8) or int8 (NORM_INT8), as
+    the dynamic linears and gemv_int4g128_a8 read them."""
+    import torch
+
+    rows, width = input.shape
+    f16 = (torch.float16,)
+    _check("rms_norm_quantize", ("input", input, f16, None), ("residual", residual, f16, (rows, width)), ("weight", weight, f16, (width,)),
+           ("residual_out", residual_out, f16, (rows, width)), ("scales", scales, (torch.float32,), (rows,)),
+           ("output", output, (torch.int8,) if kind == NORM_INT8 else (torch.uint8, torch.float8_e4m3fn), (rows, width)))
+    _dense("rms_norm_quantize", ("input", input), ("residual", residual), ("weight", weight), ("residual_out", residual_out), ("output", output),
+           ("scales", scales))
+    call("pk_rms_norm_quantize", kind, input, residual, weight, residual_out, output, scales, rows, width, epsilon, stream=stream)
+
+
+def _gemv(name, input, input_scales, weight_q, weight_scales, weight_zeros, bias, output, stream):
+    import torch
+
+    (m, k), n = input.shape, weight_q.shape[0]
+    f16 = (torch.float16,)
+    _check(name, ("input", input, f16 if input_scales is None else (torch.int8,), None), ("input_scales", input_scales, (torch.float32,), (m,)),
+           ("weight_q", weight_q, (torch.int32, torch.uint32), (n, k // 8)), ("weight_scales", weight_scales, f16, (n, k // 128)),
+           ("weight_zeros", weight_zeros, f16, (n, k // 128)), ("bias", bias, (torch.float32,), (n,)),
+           ("output", output, (torch.float16, torch.float32), (m, n)))
+    _dense(name, ("input", input), ("input_scales", input_scales), ("weight_q", weight_q), ("weight_scales", weight_scales),
+           ("weight_zeros", weight_zeros), ("bias", bias), ("output", output))
+    rows = (input,) if input_scales is None else (input, input_scales)
+    call("pk_" + name, *rows, weight_q, weight_scales, weight_zeros, bias, output, int(output.dtype == torch.float32), m, n, k, stream=stream)
+
+
+def gemv_int4g128(input, weight_q, weight_scales, weight_zeros, bias, output, stream=None):
+    """fp16 rows [m <= 16 x k] x INT4-g128 weights (pk_pack_int4_g128) -> fp16 or fp32 [m x n]; bias may be None."""
+    _gemv("gemv_int4g128", input, None, weight_q, weight_scales, weight_zeros, bias, output, stream)
+
+
+def gemv_int4g128_a8(input, input_scales, weight_q, weight_scales, weight_zeros, bias, output, stream=None):
+    """gemv_int4g128 on INT8 rows with their scales (rms_norm_quantize, pk_quantize_rows)."""
+    if input_scales is None:
+        raise ValueError("gemv_int4g128_a8: input_scales must not be None")
+    _gemv("gemv_int4g128_a8", input, input_scales, weight_q, weight_scales, weight_zeros, bias, output, stream)
+
+
+def page_plan(held, added, free_pages, free_range, block_table, query_starts, key_lengths, slots, positions, info, page_size, stream=None):
+    """Pages, block tables and slots of one step from the requests' lengths, all int32 on the GPU; see pk_page_plan in
+    include/pk_linear.h.  The sizes are the tensors': requests = len(held), token capacity = len(slots)."""
+    import torch
+
+    requests, max_pages = block_table.shape
+    i32 = (torch.int32,)
+    capacity = slots.shape[0]
+    arrays = (("held", held, i32, (requests,)), ("added", added, i32, (requests,)), ("free_pages", free_pages, i32, (free_pages.numel(),)),
+              ("free_range", free_range, i32, (2,)), ("block_table", block_table, i32, None), ("query_starts", query_starts, i32, (requests + 1,)),
+              ("key_lengths", key_lengths, i32, (requests,)), ("slots", slots, i32, (capacity,)), ("positions", positions, i32, (capacity,)),
+              ("info", info, i32, (4,)))
+    _check("page_plan", *arrays)
+    _dense("page_plan", *(a[:2] for a in arrays))
+    call("pk_page_plan", held, added, free_pages, free_range, free_pages.numel(), block_table, query_starts, key_lengths, slots, positions, info,
+         requests, max_pages, page_size, capacity, stream=stream)
+
+
+def _cache_of(what, key_cache, value_cache):
+    """(kind, pages, kv heads, page size, head dim) of a layer's cache."""
+    import torch
+
+    pages, kv_heads, page_size, head_dim = key_cache.shape
+    types = (torch.float16, torch.uint8, torch.float8_e4m3fn)
+    _check(what, ("key_cache", key_cache, types, None), ("value_cache", value_cache, (key_cache.dtype,), (pages, kv_heads, head_dim, page_size)))
+    _dense(what, ("key_cache", key_cache), ("value_cache", value_cache))
+    return CACHE_FP16 if key_cache.dtype == torch.float16 else CACHE_FP8, pages, kv_heads, page_size, head_dim
+
+
+def _row_stride(what, name, t):
+    """Elements between tokens of a [tokens x heads x head_dim] tensor whose heads lie next to each other."""
+    tokens, heads, head_dim = t.shape
+    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != head_dim):
+        raise ValueError(f"{what}: {name} must hold each token's heads contiguously")
+    return t.stride(0) if tokens > 1 else max(t.stride(0), heads * head_dim)
+
+
+def paged_cache_write(key, value, slots, key_cache, value_cache, key_inverse_scale=1.0, value_inverse_scale=1.0, stream=None):
+    """New keys and values [tokens x kv_heads x head_dim] (fp16, a stride between tokens) into their slots (-1: none) of a
+    cache [pages x kv_heads x page_size x head_dim] / [pages x kv_heads x head_dim x page_size]: fp16, or e4m3 bytes of
+    x * inverse_scale."""
+    import torch
+
+    kind, pages, kv_heads, page_size, head_dim = _cache_of("paged_cache_write", key_cache, value_cache)
+    tokens = slots.shape[0]
+    _check("paged_cache_write", ("key", key, (torch.float16,), (tokens, kv_heads, head_dim)),
+           ("value", value, (torch.float16,), (tokens, kv_heads, head_dim)), ("slots", slots, (torch.int32,), (tokens,)))
+    _dense("paged_cache_write", ("slots", slots))
+    call("pk_paged_cache_write", kind, key, _row_stride("paged_cache_write", "key", key), value, _row_stride("paged_cache_write", "value", value),
+         slots, key_cache, value_cache, tokens, kv_heads, head_dim, page_size, pages, key_inverse_scale, value_inverse_scale, stream=stream)
+
+
+def paged_attention_workspace_bytes(tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, max_pages):
+    """Bytes of workspace that paged_attention needs for these sizes (host only)."""
+    size = lib.pk_paged_attention_workspace_bytes(tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, max_pages)
+    if size < 0:
+        raise PkError(f"pk_paged_attention_workspace_bytes: status {size}: {last_error()}")
+    return size
+
+
+def paged_attention(query, key_cache, value_cache, block_table, query_starts, key_lengths, output, workspace, *, max_queries, left=-1, right=0,
+                    scale=None, key_scale=1.0, value_scale=1.0, stream=None):
+    """Attention of new tokens [tokens x heads x head_dim] over the paged cache; see pk_paged_attention in
+    include/pk_linear.h.  scale None: 1 / sqrt(head_dim); workspace: a uint8 tensor of paged_attention_workspace_bytes,
+    used by one call at a time."""
+    import torch
+
+    kind, pages, kv_heads, page_size, head_dim = _cache_of("paged_attention", key_cache, value_cache)
+    tokens, heads = query.shape[:2]
+    sequences, max_pages = block_table.shape
+    i32 = (torch.int32,)
+    _check("paged_attention", ("query", query, (torch.float16,), (tokens, heads, head_dim)), ("output", output, (torch.float16,), (tokens, heads, head_dim)),
+           ("block_table", block_table, i32, None), ("query_starts", query_starts, i32, (sequences + 1,)), ("key_lengths", key_lengths, i32, (sequences,)),
+           ("workspace", workspace, (torch.uint8,), None))
+    _dense("paged_attention", ("block_table", block_table), ("query_starts", query_starts), ("key_lengths", key_lengths), ("workspace", workspace))
+    call("pk_paged_attention", kind, query, _row_stride("paged_attention", "query", query), key_cache, value_cache, block_table, query_starts, key_lengths,
+         output, _row_stride("paged_attention", "output", output), tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, pages, max_pages,
+         left, right, head_dim**-0.5 if scale is None else scale, key_scale, value_scale, workspace,
+         0 if workspace is None else workspace.numel(), stream=stream)

@@ -1,0 +1,299 @@
+"""The operators of a serving step against their definitions in 64 bits: norm, matrix-vector products, page plan, cache write."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import serving_plain as plain  # noqa: E402
+from test_gpu_parity import pk  # noqa: E402, F401
+
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def randn(g, *shape, scale=1.0):
+    return (torch.randn(shape, generator=g, device="cuda") * scale).half()
+
+
+# ---- norm ---------------------------------------------------------------------------
+
+def check_norm(pk, kind, x, r, w, eps, keep=True, in_place=False):  # noqa: F811
+    rows, width = x.shape
+    most = 127 if kind == pk.NORM_INT8 else 448
+    h, y = plain.rms_norm(x, r, w, eps)
+    want_scale = y.abs().amax(1) / most
+    r_out = None if not keep else (r if in_place else torch.full_like(x, 7))
+    out = torch.full((rows, width), 99, dtype=torch.int8 if kind == pk.NORM_INT8 else torch.uint8, device="cuda")
+    scales = torch.full((rows,), -1.0, device="cuda")
+    pk.rms_norm_quantize(kind, x, r, w, r_out, out, scales, eps)
+    if keep:
+        # the fp32 sum, then fp16: two roundings
+        plain.close(r_out, h, h.abs() * (plain.U16 + 2 * plain.U32) + plain.TINY16, "residual")
+    # sum of squares: at most 64 fused steps in a lane and 10 levels, half of it after the root; five more roundings
+    rel = (74 / 2 + 6) * plain.U32
+    plain.close(scales, torch.where(want_scale > 0, want_scale, torch.ones_like(want_scale)), want_scale * rel, "scales")
+    s = scales.double()[:, None]
+    if kind == pk.NORM_INT8:
+        assert int(out.abs().max()) <= 127
+        plain.close(out.double() * s, y, 0.5 * s + 2 * rel * y.abs() + s * 1e-6, "codes")
+    else:  # e4m3: half a step is 2^-4 of the value, 2^-10 of the scale below its smallest normal
+        plain.close(plain.e4m3_values(out) * s, y, y.abs() * (2.0**-4 + 2 * rel) + s * 2.0**-10, "codes")
+
+
+@pytest.mark.parametrize("rows,width", [(1, 8), (1, 1024), (3, 504), (5, 512), (7, 520), (2, 1000), (9, 1032), (130, 1024), (4, 2048), (3, 2056), (6, 4096),
+                                        (2, 4104), (3, 8192), (2, 8200), (1, 16384), (1025, 640)])
+@pytest.mark.parametrize("kind", [0, 1])
+def test_norm(pk, kind, rows, width):  # noqa: F811
+    g = gen(rows * 31 + width + kind)
+    x, r, w = randn(g, rows, width), randn(g, rows, width, scale=4.0), randn(g, width)
+    check_norm(pk, kind, x, r, w, 1e-5)
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+def test_norm_without_residual_and_in_place(pk, kind):  # noqa: F811
+    g = gen(5)
+    x, r, w = randn(g, 33, 1024), randn(g, 33, 1024), randn(g, 1024)
+    check_norm(pk, kind, x, None, w, 1e-6, keep=False)
+    check_norm(pk, kind, x, None, w, 1e-6)
+    check_norm(pk, kind, x, r, w, 1e-6, keep=False)
+    first = x.clone()
+    check_norm(pk, kind, x, r, w, 1e-6, in_place=True)
+    assert torch.equal(x, first)
+    out, scales = torch.empty((33, 1024), dtype=torch.int8 if kind else torch.uint8, device="cuda"), torch.empty(33, device="cuda")
+    again, also = torch.empty_like(out), torch.empty_like(scales)
+    pk.rms_norm_quantize(kind, x, r, w, None, out, scales, 1e-6)
+    pk.rms_norm_quantize(kind, x, r, w, x, again, also, 1e-6)  # the sum over the input
+    assert torch.equal(out, again) and torch.equal(scales, also) and not torch.equal(x, first)
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("scale", [2.0**-20, 1.0, 8000.0])
+def test_norm_small_and_large_rows(pk, kind, scale):  # noqa: F811
+    g = gen(8)
+    x, r, w = randn(g, 5, 1536, scale=scale), randn(g, 5, 1536, scale=scale), randn(g, 1536, scale=0.01)
+    for eps in (0.0, 1e-5):
+        check_norm(pk, kind, x, r, w, eps)
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("width", [1024, 4096])
+def test_norm_rows_of_zeros_and_not_finite(pk, kind, width):  # noqa: F811
+    g = gen(9)
+    x, w = randn(g, 6, width), randn(g, width)
+    x[1] = 0
+    x[3, 17] = float("inf")
+    x[4, width - 1] = float("nan")
+    clean = x.clone()
+    clean[3:5] = 1
+    out = torch.empty((6, width), dtype=torch.int8 if kind else torch.uint8, device="cuda")
+    scales, want, want_scales = torch.empty(6, device="cuda"), torch.empty_like(out), torch.empty(6, device="cuda")
+    for eps in (0.0, 1e-5):
+        pk.rms_norm_quantize(kind, x, None, w, None, out, scales, eps)
+        pk.rms_norm_quantize(kind, clean, None, w, None, want, want_scales, eps)
+        assert scales[1] == 1 and not (out[1] & 0x7F).any()  # 0 * -w is -0, whose code is 0x80
+        assert torch.isnan(scales[3:5]).all() and (out[3:5] == (0 if kind else 0x7F)).all()
+        for row in (0, 1, 2, 5):  # the others do not see it
+            assert torch.equal(out[row], want[row]) and scales[row] == want_scales[row]
+
+
+def test_norm_result_does_not_depend_on_the_batch(pk):  # noqa: F811
+    g = gen(10)
+    x, w = randn(g, 300, 1024), randn(g, 1024)
+    out, scales = torch.empty((300, 1024), dtype=torch.uint8, device="cuda"), torch.empty(300, device="cuda")
+    pk.rms_norm_quantize(0, x, None, w, None, out, scales, 1e-5)
+    one, s = torch.empty((1, 1024), dtype=torch.uint8, device="cuda"), torch.empty(1, device="cuda")
+    for row in (0, 63, 299):
+        pk.rms_norm_quantize(0, x[row:row + 1], None, w, None, one, s, 1e-5)
+        assert torch.equal(one[0], out[row]) and s[0] == scales[row]
+
+
+# ---- matrix-vector products -----------------------------------------------------------
+
+def weights(g, n, k):
+    q = torch.randint(0, 256, (n, k // 2), generator=g, device="cuda", dtype=torch.uint8).view(torch.int32)
+    scales = (torch.rand((n, k // 128), generator=g, device="cuda") * 0.02 + 0.001).half()
+    zeros = torch.randint(0, 16, (n, k // 128), generator=g, device="cuda").half()
+    return q, scales, zeros
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1, 128), (1, 16, 128), (2, 17, 256), (16, 33, 384), (1, 1030, 640), (3, 100, 1024), (5, 1024, 4096), (16, 4096, 1024),
+                                   (8, 250, 8192), (7, 40, 16384), (1, 15, 65536), (13, 5000, 512), (4, 3000, 4096), (16, 12321, 896)])
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("fp32", [False, True])
+def test_gemv(pk, m, n, k, int8, fp32):  # noqa: F811
+    g = gen(m + n + k + int8)
+    q, scales, zeros = weights(g, n, k)
+    bias = torch.randn(n, generator=g, device="cuda") if (m + n) % 3 else None
+    # whatever lies behind the rows and the outputs must not matter and must stay
+    if int8:
+        rows = torch.randint(-127, 128, (m + 2, k), generator=g, device="cuda", dtype=torch.int8)
+        xs = torch.rand(m, generator=g, device="cuda") * 0.02
+    else:
+        rows, xs = randn(g, m + 2, k), None
+        rows[m:] = float("nan")
+    x = rows[:m]
+    whole = torch.full((m + 1, n), -3.0, dtype=torch.float32 if fp32 else torch.float16, device="cuda")
+    if int8:
+        pk.gemv_int4g128_a8(x, xs, q, scales, zeros, bias, whole[:m])
+    else:
+        pk.gemv_int4g128(x, q, scales, zeros, bias, whole[:m])
+    y, bound = plain.gemv(x, xs, q, scales, zeros, bias)
+    plain.close(whole[:m], y, bound + (0 if fp32 else y.abs() * plain.U16 * (1 + 2.0**-10) + plain.TINY16), f"{m} x {n} x {k}")
+    assert (whole[m] == -3).all()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_gemv_against_the_linear(pk, int8):  # noqa: F811
+    """One row of the 16-row product equals the one-row product; the packer's weights multiply as in the linear."""
+    g = gen(3)
+    n, k = 1024, 1024
+    w = randn(g, n, k, scale=0.02)
+    q = torch.empty((n, k // 8), dtype=torch.int32, device="cuda")
+    scales, zeros = torch.empty((n, k // 128), dtype=torch.float16, device="cuda"), torch.empty((n, k // 128), dtype=torch.float16, device="cuda")
+    pk.call("pk_pack_int4_g128", w, n, k, q, scales, zeros)
+    x, out, one, lin = randn(g, 16, k), torch.empty((16, n), device="cuda"), torch.empty((1, n), device="cuda"), torch.empty((16, n), device="cuda")
+    if int8:
+        x8, xs = torch.empty((16, k), dtype=torch.int8, device="cuda"), torch.empty(16, device="cuda")
+        pk.call("pk_quantize_rows", 1, x, x8, xs, 16, 16, k)
+        pk.gemv_int4g128_a8(x8, xs, q, scales, zeros, None, out)
+        pk.gemv_int4g128_a8(x8[3:4], xs[3:4], q, scales, zeros, None, one)
+        pk.call("pk_linear_int4g128_a8", x8, xs, q, scales, zeros, None, lin, 1, 16, n, k)
+        rows, xs_ = x8, xs
+    else:
+        pk.gemv_int4g128(x, q, scales, zeros, None, out)
+        pk.gemv_int4g128(x[3:4], q, scales, zeros, None, one)
+        pk.call("pk_linear_int4g128", x, q, scales, zeros, None, lin, 1, 16, n, k)
+        rows, xs_ = x, None
+    assert torch.equal(one[0], out[3])
+    y, bound = plain.gemv(rows, xs_, q, scales, zeros, None)
+    plain.close(out, y, bound)
+    if int8:  # the linear's bound is the same
+        plain.close(lin, y, bound)
+    else:  # each of the linear's weights is rounded to fp16
+        plain.close(lin, y, bound + (x.double().abs() @ w.double().abs().t()) * 1.2 * plain.U16)
+
+
+def test_gemv_infinity_and_nan_rows_stay_in_their_row(pk):  # noqa: F811
+    g = gen(4)
+    q, scales, zeros = weights(g, 64, 512)
+    x = randn(g, 4, 512)
+    x[1, 100], x[2, 7] = float("inf"), float("nan")
+    out, clean = torch.empty((4, 64), device="cuda"), torch.empty((4, 64), device="cuda")
+    pk.gemv_int4g128(x, q, scales, zeros, None, out)
+    y = x.clone()
+    y[1:3] = 0
+    pk.gemv_int4g128(y, q, scales, zeros, None, clean)
+    assert torch.equal(out[0], clean[0]) and torch.equal(out[3], clean[3])
+    assert not torch.isfinite(out[1:3]).any()
+
+
+# ---- page plan ------------------------------------------------------------------------
+
+def run_plan(pk, held, added, free, begin, end, table, page, capacity, positions=True):  # noqa: F811
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    n = len(held)
+    t = dict(held=i32(held), added=i32(added), free=i32(free), range=i32([begin, end]), table=i32(table), starts=i32([-5] * (n + 1)), lengths=i32([-5] * n),
+             slots=i32([-5] * capacity), positions=i32([-5] * capacity) if positions else None, info=i32([-5] * 4))
+    pk.page_plan(*t.values(), page)
+    got = [t[k].tolist() if t[k] is not None else None for k in ("table", "starts", "lengths", "slots", "positions", "info")]
+    want = list(plain.plan(held, added, free, begin, end, table, page, capacity))
+    if not positions:
+        want[4] = None
+    for name, a, b in zip(("table", "starts", "lengths", "slots", "positions", "info"), got, want):
+        assert a == b, name
+    return got[5]
+
+
+def plan_case(seed, n, page, most, grow, capacity_more=5):
+    import random
+
+    rng = random.Random(seed)
+    held = [rng.choice([0, 1, page - 1, page, page + 1, rng.randint(0, most)]) for _ in range(n)]
+    added = [rng.choice([0, 1, 1, 1, rng.randint(0, grow)]) for _ in range(n)]
+    up = lambda t: -(-t // page)  # noqa: E731
+    columns = max(up(h + a) for h, a in zip(held, added)) + rng.randint(0, 3)
+    ids = list(range(10 ** 5))
+    rng.shuffle(ids)
+    table, at = [], 0
+    for h in held:
+        table.append(ids[at:at + up(h)] + [-7] * (columns - up(h)))
+        at += up(h)
+    need = sum(up(h + a) - up(h) for h, a in zip(held, added))
+    free = ids[at:at + need + 4]
+    return held, added, free, 2, need + 3, [r[:max(columns, 1)] or [-7] for r in table], page, sum(added) + rng.randint(0, capacity_more)
+
+
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 255, 256, 257, 700, 4096])
+@pytest.mark.parametrize("page", [16, 256])
+def test_plan(pk, n, page):  # noqa: F811
+    case = plan_case(n + page, n, page, 40 if n > 1000 else 700, 8 if n > 1000 else 300)
+    case = [max(c, 1) if isinstance(c, int) and i == 7 else c for i, c in enumerate(case)]
+    if not case[5][0]:
+        case[5] = [[-7] for _ in case[5]]
+    assert run_plan(pk, *case)[2] == 0
+    run_plan(pk, *case, positions=False)
+
+
+def test_plan_long_prompt_and_nothing_to_add(pk):  # noqa: F811
+    assert run_plan(pk, [0, 5], [30000, 0], list(range(2000)), 0, 2000, [[-7] * 1900, [1999] + [-7] * 1899], 16, 30001) == [30000, 1875, 0, 0]
+    assert run_plan(pk, [0, 5], [0, 0], [3], 0, 1, [[-7], [2]], 16, 4) == [0, 0, 0, 0]
+
+
+def test_plan_all_or_nothing(pk):  # noqa: F811
+    held, added, free, begin, end, table, page, capacity = plan_case(77, 40, 32, 300, 90)
+    tokens = sum(added)
+    ok = (held, added, free, begin, end, table, page, capacity)
+    assert run_plan(pk, *ok)[2] == 0
+    assert run_plan(pk, held, added, free, begin, end - 2, table, page, capacity)[2] == 1
+    assert run_plan(pk, held, added, free[:-3], begin, 10 ** 6, table, page, capacity)[2] == 1
+    assert run_plan(pk, held, added, free, begin, end, table, page, tokens - 1)[2] == 4
+    assert run_plan(pk, held, added, free, -1, end, table, page, capacity)[2] == 8
+    assert run_plan(pk, held, added[:-1] + [-1], free, begin, end, table, page, capacity)[2] & 8
+    assert run_plan(pk, held[:-1] + [-3], added, free, begin, end, table, page, capacity)[2] & 8
+    assert run_plan(pk, held, added[:-1] + [100000], free, begin, end, table, page, capacity)[2] & 7 == 7
+    big = 2 ** 31 - 1
+    assert run_plan(pk, [0, 0, 0], [big, big, big], free, 0, 4, [[1], [2], [3]], 16, 9)[2] & 7 == 7
+
+
+def test_plan_of_a_negative_page(pk):  # noqa: F811
+    assert run_plan(pk, [3, 16], [2, 1], [-9, 4], 0, 2, [[5, -7], [6, -7]], 16, 4)[2] == 0  # its slots are -1
+
+
+# ---- cache write ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens,kv,d,page", [(1, 1, 64, 16), (1, 8, 128, 16), (61, 8, 128, 16), (70, 3, 64, 32), (257, 2, 128, 64), (300, 1, 128, 256),
+                                              (513, 5, 64, 128), (1000, 8, 128, 32)])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("order", ["runs", "shuffled", "offset"])
+def test_write(pk, tokens, kv, d, page, fp8, order):  # noqa: F811
+    g = gen(tokens + d + page)
+    pages = -(-tokens // page) + 4
+    slots = torch.arange(tokens, device="cuda")
+    if order == "offset":
+        slots = slots + 5
+    slots = torch.randperm(pages, generator=g, device="cuda")[slots // page] * page + slots % page
+    if order == "shuffled":
+        slots = torch.randperm(pages * page, generator=g, device="cuda")[:tokens]
+    slots[tokens // 2] = -1
+    if tokens > 8:
+        slots[3], slots[tokens - 1] = pages * page, 2 ** 31 - 1
+    slots = slots.int()
+    rows = randn(g, tokens, 3 * kv * d, scale=100.0)
+    rows[0, :3] = torch.tensor([float("inf"), float("nan"), -60000.0], dtype=torch.float16)
+    k, v = rows[:, kv * d:2 * kv * d].unflatten(1, (kv, d)), rows[:, 2 * kv * d:].unflatten(1, (kv, d))
+    inverse = (0.7, 3.0) if fp8 else (1.0, 1.0)
+    kind = torch.uint8 if fp8 else torch.float16
+    key, value = torch.full((pages, kv, page, d), 5, dtype=kind, device="cuda"), torch.full((pages, kv, d, page), 6, dtype=kind, device="cuda")
+    want_key, want_value = key.clone(), value.clone()
+    pk.paged_cache_write(k, v, slots, key, value, *inverse)
+    real = (slots >= 0) & (slots < pages * page)
+    at = slots[real].long()
+    enc = lambda x, i: (x[real].float() * i).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8) if fp8 else x[real]  # noqa: E731
+    want_key[at // page, :, at % page] = enc(k, inverse[0])
+    want_value.transpose(2, 3)[at // page, :, at % page] = enc(v, inverse[1])
+    bits = lambda x: x if fp8 else x.view(torch.int16)  # noqa: E731
+    assert torch.equal(bits(key), bits(want_key)) and torch.equal(bits(value), bits(want_value))
