@@ -730,7 +730,7 @@ int32_t pk_paged_cache_write(int32_t kind, const uint16_t* key, int64_t key_stri
  * values that a query does not see do not reach it.  Keys of a page id outside
  * [0, pages) count as not there; lengths beyond max_pages * page_size are cut.
  * Rows of output outside the sequences' ranges stay as they were.  max_queries
- * (<= tokens) is at least the largest n, tokens <= 2^20, sequences <= 65535.
+ * (<= tokens) is at least the largest n, tokens <= 2^20, sequences <= 4096.
  * Scores, the running maximum and sum and the output's sum are fp32; scores
  * multiply fp16 queries with fp16 or e4m3 keys exactly, probabilities are
  * rounded to fp16 for the second product (their sum is not).

@@ -1023,9 +1023,9 @@ static int32_t paged_shape(int32_t tokens, int32_t max_queries, int32_t sequence
         set_error("heads must be a multiple of kv_heads up to 1024, got %d for %d", heads, kv_heads);
         return PK_E_SHAPE;
     }
-    if (tokens < 0 || tokens > 1 << 20 || max_queries < 0 || max_queries > tokens || sequences < 0 || sequences > 65535 || max_pages <= 0 ||
+    if (tokens < 0 || tokens > 1 << 20 || max_queries < 0 || max_queries > tokens || sequences < 0 || sequences > 4096 || max_pages <= 0 ||
         max_pages > (1 << 30) >> shift) {
-        set_error("paged attention needs tokens <= 2^20, max_queries <= tokens, sequences <= 65535 and max_pages * page_size <= 2^30 "
+        set_error("paged attention needs tokens <= 2^20, max_queries <= tokens, sequences <= 4096 and max_pages * page_size <= 2^30 "
                   "(tokens=%d max_queries=%d sequences=%d max_pages=%d)", tokens, max_queries, sequences, max_pages);
         return PK_E_SHAPE;
     }
@@ -1036,7 +1036,7 @@ int64_t pk_paged_attention_workspace_bytes(int32_t tokens, int32_t max_queries, 
                                            int32_t head_dim, int32_t page_size, int32_t max_pages) {
     const int32_t shift = paged_shape(tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, max_pages);
     if (shift < 0) return shift;
-    return 0;
+    return (int64_t)paged_attention_workspace(head_dim, shift, max_pages);
 }
 
 int32_t pk_paged_attention(int32_t kind, const uint16_t* query, int64_t query_stride, const void* key_cache, const void* value_cache,
@@ -1091,7 +1091,7 @@ int32_t pk_paged_attention(int32_t kind, const uint16_t* query, int64_t query_st
     a.right = right < 0 || right > 1 << 30 ? -1 : right;
     a.scale_log2 = scale * (kind == PK_CACHE_FP8 ? key_scale : 1.0f) * 1.4426950408889634f;
     a.value_scale = kind == PK_CACHE_FP8 ? value_scale : 1.0f;
-    launch_paged_attention(kind, a, head_dim, max_queries, STREAM);
+    launch_paged_attention(kind, a, head_dim, max_queries, workspace, STREAM);
     return check_launch("paged_attention");
 }
 

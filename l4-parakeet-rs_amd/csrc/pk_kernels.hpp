@@ -101,7 +101,8 @@ struct PagedArgs {
     int tokens, sequences, kv_heads, group, shift, pages, max_pages, left, right;
     float scale_log2, value_scale;
 };
-void launch_paged_attention(int kind, const PagedArgs& args, int head_dim, int max_queries, hipStream_t s);
+size_t paged_attention_workspace(int head_dim, int page_shift, int max_pages);
+void launch_paged_attention(int kind, const PagedArgs& args, int head_dim, int max_queries, void* workspace, hipStream_t s);
 void set_error(const char* fmt, ...);
 int cu_count();
 int launch_sparse24_contract(const uint8_t* data, const uint8_t* meta, const uint8_t* w, const float* w_scales, float in_scale,

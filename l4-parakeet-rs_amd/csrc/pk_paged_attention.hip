@@ -38,41 +38,54 @@ template <bool kF8> __device__ __forceinline__ v8h operand(const uint4& raw, int
     }
 }
 
-// Whether any of eight fp16 values is an infinity or a NaN (exponent all ones: adding
-// one there carries into the sign bit, and nowhere else).
-__device__ __forceinline__ uint32_t not_finite(const v8h& v) {
-    const uint4 w = __builtin_bit_cast(uint4, v);
-    const uint32_t e = 0x7c007c00u, one = 0x04000400u;
-    return (((w.x & e) + one) | ((w.y & e) + one) | ((w.z & e) + one) | ((w.w & e) + one)) & 0x80008000u;
+// Nonzero where 16 bytes of cache values hold an infinity or a NaN: all ones under the sign
+// (e4m3: exponent and mantissa, its only NaN; fp16: the exponent), so that adding one
+// there carries into the sign bit, and nowhere else.
+template <bool kF8> __device__ __forceinline__ uint32_t not_finite(const uint4& w) {
+    const uint32_t e = kF8 ? 0x7f7f7f7fu : 0x7c007c00u, one = kF8 ? 0x01010101u : 0x04000400u;
+    return (((w.x & e) + one) | ((w.y & e) + one) | ((w.z & e) + one) | ((w.w & e) + one)) & (kF8 ? 0x80808080u : 0x80008000u);
 }
 
-// o += V P for an operand with infinities or NaN in it, where a product with the
-// zero of a masked key would spoil rows that do not see that key: the finite values
-// are multiplied, and each kind of the others counted over the keys a row sees.
-__device__ __forceinline__ v4f add_not_finite(const v8h& v, const v8h& p, uint32_t seen, v4f o) {
-    const _Float16 one = (_Float16)1.0f, zero = (_Float16)0.0f, inf = (_Float16)__builtin_inff();
-    v8h fin, pos, neg, nan, vis;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const bool is_pos = v[j] == inf, is_neg = v[j] == -inf, is_nan = v[j] != v[j];
-        fin[j] = is_pos || is_neg || is_nan ? zero : v[j];
-        pos[j] = is_pos ? one : zero;
-        neg[j] = is_neg ? one : zero;
-        nan[j] = is_nan ? one : zero;
-        vis[j] = (seen >> j) & 1u ? one : zero;
+// Which values of a word are NaN (0), +inf (1) or -inf (2): the cache's 1.0 where so.
+template <bool kF8> __device__ __forceinline__ uint32_t odd_ones(uint32_t w, int which) {
+    if constexpr (kF8) {
+        return (((w & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 0x38u;
+    } else {
+        const uint32_t odd = (((w & 0x7c007c00u) + 0x04000400u) >> 15) & 0x00010001u;
+        const uint32_t nan = odd & (((w & 0x03ff03ffu) + 0x03ff03ffu) >> 10);
+        const uint32_t sign = (w >> 15) & 0x00010001u, inf = odd & ~nan;
+        return (which == 0 ? nan : (which == 1 ? inf & ~sign : inf & sign)) * 0x3c00u;
     }
-    const v4f none{};
-    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(fin, p, o, 0, 0, 0);
-    const v4f up = __builtin_amdgcn_mfma_f32_16x16x32_f16(pos, vis, none, 0, 0, 0);
-    const v4f down = __builtin_amdgcn_mfma_f32_16x16x32_f16(neg, vis, none, 0, 0, 0);
-    const v4f bad = __builtin_amdgcn_mfma_f32_16x16x32_f16(nan, vis, none, 0, 0, 0);
+}
+template <bool kF8> __device__ __forceinline__ uint32_t odd_cleared(uint32_t w) {
+    if constexpr (kF8) return w & ~((((w & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 0xffu);
+    else return w & ~(((((w & 0x7c007c00u) + 0x04000400u) >> 15) & 0x00010001u) * 0xffffu);
+}
+
+// Infinities and NaN in values, where a product with the zero of a masked key would
+// spoil rows that do not see that key: each kind is counted over the keys that a row
+// sees (bits of `seen`), added to the rows that see one, and cleared from the operand.
+// Rare; in place and one kind after the other, so that it needs few registers.
+template <bool kF8> __device__ __forceinline__ void add_not_finite(uint4& raw, uint32_t seen, v4f& o) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        if (up[r] > 0.0f) o[r] += __builtin_inff();
-        if (down[r] > 0.0f) o[r] -= __builtin_inff();
-        if (bad[r] > 0.0f) o[r] = __builtin_nanf("");
+    for (int kind = 0; kind < (kF8 ? 1 : 3); ++kind) {
+        const uint4 ones{odd_ones<kF8>(raw.x, kind), odd_ones<kF8>(raw.y, kind), odd_ones<kF8>(raw.z, kind), odd_ones<kF8>(raw.w, kind)};
+        v4f count{};
+#pragma unroll
+        for (int u = 0; u < (kF8 ? 2 : 1); ++u) {
+            uint32_t vis[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vis[i] = ((seen >> (8 * u + 2 * i) & 1u) | (seen >> (8 * u + 2 * i + 1) & 1u) << 16) * 0x3c00u;
+            count = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand<kF8>(ones, u), __builtin_bit_cast(v8h, uint4{vis[0], vis[1], vis[2], vis[3]}), count,
+                                                           0, 0, 0);
+        }
+        const float add = kind == 0 ? __builtin_nanf("") : (kind == 1 ? __builtin_inff() : -__builtin_inff());
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (count[r] > 0.0f) o[r] += add;
+        __builtin_amdgcn_sched_barrier(0);
     }
-    return o;
+    raw = uint4{odd_cleared<kF8>(raw.x), odd_cleared<kF8>(raw.y), odd_cleared<kF8>(raw.z), odd_cleared<kF8>(raw.w)};
 }
 
 // One sequence's view for a tile of 16 query rows.
@@ -89,6 +102,13 @@ __device__ __forceinline__ RowTile sequence_of(const PagedArgs& a, int seq) {
     return {s, (e - s) * a.group, len, len - (e - s)};
 }
 
+// The same for a sequence that the whole wave works on, in scalar registers.
+__device__ __forceinline__ RowTile wave_sequence(const PagedArgs& a, int seq) {
+    const RowTile t = sequence_of(a, seq);
+    return {__builtin_amdgcn_readfirstlane(t.start), __builtin_amdgcn_readfirstlane(t.rows), __builtin_amdgcn_readfirstlane(t.length),
+            __builtin_amdgcn_readfirstlane(t.first_pos)};
+}
+
 // Keys [lo, hi) that a query at `pos` sees.
 __device__ __forceinline__ void window(const PagedArgs& a, int pos, int length, int& lo, int& hi) {
     lo = a.left < 0 || pos < a.left ? 0 : pos - a.left;
@@ -96,194 +116,441 @@ __device__ __forceinline__ void window(const PagedArgs& a, int pos, int length, 
     if (hi < 0) hi = 0;
 }
 
-template <int kD, bool kF8>
-__global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
-    constexpr int kSteps = kD / 32, kBlocks = kD / 16;  // MFMA steps of S over features, feature blocks of O
-    constexpr int kU = kF8 ? 2 : 1, kKeys = 32 * kU;    // 16 bytes of a value row hold 8 * kU keys; keys a wave tile
-    constexpr int kBytes = kF8 ? 1 : 2;
-    constexpr int kLoads = kSteps / kU;                 // 16-byte loads of a key row
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
-    const int kvh = blockIdx.x, seq = blockIdx.z;
-    const RowTile t = sequence_of(a, seq);
-    const int row0 = blockIdx.y * 16;
-    if (row0 >= t.rows) return;
-    const int last = t.rows - row0 < 16 ? t.rows - row0 - 1 : 15;
-    const int row = row0 + (l16 < last ? l16 : last);  // rows behind the last repeat it and are not stored
-    const int tok = row / a.group, head = kvh * a.group + row % a.group;
-    int lo, hi, tile_lo, tile_hi, full_lo, full_hi;
-    window(a, t.first_pos + tok, t.length, lo, hi);
-    window(a, t.first_pos + row0 / a.group, t.length, tile_lo, full_hi);       // first row: lowest bounds
-    window(a, t.first_pos + (row0 + last) / a.group, t.length, full_lo, tile_hi);  // last row: highest
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
+// One wave's pass over key tiles for 16 query rows.  Loads are issued a stage ahead: a
+// tile's values while its scores are computed, the next tile's keys before the softmax,
+// and page ids two tiles ahead, since loads return in order.
+template <int kD, bool kF8> struct RowPass {
+    static constexpr int kSteps = kD / 32, kBlocks = kD / 16;  // MFMA steps of S over features, feature blocks of O
+    static constexpr int kU = kF8 ? 2 : 1, kKeys = 32 * kU;    // 16 bytes of a value row hold 8 * kU keys; keys a wave tile
+    static constexpr int kBytes = kF8 ? 1 : 2;
+    static constexpr int kLoads = kSteps / kU;                 // 16-byte loads of a key row
+    static constexpr int kSpan = 4 * kKeys;                    // keys that the four waves take at once
+
+    const PagedArgs& a;
+    const int lane, l16, g, kvh;
+    RowTile t;
+    const int* table;
+    int last_page;
+    int row0, last;              // first row of the tile, index of its last row in it
+    int lo, hi;                  // keys this lane's row sees
+    int tile_lo, tile_hi;        // keys that any row sees
+    int full_lo, full_hi;        // keys that all rows see
     v8h qf[kSteps];
-    const uint16_t* qp = a.query + (size_t)(t.start + tok) * a.query_stride + (size_t)head * kD;
+    v4f acc[kBlocks];
+    float top, total;
+
+    __device__ __forceinline__ RowPass(const PagedArgs& args, int kv_head) : a(args), lane(threadIdx.x & 63), l16(lane & 15), g(lane >> 4), kvh(kv_head) {}
+
+    __device__ __forceinline__ void start(int seq, const RowTile& rows, int first_row) {
+        t = rows;
+        row0 = first_row;
+        table = a.table + (size_t)seq * a.max_pages;
+        last_page = t.length > 0 ? (t.length - 1) >> a.shift : 0;
+        last = t.rows - row0 < 16 ? t.rows - row0 - 1 : 15;
+        const int row = row0 + (l16 < last ? l16 : last);  // rows behind the last repeat it and are not stored
+        const int tok = row / a.group, head = kvh * a.group + row % a.group;
+        window(a, t.first_pos + tok, t.length, lo, hi);
+        window(a, t.first_pos + row0 / a.group, t.length, tile_lo, full_hi);           // the first row's bounds are the lowest
+        window(a, t.first_pos + (row0 + last) / a.group, t.length, full_lo, tile_hi);  // the last row's the highest
+        const uint16_t* qp = a.query + (size_t)(t.start + tok) * a.query_stride + (size_t)head * kD;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-        const int d = kF8 ? (s >> 1) * 64 + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
-        qf[s] = *(const v8h*)(qp + d);
+        for (int s = 0; s < kSteps; ++s) qf[s] = *(const v8h*)(qp + (kF8 ? (s >> 1) * 64 + 16 * g + 8 * (s & 1) : 32 * s + 8 * g));
+#pragma unroll
+        for (int c = 0; c < kBlocks; ++c) acc[c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        top = kNegInf;
+        total = 0.0f;
     }
 
-    v4f acc[kBlocks];
+    // This lane reads keys (as rows of S) and values (as columns of O) from one page each.
+    struct Ids {
+        int key, value;
+    };
+    __device__ __forceinline__ Ids ids(int k0) const {
+        int kc = (k0 + 8 * kU * (l16 >> 2)) >> a.shift, vc = (k0 + 8 * kU * g) >> a.shift;
+        kc = kc > last_page ? last_page : kc;
+        vc = vc > last_page ? last_page : vc;
+        return {table[kc], table[vc]};
+    }
+    __device__ __forceinline__ size_t page_of(int id) const {
+        id = (unsigned)id < (unsigned)a.pages ? id : 0;
+        return ((size_t)id * a.kv_heads + kvh) * ((size_t)kD * kBytes << a.shift);
+    }
+    __device__ __forceinline__ void load_keys(int k0, int id, uint4 (&raw)[kU][2][kLoads]) const {
+        const int key = k0 + 8 * kU * (l16 >> 2) + (l16 & 3);
+        const uint8_t* p = a.key + page_of(id) + (size_t)(key & ((1 << a.shift) - 1)) * (kD * kBytes) + 16 * g;
 #pragma unroll
-    for (int c = 0; c < kBlocks; ++c) acc[c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    float top = kNegInf, total = 0.0f;
-    const int* table = a.table + (size_t)seq * a.max_pages;
-    const int last_page = t.length > 0 ? (t.length - 1) >> a.shift : 0;
-    const int in_page = (1 << a.shift) - 1;
-    const size_t page_bytes = (size_t)kD * kBytes << a.shift;
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int s = 0; s < kLoads; ++s) raw[u][b][s] = *(const uint4*)(p + (8 * u + 4 * b) * kD * kBytes + 64 * s);
+    }
+    __device__ __forceinline__ void load_values(int k0, int id, uint4 (&raw)[kBlocks]) const {
+        const int key = k0 + 8 * kU * g;
+        const uint8_t* p = a.value + page_of(id) + (((size_t)l16 << a.shift) + (key & ((1 << a.shift) - 1))) * kBytes;
+#pragma unroll
+        for (int c = 0; c < kBlocks; ++c) raw[c] = *(const uint4*)(p + (((size_t)c * 16) << a.shift) * kBytes);
+    }
 
-    for (int k0 = (tile_lo & ~(kKeys - 1)) + wave * kKeys; k0 < tile_hi; k0 += 4 * kKeys) {
-        // this lane's 8 * kU keys (its values and scores) lie in one page
-        const int mine = k0 + 8 * kU * g;
-        int col = mine >> a.shift;
-        if (col > last_page) col = last_page;
-        int id = table[col];
-        const bool ok = (unsigned)id < (unsigned)a.pages;
-        if (!ok) id = 0;
-        const int there = ok ? t.length - mine : 0;  // keys from `mine` on that exist
+    // Tiles k0, k0 + kSpan, ... below `end` (and inside the rows' range).
+    __device__ __forceinline__ void run(int k0, int end) {
+        while (k0 + kKeys <= tile_lo) k0 += kSpan;
+        if (end > tile_hi) end = tile_hi;
+        if (k0 >= end) return;
+        Ids id = ids(k0), next = ids(k0 + kSpan);
         uint4 kraw[kU][2][kLoads], vraw[kBlocks];
-        const uint8_t* vp = a.value + ((size_t)id * a.kv_heads + kvh) * page_bytes + (((size_t)l16 << a.shift) + (mine & in_page)) * kBytes;
+        load_keys(k0, id.key, kraw);
+        for (; k0 < end; k0 += kSpan) {
+            load_values(k0, id.value, vraw);
+            __builtin_amdgcn_sched_barrier(0);  // out before the wait for this tile's keys
+            const int mine = k0 + 8 * kU * g;
+            const bool ok = (unsigned)id.value < (unsigned)a.pages;
+            const int there = ok ? t.length - mine : 0;  // keys from `mine` on that exist
+            float p[8 * kU];
 #pragma unroll
-        for (int u = 0; u < kU; ++u)
+            for (int u = 0; u < kU; ++u)
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int key = k0 + 8 * kU * (l16 >> 2) + 8 * u + 4 * b + (l16 & 3);
-                int kcol = key >> a.shift;
-                if (kcol > last_page) kcol = last_page;
-                int kid = table[kcol];
-                if ((unsigned)kid >= (unsigned)a.pages) kid = 0;
-                const uint8_t* kp = a.key + ((size_t)kid * a.kv_heads + kvh) * page_bytes + (size_t)(key & in_page) * kD * kBytes + 16 * g;
+                for (int b = 0; b < 2; ++b) {
+                    v4f sc{};
 #pragma unroll
-                for (int s = 0; s < kLoads; ++s) kraw[u][b][s] = *(const uint4*)(kp + 64 * s);
+                    for (int s = 0; s < kSteps; ++s)
+                        sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand<kF8>(kraw[u][b][s / kU], s % kU), qf[s], sc, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p[8 * u + 4 * b + r] = sc[r] * a.scale_log2;
+                }
+            if (k0 + kSpan < end) load_keys(k0 + kSpan, next.key, kraw);
+            const Ids later = ids(k0 + 2 * kSpan);
+            __builtin_amdgcn_sched_barrier(0);
+            const bool whole = k0 >= full_lo && k0 + kKeys <= full_hi && __all(ok);
+            uint32_t seen = 0;  // bit j: this lane's row sees key mine + j
+            if (!whole) {
+#pragma unroll
+                for (int j = 0; j < 8 * kU; ++j) {
+                    const bool see = mine + j >= lo && mine + j < hi && j < there;
+                    seen |= (uint32_t)see << j;
+                    if (!see) p[j] = kNegInf;
+                }
             }
+            float m = p[0];
 #pragma unroll
-        for (int c = 0; c < kBlocks; ++c) vraw[c] = *(const uint4*)(vp + (((size_t)c * 16) << a.shift) * kBytes);
-
-        float p[8 * kU];
-#pragma unroll
-        for (int u = 0; u < kU; ++u)
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                v4f sc{};
-#pragma unroll
-                for (int s = 0; s < kSteps; ++s)
-                    sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand<kF8>(kraw[u][b][s / kU], s % kU), qf[s], sc, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) p[8 * u + 4 * b + r] = sc[r] * a.scale_log2;
-            }
-        const bool whole = k0 >= full_lo && k0 + kKeys <= full_hi && __all(ok);
-        uint32_t seen = 0;  // bit j: this lane's row sees key mine + j
-        if (!whole) {
+            for (int j = 1; j < 8 * kU; ++j) m = __builtin_fmaxf(m, p[j]);
+            m = max_level(max_level(m, 16), 32);
+            const float new_top = __builtin_fmaxf(top, m);
+            const float base = new_top == kNegInf ? 0.0f : new_top;
+            const float keep = __builtin_amdgcn_exp2f(top - base);
+            top = new_top;
+            float sum = 0.0f;
+            v8h pf[kU];
 #pragma unroll
             for (int j = 0; j < 8 * kU; ++j) {
-                const bool see = mine + j >= lo && mine + j < hi && j < there;
-                seen |= (uint32_t)see << j;
-                if (!see) p[j] = kNegInf;
+                p[j] = __builtin_amdgcn_exp2f(p[j] - base);
+                sum += p[j];
+                pf[j >> 3][j & 7] = (_Float16)p[j];
             }
-        }
-        float m = p[0];
+            total = total * keep + sum;
 #pragma unroll
-        for (int j = 1; j < 8 * kU; ++j) m = __builtin_fmaxf(m, p[j]);
-        m = max_level(max_level(m, 16), 32);
-        const float new_top = __builtin_fmaxf(top, m);
-        const float base = new_top == kNegInf ? 0.0f : new_top;
-        const float keep = __builtin_amdgcn_exp2f(top - base);
-        top = new_top;
-        float sum = 0.0f;
-        v8h pf[kU];
+            for (int c = 0; c < kBlocks; ++c) acc[c] = acc[c] * keep;
+            if (!whole) {
+                uint32_t odd = 0;
+                // keys that do not exist hold anything: their values are taken as zero
+                constexpr int kPerWord = 4 / kBytes;
+                uint32_t there_mask[4];
 #pragma unroll
-        for (int j = 0; j < 8 * kU; ++j) {
-            p[j] = __builtin_amdgcn_exp2f(p[j] - base);
-            sum += p[j];
-            pf[j >> 3][j & 7] = (_Float16)p[j];
-        }
-        total = total * keep + sum;
-#pragma unroll
-        for (int c = 0; c < kBlocks; ++c) acc[c] = acc[c] * keep;
-        if (whole) {
-#pragma unroll
-            for (int c = 0; c < kBlocks; ++c)
-#pragma unroll
-                for (int u = 0; u < kU; ++u)
-                    acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand<kF8>(vraw[c], u), pf[u], acc[c], 0, 0, 0);
-        } else {
-            // keys that do not exist hold anything: their values are taken as zero
-            v8h vf[kBlocks][kU];
-            uint32_t odd = 0;
-#pragma unroll
-            for (int c = 0; c < kBlocks; ++c)
-#pragma unroll
-                for (int u = 0; u < kU; ++u) {
-                    vf[c][u] = operand<kF8>(vraw[c], u);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (8 * u + j >= there) vf[c][u][j] = (_Float16)0.0f;
-                    odd |= not_finite(vf[c][u]);
+                for (int w = 0; w < 4; ++w) {
+                    const int n = there - w * kPerWord;  // keys of this word that exist
+                    there_mask[w] = n >= kPerWord ? 0xffffffffu : (n <= 0 ? 0u : (1u << (8 * kBytes * n)) - 1u);
                 }
-            if (__any(odd != 0)) {
 #pragma unroll
-                for (int c = 0; c < kBlocks; ++c)
+                for (int c = 0; c < kBlocks; ++c) {
+                    vraw[c].x &= there_mask[0];
+                    vraw[c].y &= there_mask[1];
+                    vraw[c].z &= there_mask[2];
+                    vraw[c].w &= there_mask[3];
+                    odd |= not_finite<kF8>(vraw[c]);
+                }
+                if (__any(odd != 0)) {
 #pragma unroll
-                    for (int u = 0; u < kU; ++u) acc[c] = add_not_finite(vf[c][u], pf[u], seen >> (8 * u), acc[c]);
-            } else {
-#pragma unroll
-                for (int c = 0; c < kBlocks; ++c)
-#pragma unroll
-                    for (int u = 0; u < kU; ++u) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[c][u], pf[u], acc[c], 0, 0, 0);
+                    for (int c = 0; c < kBlocks; ++c) add_not_finite<kF8>(vraw[c], seen, acc[c]);
+                }
             }
+#pragma unroll
+            for (int c = 0; c < kBlocks; ++c)
+#pragma unroll
+                for (int u = 0; u < kU; ++u) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand<kF8>(vraw[c], u), pf[u], acc[c], 0, 0, 0);
+            id = next;
+            next = later;
         }
     }
+};
 
-    // join the four waves' parts
-    total = add_level(add_level(total, 16), 32);
-    __shared__ float part[4][16][kD + 4];
-    __shared__ float part_top[4][16], part_total[4][16];
+// What the four waves hold of 16 rows, side by side in LDS.
+template <int kD> struct Parts {
+    float acc[4][16][kD + 4];
+    float top[4][16], total[4][16];
+};
+
+template <int kD, bool kF8> __device__ __forceinline__ void to_lds(RowPass<kD, kF8>& pass, Parts<kD>& parts) {
+    const int wave = threadIdx.x >> 6;
+    const float total = add_level(add_level(pass.total, 16), 32);
 #pragma unroll
-    for (int c = 0; c < kBlocks; ++c) *(v4f*)&part[wave][l16][16 * c + 4 * g] = acc[c];
-    if (g == 0) {
-        part_top[wave][l16] = top;
-        part_total[wave][l16] = total;
-    }
-    __syncthreads();
-    const int r = threadIdx.x >> 4;
-    if (r > last) return;
-    float best = part_top[0][r];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) best = __builtin_fmaxf(best, part_top[w][r]);
-    if (best == kNegInf) best = 0.0f;
-    float f[4], sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        f[w] = __builtin_amdgcn_exp2f(part_top[w][r] - best);
-        sum += part_total[w][r] * f[w];
-    }
-    const float inv = sum == 0.0f ? 0.0f : a.value_scale / sum;
-    const int orow = row0 + r;
-    uint16_t* op = a.out + (size_t)(t.start + orow / a.group) * a.out_stride + (size_t)(kvh * a.group + orow % a.group) * kD;
-    constexpr int kEach = kD / 16;
-    const int d0 = (threadIdx.x & 15) * kEach;
-#pragma unroll
-    for (int j = 0; j < kEach; j += 2) {
-        float v[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float x2 = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) x2 += part[w][r][d0 + j + e] * f[w];
-            v[e] = x2 * inv;
-        }
-        *(uint32_t*)(op + d0 + j) = (uint32_t)f2h(v[0]) | ((uint32_t)f2h(v[1]) << 16);
+    for (int c = 0; c < kD / 16; ++c) *(v4f*)&parts.acc[wave][pass.l16][16 * c + 4 * pass.g] = pass.acc[c];
+    if (pass.g == 0) {
+        parts.top[wave][pass.l16] = pass.top;
+        parts.total[wave][pass.l16] = total;
     }
 }
 
-void launch_paged_attention(int kind, const PagedArgs& a, int head_dim, int max_queries, hipStream_t s) {
-    const dim3 grid((unsigned)a.kv_heads, (unsigned)((max_queries * a.group + 15) / 16), (unsigned)a.sequences);
+// Row r of the joined waves: its maximum and sum, and kD / 16 features from d0 on.
+template <int kD> __device__ __forceinline__ void join(const Parts<kD>& parts, int r, int d0, float& best, float& total, float (&v)[kD / 16]) {
+    best = parts.top[0][r];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) best = __builtin_fmaxf(best, parts.top[w][r]);
+    const float base = best == kNegInf ? 0.0f : best;
+    total = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kD / 16; ++j) v[j] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = __builtin_amdgcn_exp2f(parts.top[w][r] - base);
+        total += parts.total[w][r] * f;
+#pragma unroll
+        for (int j = 0; j < kD / 16; ++j) v[j] += parts.acc[w][r][d0 + j] * f;
+    }
+}
+
+template <int kN>
+__device__ __forceinline__ void store_row(const PagedArgs& a, const RowTile& t, int kvh, int row, int dim, int d0, float total, const float (&v)[kN]) {
+    const float inv = total == 0.0f ? 0.0f : a.value_scale / total;
+    uint16_t* op = a.out + (size_t)(t.start + row / a.group) * a.out_stride + (size_t)(kvh * a.group + row % a.group) * dim + d0;
+    uint32_t w[kN / 2];
+#pragma unroll
+    for (int j = 0; j < kN / 2; ++j) w[j] = (uint32_t)f2h(v[2 * j] * inv) | ((uint32_t)f2h(v[2 * j + 1] * inv) << 16);
+    if constexpr (kN == 8) *(uint4*)op = uint4{w[0], w[1], w[2], w[3]};
+    else *(uint2*)op = uint2{w[0], w[1]};
+}
+
+// Short contexts: one workgroup for the keys of a (sequence, kv head, 16 rows).
+template <int kD, bool kF8> __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs a) {
+    __shared__ Parts<kD> parts;
+    const int kvh = blockIdx.x, seq = blockIdx.z, row0 = blockIdx.y * 16;
+    const RowTile t = wave_sequence(a, seq);
+    if (row0 >= t.rows) return;
+    RowPass<kD, kF8> pass(a, kvh);
+    pass.start(seq, t, row0);
+    pass.run((pass.tile_lo & ~(pass.kKeys - 1)) + wave_index() * pass.kKeys, pass.tile_hi);
+    to_lds<kD, kF8>(pass, parts);
+    __syncthreads();
+    const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (kD / 16);
+    if (r > pass.last) return;
+    float best, total, v[kD / 16];
+    join<kD>(parts, r, d0, best, total, v);
+    store_row<kD / 16>(a, t, kvh, row0 + r, kD, d0, total, v);
+}
+
+// ---- long contexts: the work of all sequences in equal shares --------------------------
+//
+// An item is a (sequence, kv head, 16 rows); its keys are a run of blocks of kSpan keys,
+// and the items' blocks in a row are dealt to kShares workgroups in equal contiguous
+// shares, so that one long sequence among short ones, or a single one, keeps the whole
+// GPU busy.  A share boundary inside an item leaves it in parts: at most two a workgroup
+// (the item its share begins in and the one it ends in), which a second launch joins.
+constexpr int kShares = 512;  // two workgroups on each of 256 CUs
+constexpr int kLeastShare = 2;
+
+template <int kD> struct Part {
+    float acc[16][kD];
+    float top[16], total[16];
+};
+struct Join {  // for the workgroup in whose share a divided item begins
+    int seq, item, count, first_slot;
+};
+
+__device__ __forceinline__ long long uniform(long long v) {
+    return (long long)((unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+// Blocks of one item of a sequence (0: the sequence has no rows) and its first block.
+template <int kSpan> __device__ __forceinline__ int item_blocks(const PagedArgs& a, const RowTile& t, int& first) {
+    first = 0;
+    if (t.rows == 0) return 0;
+    int lo, hi, none;
+    window(a, t.first_pos, t.length, lo, none);
+    window(a, t.first_pos + (t.rows - 1) / a.group, t.length, none, hi);
+    first = lo / kSpan;
+    const int blocks = (hi + kSpan - 1) / kSpan - first;
+    return blocks > 0 ? blocks : 1;  // rows that see nothing are still written
+}
+__device__ __forceinline__ int items_of(const PagedArgs& a, const RowTile& t) { return ((t.rows + 15) >> 4) * a.kv_heads; }
+
+template <int kD, bool kF8> __global__ __launch_bounds__(256, 2) void paged_attention_shares_kernel(PagedArgs a, Part<kD>* slots, Join* joins) {
+    constexpr int kSpan = RowPass<kD, kF8>::kSpan;
+    __shared__ Parts<kD> parts;
+    __shared__ long long wave_total[4], found_offset;
+    __shared__ int found_seq;
+    // where the shares lie: every workgroup sums the blocks of all sequences
+    const int per = (a.sequences + 255) / 256, s0 = threadIdx.x * per;
+    long long mine = 0;
+    for (int s = s0; s < s0 + per && s < a.sequences; ++s) {
+        const RowTile t = sequence_of(a, s);
+        int first;
+        mine += (long long)item_blocks<kSpan>(a, t, first) * items_of(a, t);
+    }
+    long long end = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const long long up = __shfl_up(end, off, 64);
+        if ((threadIdx.x & 63) >= off) end += up;
+    }
+    if ((threadIdx.x & 63) == 63) wave_total[threadIdx.x >> 6] = end;
+    __syncthreads();
+    for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) end += wave_total[w];
+    const long long all = uniform((wave_total[0] + wave_total[1]) + (wave_total[2] + wave_total[3]));
+    long long share = (all + kShares - 1) / kShares;
+    if (share < kLeastShare) share = kLeastShare;
+    const long long from = blockIdx.x * share, to = from + share < all ? from + share : all;
+    if (threadIdx.x == 0) joins[blockIdx.x].count = 0;
+    if (from >= all) return;
+    if (end - mine <= from && from < end) {
+        long long at = end - mine;
+        for (int s = s0;; ++s) {
+            const RowTile t = sequence_of(a, s);
+            int first;
+            const long long n = (long long)item_blocks<kSpan>(a, t, first) * items_of(a, t);
+            if (from < at + n) {
+                found_seq = s;
+                found_offset = from - at;
+                break;
+            }
+            at += n;
+        }
+    }
+    __syncthreads();
+
+    int seq = __builtin_amdgcn_readfirstlane(found_seq);
+    long long at = from, offset = uniform(found_offset);  // offset: blocks of `seq` before `at`
+    const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (kD / 16);
+    while (at < to) {
+        const RowTile t = wave_sequence(a, seq);
+        int first;
+        const int blocks = item_blocks<kSpan>(a, t, first), items = items_of(a, t);
+        for (int item = blocks ? (int)(offset / blocks) : 0; blocks && item < items && at < to; ++item) {
+            const int b0 = (int)(offset - (long long)item * blocks);
+            const int n = to - at < blocks - b0 ? (int)(to - at) : blocks - b0;
+            const int kvh = item % a.kv_heads, row0 = item / a.kv_heads * 16;
+            RowPass<kD, kF8> pass(a, kvh);
+            pass.start(seq, t, row0);
+            pass.run((first + b0) * kSpan + wave_index() * pass.kKeys, (first + b0 + n) * kSpan);
+            __syncthreads();  // the previous item's parts are read
+            to_lds<kD, kF8>(pass, parts);
+            __syncthreads();
+            float best, total, v[kD / 16];
+            join<kD>(parts, r, d0, best, total, v);
+            if (n == blocks) {
+                if (r <= pass.last) store_row<kD / 16>(a, t, kvh, row0 + r, kD, d0, total, v);
+            } else {
+                Part<kD>& slot = slots[2 * blockIdx.x + (at == from ? 0 : 1)];
+#pragma unroll
+                for (int j = 0; j < kD / 16; j += 4) *(v4f*)&slot.acc[r][d0 + j] = v4f{v[j], v[j + 1], v[j + 2], v[j + 3]};
+                if (d0 == 0) {
+                    slot.top[r] = best;
+                    slot.total[r] = total;
+                }
+                if (b0 == 0 && threadIdx.x == 0) {
+                    const long long item_end = at + blocks;
+                    joins[blockIdx.x] = {seq, item, (int)((item_end - 1) / share - blockIdx.x) + 1, at == from ? 0 : 1};
+                }
+            }
+            at += n;
+            offset += n;
+        }
+        ++seq;
+        offset = 0;
+    }
+}
+
+// The parts of a divided item: the slot its first workgroup ended in, and the first slot
+// of each of the following workgroups.  A workgroup joins one row; kJoinGroups groups of
+// lanes take every kJoinGroups-th part each, because a single long sequence is divided
+// into as many parts as there are shares (grouped: 9 us for 469 parts; a thread that
+// takes all parts of its features in turn: 130 us).
+constexpr int kJoinGroups = 16;
+
+template <int kD> __global__ __launch_bounds__(kJoinGroups * kD / 4) void paged_attention_join_kernel(PagedArgs a, const Part<kD>* slots, const Join* joins) {
+    constexpr int kLanes = kD / 4;  // 4 features each
+    __shared__ float part_acc[kJoinGroups][kD], part_top[kJoinGroups], part_total[kJoinGroups];
+    const Join job = joins[blockIdx.x];
+    const int r = blockIdx.y;
+    if (job.count == 0) return;
+    const RowTile t = sequence_of(a, job.seq);
+    const int kvh = job.item % a.kv_heads, row0 = job.item / a.kv_heads * 16;
+    if (row0 + r >= t.rows) return;
+    const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    const Part<kD>* first = slots + 2 * blockIdx.x;
+    float top = kNegInf, total = 0.0f;
+    v4f v{};
+#pragma unroll 4
+    for (int i = group; i < job.count; i += kJoinGroups) {
+        const Part<kD>& slot = first[2 * i + (i == 0 ? job.first_slot : 0)];
+        const float new_top = __builtin_fmaxf(top, slot.top[r]);
+        const float base = new_top == kNegInf ? 0.0f : new_top;
+        const float f = __builtin_amdgcn_exp2f(slot.top[r] - base), keep = __builtin_amdgcn_exp2f(top - base);
+        total = total * keep + slot.total[r] * f;
+        v = v * keep + *(const v4f*)&slot.acc[r][4 * lane] * f;
+        top = new_top;
+    }
+    *(v4f*)&part_acc[group][4 * lane] = v;
+    if (lane == 0) {
+        part_top[group] = top;
+        part_total[group] = total;
+    }
+    __syncthreads();
+    if (group != 0) return;
+    float best = kNegInf;
+#pragma unroll
+    for (int w = 0; w < kJoinGroups; ++w) best = __builtin_fmaxf(best, part_top[w]);
+    const float base = best == kNegInf ? 0.0f : best;
+    total = 0.0f;
+    v = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kJoinGroups; ++w) {
+        const float f = __builtin_amdgcn_exp2f(part_top[w] - base);
+        total += part_total[w] * f;
+        v = v + *(const v4f*)&part_acc[w][4 * lane] * f;
+    }
+    const float o[4] = {v[0], v[1], v[2], v[3]};
+    store_row<4>(a, t, kvh, row0 + r, kD, 4 * lane, total, o);
+}
+
+// Whether one workgroup an item does: at most kDirectKeys keys each, by the table's width.
+constexpr int kDirectKeys = 512;
+
+size_t paged_attention_workspace(int head_dim, int page_shift, int max_pages) {
+    if ((long long)max_pages << page_shift <= kDirectKeys) return 0;
+    return 2 * kShares * (head_dim == 128 ? sizeof(Part<128>) : sizeof(Part<64>)) + kShares * sizeof(Join);
+}
+
+template <int kD, bool kF8> static void launch_rows(const PagedArgs& a, int max_queries, void* workspace, hipStream_t s) {
+    if ((long long)a.max_pages << a.shift <= kDirectKeys) {
+        const dim3 grid((unsigned)a.kv_heads, (unsigned)((max_queries * a.group + 15) / 16), (unsigned)a.sequences);
+        paged_attention_rows_kernel<kD, kF8><<<grid, 256, 0, s>>>(a);
+        return;
+    }
+    Part<kD>* slots = (Part<kD>*)workspace;
+    Join* joins = (Join*)(slots + 2 * kShares);
+    paged_attention_shares_kernel<kD, kF8><<<kShares, 256, 0, s>>>(a, slots, joins);
+    const int rows = max_queries * a.group < 16 ? max_queries * a.group : 16;
+    paged_attention_join_kernel<kD><<<dim3(kShares, (unsigned)rows), kJoinGroups * kD / 4, 0, s>>>(a, slots, joins);
+}
+
+void launch_paged_attention(int kind, const PagedArgs& a, int head_dim, int max_queries, void* workspace, hipStream_t s) {
     if (head_dim == 128) {
-        if (kind == 1) paged_attention_kernel<128, true><<<grid, 256, 0, s>>>(a);
-        else paged_attention_kernel<128, false><<<grid, 256, 0, s>>>(a);
+        if (kind == 1) launch_rows<128, true>(a, max_queries, workspace, s);
+        else launch_rows<128, false>(a, max_queries, workspace, s);
     } else {
-        if (kind == 1) paged_attention_kernel<64, true><<<grid, 256, 0, s>>>(a);
-        else paged_attention_kernel<64, false><<<grid, 256, 0, s>>>(a);
+        if (kind == 1) launch_rows<64, true>(a, max_queries, workspace, s);
+        else launch_rows<64, false>(a, max_queries, workspace, s);
     }
 }
 

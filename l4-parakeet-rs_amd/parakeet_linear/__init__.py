@@ -406,63 +406,101 @@ def launch_decode(encoder_projection, frames, lstm, projection, joint, tokens, r
 
 
 # ---- a decoder layer's serving step (no reference counterpart) -----------------------
+#
+# These calls take their sizes from the tensors, so they check what they are given: a
+# single token's step is a few microseconds of GPU time, so the checks are one plain
+# condition each, and only a call that fails it is looked at again to say why.
 
 NORM_FP8, NORM_INT8 = 0, 1
 CACHE_FP16, CACHE_FP8 = 0, 1
 
+_torch = None
 
-def _check(what, *tensors):
-    """(name, tensor, dtypes, shape) each: the types and shapes that a call takes its sizes from, and the
-    current device, whose stream the call goes to."""
+
+def _types():
+    global _torch
     import torch
 
-    device = torch.cuda.current_device()
-    for name, t, dtypes, shape in tensors:
+    _torch = torch
+    return torch
+
+
+def _device_and_stream(stream):
+    """The current device, and the stream a call goes to."""
+    torch = _torch
+    if not torch.cuda.is_initialized():
+        torch.cuda.init()
+    device = torch._C._cuda_getDevice()
+    if stream is None:
+        return device, torch._C._cuda_getCurrentRawStream(device)
+    return device, stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _refuse(what, device, *tensors):
+    """Raises for the first of (name, tensor, dtypes, shape or None, dense) that is not as asked."""
+    for name, t, dtypes, shape, dense in tensors:
         if t is None:
             continue
         if t.dtype not in dtypes:
             raise ValueError(f"{what}: {name} is {t.dtype}, expected {' or '.join(map(str, dtypes))}")
-        if t.device.type != "cuda" or t.device.index != device:
+        if t.get_device() != device:
             raise ValueError(f"{what}: {name} is on {t.device}, not on the current device cuda:{device}")
-        if shape is not None and tuple(t.shape) != shape:
+        if shape is not None and t.shape != shape:
             raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
-
-
-def _dense(what, *tensors):
-    for name, t in tensors:
-        if t is not None and not t.is_contiguous():
+        if dense and not t.is_contiguous():
             raise ValueError(f"{what}: {name} must be contiguous")
+    raise ValueError(f"{what}: the tensors do not fit together")
+
+
+def _done(name, status):
+    if status < 0:
+        raise PkError(f"{name}: status {status}: {last_error()}")
 
 
 def rms_norm_quantize(kind, input, residual, weight, residual_out, output, scales, epsilon, stream=None):
     """h = input + residual (residual None: input), residual_out = fp16(h) (None: not kept), output = the 8-bit rows
     of h's root-mean-square norm times weight with their scales: e4m3 bytes (kind NORM_FP8) or int8 (NORM_INT8), as
     the dynamic linears and gemv_int4g128_a8 read them."""
-    import torch
-
-    rows, width = input.shape
-    f16 = (torch.float16,)
-    _check("rms_norm_quantize", ("input", input, f16, None), ("residual", residual, f16, (rows, width)), ("weight", weight, f16, (width,)),
-           ("residual_out", residual_out, f16, (rows, width)), ("scales", scales, (torch.float32,), (rows,)),
-           ("output", output, (torch.int8,) if kind == NORM_INT8 else (torch.uint8, torch.float8_e4m3fn), (rows, width)))
-    _dense("rms_norm_quantize", ("input", input), ("residual", residual), ("weight", weight), ("residual_out", residual_out), ("output", output),
-           ("scales", scales))
-    call("pk_rms_norm_quantize", kind, input, residual, weight, residual_out, output, scales, rows, width, epsilon, stream=stream)
+    torch = _torch or _types()
+    device, stream = _device_and_stream(stream)
+    f16, shape = torch.float16, input.shape
+    rows, width = shape
+    codes = (torch.int8,) if kind == NORM_INT8 else (torch.uint8, torch.float8_e4m3fn)
+    if not (input.dtype is f16 and weight.dtype is f16 and output.dtype in codes and scales.dtype is torch.float32 and output.shape == shape
+            and weight.shape == (width,) and scales.shape == (rows,) and input.is_contiguous() and weight.is_contiguous() and output.is_contiguous()
+            and scales.is_contiguous() and input.get_device() == weight.get_device() == output.get_device() == scales.get_device() == device
+            and all(t is None or (t.dtype is f16 and t.shape == shape and t.is_contiguous() and t.get_device() == device)
+                    for t in (residual, residual_out))):
+        _refuse("rms_norm_quantize", device, ("input", input, (f16,), None, True), ("residual", residual, (f16,), (rows, width), True),
+                ("weight", weight, (f16,), (width,), True), ("residual_out", residual_out, (f16,), (rows, width), True),
+                ("output", output, codes, (rows, width), True), ("scales", scales, (torch.float32,), (rows,), True))
+    _done("pk_rms_norm_quantize", lib.pk_rms_norm_quantize(
+        kind, input.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(),
+        None if residual_out is None else residual_out.data_ptr(), output.data_ptr(), scales.data_ptr(), rows, width, epsilon, stream))
 
 
 def _gemv(name, input, input_scales, weight_q, weight_scales, weight_zeros, bias, output, stream):
-    import torch
-
+    torch = _torch or _types()
+    device, stream = _device_and_stream(stream)
     (m, k), n = input.shape, weight_q.shape[0]
-    f16 = (torch.float16,)
-    _check(name, ("input", input, f16 if input_scales is None else (torch.int8,), None), ("input_scales", input_scales, (torch.float32,), (m,)),
-           ("weight_q", weight_q, (torch.int32, torch.uint32), (n, k // 8)), ("weight_scales", weight_scales, f16, (n, k // 128)),
-           ("weight_zeros", weight_zeros, f16, (n, k // 128)), ("bias", bias, (torch.float32,), (n,)),
-           ("output", output, (torch.float16, torch.float32), (m, n)))
-    _dense(name, ("input", input), ("input_scales", input_scales), ("weight_q", weight_q), ("weight_scales", weight_scales),
-           ("weight_zeros", weight_zeros), ("bias", bias), ("output", output))
-    rows = (input,) if input_scales is None else (input, input_scales)
-    call("pk_" + name, *rows, weight_q, weight_scales, weight_zeros, bias, output, int(output.dtype == torch.float32), m, n, k, stream=stream)
+    f16, f32, groups = torch.float16, torch.float32, (n, k // 128)
+    row_type, words, outs = f16 if input_scales is None else torch.int8, (torch.int32, torch.uint32), (f16, f32)
+    if not (input.dtype is row_type and weight_q.dtype in words and weight_scales.dtype is f16 and weight_zeros.dtype is f16 and output.dtype in outs
+            and weight_q.shape == (n, k // 8) and weight_scales.shape == groups and weight_zeros.shape == groups and output.shape == (m, n)
+            and input.is_contiguous() and weight_q.is_contiguous() and weight_scales.is_contiguous() and weight_zeros.is_contiguous()
+            and output.is_contiguous()
+            and input.get_device() == weight_q.get_device() == weight_scales.get_device() == weight_zeros.get_device() == output.get_device() == device
+            and all(t is None or (t.dtype is f32 and t.shape == (size,) and t.is_contiguous() and t.get_device() == device)
+                    for t, size in ((bias, n), (input_scales, m)))):
+        _refuse(name, device, ("input", input, (row_type,), None, True), ("input_scales", input_scales, (f32,), (m,), True),
+                ("weight_q", weight_q, words, (n, k // 8), True), ("weight_scales", weight_scales, (f16,), groups, True),
+                ("weight_zeros", weight_zeros, (f16,), groups, True), ("bias", bias, (f32,), (n,), True), ("output", output, outs, (m, n), True))
+    rest = (weight_q.data_ptr(), weight_scales.data_ptr(), weight_zeros.data_ptr(), None if bias is None else bias.data_ptr(), output.data_ptr(),
+            output.dtype is f32, m, n, k, stream)
+    if input_scales is None:
+        _done("pk_gemv_int4g128", lib.pk_gemv_int4g128(input.data_ptr(), *rest))
+    else:
+        _done("pk_gemv_int4g128_a8", lib.pk_gemv_int4g128_a8(input.data_ptr(), input_scales.data_ptr(), *rest))
 
 
 def gemv_int4g128(input, weight_q, weight_scales, weight_zeros, bias, output, stream=None):
@@ -479,61 +517,66 @@ def gemv_int4g128_a8(input, input_scales, weight_q, weight_scales, weight_zeros,
 
 def page_plan(held, added, free_pages, free_range, block_table, query_starts, key_lengths, slots, positions, info, page_size, stream=None):
     """Pages, block tables and slots of one step from the requests' lengths, all int32 on the GPU; see pk_page_plan in
-    include/pk_linear.h.  The sizes are the tensors': requests = len(held), token capacity = len(slots)."""
-    import torch
-
+    include/pk_linear.h.  The sizes are the tensors': requests = len(held), token capacity = len(slots); positions may
+    be None."""
+    torch = _torch or _types()
+    device, stream = _device_and_stream(stream)
+    i32 = torch.int32
     requests, max_pages = block_table.shape
-    i32 = (torch.int32,)
-    capacity = slots.shape[0]
-    arrays = (("held", held, i32, (requests,)), ("added", added, i32, (requests,)), ("free_pages", free_pages, i32, (free_pages.numel(),)),
-              ("free_range", free_range, i32, (2,)), ("block_table", block_table, i32, None), ("query_starts", query_starts, i32, (requests + 1,)),
-              ("key_lengths", key_lengths, i32, (requests,)), ("slots", slots, i32, (capacity,)), ("positions", positions, i32, (capacity,)),
-              ("info", info, i32, (4,)))
-    _check("page_plan", *arrays)
-    _dense("page_plan", *(a[:2] for a in arrays))
-    call("pk_page_plan", held, added, free_pages, free_range, free_pages.numel(), block_table, query_starts, key_lengths, slots, positions, info,
-         requests, max_pages, page_size, capacity, stream=stream)
-
-
-def _cache_of(what, key_cache, value_cache):
-    """(kind, pages, kv heads, page size, head dim) of a layer's cache."""
-    import torch
-
-    pages, kv_heads, page_size, head_dim = key_cache.shape
-    types = (torch.float16, torch.uint8, torch.float8_e4m3fn)
-    _check(what, ("key_cache", key_cache, types, None), ("value_cache", value_cache, (key_cache.dtype,), (pages, kv_heads, head_dim, page_size)))
-    _dense(what, ("key_cache", key_cache), ("value_cache", value_cache))
-    return CACHE_FP16 if key_cache.dtype == torch.float16 else CACHE_FP8, pages, kv_heads, page_size, head_dim
+    capacity, one = slots.numel(), (requests,)
+    arrays = (held, added, free_pages, free_range, block_table, query_starts, key_lengths, slots, info)
+    if not (all(t.dtype is i32 and t.get_device() == device and t.is_contiguous() for t in arrays) and held.shape == one and added.shape == one
+            and key_lengths.shape == one and query_starts.shape == (requests + 1,) and free_range.shape == (2,) and info.shape == (4,)
+            and free_pages.dim() == slots.dim() == 1
+            and (positions is None or (positions.dtype is i32 and positions.shape == slots.shape and positions.get_device() == device
+                                       and positions.is_contiguous()))):
+        i32 = (i32,)
+        _refuse("page_plan", device, ("held", held, i32, one, True), ("added", added, i32, one, True),
+                ("free_pages", free_pages, i32, (free_pages.numel(),), True), ("free_range", free_range, i32, (2,), True),
+                ("block_table", block_table, i32, None, True), ("query_starts", query_starts, i32, (requests + 1,), True),
+                ("key_lengths", key_lengths, i32, one, True), ("slots", slots, i32, (capacity,), True),
+                ("positions", positions, i32, (capacity,), True), ("info", info, i32, (4,), True))
+    _done("pk_page_plan", lib.pk_page_plan(
+        held.data_ptr(), added.data_ptr(), free_pages.data_ptr(), free_range.data_ptr(), free_pages.numel(), block_table.data_ptr(),
+        query_starts.data_ptr(), key_lengths.data_ptr(), slots.data_ptr(), None if positions is None else positions.data_ptr(), info.data_ptr(),
+        requests, max_pages, page_size, capacity, stream))
 
 
 def _row_stride(what, name, t):
-    """Elements between tokens of a [tokens x heads x head_dim] tensor whose heads lie next to each other."""
+    """Elements between the tokens of a [tokens x heads x head_dim] tensor whose heads lie next to each other."""
     tokens, heads, head_dim = t.shape
-    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != head_dim):
+    step, head, one = t.stride()
+    if one != 1 or (heads > 1 and head != head_dim):
         raise ValueError(f"{what}: {name} must hold each token's heads contiguously")
-    return t.stride(0) if tokens > 1 else max(t.stride(0), heads * head_dim)
+    return step if tokens > 1 else max(step, heads * head_dim)
 
 
 def paged_cache_write(key, value, slots, key_cache, value_cache, key_inverse_scale=1.0, value_inverse_scale=1.0, stream=None):
     """New keys and values [tokens x kv_heads x head_dim] (fp16, a stride between tokens) into their slots (-1: none) of a
     cache [pages x kv_heads x page_size x head_dim] / [pages x kv_heads x head_dim x page_size]: fp16, or e4m3 bytes of
     x * inverse_scale."""
-    import torch
-
-    kind, pages, kv_heads, page_size, head_dim = _cache_of("paged_cache_write", key_cache, value_cache)
-    tokens = slots.shape[0]
-    _check("paged_cache_write", ("key", key, (torch.float16,), (tokens, kv_heads, head_dim)),
-           ("value", value, (torch.float16,), (tokens, kv_heads, head_dim)), ("slots", slots, (torch.int32,), (tokens,)))
-    _dense("paged_cache_write", ("slots", slots))
-    call("pk_paged_cache_write", kind, key, _row_stride("paged_cache_write", "key", key), value, _row_stride("paged_cache_write", "value", value),
-         slots, key_cache, value_cache, tokens, kv_heads, head_dim, page_size, pages, key_inverse_scale, value_inverse_scale, stream=stream)
+    torch = _torch or _types()
+    device, stream = _device_and_stream(stream)
+    pages, kv_heads, page_size, head_dim = key_cache.shape
+    f16, kind, kinds = torch.float16, key_cache.dtype, (torch.float16, torch.uint8, torch.float8_e4m3fn)
+    tokens = slots.numel()
+    new, transposed = (tokens, kv_heads, head_dim), (pages, kv_heads, head_dim, page_size)
+    if not (kind in kinds and value_cache.dtype is kind and key.dtype is f16 and value.dtype is f16 and slots.dtype is torch.int32
+            and value_cache.shape == transposed and key.shape == new and value.shape == new and slots.dim() == 1 and key_cache.is_contiguous()
+            and value_cache.is_contiguous() and slots.is_contiguous()
+            and key_cache.get_device() == value_cache.get_device() == key.get_device() == value.get_device() == slots.get_device() == device):
+        _refuse("paged_cache_write", device, ("key_cache", key_cache, kinds, None, True), ("value_cache", value_cache, (kind,), transposed, True),
+                ("key", key, (f16,), new, False), ("value", value, (f16,), new, False), ("slots", slots, (torch.int32,), (tokens,), True))
+    _done("pk_paged_cache_write", lib.pk_paged_cache_write(
+        CACHE_FP16 if kind is f16 else CACHE_FP8, key.data_ptr(), _row_stride("paged_cache_write", "key", key), value.data_ptr(),
+        _row_stride("paged_cache_write", "value", value), slots.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), tokens, kv_heads, head_dim,
+        page_size, pages, key_inverse_scale, value_inverse_scale, stream))
 
 
 def paged_attention_workspace_bytes(tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, max_pages):
     """Bytes of workspace that paged_attention needs for these sizes (host only)."""
     size = lib.pk_paged_attention_workspace_bytes(tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, max_pages)
-    if size < 0:
-        raise PkError(f"pk_paged_attention_workspace_bytes: status {size}: {last_error()}")
+    _done("pk_paged_attention_workspace_bytes", size)
     return size
 
 
@@ -541,18 +584,29 @@ def paged_attention(query, key_cache, value_cache, block_table, query_starts, ke
                     scale=None, key_scale=1.0, value_scale=1.0, stream=None):
     """Attention of new tokens [tokens x heads x head_dim] over the paged cache; see pk_paged_attention in
     include/pk_linear.h.  scale None: 1 / sqrt(head_dim); workspace: a uint8 tensor of paged_attention_workspace_bytes,
-    used by one call at a time."""
-    import torch
-
-    kind, pages, kv_heads, page_size, head_dim = _cache_of("paged_attention", key_cache, value_cache)
-    tokens, heads = query.shape[:2]
+    used by one call at a time (None where that is 0)."""
+    torch = _torch or _types()
+    device, stream = _device_and_stream(stream)
+    pages, kv_heads, page_size, head_dim = key_cache.shape
+    rows = query.shape
+    tokens, heads, _ = rows
     sequences, max_pages = block_table.shape
-    i32 = (torch.int32,)
-    _check("paged_attention", ("query", query, (torch.float16,), (tokens, heads, head_dim)), ("output", output, (torch.float16,), (tokens, heads, head_dim)),
-           ("block_table", block_table, i32, None), ("query_starts", query_starts, i32, (sequences + 1,)), ("key_lengths", key_lengths, i32, (sequences,)),
-           ("workspace", workspace, (torch.uint8,), None))
-    _dense("paged_attention", ("block_table", block_table), ("query_starts", query_starts), ("key_lengths", key_lengths), ("workspace", workspace))
-    call("pk_paged_attention", kind, query, _row_stride("paged_attention", "query", query), key_cache, value_cache, block_table, query_starts, key_lengths,
-         output, _row_stride("paged_attention", "output", output), tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, pages, max_pages,
-         left, right, head_dim**-0.5 if scale is None else scale, key_scale, value_scale, workspace,
-         0 if workspace is None else workspace.numel(), stream=stream)
+    f16, i32, kind, kinds = torch.float16, torch.int32, key_cache.dtype, (torch.float16, torch.uint8, torch.float8_e4m3fn)
+    transposed = (pages, kv_heads, head_dim, page_size)
+    if not (kind in kinds and value_cache.dtype is kind and query.dtype is f16 and output.dtype is f16 and value_cache.shape == transposed
+            and rows[2] == head_dim and output.shape == rows and query_starts.shape == (sequences + 1,) and key_lengths.shape == (sequences,)
+            and key_cache.is_contiguous() and value_cache.is_contiguous()
+            and key_cache.get_device() == value_cache.get_device() == query.get_device() == output.get_device() == device
+            and all(t.dtype is i32 and t.is_contiguous() and t.get_device() == device for t in (block_table, query_starts, key_lengths))
+            and (workspace is None or (workspace.dtype is torch.uint8 and workspace.is_contiguous() and workspace.get_device() == device))):
+        i32 = (i32,)
+        _refuse("paged_attention", device, ("key_cache", key_cache, kinds, None, True), ("value_cache", value_cache, (kind,), transposed, True),
+                ("query", query, (f16,), (tokens, heads, head_dim), False), ("output", output, (f16,), (tokens, heads, head_dim), False),
+                ("block_table", block_table, i32, None, True), ("query_starts", query_starts, i32, (sequences + 1,), True),
+                ("key_lengths", key_lengths, i32, (sequences,), True), ("workspace", workspace, (torch.uint8,), None, True))
+    _done("pk_paged_attention", lib.pk_paged_attention(
+        CACHE_FP16 if kind is f16 else CACHE_FP8, query.data_ptr(), _row_stride("paged_attention", "query", query), key_cache.data_ptr(),
+        value_cache.data_ptr(), block_table.data_ptr(), query_starts.data_ptr(), key_lengths.data_ptr(), output.data_ptr(),
+        _row_stride("paged_attention", "output", output), tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, pages, max_pages, left,
+        right, head_dim**-0.5 if scale is None else scale, key_scale, value_scale, None if workspace is None else workspace.data_ptr(),
+        0 if workspace is None else workspace.numel(), stream))

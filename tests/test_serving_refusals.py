@@ -89,7 +89,7 @@ def test_write(want, kw):
 
 @pytest.mark.parametrize("want,kw", [
     (ARG, {"kind": 3}), (SHAPE, {"page_size": 20}), (SHAPE, {"head_dim": 80}), (SHAPE, {"heads": 12}), (SHAPE, {"heads": 0}), (SHAPE, {"heads": 2048}),
-    (SHAPE, {"kv_heads": 0}), (SHAPE, {"tokens": -1}), (SHAPE, {"tokens": (1 << 20) + 1}), (SHAPE, {"max_queries": 6}), (SHAPE, {"sequences": 65536}),
+    (SHAPE, {"kv_heads": 0}), (SHAPE, {"tokens": -1}), (SHAPE, {"tokens": (1 << 20) + 1}), (SHAPE, {"max_queries": 6}), (SHAPE, {"sequences": 4097}),
     (SHAPE, {"max_pages": 0}), (SHAPE, {"max_pages": (1 << 26) + 1}), (SHAPE, {"pages": 0}), (SHAPE, {"query_stride": 2040}),
     (SHAPE, {"output_stride": 0}), (ARG, {"query": None}), (ARG, {"key_cache": None}), (ARG, {"value_cache": None}), (ARG, {"block_table": None}),
     (ARG, {"query_starts": None}), (ARG, {"key_lengths": None}), (ARG, {"output": None}), (ALIGN, {"query": P + 8}), (ALIGN, {"query_stride": 2052}),
