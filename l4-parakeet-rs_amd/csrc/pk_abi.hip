@@ -1036,7 +1036,7 @@ int64_t pk_paged_attention_workspace_bytes(int32_t tokens, int32_t max_queries, 
                                            int32_t head_dim, int32_t page_size, int32_t max_pages) {
     const int32_t shift = paged_shape(tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, max_pages);
     if (shift < 0) return shift;
-    return (int64_t)paged_attention_workspace(head_dim, shift, max_pages);
+    return (int64_t)paged_attention_workspace(head_dim, shift, max_pages, max_queries * (heads / kv_heads));
 }
 
 int32_t pk_paged_attention(int32_t kind, const uint16_t* query, int64_t query_stride, const void* key_cache, const void* value_cache,

@@ -101,7 +101,7 @@ struct PagedArgs {
     int tokens, sequences, kv_heads, group, shift, pages, max_pages, left, right;
     float scale_log2, value_scale;
 };
-size_t paged_attention_workspace(int head_dim, int page_shift, int max_pages);
+size_t paged_attention_workspace(int head_dim, int page_shift, int max_pages, int max_rows);
 void launch_paged_attention(int kind, const PagedArgs& args, int head_dim, int max_queries, void* workspace, hipStream_t s);
 void set_error(const char* fmt, ...);
 int cu_count();

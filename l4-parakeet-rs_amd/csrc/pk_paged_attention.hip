@@ -12,111 +12,9 @@
 // of O^T = V^T P^T.  Probabilities therefore never leave their registers, and keys
 // and (transposed) values are loaded from the cache straight into operand layout, 16
 // bytes a lane.
-#include "pk_kernels.hpp"
+#include "pk_paged_attention.hpp"
 
 namespace pk {
-
-constexpr float kNegInf = -__builtin_inff();
-
-// Eight cache values of an operand -> fp16 (e4m3 values are exact in fp16).
-template <bool kF8> __device__ __forceinline__ v8h operand(const uint4& raw, int half) {
-    if constexpr (kF8) {
-        const uint32_t w[2] = {half ? raw.z : raw.x, half ? raw.w : raw.y};
-        v8h r;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const v2h a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], 1.0f, false);
-            const v2h b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], 1.0f, true);
-            r[4 * i] = a[0];
-            r[4 * i + 1] = a[1];
-            r[4 * i + 2] = b[0];
-            r[4 * i + 3] = b[1];
-        }
-        return r;
-    } else {
-        return __builtin_bit_cast(v8h, raw);
-    }
-}
-
-// Nonzero where 16 bytes of cache values hold an infinity or a NaN: all ones under the sign
-// (e4m3: exponent and mantissa, its only NaN; fp16: the exponent), so that adding one
-// there carries into the sign bit, and nowhere else.
-template <bool kF8> __device__ __forceinline__ uint32_t not_finite(const uint4& w) {
-    const uint32_t e = kF8 ? 0x7f7f7f7fu : 0x7c007c00u, one = kF8 ? 0x01010101u : 0x04000400u;
-    return (((w.x & e) + one) | ((w.y & e) + one) | ((w.z & e) + one) | ((w.w & e) + one)) & (kF8 ? 0x80808080u : 0x80008000u);
-}
-
-// Which values of a word are NaN (0), +inf (1) or -inf (2): the cache's 1.0 where so.
-template <bool kF8> __device__ __forceinline__ uint32_t odd_ones(uint32_t w, int which) {
-    if constexpr (kF8) {
-        return (((w & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 0x38u;
-    } else {
-        const uint32_t odd = (((w & 0x7c007c00u) + 0x04000400u) >> 15) & 0x00010001u;
-        const uint32_t nan = odd & (((w & 0x03ff03ffu) + 0x03ff03ffu) >> 10);
-        const uint32_t sign = (w >> 15) & 0x00010001u, inf = odd & ~nan;
-        return (which == 0 ? nan : (which == 1 ? inf & ~sign : inf & sign)) * 0x3c00u;
-    }
-}
-template <bool kF8> __device__ __forceinline__ uint32_t odd_cleared(uint32_t w) {
-    if constexpr (kF8) return w & ~((((w & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 0xffu);
-    else return w & ~(((((w & 0x7c007c00u) + 0x04000400u) >> 15) & 0x00010001u) * 0xffffu);
-}
-
-// Infinities and NaN in values, where a product with the zero of a masked key would
-// spoil rows that do not see that key: each kind is counted over the keys that a row
-// sees (bits of `seen`), added to the rows that see one, and cleared from the operand.
-// Rare; in place and one kind after the other, so that it needs few registers.
-template <bool kF8> __device__ __forceinline__ void add_not_finite(uint4& raw, uint32_t seen, v4f& o) {
-#pragma unroll
-    for (int kind = 0; kind < (kF8 ? 1 : 3); ++kind) {
-        const uint4 ones{odd_ones<kF8>(raw.x, kind), odd_ones<kF8>(raw.y, kind), odd_ones<kF8>(raw.z, kind), odd_ones<kF8>(raw.w, kind)};
-        v4f count{};
-#pragma unroll
-        for (int u = 0; u < (kF8 ? 2 : 1); ++u) {
-            uint32_t vis[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) vis[i] = ((seen >> (8 * u + 2 * i) & 1u) | (seen >> (8 * u + 2 * i + 1) & 1u) << 16) * 0x3c00u;
-            count = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand<kF8>(ones, u), __builtin_bit_cast(v8h, uint4{vis[0], vis[1], vis[2], vis[3]}), count,
-                                                           0, 0, 0);
-        }
-        const float add = kind == 0 ? __builtin_nanf("") : (kind == 1 ? __builtin_inff() : -__builtin_inff());
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (count[r] > 0.0f) o[r] += add;
-        __builtin_amdgcn_sched_barrier(0);
-    }
-    raw = uint4{odd_cleared<kF8>(raw.x), odd_cleared<kF8>(raw.y), odd_cleared<kF8>(raw.z), odd_cleared<kF8>(raw.w)};
-}
-
-// One sequence's view for a tile of 16 query rows.
-struct RowTile {
-    int start, rows, length, first_pos;  // first_pos: position of the sequence's first new token
-};
-
-__device__ __forceinline__ RowTile sequence_of(const PagedArgs& a, int seq) {
-    int s = a.starts[seq], e = a.starts[seq + 1], len = a.lengths[seq];
-    s = s < 0 ? 0 : (s > a.tokens ? a.tokens : s);
-    e = e < s ? s : (e > a.tokens ? a.tokens : e);
-    const int most = a.max_pages << a.shift;
-    len = len < 0 ? 0 : (len > most ? most : len);
-    return {s, (e - s) * a.group, len, len - (e - s)};
-}
-
-// The same for a sequence that the whole wave works on, in scalar registers.
-__device__ __forceinline__ RowTile wave_sequence(const PagedArgs& a, int seq) {
-    const RowTile t = sequence_of(a, seq);
-    return {__builtin_amdgcn_readfirstlane(t.start), __builtin_amdgcn_readfirstlane(t.rows), __builtin_amdgcn_readfirstlane(t.length),
-            __builtin_amdgcn_readfirstlane(t.first_pos)};
-}
-
-// Keys [lo, hi) that a query at `pos` sees.
-__device__ __forceinline__ void window(const PagedArgs& a, int pos, int length, int& lo, int& hi) {
-    lo = a.left < 0 || pos < a.left ? 0 : pos - a.left;
-    hi = a.right < 0 || length - pos <= a.right ? length : pos + a.right + 1;
-    if (hi < 0) hi = 0;
-}
-
-__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // One wave's pass over key tiles for 16 query rows.  Loads are issued a stage ahead: a
 // tile's values while its scores are computed, the next tile's keys before the softmax,
@@ -320,17 +218,6 @@ template <int kD> __device__ __forceinline__ void join(const Parts<kD>& parts, i
     }
 }
 
-template <int kN>
-__device__ __forceinline__ void store_row(const PagedArgs& a, const RowTile& t, int kvh, int row, int dim, int d0, float total, const float (&v)[kN]) {
-    const float inv = total == 0.0f ? 0.0f : a.value_scale / total;
-    uint16_t* op = a.out + (size_t)(t.start + row / a.group) * a.out_stride + (size_t)(kvh * a.group + row % a.group) * dim + d0;
-    uint32_t w[kN / 2];
-#pragma unroll
-    for (int j = 0; j < kN / 2; ++j) w[j] = (uint32_t)f2h(v[2 * j] * inv) | ((uint32_t)f2h(v[2 * j + 1] * inv) << 16);
-    if constexpr (kN == 8) *(uint4*)op = uint4{w[0], w[1], w[2], w[3]};
-    else *(uint2*)op = uint2{w[0], w[1]};
-}
-
 // Short contexts: one workgroup for the keys of a (sequence, kv head, 16 rows).
 template <int kD, bool kF8> __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs a) {
     __shared__ Parts<kD> parts;
@@ -359,18 +246,6 @@ template <int kD, bool kF8> __global__ __launch_bounds__(256, 2) void paged_atte
 constexpr int kShares = 512;  // two workgroups on each of 256 CUs
 constexpr int kLeastShare = 2;
 
-template <int kD> struct Part {
-    float acc[16][kD];
-    float top[16], total[16];
-};
-struct Join {  // for the workgroup in whose share a divided item begins
-    int seq, item, count, first_slot;
-};
-
-__device__ __forceinline__ long long uniform(long long v) {
-    return (long long)((unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
-}
-
 // Blocks of one item of a sequence (0: the sequence has no rows) and its first block.
 template <int kSpan> __device__ __forceinline__ int item_blocks(const PagedArgs& a, const RowTile& t, int& first) {
     first = 0;
@@ -384,60 +259,28 @@ template <int kSpan> __device__ __forceinline__ int item_blocks(const PagedArgs&
 }
 __device__ __forceinline__ int items_of(const PagedArgs& a, const RowTile& t) { return ((t.rows + 15) >> 4) * a.kv_heads; }
 
-template <int kD, bool kF8> __global__ __launch_bounds__(256, 2) void paged_attention_shares_kernel(PagedArgs a, Part<kD>* slots, Join* joins) {
+template <int kD, bool kF8>
+__global__ __launch_bounds__(256, 2) void paged_attention_shares_kernel(PagedArgs a, Part<kD, 16>* slots, Join* joins) {
     constexpr int kSpan = RowPass<kD, kF8>::kSpan;
     __shared__ Parts<kD> parts;
-    __shared__ long long wave_total[4], found_offset;
-    __shared__ int found_seq;
-    // where the shares lie: every workgroup sums the blocks of all sequences
-    const int per = (a.sequences + 255) / 256, s0 = threadIdx.x * per;
-    long long mine = 0;
-    for (int s = s0; s < s0 + per && s < a.sequences; ++s) {
-        const RowTile t = sequence_of(a, s);
-        int first;
-        mine += (long long)item_blocks<kSpan>(a, t, first) * items_of(a, t);
-    }
-    long long end = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const long long up = __shfl_up(end, off, 64);
-        if ((threadIdx.x & 63) >= off) end += up;
-    }
-    if ((threadIdx.x & 63) == 63) wave_total[threadIdx.x >> 6] = end;
-    __syncthreads();
-    for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) end += wave_total[w];
-    const long long all = uniform((wave_total[0] + wave_total[1]) + (wave_total[2] + wave_total[3]));
-    long long share = (all + kShares - 1) / kShares;
-    if (share < kLeastShare) share = kLeastShare;
-    const long long from = blockIdx.x * share, to = from + share < all ? from + share : all;
     if (threadIdx.x == 0) joins[blockIdx.x].count = 0;
-    if (from >= all) return;
-    if (end - mine <= from && from < end) {
-        long long at = end - mine;
-        for (int s = s0;; ++s) {
-            const RowTile t = sequence_of(a, s);
-            int first;
-            const long long n = (long long)item_blocks<kSpan>(a, t, first) * items_of(a, t);
-            if (from < at + n) {
-                found_seq = s;
-                found_offset = from - at;
-                break;
-            }
-            at += n;
-        }
-    }
-    __syncthreads();
+    Share share;
+    const auto blocks_of = [&](const RowTile& t) {
+        int first;
+        return (long long)item_blocks<kSpan>(a, t, first) * items_of(a, t);
+    };
+    if (!deal(a, kShares, kLeastShare, blockIdx.x, blocks_of, share)) return;
 
-    int seq = __builtin_amdgcn_readfirstlane(found_seq);
-    long long at = from, offset = uniform(found_offset);  // offset: blocks of `seq` before `at`
+    int seq = share.seq;
+    long long at = share.from, offset = share.offset;
     const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (kD / 16);
-    while (at < to) {
+    while (at < share.to) {
         const RowTile t = wave_sequence(a, seq);
         int first;
         const int blocks = item_blocks<kSpan>(a, t, first), items = items_of(a, t);
-        for (int item = blocks ? (int)(offset / blocks) : 0; blocks && item < items && at < to; ++item) {
+        for (int item = blocks ? (int)(offset / blocks) : 0; blocks && item < items && at < share.to; ++item) {
             const int b0 = (int)(offset - (long long)item * blocks);
-            const int n = to - at < blocks - b0 ? (int)(to - at) : blocks - b0;
+            const int n = share.to - at < blocks - b0 ? (int)(share.to - at) : blocks - b0;
             const int kvh = item % a.kv_heads, row0 = item / a.kv_heads * 16;
             RowPass<kD, kF8> pass(a, kvh);
             pass.start(seq, t, row0);
@@ -450,17 +293,15 @@ template <int kD, bool kF8> __global__ __launch_bounds__(256, 2) void paged_atte
             if (n == blocks) {
                 if (r <= pass.last) store_row<kD / 16>(a, t, kvh, row0 + r, kD, d0, total, v);
             } else {
-                Part<kD>& slot = slots[2 * blockIdx.x + (at == from ? 0 : 1)];
+                Part<kD, 16>& slot = slots[2 * blockIdx.x + (at == share.from ? 0 : 1)];
 #pragma unroll
                 for (int j = 0; j < kD / 16; j += 4) *(v4f*)&slot.acc[r][d0 + j] = v4f{v[j], v[j + 1], v[j + 2], v[j + 3]};
                 if (d0 == 0) {
                     slot.top[r] = best;
                     slot.total[r] = total;
                 }
-                if (b0 == 0 && threadIdx.x == 0) {
-                    const long long item_end = at + blocks;
-                    joins[blockIdx.x] = {seq, item, (int)((item_end - 1) / share - blockIdx.x) + 1, at == from ? 0 : 1};
-                }
+                if (b0 == 0 && threadIdx.x == 0)
+                    joins[blockIdx.x] = {t.start, t.rows, kvh, row0, (int)((at + blocks - 1) / share.size - blockIdx.x) + 1, at == share.from ? 0 : 1, {}};
             }
             at += n;
             offset += n;
@@ -477,22 +318,20 @@ template <int kD, bool kF8> __global__ __launch_bounds__(256, 2) void paged_atte
 // takes all parts of its features in turn: 130 us).
 constexpr int kJoinGroups = 16;
 
-template <int kD> __global__ __launch_bounds__(kJoinGroups * kD / 4) void paged_attention_join_kernel(PagedArgs a, const Part<kD>* slots, const Join* joins) {
+template <int kD> __global__ __launch_bounds__(kJoinGroups * kD / 4) void paged_attention_join_kernel(PagedArgs a, const Part<kD, 16>* slots, const Join* joins) {
     constexpr int kLanes = kD / 4;  // 4 features each
     __shared__ float part_acc[kJoinGroups][kD], part_top[kJoinGroups], part_total[kJoinGroups];
     const Join job = joins[blockIdx.x];
     const int r = blockIdx.y;
     if (job.count == 0) return;
-    const RowTile t = sequence_of(a, job.seq);
-    const int kvh = job.item % a.kv_heads, row0 = job.item / a.kv_heads * 16;
-    if (row0 + r >= t.rows) return;
+    if (job.row0 + r >= job.rows) return;
     const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-    const Part<kD>* first = slots + 2 * blockIdx.x;
+    const Part<kD, 16>* first = slots + 2 * blockIdx.x;
     float top = kNegInf, total = 0.0f;
     v4f v{};
 #pragma unroll 4
     for (int i = group; i < job.count; i += kJoinGroups) {
-        const Part<kD>& slot = first[2 * i + (i == 0 ? job.first_slot : 0)];
+        const Part<kD, 16>& slot = first[2 * i + (i == 0 ? job.first_slot : 0)];
         const float new_top = __builtin_fmaxf(top, slot.top[r]);
         const float base = new_top == kNegInf ? 0.0f : new_top;
         const float f = __builtin_amdgcn_exp2f(slot.top[r] - base), keep = __builtin_amdgcn_exp2f(top - base);
@@ -520,37 +359,46 @@ template <int kD> __global__ __launch_bounds__(kJoinGroups * kD / 4) void paged_
         v = v + *(const v4f*)&part_acc[w][4 * lane] * f;
     }
     const float o[4] = {v[0], v[1], v[2], v[3]};
-    store_row<4>(a, t, kvh, row0 + r, kD, 4 * lane, total, o);
+    store_row<4>(a, {job.start, job.rows, 0, 0}, job.kvh, job.row0 + r, kD, 4 * lane, total, o);
 }
 
 // Whether one workgroup an item does: at most kDirectKeys keys each, by the table's width.
 constexpr int kDirectKeys = 512;
 
-size_t paged_attention_workspace(int head_dim, int page_shift, int max_pages) {
+// From this many query rows a sequence on, chunks of 128 rows share their loads.
+constexpr int kChunksFrom = 17;
+
+size_t paged_attention_workspace(int head_dim, int page_shift, int max_pages, int max_rows) {
     if ((long long)max_pages << page_shift <= kDirectKeys) return 0;
-    return 2 * kShares * (head_dim == 128 ? sizeof(Part<128>) : sizeof(Part<64>)) + kShares * sizeof(Join);
+    if (max_rows >= kChunksFrom) return paged_chunks_workspace(head_dim);
+    return 2 * kShares * (head_dim == 128 ? sizeof(Part<128, 16>) : sizeof(Part<64, 16>)) + kShares * sizeof(Join);
 }
 
-template <int kD, bool kF8> static void launch_rows(const PagedArgs& a, int max_queries, void* workspace, hipStream_t s) {
-    if ((long long)a.max_pages << a.shift <= kDirectKeys) {
-        const dim3 grid((unsigned)a.kv_heads, (unsigned)((max_queries * a.group + 15) / 16), (unsigned)a.sequences);
+template <int kD, bool kF8> static void launch_rows(const PagedArgs& a, bool direct, int max_queries, void* workspace, hipStream_t s) {
+    const unsigned rows = (unsigned)(max_queries * a.group);
+    if (direct) {
+        const dim3 grid((unsigned)a.kv_heads, (rows + 15) / 16, (unsigned)a.sequences);
         paged_attention_rows_kernel<kD, kF8><<<grid, 256, 0, s>>>(a);
         return;
     }
-    Part<kD>* slots = (Part<kD>*)workspace;
+    auto* slots = (Part<kD, 16>*)workspace;
     Join* joins = (Join*)(slots + 2 * kShares);
     paged_attention_shares_kernel<kD, kF8><<<kShares, 256, 0, s>>>(a, slots, joins);
-    const int rows = max_queries * a.group < 16 ? max_queries * a.group : 16;
-    paged_attention_join_kernel<kD><<<dim3(kShares, (unsigned)rows), kJoinGroups * kD / 4, 0, s>>>(a, slots, joins);
+    paged_attention_join_kernel<kD><<<dim3(kShares, rows < 16 ? rows : 16), kJoinGroups * kD / 4, 0, s>>>(a, slots, joins);
 }
 
 void launch_paged_attention(int kind, const PagedArgs& a, int head_dim, int max_queries, void* workspace, hipStream_t s) {
+    const bool direct = (long long)a.max_pages << a.shift <= kDirectKeys;
+    if (max_queries * a.group >= kChunksFrom) {
+        launch_paged_chunks(kind, a, head_dim, direct, max_queries, workspace, s);
+        return;
+    }
     if (head_dim == 128) {
-        if (kind == 1) launch_rows<128, true>(a, max_queries, workspace, s);
-        else launch_rows<128, false>(a, max_queries, workspace, s);
+        if (kind == 1) launch_rows<128, true>(a, direct, max_queries, workspace, s);
+        else launch_rows<128, false>(a, direct, max_queries, workspace, s);
     } else {
-        if (kind == 1) launch_rows<64, true>(a, max_queries, workspace, s);
-        else launch_rows<64, false>(a, max_queries, workspace, s);
+        if (kind == 1) launch_rows<64, true>(a, direct, max_queries, workspace, s);
+        else launch_rows<64, false>(a, direct, max_queries, workspace, s);
     }
 }
 

@@ -1,0 +1,533 @@
+// The paged attention for chunks of new tokens: 128 query rows a workgroup, 32 a wave.
+//
+// The same two products as for few rows (S^T = K Q^T, O^T = V^T P^T, probabilities in
+// registers), on 32 x 32 x 16 MFMAs.  The four waves share 64-key tiles of keys and
+// values in LDS, which the loads fill directly while the previous tile is multiplied
+// (two buffers, one barrier a tile; two workgroups a CU, so that one's softmax runs
+// under the other's products).  Tile rows are whole key or value rows whose 16-byte chunks
+// are XOR-swizzled at the source, since such loads write LDS in lane order.
+//
+// Bound by the softmax's vector instructions next to the MFMAs: 32 scores a lane and
+// tile, each a maximum, a fused scale and subtraction, an exponential, a sum and half a
+// conversion; the running output is only rescaled on tiles that raise some row's maximum.
+#include "pk_paged_attention.hpp"
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+namespace pk {
+
+constexpr int kChunkRows = 128, kTileKeys = 64;
+constexpr int kChunkShares = 512;  // two workgroups on each of 256 CUs
+constexpr int kLeastChunkShare = 4;
+
+// Blocks (tiles of keys) that the rows of one row tile see, from block `first` on.
+__device__ __forceinline__ int chunk_blocks(const PagedArgs& a, const RowTile& t, int tile, int& first) {
+    const int r0 = tile * kChunkRows, r1 = r0 + kChunkRows < t.rows ? r0 + kChunkRows - 1 : t.rows - 1;
+    int lo, hi, none;
+    window(a, t.first_pos + r0 / a.group, t.length, lo, none);
+    window(a, t.first_pos + r1 / a.group, t.length, none, hi);
+    first = lo / kTileKeys;
+    const int n = (hi + kTileKeys - 1) / kTileKeys - first;
+    return n > 0 ? n : 1;
+}
+
+// With a causal mask the row tiles of a sequence differ in length; tile j and tile n - 1 -
+// j together hardly do (their blocks are concave in j), so they are dealt as one item of
+// `pair` blocks, the most any pair has; the middle tile of an odd number is an item by
+// itself.
+struct Pairs {
+    int tiles, pair, middle;
+    long long per_head;
+};
+__device__ __forceinline__ Pairs pairs_of(const PagedArgs& a, const RowTile& t) {
+    Pairs p{};
+    p.tiles = (t.rows + kChunkRows - 1) / kChunkRows;
+    if (p.tiles == 0) return p;
+    int first;
+    const int mid = chunk_blocks(a, t, p.tiles / 2, first);
+    if (p.tiles & 1) p.middle = mid;
+    if (p.tiles > 1) p.pair = mid + chunk_blocks(a, t, (p.tiles - 1) / 2, first) + 2;  // + 2: blocks are whole
+    p.per_head = (long long)(p.tiles / 2) * p.pair + p.middle;
+    return p;
+}
+
+template <int kD, bool kF8> struct ChunkPass {
+    static constexpr int kBytes = kF8 ? 1 : 2;
+    static constexpr int kSteps = kD / 16, kBlocks = kD / 32;          // MFMA steps of S over features, feature blocks of O
+    static constexpr int kKeyBytes = kD * kBytes, kValueBytes = kTileKeys * kBytes;  // tile rows
+    static constexpr int kKeyTile = kTileKeys * kKeyBytes, kValueTile = kD * kValueBytes;
+    static constexpr int kBuffer = kKeyTile + kValueTile;
+    static constexpr int kKeyChunks = kKeyBytes / 16, kValueChunks = kValueBytes / 16;
+    static constexpr uint32_t kAllPages = (1u << kValueChunks) - 1u;
+    static constexpr int kKeyLoads = kKeyTile / 4096, kValueLoads = kValueTile / 4096;  // 16 bytes a lane, of 4 waves
+
+    const PagedArgs& a;
+    uint8_t* lds;
+    const int lane, wave, l32, h, kvh;
+    RowTile t;
+    const int* table;
+    int last_page;
+    int row0, last, row;      // this wave's first row, its last row's index (< 0: none), this lane's row
+    int lo, hi, full_lo, full_hi, wave_lo, wave_hi;
+    int tile_full_lo, tile_full_hi;  // keys that all 128 rows see
+    float scale, sign;
+    v8h qf[kSteps];
+    v16f acc[kBlocks];
+    float top, total;         // in raw scores; total of this lane's keys
+
+    __device__ __forceinline__ ChunkPass(const PagedArgs& args, uint8_t* buffers, int kv_head)
+        : a(args), lds(buffers), lane(threadIdx.x & 63), wave(wave_index()), l32(lane & 31), h(lane >> 5), kvh(kv_head) {
+        // a negative scale turns the queries' signs, so that the largest score has the largest
+        // product; 0 becomes tiny, so that -inf stays -inf
+        sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
+        scale = __builtin_fmaxf(__builtin_fabsf(a.scale_log2), 1e-30f);
+    }
+
+    __device__ __forceinline__ void start(int seq, const RowTile& rows, int tile) {
+        t = rows;
+        table = a.table + (size_t)seq * a.max_pages;
+        last_page = t.length > 0 ? (t.length - 1) >> a.shift : 0;
+        row0 = tile * kChunkRows + wave * 32;
+        last = t.rows - row0 < 32 ? t.rows - row0 - 1 : 31;
+        const int at = row0 + (l32 < last ? l32 : last);
+        row = at < 0 ? 0 : (at < t.rows ? at : t.rows - 1);
+        const int tok = row / a.group, head = kvh * a.group + row % a.group;
+        window(a, t.first_pos + tok, t.length, lo, hi);
+        if (last >= 0) {
+            window(a, t.first_pos + row0 / a.group, t.length, wave_lo, full_hi);
+            window(a, t.first_pos + (row0 + last) / a.group, t.length, full_lo, wave_hi);
+        } else {
+            wave_lo = wave_hi = full_lo = full_hi = 0;
+        }
+        int none;
+        const int tile_last = (tile + 1) * kChunkRows < t.rows ? (tile + 1) * kChunkRows - 1 : t.rows - 1;
+        window(a, t.first_pos + tile * kChunkRows / a.group, t.length, none, tile_full_hi);
+        window(a, t.first_pos + tile_last / a.group, t.length, tile_full_lo, none);
+        const uint16_t* qp = a.query + (size_t)(t.start + tok) * a.query_stride + (size_t)head * kD;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            qf[s] = *(const v8h*)(qp + (kF8 ? 32 * (s >> 1) + 16 * h + 8 * (s & 1) : 16 * s + 8 * h));
+            if (sign < 0.0f) qf[s] = -qf[s];
+        }
+#pragma unroll
+        for (int c = 0; c < kBlocks; ++c) acc[c] = v16f{};
+        top = kNegInf;
+        total = 0.0f;
+    }
+
+    // ---- tiles ----
+
+    // A wave fills 16 keys' rows (in one page), and value chunks of one place among the
+    // tile's keys a lane (in one page).
+    struct Ids {
+        int key, value;
+    };
+    __device__ __forceinline__ int column(int key) const {
+        const int c = key >> a.shift;
+        return c > last_page ? last_page : c;
+    }
+    __device__ __forceinline__ static int key_swizzle(int key) {
+        if constexpr (kKeyBytes == 256) return key & 15;
+        else if constexpr (kKeyBytes == 128) return ((key >> 1) ^ (key >> 3)) & 7;
+        else return ((key >> 4) ^ (key >> 2)) & 3;
+    }
+    __device__ __forceinline__ static int value_swizzle(int d) {
+        if constexpr (kValueBytes == 128) return d & 7;
+        else return (d >> 2) & 3;
+    }
+    __device__ __forceinline__ int value_chunk() const {  // of this lane's loads: their rows differ by multiples of the swizzle
+        return (lane & (kValueChunks - 1)) ^ value_swizzle(lane / kValueChunks);
+    }
+    __device__ __forceinline__ Ids ids(int block) const {
+        const int k0 = block * kTileKeys;
+        return {table[column(k0 + 16 * wave)], table[column(k0 + value_chunk() * (16 / kBytes))]};
+    }
+    __device__ __forceinline__ size_t page_of(int id) const {
+        id = (unsigned)id < (unsigned)a.pages ? id : 0;
+        return ((size_t)id * a.kv_heads + kvh) * ((size_t)kD * kBytes << a.shift);
+    }
+    __device__ __forceinline__ void issue(int block, int buffer, const Ids& id) const {
+        const int k0 = block * kTileKeys, in_page = (1 << a.shift) - 1;
+        const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + buffer * kBuffer;
+        const uint8_t* kp = a.key + page_of(__builtin_amdgcn_readfirstlane(id.key));
+#pragma unroll
+        for (int i = 0; i < kKeyLoads; ++i) {
+            const int slot = (wave * kKeyLoads + i) * 64 + lane, key = slot / kKeyChunks;
+            const int chunk = (slot & (kKeyChunks - 1)) ^ key_swizzle(key);
+            dma16(kp + ((k0 + key) & in_page) * kKeyBytes + chunk * 16, base + (wave * kKeyLoads + i) * 1024);
+        }
+        const uint8_t* vp = a.value + page_of(id.value) + ((k0 + value_chunk() * (16 / kBytes)) & in_page) * kBytes;
+#pragma unroll
+        for (int i = 0; i < kValueLoads; ++i) {
+            const int d = (wave * kValueLoads + i) * (64 / kValueChunks) + lane / kValueChunks;
+            dma16(vp + ((size_t)(d * kBytes) << a.shift), base + kKeyTile + (wave * kValueLoads + i) * 1024);
+        }
+    }
+    // Bit c: the page of value chunk c of the tile exists.
+    __device__ __forceinline__ uint32_t pages_ok(const Ids& id) const {
+        return (uint32_t)__ballot((unsigned)id.value < (unsigned)a.pages) & kAllPages;
+    }
+
+    // First of the 8 consecutive keys of step s (of 4) that this lane holds scores of.
+    __device__ __forceinline__ int step_key(int s) const { return kF8 ? 32 * (s >> 1) + 16 * h + 8 * (s & 1) : 16 * s + 8 * h; }
+
+    // Bit j: this lane's row sees key j of step s.
+    __device__ __forceinline__ uint32_t sees(int k0, int s, uint32_t ok) const {
+        if (!(ok >> (step_key(s) * kBytes / 16) & 1u)) return 0;
+        const int k = k0 + step_key(s), from = lo - k, to = (hi < t.length ? hi : t.length) - k;
+        if (to <= 0 || from >= 8) return 0;
+        return (to >= 8 ? 0xffu : (1u << to) - 1u) & (from <= 0 ? 0xffu : 0xffu << from);
+    }
+
+    // Before a tile at an edge of some row's keys is multiplied (all waves): values of keys
+    // that do not exist hold anything and are cleared.  Whether the others hold
+    // infinities or NaN, which a product with the zero of a masked key would carry into
+    // rows that do not see them.
+    __device__ __forceinline__ bool clear_values(int block, int buffer, uint32_t ok) {
+        const int k0 = block * kTileKeys;
+        uint8_t* vt = lds + buffer * kBuffer + kKeyTile;
+        const int chunk = value_chunk();  // (the loads' places)
+        const int there = ok >> chunk & 1u ? t.length - k0 - chunk * (16 / kBytes) : 0;
+        uint32_t odd = 0;
+#pragma unroll
+        for (int i = 0; i < kValueLoads; ++i) {
+            uint4* p = (uint4*)(vt + (wave * kValueLoads + i) * 1024) + lane;
+            const uint4 old = *p;
+            uint32_t w[4] = {old.x, old.y, old.z, old.w};
+            constexpr int kPerWord = 4 / kBytes;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int n = there - j * kPerWord;  // keys of this word that exist
+                w[j] &= n >= kPerWord ? 0xffffffffu : (n <= 0 ? 0u : (1u << (8 * kBytes * n)) - 1u);
+            }
+            const uint4 now{w[0], w[1], w[2], w[3]};
+            odd |= not_finite<kF8>(now);
+            *p = now;
+        }
+        return __syncthreads_or(odd != 0) != 0;
+    }
+
+    // For such a tile: which of the lane's outputs become NaN, +inf and -inf, counted over
+    // the keys its row sees, into LDS; then the values are cleared of them (all waves).
+    __device__ __forceinline__ void take_out_odd(int block, int buffer, uint32_t ok, uint32_t (*marks)[6]) {
+        const uint8_t* vt = lds + buffer * kBuffer + kKeyTile;
+#pragma unroll 1
+        for (int kind = 0; kind < (kF8 ? 1 : 3); ++kind) {
+#pragma unroll 1
+            for (int half = 0; half < kBlocks; half += 2) {
+                uint32_t mark = 0;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int d = 32 * (half + e) + l32;
+                    v16f count{};
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        const uint4 r = *(const uint4*)(vt + d * kValueBytes + ((kF8 ? 2 * (s >> 1) + h : 2 * s + h) ^ value_swizzle(d)) * 16);
+                        const uint4 ones{odd_ones<kF8>(r.x, kind), odd_ones<kF8>(r.y, kind), odd_ones<kF8>(r.z, kind), odd_ones<kF8>(r.w, kind)};
+                        const uint32_t seen = sees(block * kTileKeys, s, ok);
+                        uint32_t vis[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) vis[i] = ((seen >> (2 * i) & 1u) | (seen >> (2 * i + 1) & 1u) << 16) * 0x3c00u;
+                        count = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<kF8>(ones, s & 1), __builtin_bit_cast(v8h, uint4{vis[0], vis[1], vis[2], vis[3]}),
+                                                                       count, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) mark |= (uint32_t)(count[i] > 0.0f) << (16 * e + i);
+                }
+                marks[threadIdx.x][2 * kind + half / 2] = mark;
+            }
+        }
+        __syncthreads();  // the values are read
+#pragma unroll
+        for (int i = 0; i < kValueLoads; ++i) {
+            uint4* p = (uint4*)(lds + buffer * kBuffer + kKeyTile + (wave * kValueLoads + i) * 1024) + lane;
+            const uint4 v = *p;
+            *p = uint4{odd_cleared<kF8>(v.x), odd_cleared<kF8>(v.y), odd_cleared<kF8>(v.z), odd_cleared<kF8>(v.w)};
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ void put_odd(const uint32_t (*marks)[6]) {
+#pragma unroll
+        for (int kind = 0; kind < (kF8 ? 1 : 3); ++kind) {
+            const float add = kind == 0 ? __builtin_nanf("") : (kind == 1 ? __builtin_inff() : -__builtin_inff());
+#pragma unroll
+            for (int half = 0; half < kBlocks; half += 2) {
+                const uint32_t mark = marks[threadIdx.x][2 * kind + half / 2];
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (mark >> i & 1u) acc[half + (i >> 4)][i & 15] += add;
+            }
+        }
+    }
+
+    __device__ __forceinline__ void multiply(int block, int buffer, uint32_t ok) {
+        const int k0 = block * kTileKeys;
+        if (k0 >= wave_hi || k0 + kTileKeys <= wave_lo) return;
+        const uint8_t* kt = lds + buffer * kBuffer;
+        const uint8_t* vt = kt + kKeyTile;
+
+        v16f sc[2];
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+            // row m of the MFMA is the key whose score lands in place: see step_key
+            const int m = l32, quad = (m >> 3) & 3, half = (m >> 2) & 1, b = m & 3;
+            const int key = 32 * blk + (kF8 ? 16 * half + 8 * (quad >> 1) : 16 * (quad >> 1) + 8 * half) + 4 * (quad & 1) + b;
+            const uint8_t* kr = kt + key * kKeyBytes;
+            const int swz = key_swizzle(key);
+            sc[blk] = v16f{};
+#pragma unroll
+            for (int s = 0; s < kSteps; s += kF8 ? 2 : 1) {
+                const uint4 raw = *(const uint4*)(kr + (((kF8 ? s : 2 * s) + h) ^ swz) * 16);
+#pragma unroll
+                for (int e = 0; e < (kF8 ? 2 : 1); ++e)
+                    sc[blk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<kF8>(raw, e), qf[s + e], sc[blk], 0, 0, 0);
+            }
+        }
+
+        const bool whole = k0 >= full_lo && k0 + kTileKeys <= full_hi && ok == kAllPages;
+        if (!whole) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const uint32_t seen = sees(k0, s, ok);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (!(seen >> j & 1u)) sc[s >> 1][8 * (s & 1) + j] = kNegInf;
+            }
+        }
+        float m = __builtin_fmaxf(sc[0][0], sc[1][0]);
+#pragma unroll
+        for (int j = 1; j < 16; ++j) m = __builtin_fmaxf(m, __builtin_fmaxf(sc[0][j], sc[1][j]));
+        m = max_level(m, 32);
+        if (__any(m > top)) {  // else every factor is 1
+            const float new_top = __builtin_fmaxf(top, m);
+            const float keep = new_top == kNegInf ? 1.0f : __builtin_amdgcn_exp2f((top - new_top) * scale);
+            top = new_top;
+            total *= keep;
+#pragma unroll
+            for (int c = 0; c < kBlocks; ++c) acc[c] = acc[c] * keep;
+        }
+        const float base = top == kNegInf ? 0.0f : top * scale;
+        v8h pf[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[s >> 1][8 * (s & 1) + j], scale, -base));
+                total += p;
+                pf[s][j] = (_Float16)p;
+            }
+
+#pragma unroll
+        for (int c = 0; c < kBlocks; ++c) {
+            const int d = 32 * c + l32;
+            const uint8_t* vr = vt + d * kValueBytes;
+            const int swz = value_swizzle(d);
+            uint4 raw[kF8 ? 2 : 4];
+#pragma unroll
+            for (int s = 0; s < (kF8 ? 2 : 4); ++s) raw[s] = *(const uint4*)(vr + ((2 * s + h) ^ swz) * 16);
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<kF8>(raw[kF8 ? s >> 1 : s], s & 1), pf[s], acc[c], 0, 0, 0);
+        }
+    }
+
+    // Blocks [from, to); `buffer`: the one to fill next, which no wave reads any more.
+    __device__ __forceinline__ void run(int from, int to, int& buffer, uint32_t (*marks)[6]) {
+        Ids id = ids(from), next = ids(from + 1);
+        uint32_t ok = pages_ok(id), next_ok = 0;
+        issue(from, buffer, id);
+        for (int b = from; b < to; ++b) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();  // the tile is there, and every wave is done with the other buffer
+            if (b + 1 < to) {
+                next_ok = pages_ok(next);
+                issue(b + 1, buffer ^ 1, next);
+                next = ids(b + 2);
+            }
+            bool odd = false;
+            if (b * kTileKeys < tile_full_lo || (b + 1) * kTileKeys > tile_full_hi || ok != kAllPages) odd = clear_values(b, buffer, ok);
+            if (odd) take_out_odd(b, buffer, ok, marks);
+            multiply(b, buffer, ok);
+            if (odd) put_odd(marks);
+            ok = next_ok;
+            buffer ^= 1;
+        }
+    }
+
+    // The lane's row (unless it repeats the last) of the output, or of a part.
+    __device__ __forceinline__ void finish(bool whole, Part<kD, kChunkRows>* slot) {
+        int sum_a, sum_b;
+        pair_of(__float_as_int(total), 32, sum_a, sum_b);
+        const float sum = __int_as_float(sum_a) + __int_as_float(sum_b);
+        if (l32 > last) return;
+        const int r = wave * 32 + l32;
+        const float inv = sum == 0.0f ? 0.0f : a.value_scale / sum;
+        uint16_t* op = a.out + (size_t)(t.start + row / a.group) * a.out_stride + (size_t)(kvh * a.group + row % a.group) * kD;
+#pragma unroll
+        for (int c = 0; c < kBlocks; ++c)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int d = 32 * c + 8 * q + 4 * h;
+                const v4f v{acc[c][4 * q], acc[c][4 * q + 1], acc[c][4 * q + 2], acc[c][4 * q + 3]};
+                if (whole)
+                    *(uint2*)(op + d) = uint2{(uint32_t)f2h(v[0] * inv) | ((uint32_t)f2h(v[1] * inv) << 16),
+                                              (uint32_t)f2h(v[2] * inv) | ((uint32_t)f2h(v[3] * inv) << 16)};
+                else
+                    *(v4f*)&slot->acc[r][d] = v;
+            }
+        if (!whole && h == 0) {
+            slot->top[r] = top == kNegInf ? kNegInf : top * scale;
+            slot->total[r] = sum;
+        }
+    }
+};
+
+// Short contexts: a workgroup for all keys of a (sequence, kv head, 128 rows).
+template <int kD, bool kF8> __global__ __launch_bounds__(256, 2) void paged_chunks_direct_kernel(PagedArgs a) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * ChunkPass<kD, kF8>::kBuffer];
+    __shared__ uint32_t marks[256][6];
+    const int kvh = blockIdx.x, seq = blockIdx.z, tile = blockIdx.y;
+    const RowTile t = wave_sequence(a, seq);
+    if (tile * kChunkRows >= t.rows) return;
+    int first, buffer = 0;
+    const int blocks = chunk_blocks(a, t, tile, first);
+    ChunkPass<kD, kF8> pass(a, lds, kvh);
+    pass.start(seq, t, tile);
+    pass.run(first, first + blocks, buffer, marks);
+    pass.finish(true, nullptr);
+}
+
+template <int kD, bool kF8>
+__global__ __launch_bounds__(256, 2) void paged_chunks_shares_kernel(PagedArgs a, Part<kD, kChunkRows>* slots, Join* joins) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * ChunkPass<kD, kF8>::kBuffer];
+    __shared__ uint32_t marks[256][6];
+    // neighbouring shares read the same keys: they go to one XCD's L2
+    const int index = (blockIdx.x & 7) * (kChunkShares / 8) + (blockIdx.x >> 3);
+    if (threadIdx.x == 0) joins[index].count = 0;
+    Share share;
+    const auto blocks_of = [&](const RowTile& t) { return pairs_of(a, t).per_head * a.kv_heads; };
+    if (!deal(a, kChunkShares, kLeastChunkShare, index, blocks_of, share)) return;
+
+    int seq = share.seq, buffer = 0;
+    long long at = share.from, offset = share.offset;  // offset: of `at` in the sequence's blocks
+    while (at < share.to) {
+        const RowTile t = wave_sequence(a, seq);
+        const Pairs p = pairs_of(a, t);
+        const long long all = p.per_head * a.kv_heads;
+        while (offset < all && at < share.to) {
+            const int kvh = (int)(offset / p.per_head);
+            const int in_head = (int)(offset - kvh * p.per_head);
+            const int pair = p.pair ? in_head / p.pair : 0;
+            const bool middle = pair == p.tiles / 2;
+            const int in_pair = in_head - pair * p.pair, pair_blocks = middle ? p.middle : p.pair;
+            int first_a, first_b = 0;
+            const int blocks_a = chunk_blocks(a, t, pair, first_a);
+            const int blocks_b = middle ? 0 : chunk_blocks(a, t, p.tiles - 1 - pair, first_b);
+            // the part of the item at `offset`: its first tile, its second, or what the pair has too many
+            const bool second = in_pair >= blocks_a;
+            const int b0 = second ? in_pair - blocks_a : in_pair, blocks = second ? blocks_b : blocks_a;
+            int n;
+            if (second && b0 >= blocks_b) {
+                n = pair_blocks - in_pair;
+                if (n > share.to - at) n = (int)(share.to - at);
+            } else {
+                n = share.to - at < blocks - b0 ? (int)(share.to - at) : blocks - b0;
+                const int tile = second ? p.tiles - 1 - pair : pair, first = (second ? first_b : first_a) + b0;
+                ChunkPass<kD, kF8> pass(a, lds, kvh);
+                pass.start(seq, t, tile);
+                pass.run(first, first + n, buffer, marks);
+                const int which = at == share.from ? 0 : 1;
+                pass.finish(n == blocks, slots + 2 * index + which);
+                if (n != blocks && b0 == 0 && threadIdx.x == 0)
+                    joins[index] = {t.start, t.rows, kvh, tile * kChunkRows, (int)((at + blocks - 1) / share.size - index) + 1, which, {}};
+            }
+            at += n;
+            offset += n;
+        }
+        ++seq;
+        offset = 0;
+    }
+}
+
+// Joins the parts of the divided row tiles, 16 rows a workgroup: a row a group of lanes
+// where the parts are few, else a row at a time with the groups taking parts in turn.
+template <int kD> __global__ __launch_bounds__(16 * kD / 4) void paged_chunks_join_kernel(PagedArgs a, const Part<kD, kChunkRows>* slots, const Join* joins) {
+    constexpr int kLanes = kD / 4;
+    __shared__ float part_acc[16][kD], part_top[16], part_total[16];
+    const Join job = joins[blockIdx.x];
+    const int r0 = blockIdx.y * 16;
+    if (job.count == 0 || job.row0 + r0 >= job.rows) return;
+    const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    const Part<kD, kChunkRows>* first = slots + 2 * blockIdx.x;
+    const bool few = job.count <= 16;
+    for (int row = few ? group : 0; row < 16; row += few ? 16 : 1) {
+        const int r = r0 + row;
+        if (job.row0 + r >= job.rows) break;
+        float top = kNegInf, total = 0.0f;
+        v4f v{};
+#pragma unroll 4
+        for (int i = few ? 0 : group; i < job.count; i += few ? 1 : 16) {
+            const Part<kD, kChunkRows>& slot = first[2 * i + (i == 0 ? job.first_slot : 0)];
+            const float new_top = __builtin_fmaxf(top, slot.top[r]);
+            const float base = new_top == kNegInf ? 0.0f : new_top;
+            const float f = __builtin_amdgcn_exp2f(slot.top[r] - base), keep = __builtin_amdgcn_exp2f(top - base);
+            total = total * keep + slot.total[r] * f;
+            v = v * keep + *(const v4f*)&slot.acc[r][4 * lane] * f;
+            top = new_top;
+        }
+        if (!few) {
+            __syncthreads();  // the row before is read
+            *(v4f*)&part_acc[group][4 * lane] = v;
+            if (lane == 0) {
+                part_top[group] = top;
+                part_total[group] = total;
+            }
+            __syncthreads();
+            if (group != 0) continue;
+            float best = kNegInf;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) best = __builtin_fmaxf(best, part_top[w]);
+            const float base = best == kNegInf ? 0.0f : best;
+            total = 0.0f;
+            v = v4f{};
+#pragma unroll
+            for (int w = 0; w < 16; ++w) {
+                const float f = __builtin_amdgcn_exp2f(part_top[w] - base);
+                total += part_total[w] * f;
+                v = v + *(const v4f*)&part_acc[w][4 * lane] * f;
+            }
+        }
+        const float o[4] = {v[0], v[1], v[2], v[3]};
+        store_row<4>(a, {job.start, job.rows, 0, 0}, job.kvh, job.row0 + r, kD, 4 * lane, total, o);
+    }
+}
+
+size_t paged_chunks_workspace(int head_dim) {
+    return 2 * kChunkShares * (head_dim == 128 ? sizeof(Part<128, kChunkRows>) : sizeof(Part<64, kChunkRows>)) + kChunkShares * sizeof(Join);
+}
+
+template <int kD, bool kF8> static void launch_chunks(const PagedArgs& a, bool direct, int max_queries, void* workspace, hipStream_t s) {
+    const int rows = max_queries * a.group;
+    if (direct) {
+        const dim3 grid((unsigned)a.kv_heads, (unsigned)((rows + kChunkRows - 1) / kChunkRows), (unsigned)a.sequences);
+        paged_chunks_direct_kernel<kD, kF8><<<grid, 256, 0, s>>>(a);
+        return;
+    }
+    auto* slots = (Part<kD, kChunkRows>*)workspace;
+    Join* joins = (Join*)(slots + 2 * kChunkShares);
+    paged_chunks_shares_kernel<kD, kF8><<<kChunkShares, 256, 0, s>>>(a, slots, joins);
+    const int part_rows = rows < kChunkRows ? rows : kChunkRows;
+    paged_chunks_join_kernel<kD><<<dim3(kChunkShares, (unsigned)((part_rows + 15) / 16)), 16 * kD / 4, 0, s>>>(a, slots, joins);
+}
+
+void launch_paged_chunks(int kind, const PagedArgs& a, int head_dim, bool direct, int max_queries, void* workspace, hipStream_t s) {
+    if (head_dim == 128) {
+        if (kind == 1) launch_chunks<128, true>(a, direct, max_queries, workspace, s);
+        else launch_chunks<128, false>(a, direct, max_queries, workspace, s);
+    } else {
+        if (kind == 1) launch_chunks<64, true>(a, direct, max_queries, workspace, s);
+        else launch_chunks<64, false>(a, direct, max_queries, workspace, s);
+    }
+}
+
+}  // namespace pk
