@@ -93,7 +93,7 @@ template <int kD, bool kF8> struct RowPass {
     }
 
     // Tiles k0, k0 + kSpan, ... below `end` (and inside the rows' range).
-    __device__ __forceinline__ void run(int k0, int end) {
+    __device__ __forceinline__ void run(int k0, int end, Odd<kD, 16>& odd) {
         while (k0 + kKeys <= tile_lo) k0 += kSpan;
         if (end > tile_hi) end = tile_hi;
         if (k0 >= end) return;
@@ -122,14 +122,10 @@ template <int kD, bool kF8> struct RowPass {
             const Ids later = ids(k0 + 2 * kSpan);
             __builtin_amdgcn_sched_barrier(0);
             const bool whole = k0 >= full_lo && k0 + kKeys <= full_hi && __all(ok);
-            uint32_t seen = 0;  // bit j: this lane's row sees key mine + j
             if (!whole) {
 #pragma unroll
-                for (int j = 0; j < 8 * kU; ++j) {
-                    const bool see = mine + j >= lo && mine + j < hi && j < there;
-                    seen |= (uint32_t)see << j;
-                    if (!see) p[j] = kNegInf;
-                }
+                for (int j = 0; j < 8 * kU; ++j)
+                    if (mine + j < lo || mine + j >= hi || j >= there) p[j] = kNegInf;
             }
             float m = p[0];
 #pragma unroll
@@ -151,7 +147,6 @@ template <int kD, bool kF8> struct RowPass {
 #pragma unroll
             for (int c = 0; c < kBlocks; ++c) acc[c] = acc[c] * keep;
             if (!whole) {
-                uint32_t odd = 0;
                 // keys that do not exist hold anything: their values are taken as zero
                 constexpr int kPerWord = 4 / kBytes;
                 uint32_t there_mask[4];
@@ -166,11 +161,10 @@ template <int kD, bool kF8> struct RowPass {
                     vraw[c].y &= there_mask[1];
                     vraw[c].z &= there_mask[2];
                     vraw[c].w &= there_mask[3];
-                    odd |= not_finite<kF8>(vraw[c]);
-                }
-                if (__any(odd != 0)) {
-#pragma unroll
-                    for (int c = 0; c < kBlocks; ++c) add_not_finite<kF8>(vraw[c], seen, acc[c]);
+                    odd.template take<kF8>(vraw[c], 16 * c + l16, mine, [&](int r, int& from, int& to) {
+                        from = lo;  // lane r < 16 has row r
+                        to = r <= last ? hi : lo;
+                    });
                 }
             }
 #pragma unroll
@@ -218,21 +212,34 @@ template <int kD> __device__ __forceinline__ void join(const Parts<kD>& parts, i
     }
 }
 
+template <int kD> __device__ __forceinline__ bool put_odd(const Odd<kD, 16>& odd, int r, int d0, float (&v)[kD / 16]) {
+    const bool any = __builtin_amdgcn_readfirstlane((int)odd.any) != 0;
+    if (__builtin_expect(any, 0)) {
+#pragma unroll
+        for (int j = 0; j < kD / 16; ++j) v[j] = odd.put(v[j], r, d0 + j);
+    }
+    return any;
+}
+
 // Short contexts: one workgroup for the keys of a (sequence, kv head, 16 rows).
 template <int kD, bool kF8> __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs a) {
     __shared__ Parts<kD> parts;
+    __shared__ Odd<kD, 16> odd;
+    odd.clear(256);
+    __syncthreads();
     const int kvh = blockIdx.x, seq = blockIdx.z, row0 = blockIdx.y * 16;
     const RowTile t = wave_sequence(a, seq);
     if (row0 >= t.rows) return;
     RowPass<kD, kF8> pass(a, kvh);
     pass.start(seq, t, row0);
-    pass.run((pass.tile_lo & ~(pass.kKeys - 1)) + wave_index() * pass.kKeys, pass.tile_hi);
+    pass.run((pass.tile_lo & ~(pass.kKeys - 1)) + wave_index() * pass.kKeys, pass.tile_hi, odd);
     to_lds<kD, kF8>(pass, parts);
     __syncthreads();
     const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (kD / 16);
     if (r > pass.last) return;
     float best, total, v[kD / 16];
     join<kD>(parts, r, d0, best, total, v);
+    put_odd<kD>(odd, r, d0, v);
     store_row<kD / 16>(a, t, kvh, row0 + r, kD, d0, total, v);
 }
 
@@ -263,13 +270,15 @@ template <int kD, bool kF8>
 __global__ __launch_bounds__(256, 2) void paged_attention_shares_kernel(PagedArgs a, Part<kD, 16>* slots, Join* joins) {
     constexpr int kSpan = RowPass<kD, kF8>::kSpan;
     __shared__ Parts<kD> parts;
+    __shared__ Odd<kD, 16> odd;
+    odd.clear(256);
     if (threadIdx.x == 0) joins[blockIdx.x].count = 0;
     Share share;
     const auto blocks_of = [&](const RowTile& t) {
         int first;
         return (long long)item_blocks<kSpan>(a, t, first) * items_of(a, t);
     };
-    if (!deal(a, kShares, kLeastShare, blockIdx.x, blocks_of, share)) return;
+    if (!deal<256>(a, kShares, kLeastShare, blockIdx.x, blocks_of, share)) return;
 
     int seq = share.seq;
     long long at = share.from, offset = share.offset;
@@ -284,12 +293,13 @@ __global__ __launch_bounds__(256, 2) void paged_attention_shares_kernel(PagedArg
             const int kvh = item % a.kv_heads, row0 = item / a.kv_heads * 16;
             RowPass<kD, kF8> pass(a, kvh);
             pass.start(seq, t, row0);
-            pass.run((first + b0) * kSpan + wave_index() * pass.kKeys, (first + b0 + n) * kSpan);
+            pass.run((first + b0) * kSpan + wave_index() * pass.kKeys, (first + b0 + n) * kSpan, odd);
             __syncthreads();  // the previous item's parts are read
             to_lds<kD, kF8>(pass, parts);
             __syncthreads();
             float best, total, v[kD / 16];
             join<kD>(parts, r, d0, best, total, v);
+            const bool any_odd = put_odd<kD>(odd, r, d0, v);
             if (n == blocks) {
                 if (r <= pass.last) store_row<kD / 16>(a, t, kvh, row0 + r, kD, d0, total, v);
             } else {
@@ -302,6 +312,11 @@ __global__ __launch_bounds__(256, 2) void paged_attention_shares_kernel(PagedArg
                 }
                 if (b0 == 0 && threadIdx.x == 0)
                     joins[blockIdx.x] = {t.start, t.rows, kvh, row0, (int)((at + blocks - 1) / share.size - blockIdx.x) + 1, at == share.from ? 0 : 1, {}};
+            }
+            if (any_odd) {
+                __syncthreads();
+                odd.clear(256);
+                __syncthreads();
             }
             at += n;
             offset += n;

@@ -36,48 +36,58 @@ template <bool kF8> __device__ __forceinline__ uint32_t not_finite(const uint4& 
     return (((w.x & e) + one) | ((w.y & e) + one) | ((w.z & e) + one) | ((w.w & e) + one)) & (kF8 ? 0x80808080u : 0x80008000u);
 }
 
-// Which values of a word are NaN (0), +inf (1) or -inf (2): the cache's 1.0 where so.
-template <bool kF8> __device__ __forceinline__ uint32_t odd_ones(uint32_t w, int which) {
-    if constexpr (kF8) {
-        return (((w & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 0x38u;
-    } else {
-        const uint32_t odd = (((w & 0x7c007c00u) + 0x04000400u) >> 15) & 0x00010001u;
-        const uint32_t nan = odd & (((w & 0x03ff03ffu) + 0x03ff03ffu) >> 10);
-        const uint32_t sign = (w >> 15) & 0x00010001u, inf = odd & ~nan;
-        return (which == 0 ? nan : (which == 1 ? inf & ~sign : inf & sign)) * 0x3c00u;
-    }
-}
 template <bool kF8> __device__ __forceinline__ uint32_t odd_cleared(uint32_t w) {
     if constexpr (kF8) return w & ~((((w & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 0xffu);
     else return w & ~(((((w & 0x7c007c00u) + 0x04000400u) >> 15) & 0x00010001u) * 0xffffu);
 }
 
-// Infinities and NaN in values, where a product with the zero of a masked key would
-// spoil rows that do not see that key: each kind is counted over the keys that a row
-// sees (bits of `seen`), added to the rows that see one, and cleared from the operand.
-// Rare; in place and one kind after the other, so that it needs few registers.
-template <bool kF8> __device__ __forceinline__ void add_not_finite(uint4& raw, uint32_t seen, v4f& o) {
-#pragma unroll
-    for (int kind = 0; kind < (kF8 ? 1 : 3); ++kind) {
-        asm volatile("" : "+v"(seen));  // operands are made anew: not kept in registers
-        const uint4 ones{odd_ones<kF8>(raw.x, kind), odd_ones<kF8>(raw.y, kind), odd_ones<kF8>(raw.z, kind), odd_ones<kF8>(raw.w, kind)};
-        v4f count{};
-#pragma unroll
-        for (int u = 0; u < (kF8 ? 2 : 1); ++u) {
-            uint32_t vis[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) vis[i] = ((seen >> (8 * u + 2 * i) & 1u) | (seen >> (8 * u + 2 * i + 1) & 1u) << 16) * 0x3c00u;
-            count = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand<kF8>(ones, u), __builtin_bit_cast(v8h, uint4{vis[0], vis[1], vis[2], vis[3]}), count,
-                                                           0, 0, 0);
-        }
-        const float add = kind == 0 ? __builtin_nanf("") : (kind == 1 ? __builtin_inff() : -__builtin_inff());
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (count[r] > 0.0f) o[r] += add;
-        __builtin_amdgcn_sched_barrier(0);
+// Infinities and NaN in values: a product with the zero of a masked key would spoil rows
+// that do not see that key.  At the edges of the rows' keys they are therefore taken out
+// of the operands, and which outputs they belong to (those of the rows that do see the
+// key) is noted in LDS, for the end.  Rare, and kept out of the way of everything else.
+template <int kD, int kRows> struct Odd {
+    static constexpr int kWords = (kRows + 31) / 32;
+    uint32_t any;
+    uint32_t marks[3][kD][kWords];  // NaN, +inf, -inf: bit of the row
+
+    __device__ __forceinline__ void clear(int threads) {
+        for (int i = threadIdx.x; i < 3 * kD * kWords; i += threads) (&marks[0][0][0])[i] = 0;
+        if (threadIdx.x == 0) any = 0;
     }
-    raw = uint4{odd_cleared<kF8>(raw.x), odd_cleared<kF8>(raw.y), odd_cleared<kF8>(raw.z), odd_cleared<kF8>(raw.w)};
-}
+    // 16 bytes of values of feature d from key `key` on, a lane; window(r, lo, hi): the keys that row r of this lane sees.
+    template <bool kF8, class Window> __device__ __forceinline__ void take(uint4& raw, int d, int key, Window window) {
+        const int lane = threadIdx.x & 63;
+        unsigned long long todo = __ballot(not_finite<kF8>(raw) != 0);
+        while (__builtin_expect(todo != 0, 0)) {
+            const int from = __builtin_ctzll(todo);
+            todo &= todo - 1;
+            const uint32_t w[4] = {(uint32_t)__builtin_amdgcn_readlane((int)raw.x, from), (uint32_t)__builtin_amdgcn_readlane((int)raw.y, from),
+                                   (uint32_t)__builtin_amdgcn_readlane((int)raw.z, from), (uint32_t)__builtin_amdgcn_readlane((int)raw.w, from)};
+            const int feature = __builtin_amdgcn_readlane(d, from), first = __builtin_amdgcn_readlane(key, from);
+#pragma unroll 1
+            for (int j = 0; j < (kF8 ? 16 : 8); ++j) {
+                const int at = kF8 ? j >> 2 : j >> 1;
+                const uint32_t word = at == 0 ? w[0] : (at == 1 ? w[1] : (at == 2 ? w[2] : w[3]));
+                const uint32_t v = kF8 ? word >> (8 * (j & 3)) & 0xffu : word >> (16 * (j & 1)) & 0xffffu;
+                if (kF8 ? (v & 0x7fu) != 0x7fu : (v & 0x7c00u) != 0x7c00u) continue;
+                const int kind = kF8 || v & 0x3ffu ? 0 : (v >> 15 ? 2 : 1);
+                for (int r = lane; r < kRows; r += 64) {
+                    int lo, hi;
+                    window(r, lo, hi);
+                    if (first + j >= lo && first + j < hi) atomicOr(&marks[kind][feature][r >> 5], 1u << (r & 31));
+                }
+                if (lane == 0) any = 1;
+            }
+        }
+        raw = uint4{odd_cleared<kF8>(raw.x), odd_cleared<kF8>(raw.y), odd_cleared<kF8>(raw.z), odd_cleared<kF8>(raw.w)};
+    }
+    // What row r's sum of feature d becomes.
+    __device__ __forceinline__ float put(float v, int r, int d) const {
+        if (marks[1][d][r >> 5] >> (r & 31) & 1u) v += __builtin_inff();
+        if (marks[2][d][r >> 5] >> (r & 31) & 1u) v -= __builtin_inff();
+        return marks[0][d][r >> 5] >> (r & 31) & 1u ? __builtin_nanf("") : v;
+    }
+};
 
 // One sequence's view for a tile of 16 query rows.
 struct RowTile {
@@ -125,18 +135,18 @@ __device__ __forceinline__ void store_row(const PagedArgs& a, const RowTile& t, 
 }
 
 // The work of all sequences in a row, in blocks of keys, dealt to `shares` workgroups in
-// equal contiguous shares: every workgroup sums the blocks of all sequences (256 threads)
-// and finds the sequence that its share begins in.
+// equal contiguous shares: every workgroup (kThreads threads) sums the blocks of all
+// sequences and finds the sequence that its share begins in.
 struct Share {
     long long from, to, size;  // its blocks, and the blocks of a full share
     long long offset;          // blocks of `seq` before `from`
     int seq;
 };
 
-template <class Blocks> __device__ __forceinline__ bool deal(const PagedArgs& a, int shares, int least, int index, Blocks blocks_of, Share& out) {
-    __shared__ long long wave_total[4], found_offset;
+template <int kThreads, class Blocks> __device__ __forceinline__ bool deal(const PagedArgs& a, int shares, int least, int index, Blocks blocks_of, Share& out) {
+    __shared__ long long wave_total[kThreads / 64], found_offset;
     __shared__ int found_seq;
-    const int per = (a.sequences + 255) / 256, s0 = threadIdx.x * per;
+    const int per = (a.sequences + kThreads - 1) / kThreads, s0 = threadIdx.x * per;
     long long mine = 0;
     for (int s = s0; s < s0 + per && s < a.sequences; ++s) mine += blocks_of(sequence_of(a, s));
     long long end = mine;
@@ -148,7 +158,9 @@ template <class Blocks> __device__ __forceinline__ bool deal(const PagedArgs& a,
     if ((threadIdx.x & 63) == 63) wave_total[threadIdx.x >> 6] = end;
     __syncthreads();
     for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) end += wave_total[w];
-    const long long all = uniform((wave_total[0] + wave_total[1]) + (wave_total[2] + wave_total[3]));
+    long long all = 0;
+    for (int w = 0; w < kThreads / 64; ++w) all += wave_total[w];
+    all = uniform(all);
     out.size = (all + shares - 1) / shares;
     if (out.size < least) out.size = least;
     out.from = index * out.size;

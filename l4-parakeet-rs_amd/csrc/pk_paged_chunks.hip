@@ -1,11 +1,11 @@
-// The paged attention for chunks of new tokens: 128 query rows a workgroup, 32 a wave.
+// The paged attention for chunks of new tokens: 256 query rows a workgroup, 32 a wave.
 //
 // The same two products as for few rows (S^T = K Q^T, O^T = V^T P^T, probabilities in
-// registers), on 32 x 32 x 16 MFMAs.  The four waves share 64-key tiles of keys and
-// values in LDS, which the loads fill directly while the previous tile is multiplied
-// (two buffers, one barrier a tile; two workgroups a CU, so that one's softmax runs
-// under the other's products).  Tile rows are whole key or value rows whose 16-byte chunks
-// are XOR-swizzled at the source, since such loads write LDS in lane order.
+// registers), on 32 x 32 x 16 MFMAs.  The eight waves share 64-key tiles of keys and
+// values in LDS, which the loads fill directly, three tiles ahead of the one that is
+// multiplied (four buffers, one barrier a tile).  Tile rows are whole key or value rows
+// whose 16-byte chunks are XOR-swizzled at the source, since such loads write LDS in lane
+// order.
 //
 // Bound by the softmax's vector instructions next to the MFMAs: 32 scores a lane and
 // tile, each a maximum, a fused scale and subtraction, an exponential, a sum and half a
@@ -16,8 +16,9 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 
 namespace pk {
 
-constexpr int kChunkRows = 128, kTileKeys = 64;
-constexpr int kChunkShares = 512;  // two workgroups on each of 256 CUs
+constexpr int kChunkWaves = 8, kChunkThreads = 64 * kChunkWaves, kChunkRows = 32 * kChunkWaves;
+constexpr int kTileKeys = 64, kBuffers = 4;
+constexpr int kChunkShares = 256;  // a workgroup on each of 256 CUs
 constexpr int kLeastChunkShare = 4;
 
 // Blocks (tiles of keys) that the rows of one row tile see, from block `first` on.
@@ -59,17 +60,25 @@ template <int kD, bool kF8> struct ChunkPass {
     static constexpr int kBuffer = kKeyTile + kValueTile;
     static constexpr int kKeyChunks = kKeyBytes / 16, kValueChunks = kValueBytes / 16;
     static constexpr uint32_t kAllPages = (1u << kValueChunks) - 1u;
-    static constexpr int kKeyLoads = kKeyTile / 4096, kValueLoads = kValueTile / 4096;  // 16 bytes a lane, of 4 waves
+    // a load of a wave fills 1 KB: the keys' units go to the waves in runs, the values' in
+    // turn; where there are fewer units than waves, the keys' go to the first waves and the
+    // values' to the others, so that every wave has kLoads a tile
+    static constexpr int kKeyUnits = kKeyTile / 1024, kValueUnits = kValueTile / 1024;
+    static constexpr bool kSplit = kKeyUnits < kChunkWaves;
+    static constexpr int kKeyLoads = kSplit ? 1 : kKeyUnits / kChunkWaves, kValueLoads = kSplit ? 1 : kValueUnits / kChunkWaves;
+    static constexpr int kLoads = kSplit ? 1 : kKeyLoads + kValueLoads;
+    static_assert(!kSplit || kKeyUnits + kValueUnits == kChunkWaves);
+    static constexpr int kKeyRun = 16 / (kSplit ? 1 : 2);  // keys that a wave loads
 
     const PagedArgs& a;
     uint8_t* lds;
     const int lane, wave, l32, h, kvh;
     RowTile t;
     const int* table;
-    int last_page;
+    int last_page, ring;      // ring: tile b lies in buffer (b + ring) mod kBuffers
     int row0, last, row;      // this wave's first row, its last row's index (< 0: none), this lane's row
     int lo, hi, full_lo, full_hi, wave_lo, wave_hi;
-    int tile_full_lo, tile_full_hi;  // keys that all 128 rows see
+    int tile_full_lo, tile_full_hi;  // keys that all of the workgroup's rows see
     float scale, sign;
     v8h qf[kSteps];
     v16f acc[kBlocks];
@@ -117,81 +126,113 @@ template <int kD, bool kF8> struct ChunkPass {
 
     // ---- tiles ----
 
-    // A wave fills 16 keys' rows (in one page), and value chunks of one place among the
-    // tile's keys a lane (in one page).
+    // Pages of the tile's four groups of 16 keys.  The table is read through the scalar
+    // cache: a vector load among the tiles' would have to wait for all of them.
     struct Ids {
-        int key, value;
+        int page[4];
     };
-    __device__ __forceinline__ int column(int key) const {
+    __device__ __forceinline__ int page_at(int key) const {
+        typedef const __attribute__((address_space(4))) int* ScalarTable;
         const int c = key >> a.shift;
-        return c > last_page ? last_page : c;
+        return ((ScalarTable)(uintptr_t)table)[__builtin_amdgcn_readfirstlane(c > last_page ? last_page : c)];
     }
+    __device__ __forceinline__ int key_id(int block) const { return page_at(block * kTileKeys + (kKeyRun * wave & (kTileKeys - 1))); }
+    __device__ __forceinline__ Ids value_ids(int block) const {
+        const int k0 = block * kTileKeys;
+        return {{page_at(k0), page_at(k0 + 16), page_at(k0 + 32), page_at(k0 + 48)}};
+    }
+    // Of one of the groups, chosen by the wave or by a lane.
+    __device__ __forceinline__ static int pick(const Ids& id, int group) {
+        const int a = id.page[0], b = id.page[1], c = id.page[2], d = id.page[3];
+        const int low = group & 1 ? b : a, high = group & 1 ? d : c;
+        return group & 2 ? high : low;
+    }
+    // Bit c: the page of value chunk c of the tile exists.
+    __device__ __forceinline__ uint32_t pages_ok(const Ids& id) const {
+        uint32_t ok = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if ((unsigned)id.page[i] < (unsigned)a.pages) ok |= kF8 ? 1u << i : 3u << (2 * i);
+        return ok;
+    }
+    // Keys that 16 lanes of a fragment read differ in bits 0-3 (fp16) or 0-2 and 4 (e4m3).
     __device__ __forceinline__ static int key_swizzle(int key) {
         if constexpr (kKeyBytes == 256) return key & 15;
-        else if constexpr (kKeyBytes == 128) return ((key >> 1) ^ (key >> 3)) & 7;
-        else return ((key >> 4) ^ (key >> 2)) & 3;
+        else if constexpr (kKeyBytes == 128) return (key >> 1 & 3) | ((key >> 3 ^ key >> 4) & 1) << 2;
+        else return (key >> 2 & 1) | ((key >> 3 ^ key >> 4) & 1) << 1;
     }
     __device__ __forceinline__ static int value_swizzle(int d) {
-        if constexpr (kValueBytes == 128) return d & 7;
-        else return (d >> 2) & 3;
+        if constexpr (kValueBytes == 128) return d >> 1 & 7;
+        else return d >> 2 & 3;
     }
-    __device__ __forceinline__ int value_chunk() const {  // of this lane's loads: their rows differ by multiples of the swizzle
-        return (lane & (kValueChunks - 1)) ^ value_swizzle(lane / kValueChunks);
-    }
-    __device__ __forceinline__ Ids ids(int block) const {
-        const int k0 = block * kTileKeys;
-        return {table[column(k0 + 16 * wave)], table[column(k0 + value_chunk() * (16 / kBytes))]};
+    __device__ __forceinline__ int value_unit(int i) const { return kSplit ? wave - kKeyUnits : wave + kChunkWaves * i; }
+    // Of this lane's loads, whose rows differ by multiples of what the swizzle sees.
+    __device__ __forceinline__ int value_chunk() const {
+        return (lane & (kValueChunks - 1)) ^ value_swizzle(value_unit(0) * (64 / kValueChunks) + lane / kValueChunks);
     }
     __device__ __forceinline__ size_t page_of(int id) const {
         id = (unsigned)id < (unsigned)a.pages ? id : 0;
         return ((size_t)id * a.kv_heads + kvh) * ((size_t)kD * kBytes << a.shift);
     }
-    __device__ __forceinline__ void issue(int block, int buffer, const Ids& id) const {
+    __device__ __forceinline__ int buffer_of(int block) const { return (block + ring) & (kBuffers - 1); }
+    __device__ __forceinline__ uint32_t lds_of(int block) const {
+        return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + buffer_of(block) * kBuffer;
+    }
+    __device__ __forceinline__ void issue_keys(int block, int id) const {
+        if (kSplit && wave >= kKeyUnits) return;
+        const uint8_t* kp = a.key + page_of(id);  // a wave's keys lie in one page
         const int k0 = block * kTileKeys, in_page = (1 << a.shift) - 1;
-        const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + buffer * kBuffer;
-        const uint8_t* kp = a.key + page_of(__builtin_amdgcn_readfirstlane(id.key));
+        const uint32_t base = lds_of(block);
 #pragma unroll
         for (int i = 0; i < kKeyLoads; ++i) {
-            const int slot = (wave * kKeyLoads + i) * 64 + lane, key = slot / kKeyChunks;
+            const int unit = wave * kKeyLoads + i, slot = unit * 64 + lane, key = slot / kKeyChunks;
             const int chunk = (slot & (kKeyChunks - 1)) ^ key_swizzle(key);
-            dma16(kp + ((k0 + key) & in_page) * kKeyBytes + chunk * 16, base + (wave * kKeyLoads + i) * 1024);
-        }
-        const uint8_t* vp = a.value + page_of(id.value) + ((k0 + value_chunk() * (16 / kBytes)) & in_page) * kBytes;
-#pragma unroll
-        for (int i = 0; i < kValueLoads; ++i) {
-            const int d = (wave * kValueLoads + i) * (64 / kValueChunks) + lane / kValueChunks;
-            dma16(vp + ((size_t)(d * kBytes) << a.shift), base + kKeyTile + (wave * kValueLoads + i) * 1024);
+            dma16(kp + ((k0 + key) & in_page) * kKeyBytes + chunk * 16, base + unit * 1024);
         }
     }
-    // Bit c: the page of value chunk c of the tile exists.
-    __device__ __forceinline__ uint32_t pages_ok(const Ids& id) const {
-        return (uint32_t)__ballot((unsigned)id.value < (unsigned)a.pages) & kAllPages;
+    __device__ __forceinline__ void issue_values(int block, const Ids& id) const {
+        if (kSplit && wave < kKeyUnits) return;
+        const int chunk = value_chunk(), k0 = block * kTileKeys, in_page = (1 << a.shift) - 1;
+        const uint8_t* vp = a.value + page_of(pick(id, chunk * 4 / kValueChunks)) + ((k0 + chunk * (16 / kBytes)) & in_page) * kBytes;
+        const uint32_t base = lds_of(block) + kKeyTile;
+#pragma unroll
+        for (int i = 0; i < kValueLoads; ++i) {
+            const int unit = value_unit(i), d = unit * (64 / kValueChunks) + lane / kValueChunks;
+            dma16(vp + ((size_t)(d * kBytes) << a.shift), base + unit * 1024);
+        }
     }
 
     // First of the 8 consecutive keys of step s (of 4) that this lane holds scores of.
     __device__ __forceinline__ int step_key(int s) const { return kF8 ? 32 * (s >> 1) + 16 * h + 8 * (s & 1) : 16 * s + 8 * h; }
 
+    // The value itself, computed from anew at this place: what only edge tiles need is not
+    // kept in registers over the loop.
+    __device__ __forceinline__ static int here(int v) {
+        asm volatile("" : "+v"(v));
+        return v;
+    }
     // Bit j: this lane's row sees key j of step s.
     __device__ __forceinline__ uint32_t sees(int k0, int s, uint32_t ok) const {
         if (!(ok >> (step_key(s) * kBytes / 16) & 1u)) return 0;
-        const int k = k0 + step_key(s), from = lo - k, to = (hi < t.length ? hi : t.length) - k;
+        const int k = k0 + step_key(s), from = here(lo) - k, to = here(hi) - k;
         if (to <= 0 || from >= 8) return 0;
         return (to >= 8 ? 0xffu : (1u << to) - 1u) & (from <= 0 ? 0xffu : 0xffu << from);
     }
 
-    // Before a tile at an edge of some row's keys is multiplied (all waves): values of keys
-    // that do not exist hold anything and are cleared.  Whether the others hold
-    // infinities or NaN, which a product with the zero of a masked key would carry into
-    // rows that do not see them.
-    __device__ __forceinline__ bool clear_values(int block, int buffer, uint32_t ok) {
-        const int k0 = block * kTileKeys;
-        uint8_t* vt = lds + buffer * kBuffer + kKeyTile;
-        const int chunk = value_chunk();  // (the loads' places)
-        const int there = ok >> chunk & 1u ? t.length - k0 - chunk * (16 / kBytes) : 0;
-        uint32_t odd = 0;
+    // The values that this wave loaded of a tile at an edge of some row's keys: those of keys
+    // that do not exist hold anything and are cleared, infinities and NaN are taken out.
+    __device__ __forceinline__ void tidy_values(int block, uint32_t ok, Odd<kD, kChunkRows>& odd) const {
+        if (kSplit && wave < kKeyUnits) return;
+        uint8_t* vt = lds + buffer_of(block) * kBuffer + kKeyTile + here(lane) * 16;
+        const int chunk = here(value_chunk()), key = block * kTileKeys + chunk * (16 / kBytes), there = ok >> chunk & 1u ? t.length - key : 0;
+        const int tile_row0 = row0 - 32 * wave;
+        const auto seen = [&](int r, int& from, int& to) {
+            from = to = 0;
+            if (tile_row0 + r < t.rows) window(a, t.first_pos + (tile_row0 + r) / a.group, t.length, from, to);
+        };
 #pragma unroll
         for (int i = 0; i < kValueLoads; ++i) {
-            uint4* p = (uint4*)(vt + (wave * kValueLoads + i) * 1024) + lane;
+            uint4* p = (uint4*)(vt + value_unit(i) * 1024);
             const uint4 old = *p;
             uint32_t w[4] = {old.x, old.y, old.z, old.w};
             constexpr int kPerWord = 4 / kBytes;
@@ -200,73 +241,14 @@ template <int kD, bool kF8> struct ChunkPass {
                 const int n = there - j * kPerWord;  // keys of this word that exist
                 w[j] &= n >= kPerWord ? 0xffffffffu : (n <= 0 ? 0u : (1u << (8 * kBytes * n)) - 1u);
             }
-            const uint4 now{w[0], w[1], w[2], w[3]};
-            odd |= not_finite<kF8>(now);
+            uint4 now{w[0], w[1], w[2], w[3]};
+            odd.template take<kF8>(now, value_unit(i) * (64 / kValueChunks) + here(lane) / kValueChunks, key, seen);
             *p = now;
         }
-        return __syncthreads_or(odd != 0) != 0;
     }
 
-    // For such a tile: which of the lane's outputs become NaN, +inf and -inf, counted over
-    // the keys its row sees, into LDS; then the values are cleared of them (all waves).
-    __device__ __forceinline__ void take_out_odd(int block, int buffer, uint32_t ok, uint32_t (*marks)[6]) {
-        const uint8_t* vt = lds + buffer * kBuffer + kKeyTile;
-#pragma unroll 1
-        for (int kind = 0; kind < (kF8 ? 1 : 3); ++kind) {
-#pragma unroll 1
-            for (int half = 0; half < kBlocks; half += 2) {
-                uint32_t mark = 0;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int d = 32 * (half + e) + l32;
-                    v16f count{};
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        const uint4 r = *(const uint4*)(vt + d * kValueBytes + ((kF8 ? 2 * (s >> 1) + h : 2 * s + h) ^ value_swizzle(d)) * 16);
-                        const uint4 ones{odd_ones<kF8>(r.x, kind), odd_ones<kF8>(r.y, kind), odd_ones<kF8>(r.z, kind), odd_ones<kF8>(r.w, kind)};
-                        const uint32_t seen = sees(block * kTileKeys, s, ok);
-                        uint32_t vis[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) vis[i] = ((seen >> (2 * i) & 1u) | (seen >> (2 * i + 1) & 1u) << 16) * 0x3c00u;
-                        count = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<kF8>(ones, s & 1), __builtin_bit_cast(v8h, uint4{vis[0], vis[1], vis[2], vis[3]}),
-                                                                       count, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) mark |= (uint32_t)(count[i] > 0.0f) << (16 * e + i);
-                }
-                marks[threadIdx.x][2 * kind + half / 2] = mark;
-            }
-        }
-        __syncthreads();  // the values are read
-#pragma unroll
-        for (int i = 0; i < kValueLoads; ++i) {
-            uint4* p = (uint4*)(lds + buffer * kBuffer + kKeyTile + (wave * kValueLoads + i) * 1024) + lane;
-            const uint4 v = *p;
-            *p = uint4{odd_cleared<kF8>(v.x), odd_cleared<kF8>(v.y), odd_cleared<kF8>(v.z), odd_cleared<kF8>(v.w)};
-        }
-        __syncthreads();
-    }
-    __device__ __forceinline__ void put_odd(const uint32_t (*marks)[6]) {
-#pragma unroll
-        for (int kind = 0; kind < (kF8 ? 1 : 3); ++kind) {
-            const float add = kind == 0 ? __builtin_nanf("") : (kind == 1 ? __builtin_inff() : -__builtin_inff());
-#pragma unroll
-            for (int half = 0; half < kBlocks; half += 2) {
-                const uint32_t mark = marks[threadIdx.x][2 * kind + half / 2];
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (mark >> i & 1u) acc[half + (i >> 4)][i & 15] += add;
-            }
-        }
-    }
-
-    __device__ __forceinline__ void multiply(int block, int buffer, uint32_t ok) {
-        const int k0 = block * kTileKeys;
-        if (k0 >= wave_hi || k0 + kTileKeys <= wave_lo) return;
-        const uint8_t* kt = lds + buffer * kBuffer;
-        const uint8_t* vt = kt + kKeyTile;
-
-        v16f sc[2];
+    __device__ __forceinline__ void scores(int block, v16f (&sc)[2]) const {
+        const uint8_t* kt = lds + buffer_of(block) * kBuffer;
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
             // row m of the MFMA is the key whose score lands in place: see step_key
@@ -283,17 +265,18 @@ template <int kD, bool kF8> struct ChunkPass {
                     sc[blk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<kF8>(raw, e), qf[s + e], sc[blk], 0, 0, 0);
             }
         }
-
-        const bool whole = k0 >= full_lo && k0 + kTileKeys <= full_hi && ok == kAllPages;
-        if (!whole) {
+    }
+    __device__ __forceinline__ void mask(int block, uint32_t ok, v16f (&sc)[2]) const {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const uint32_t seen = sees(k0, s, ok);
+        for (int s = 0; s < 4; ++s) {
+            const uint32_t seen = sees(block * kTileKeys, s, ok);
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (!(seen >> j & 1u)) sc[s >> 1][8 * (s & 1) + j] = kNegInf;
-            }
+            for (int j = 0; j < 8; ++j)
+                if (!(seen >> j & 1u)) sc[s >> 1][8 * (s & 1) + j] = kNegInf;
         }
+    }
+    // Scores -> probabilities as operands; the sums so far are scaled to the new maximum.
+    __device__ __forceinline__ void soften(const v16f (&sc)[2], v8h (&pf)[4]) {
         float m = __builtin_fmaxf(sc[0][0], sc[1][0]);
 #pragma unroll
         for (int j = 1; j < 16; ++j) m = __builtin_fmaxf(m, __builtin_fmaxf(sc[0][j], sc[1][j]));
@@ -307,7 +290,6 @@ template <int kD, bool kF8> struct ChunkPass {
             for (int c = 0; c < kBlocks; ++c) acc[c] = acc[c] * keep;
         }
         const float base = top == kNegInf ? 0.0f : top * scale;
-        v8h pf[4];
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -316,46 +298,93 @@ template <int kD, bool kF8> struct ChunkPass {
                 total += p;
                 pf[s][j] = (_Float16)p;
             }
-
+    }
+    __device__ __forceinline__ uint4 value_operand(int block, int d, int s) const {
+        return *(const uint4*)(lds + buffer_of(block) * kBuffer + kKeyTile + d * kValueBytes + (((kF8 ? s & ~1 : 2 * s) + h) ^ value_swizzle(d)) * 16);
+    }
+    __device__ __forceinline__ void accumulate(int block, const v8h (&pf)[4]) {
 #pragma unroll
         for (int c = 0; c < kBlocks; ++c) {
-            const int d = 32 * c + l32;
-            const uint8_t* vr = vt + d * kValueBytes;
-            const int swz = value_swizzle(d);
-            uint4 raw[kF8 ? 2 : 4];
+            uint4 raw[4];
 #pragma unroll
-            for (int s = 0; s < (kF8 ? 2 : 4); ++s) raw[s] = *(const uint4*)(vr + ((2 * s + h) ^ swz) * 16);
+            for (int s = 0; s < 4; s += kF8 ? 2 : 1) raw[s] = value_operand(block, 32 * c + l32, s);
 #pragma unroll
             for (int s = 0; s < 4; ++s)
-                acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<kF8>(raw[kF8 ? s >> 1 : s], s & 1), pf[s], acc[c], 0, 0, 0);
+                acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<kF8>(raw[kF8 ? s & ~1 : s], s & 1), pf[s], acc[c], 0, 0, 0);
         }
     }
+    // Loads go out in steps: K(t + 3) and V(t + 2) while tile t is worked on.  Waits until
+    // all but the last `steps` steps (of kLoads a wave) have arrived, which they do in order.
+    template <int steps> __device__ __forceinline__ static void wait_steps(bool more) {
+        if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(steps * kLoads) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    __device__ __forceinline__ static void meet() {
+        __builtin_amdgcn_sched_barrier(0);
+        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+    }
 
-    // Blocks [from, to); `buffer`: the one to fill next, which no wave reads any more.
-    __device__ __forceinline__ void run(int from, int to, int& buffer, uint32_t (*marks)[6]) {
-        Ids id = ids(from), next = ids(from + 1);
-        uint32_t ok = pages_ok(id), next_ok = 0;
-        issue(from, buffer, id);
+    // Tiles [from, to); `tick`: of the first, a number that counts the workgroup's tiles and
+    // gives each its buffer.
+    //
+    // Two waves share a SIMD (w and w + 4); the second four run half a period behind, so
+    // that one's products (the scores of a tile and the output of the one before) run under
+    // the other's softmax and loads.  Buffers: K(t + 3) replaces K(t - 1) and V(t + 2)
+    // replaces V(t - 2) after the meeting that ends tile t's products, when the waves that
+    // are behind are at theirs: they read K(t) and V(t - 1).  The waves that are behind are
+    // at their last products when the others go on to the next tiles' first loads, which
+    // go to other buffers than V(to - 1).
+    __device__ __forceinline__ void run(int from, int to, int& tick, Odd<kD, kChunkRows>& odd) {
+        ring = (tick - from) & (kBuffers - 1);
+        const bool behind = wave >= 4;
+        uint32_t ok[3];  // pages of tiles b, b + 1, b + 2
+        {
+            const Ids v0 = value_ids(from), v1 = value_ids(from + 1);
+            ok[0] = pages_ok(v0);
+            ok[1] = pages_ok(v1);
+            issue_keys(from, key_id(from));
+            if (from + 1 < to) issue_keys(from + 1, key_id(from + 1));
+            issue_values(from, v0);
+            if (from + 2 < to) issue_keys(from + 2, key_id(from + 2));
+            if (from + 1 < to) issue_values(from + 1, v1);
+        }
+        wait_steps<2>(from + 2 < to);
+        meet();
+        if (behind) meet();
+        v16f sc[2];
+        v8h pf[4];
+        bool live = false;  // whether this wave's rows see the tile
+        int kid = key_id(from + 3);
+        Ids vid = value_ids(from + 2);
         for (int b = from; b < to; ++b) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();  // the tile is there, and every wave is done with the other buffer
-            if (b + 1 < to) {
-                next_ok = pages_ok(next);
-                issue(b + 1, buffer ^ 1, next);
-                next = ids(b + 2);
+            const bool sees_any = b * kTileKeys < wave_hi && (b + 1) * kTileKeys > wave_lo;
+            if (sees_any) scores(b, sc);
+            if (live) accumulate(b - 1, pf);
+            live = sees_any;
+            wait_steps<1>(b + 2 < to);
+            const bool edge = b * kTileKeys < tile_full_lo || (b + 1) * kTileKeys > tile_full_hi || ok[0] != kAllPages;
+            if (edge) tidy_values(b, ok[0], odd);
+            meet();
+            if (b + 3 < to) issue_keys(b + 3, kid);
+            if (b + 2 < to) issue_values(b + 2, vid);
+            ok[2] = pages_ok(vid);
+            kid = key_id(b + 4);
+            vid = value_ids(b + 3);
+            if (live) {
+                if (edge && (b * kTileKeys < full_lo || (b + 1) * kTileKeys > full_hi || ok[0] != kAllPages)) mask(b, ok[0], sc);
+                soften(sc, pf);
             }
-            bool odd = false;
-            if (b * kTileKeys < tile_full_lo || (b + 1) * kTileKeys > tile_full_hi || ok != kAllPages) odd = clear_values(b, buffer, ok);
-            if (odd) take_out_odd(b, buffer, ok, marks);
-            multiply(b, buffer, ok);
-            if (odd) put_odd(marks);
-            ok = next_ok;
-            buffer ^= 1;
+            meet();
+            ok[0] = ok[1];
+            ok[1] = ok[2];
         }
+        if (live) accumulate(to - 1, pf);
+        tick += to - from;
+        if (!behind) meet();
     }
-
     // The lane's row (unless it repeats the last) of the output, or of a part.
-    __device__ __forceinline__ void finish(bool whole, Part<kD, kChunkRows>* slot) {
+    __device__ __forceinline__ void finish(bool whole, Part<kD, kChunkRows>* slot, const Odd<kD, kChunkRows>& odd, bool any_odd) {
         int sum_a, sum_b;
         pair_of(__float_as_int(total), 32, sum_a, sum_b);
         const float sum = __int_as_float(sum_a) + __int_as_float(sum_b);
@@ -368,7 +397,8 @@ template <int kD, bool kF8> struct ChunkPass {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int d = 32 * c + 8 * q + 4 * h;
-                const v4f v{acc[c][4 * q], acc[c][4 * q + 1], acc[c][4 * q + 2], acc[c][4 * q + 3]};
+                v4f v{acc[c][4 * q], acc[c][4 * q + 1], acc[c][4 * q + 2], acc[c][4 * q + 3]};
+                if (__builtin_expect(any_odd, 0)) v = v4f{odd.put(v[0], r, d), odd.put(v[1], r, d + 1), odd.put(v[2], r, d + 2), odd.put(v[3], r, d + 3)};
                 if (whole)
                     *(uint2*)(op + d) = uint2{(uint32_t)f2h(v[0] * inv) | ((uint32_t)f2h(v[1] * inv) << 16),
                                               (uint32_t)f2h(v[2] * inv) | ((uint32_t)f2h(v[3] * inv) << 16)};
@@ -382,33 +412,36 @@ template <int kD, bool kF8> struct ChunkPass {
     }
 };
 
-// Short contexts: a workgroup for all keys of a (sequence, kv head, 128 rows).
-template <int kD, bool kF8> __global__ __launch_bounds__(256, 2) void paged_chunks_direct_kernel(PagedArgs a) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * ChunkPass<kD, kF8>::kBuffer];
-    __shared__ uint32_t marks[256][6];
+// Short contexts: a workgroup for all keys of a (sequence, kv head, 256 rows).
+template <int kD, bool kF8> __global__ __launch_bounds__(kChunkThreads, 2) void paged_chunks_direct_kernel(PagedArgs a) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kBuffers * ChunkPass<kD, kF8>::kBuffer];
+    __shared__ Odd<kD, kChunkRows> odd;
+    odd.clear(kChunkThreads);
     const int kvh = blockIdx.x, seq = blockIdx.z, tile = blockIdx.y;
     const RowTile t = wave_sequence(a, seq);
     if (tile * kChunkRows >= t.rows) return;
-    int first, buffer = 0;
+    int first, tick = 0;
     const int blocks = chunk_blocks(a, t, tile, first);
     ChunkPass<kD, kF8> pass(a, lds, kvh);
     pass.start(seq, t, tile);
-    pass.run(first, first + blocks, buffer, marks);
-    pass.finish(true, nullptr);
+    pass.run(first, first + blocks, tick, odd);
+    __syncthreads();
+    pass.finish(true, nullptr, odd, odd.any != 0);
 }
 
 template <int kD, bool kF8>
-__global__ __launch_bounds__(256, 2) void paged_chunks_shares_kernel(PagedArgs a, Part<kD, kChunkRows>* slots, Join* joins) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * ChunkPass<kD, kF8>::kBuffer];
-    __shared__ uint32_t marks[256][6];
+__global__ __launch_bounds__(kChunkThreads, 2) void paged_chunks_shares_kernel(PagedArgs a, Part<kD, kChunkRows>* slots, Join* joins) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kBuffers * ChunkPass<kD, kF8>::kBuffer];
+    __shared__ Odd<kD, kChunkRows> odd;
+    odd.clear(kChunkThreads);
     // neighbouring shares read the same keys: they go to one XCD's L2
     const int index = (blockIdx.x & 7) * (kChunkShares / 8) + (blockIdx.x >> 3);
     if (threadIdx.x == 0) joins[index].count = 0;
     Share share;
     const auto blocks_of = [&](const RowTile& t) { return pairs_of(a, t).per_head * a.kv_heads; };
-    if (!deal(a, kChunkShares, kLeastChunkShare, index, blocks_of, share)) return;
+    if (!deal<kChunkThreads>(a, kChunkShares, kLeastChunkShare, index, blocks_of, share)) return;
 
-    int seq = share.seq, buffer = 0;
+    int seq = share.seq, tick = 0;
     long long at = share.from, offset = share.offset;  // offset: of `at` in the sequence's blocks
     while (at < share.to) {
         const RowTile t = wave_sequence(a, seq);
@@ -435,9 +468,15 @@ __global__ __launch_bounds__(256, 2) void paged_chunks_shares_kernel(PagedArgs a
                 const int tile = second ? p.tiles - 1 - pair : pair, first = (second ? first_b : first_a) + b0;
                 ChunkPass<kD, kF8> pass(a, lds, kvh);
                 pass.start(seq, t, tile);
-                pass.run(first, first + n, buffer, marks);
+                pass.run(first, first + n, tick, odd);
+                __syncthreads();
                 const int which = at == share.from ? 0 : 1;
-                pass.finish(n == blocks, slots + 2 * index + which);
+                const bool any_odd = __builtin_amdgcn_readfirstlane((int)odd.any) != 0;
+                pass.finish(n == blocks, slots + 2 * index + which, odd, any_odd);
+                if (any_odd) {
+                    __syncthreads();
+                    odd.clear(kChunkThreads);
+                }
                 if (n != blocks && b0 == 0 && threadIdx.x == 0)
                     joins[index] = {t.start, t.rows, kvh, tile * kChunkRows, (int)((at + blocks - 1) / share.size - index) + 1, which, {}};
             }
@@ -510,12 +549,12 @@ template <int kD, bool kF8> static void launch_chunks(const PagedArgs& a, bool d
     const int rows = max_queries * a.group;
     if (direct) {
         const dim3 grid((unsigned)a.kv_heads, (unsigned)((rows + kChunkRows - 1) / kChunkRows), (unsigned)a.sequences);
-        paged_chunks_direct_kernel<kD, kF8><<<grid, 256, 0, s>>>(a);
+        paged_chunks_direct_kernel<kD, kF8><<<grid, kChunkThreads, 0, s>>>(a);
         return;
     }
     auto* slots = (Part<kD, kChunkRows>*)workspace;
     Join* joins = (Join*)(slots + 2 * kChunkShares);
-    paged_chunks_shares_kernel<kD, kF8><<<kChunkShares, 256, 0, s>>>(a, slots, joins);
+    paged_chunks_shares_kernel<kD, kF8><<<kChunkShares, kChunkThreads, 0, s>>>(a, slots, joins);
     const int part_rows = rows < kChunkRows ? rows : kChunkRows;
     paged_chunks_join_kernel<kD><<<dim3(kChunkShares, (unsigned)((part_rows + 15) / 16)), 16 * kD / 4, 0, s>>>(a, slots, joins);
 }
