@@ -247,25 +247,6 @@ template <int kD, bool kF8> struct ChunkPass {
         }
     }
 
-    __device__ __forceinline__ void scores(int block, v16f (&sc)[2]) const {
-        const uint8_t* kt = lds + buffer_of(block) * kBuffer;
-#pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
-            // row m of the MFMA is the key whose score lands in place: see step_key
-            const int m = l32, quad = (m >> 3) & 3, half = (m >> 2) & 1, b = m & 3;
-            const int key = 32 * blk + (kF8 ? 16 * half + 8 * (quad >> 1) : 16 * (quad >> 1) + 8 * half) + 4 * (quad & 1) + b;
-            const uint8_t* kr = kt + key * kKeyBytes;
-            const int swz = key_swizzle(key);
-            sc[blk] = v16f{};
-#pragma unroll
-            for (int s = 0; s < kSteps; s += kF8 ? 2 : 1) {
-                const uint4 raw = *(const uint4*)(kr + (((kF8 ? s : 2 * s) + h) ^ swz) * 16);
-#pragma unroll
-                for (int e = 0; e < (kF8 ? 2 : 1); ++e)
-                    sc[blk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<kF8>(raw, e), qf[s + e], sc[blk], 0, 0, 0);
-            }
-        }
-    }
     __device__ __forceinline__ void mask(int block, uint32_t ok, v16f (&sc)[2]) const {
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
@@ -299,20 +280,49 @@ template <int kD, bool kF8> struct ChunkPass {
                 pf[s][j] = (_Float16)p;
             }
     }
-    __device__ __forceinline__ uint4 value_operand(int block, int d, int s) const {
-        return *(const uint4*)(lds + buffer_of(block) * kBuffer + kKeyTile + d * kValueBytes + (((kF8 ? s & ~1 : 2 * s) + h) ^ value_swizzle(d)) * 16);
-    }
-    __device__ __forceinline__ void accumulate(int block, const v8h (&pf)[4]) {
+    // The scores of tile `block` and (or) the output of the tile before it, LDS reads
+    // kAhead operands ahead of the products: one at a time, each is waited for in full (the
+    // order is pinned because the compiler brings them together again).
+    static constexpr int kAhead = 6;
+    template <bool kScores, bool kOutput> __device__ __forceinline__ void products(int block, v16f (&sc)[2], const v8h (&pf)[4]) {
+        constexpr int kPer = kF8 ? 2 : 1;  // products an operand's 16 bytes feed
+        constexpr int kScoreReads = kScores ? 2 * kSteps / kPer : 0, kReads = kScoreReads + (kOutput ? 4 * kBlocks / kPer : 0);
+        const uint8_t* kt = lds + buffer_of(block) * kBuffer;
+        const uint8_t* vt = lds + buffer_of(block - 1) * kBuffer + kKeyTile;
+        // row m of the MFMA is the key whose score lands in place: see step_key
+        const int quad = (l32 >> 3) & 3, half = (l32 >> 2) & 1;
+        const int key0 = (kF8 ? 16 * half + 8 * (quad >> 1) : 16 * (quad >> 1) + 8 * half) + 4 * (quad & 1) + (l32 & 3);
+        const auto read = [&](int i) {
+            if (i < kScoreReads) {
+                const int key = key0 + 32 * (i / (kSteps / kPer)), s = i % (kSteps / kPer);
+                return *(const uint4*)(kt + key * kKeyBytes + ((2 * s + h) ^ key_swizzle(key)) * 16);
+            }
+            const int j = i - kScoreReads, d = l32 + 32 * (j / (4 / kPer)), s = j % (4 / kPer);
+            return *(const uint4*)(vt + d * kValueBytes + ((2 * s + h) ^ value_swizzle(d)) * 16);
+        };
+        if constexpr (kScores) sc[0] = sc[1] = v16f{};
+        uint4 raw[kAhead];
 #pragma unroll
-        for (int c = 0; c < kBlocks; ++c) {
-            uint4 raw[4];
+        for (int i = 0; i < kAhead; ++i) raw[i] = read(i);
 #pragma unroll
-            for (int s = 0; s < 4; s += kF8 ? 2 : 1) raw[s] = value_operand(block, 32 * c + l32, s);
+        for (int i = 0; i < kReads; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-                acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<kF8>(raw[kF8 ? s & ~1 : s], s & 1), pf[s], acc[c], 0, 0, 0);
+            for (int e = 0; e < kPer; ++e) {
+                const v8h first = operand<kF8>(raw[i % kAhead], e);
+                if (i < kScoreReads) {
+                    const int blk = i / (kSteps / kPer);
+                    sc[blk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(first, qf[i % (kSteps / kPer) * kPer + e], sc[blk], 0, 0, 0);
+                } else {
+                    const int j = i - kScoreReads, c = j / (4 / kPer);
+                    acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(first, pf[j % (4 / kPer) * kPer + e], acc[c], 0, 0, 0);
+                }
+            }
+            if (i + kAhead < kReads) raw[i % kAhead] = read(i + kAhead);
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
+
     // Loads go out in steps: K(t + 3) and V(t + 2) while tile t is worked on.  Waits until
     // all but the last `steps` steps (of kLoads a wave) have arrived, which they do in order.
     template <int steps> __device__ __forceinline__ static void wait_steps(bool more) {
@@ -352,16 +362,13 @@ template <int kD, bool kF8> struct ChunkPass {
         wait_steps<2>(from + 2 < to);
         meet();
         if (behind) meet();
+        const bool active = last >= 0;
         v16f sc[2];
         v8h pf[4];
-        bool live = false;  // whether this wave's rows see the tile
         int kid = key_id(from + 3);
         Ids vid = value_ids(from + 2);
+        if (active) products<true, false>(from, sc, pf);
         for (int b = from; b < to; ++b) {
-            const bool sees_any = b * kTileKeys < wave_hi && (b + 1) * kTileKeys > wave_lo;
-            if (sees_any) scores(b, sc);
-            if (live) accumulate(b - 1, pf);
-            live = sees_any;
             wait_steps<1>(b + 2 < to);
             const bool edge = b * kTileKeys < tile_full_lo || (b + 1) * kTileKeys > tile_full_hi || ok[0] != kAllPages;
             if (edge) tidy_values(b, ok[0], odd);
@@ -371,18 +378,21 @@ template <int kD, bool kF8> struct ChunkPass {
             ok[2] = pages_ok(vid);
             kid = key_id(b + 4);
             vid = value_ids(b + 3);
-            if (live) {
+            if (active) {
+                // a tile that none of the wave's rows sees has probabilities of zero and tidy values
                 if (edge && (b * kTileKeys < full_lo || (b + 1) * kTileKeys > full_hi || ok[0] != kAllPages)) mask(b, ok[0], sc);
                 soften(sc, pf);
             }
             meet();
             ok[0] = ok[1];
             ok[1] = ok[2];
+            if (b + 1 < to && active) products<true, true>(b + 1, sc, pf);
         }
-        if (live) accumulate(to - 1, pf);
+        if (active) products<false, true>(to, sc, pf);
         tick += to - from;
         if (!behind) meet();
     }
+
     // The lane's row (unless it repeats the last) of the output, or of a part.
     __device__ __forceinline__ void finish(bool whole, Part<kD, kChunkRows>* slot, const Odd<kD, kChunkRows>& odd, bool any_odd) {
         int sum_a, sum_b;
