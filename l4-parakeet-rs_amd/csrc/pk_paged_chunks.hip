@@ -256,16 +256,29 @@ template <int kD, bool kF8> struct ChunkPass {
                 if (!(seen >> j & 1u)) sc[s >> 1][8 * (s & 1) + j] = kNegInf;
         }
     }
+    // The largest of three, in one instruction: the compiler's own form of it first passes
+    // products of the MFMA through another maximum each, for signalling NaN.  (A NaN among
+    // the scores comes through the exponentials.)
+    __device__ __forceinline__ static float max3(float x, float y, float z) {
+        float r;
+        asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+        return r;
+    }
+    // Scores are taken relative to a running maximum that is only raised where a row's
+    // falls kSlack short (factors of two): probabilities up to 2^8 are as exact in fp16 and
+    // fp32 as those up to 1, and the output so far is rarely rescaled.
+    static constexpr float kSlack = 8.0f;
     // Scores -> probabilities as operands; the sums so far are scaled to the new maximum.
     __device__ __forceinline__ void soften(const v16f (&sc)[2], v8h (&pf)[4]) {
-        float m = __builtin_fmaxf(sc[0][0], sc[1][0]);
+        float m = max3(sc[0][0], sc[0][1], sc[1][0]);
+        m = max3(m, sc[1][1], kNegInf);
 #pragma unroll
-        for (int j = 1; j < 16; ++j) m = __builtin_fmaxf(m, __builtin_fmaxf(sc[0][j], sc[1][j]));
+        for (int j = 2; j < 16; ++j) m = max3(m, sc[0][j], sc[1][j]);
         m = max_level(m, 32);
-        if (__any(m > top)) {  // else every factor is 1
-            const float new_top = __builtin_fmaxf(top, m);
-            const float keep = new_top == kNegInf ? 1.0f : __builtin_amdgcn_exp2f((top - new_top) * scale);
-            top = new_top;
+        const bool far = (m - top) * scale > kSlack;  // also from -inf; false while nothing is seen
+        if (__any(far)) {
+            const float keep = far ? __builtin_amdgcn_exp2f((top - m) * scale) : 1.0f;
+            top = far ? m : top;
             total *= keep;
 #pragma unroll
             for (int c = 0; c < kBlocks; ++c) acc[c] = acc[c] * keep;
@@ -320,6 +333,8 @@ template <int kD, bool kF8> struct ChunkPass {
             }
             if (i + kAhead < kReads) raw[i % kAhead] = read(i + kAhead);
         }
+        // the scores are next read by max3, before which the compiler places no wait for the MFMA
+        if constexpr (kScores && !kOutput) asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     }
 
