@@ -136,16 +136,17 @@ __device__ __forceinline__ void store_row(const PagedArgs& a, const RowTile& t, 
 
 // The work of all sequences in a row, in blocks of keys, dealt to `shares` workgroups in
 // equal contiguous shares: every workgroup (kThreads threads) sums the blocks of all
-// sequences and finds the sequence that its share begins in.
+// sequences and finds the sequences that its share begins and ends in.
 struct Share {
     long long from, to, size;  // its blocks, and the blocks of a full share
     long long offset;          // blocks of `seq` before `from`
-    int seq;
+    long long last_offset;     // and of `last_seq` before `to` - 1
+    int seq, last_seq;
 };
 
 template <int kThreads, class Blocks> __device__ __forceinline__ bool deal(const PagedArgs& a, int shares, int least, int index, Blocks blocks_of, Share& out) {
-    __shared__ long long wave_total[kThreads / 64], found_offset;
-    __shared__ int found_seq;
+    __shared__ long long wave_total[kThreads / 64], found_offset[2];
+    __shared__ int found_seq[2];
     const int per = (a.sequences + kThreads - 1) / kThreads, s0 = threadIdx.x * per;
     long long mine = 0;
     for (int s = s0; s < s0 + per && s < a.sequences; ++s) mine += blocks_of(sequence_of(a, s));
@@ -166,21 +167,27 @@ template <int kThreads, class Blocks> __device__ __forceinline__ bool deal(const
     out.from = index * out.size;
     out.to = out.from + out.size < all ? out.from + out.size : all;
     if (out.from >= all) return false;
-    if (end - mine <= out.from && out.from < end) {
+    const long long last = out.to - 1;
+    if (end - mine <= last && out.from < end) {  // this thread's sequences hold blocks of the share
         long long at = end - mine;
-        for (int s = s0;; ++s) {
+        for (int s = s0; s < s0 + per && s < a.sequences; ++s) {
             const long long n = blocks_of(sequence_of(a, s));
-            if (out.from < at + n) {
-                found_seq = s;
-                found_offset = out.from - at;
-                break;
+            if (at <= out.from && out.from < at + n) {
+                found_seq[0] = s;
+                found_offset[0] = out.from - at;
+            }
+            if (at <= last && last < at + n) {
+                found_seq[1] = s;
+                found_offset[1] = last - at;
             }
             at += n;
         }
     }
     __syncthreads();
-    out.seq = __builtin_amdgcn_readfirstlane(found_seq);
-    out.offset = uniform(found_offset);
+    out.seq = __builtin_amdgcn_readfirstlane(found_seq[0]);
+    out.offset = uniform(found_offset[0]);
+    out.last_seq = __builtin_amdgcn_readfirstlane(found_seq[1]);
+    out.last_offset = uniform(found_offset[1]);
     return true;
 }
 

@@ -78,6 +78,7 @@ template <int kD, bool kF8> struct ChunkPass {
     int last_page, ring;      // ring: tile b lies in buffer (b + ring) mod kBuffers
     int row0, last, row;      // this wave's first row, its last row's index (< 0: none), this lane's row
     int lo, hi, full_lo, full_hi, wave_lo, wave_hi;
+    uint32_t key_off[kKeyLoads], value_off[kValueLoads];
     int tile_full_lo, tile_full_hi;  // keys that all of the workgroup's rows see
     float scale, sign;
     v8h qf[kSteps];
@@ -90,6 +91,7 @@ template <int kD, bool kF8> struct ChunkPass {
         // product; 0 becomes tiny, so that -inf stays -inf
         sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
         scale = __builtin_fmaxf(__builtin_fabsf(a.scale_log2), 1e-30f);
+        place_loads();
     }
 
     __device__ __forceinline__ void start(int seq, const RowTile& rows, int tile) {
@@ -136,10 +138,16 @@ template <int kD, bool kF8> struct ChunkPass {
         const int c = key >> a.shift;
         return ((ScalarTable)(uintptr_t)table)[__builtin_amdgcn_readfirstlane(c > last_page ? last_page : c)];
     }
-    __device__ __forceinline__ int key_id(int block) const { return page_at(block * kTileKeys + (kKeyRun * wave & (kTileKeys - 1))); }
-    __device__ __forceinline__ Ids value_ids(int block) const {
+    __device__ __forceinline__ Ids tile_ids(int block) const {
         const int k0 = block * kTileKeys;
-        return {{page_at(k0), page_at(k0 + 16), page_at(k0 + 32), page_at(k0 + 48)}};
+        Ids r;
+        r.page[0] = r.page[1] = r.page[2] = r.page[3] = page_at(k0);
+        if (a.shift < 6) {  // else a tile lies in one page
+            r.page[1] = page_at(k0 + 16);
+            r.page[2] = page_at(k0 + 32);
+            r.page[3] = page_at(k0 + 48);
+        }
+        return r;
     }
     // Of one of the groups, chosen by the wave or by a lane.
     __device__ __forceinline__ static int pick(const Ids& id, int group) {
@@ -172,34 +180,55 @@ template <int kD, bool kF8> struct ChunkPass {
     }
     __device__ __forceinline__ size_t page_of(int id) const {
         id = (unsigned)id < (unsigned)a.pages ? id : 0;
-        return ((size_t)id * a.kv_heads + kvh) * ((size_t)kD * kBytes << a.shift);
+        return ((size_t)id * a.kv_heads + kvh) << (a.shift + (kD == 128 ? 7 : 6) + (kF8 ? 0 : 1));
     }
     __device__ __forceinline__ int buffer_of(int block) const { return (block + ring) & (kBuffers - 1); }
     __device__ __forceinline__ uint32_t lds_of(int block) const {
         return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + buffer_of(block) * kBuffer;
     }
-    __device__ __forceinline__ void issue_keys(int block, int id) const {
-        if (kSplit && wave >= kKeyUnits) return;
-        const uint8_t* kp = a.key + page_of(id);  // a wave's keys lie in one page
-        const int k0 = block * kTileKeys, in_page = (1 << a.shift) - 1;
-        const uint32_t base = lds_of(block);
+    // Where the lane's loads lie, from the wave's first key (one page) or the first value of
+    // its place in a page on: the same for every tile.
+    __device__ __forceinline__ void place_loads() {
 #pragma unroll
         for (int i = 0; i < kKeyLoads; ++i) {
-            const int unit = wave * kKeyLoads + i, slot = unit * 64 + lane, key = slot / kKeyChunks;
-            const int chunk = (slot & (kKeyChunks - 1)) ^ key_swizzle(key);
-            dma16(kp + ((k0 + key) & in_page) * kKeyBytes + chunk * 16, base + unit * 1024);
+            const int slot = (wave * kKeyLoads + i) * 64 + lane, key = slot / kKeyChunks;
+            key_off[i] = (uint32_t)((key & (kKeyRun - 1)) * kKeyBytes + ((slot & (kKeyChunks - 1)) ^ key_swizzle(key)) * 16);
         }
-    }
-    __device__ __forceinline__ void issue_values(int block, const Ids& id) const {
-        if (kSplit && wave < kKeyUnits) return;
-        const int chunk = value_chunk(), k0 = block * kTileKeys, in_page = (1 << a.shift) - 1;
-        const uint8_t* vp = a.value + page_of(pick(id, chunk * 4 / kValueChunks)) + ((k0 + chunk * (16 / kBytes)) & in_page) * kBytes;
-        const uint32_t base = lds_of(block) + kKeyTile;
 #pragma unroll
         for (int i = 0; i < kValueLoads; ++i) {
-            const int unit = value_unit(i), d = unit * (64 / kValueChunks) + lane / kValueChunks;
-            dma16(vp + ((size_t)(d * kBytes) << a.shift), base + unit * 1024);
+            const int d = value_unit(i) * (64 / kValueChunks) + lane / kValueChunks;
+            value_off[i] = (uint32_t)(((d * kBytes) << a.shift) + (value_chunk() * 16 & ((kBytes << a.shift) - 1)));
         }
+    }
+    // The wave's loads of a step, one by one: the keys of a tile, then the values of another.
+    struct Step {
+        bool keys, values;
+        const uint8_t *key, *value;  // value: the lane's where its place decides the page, else the wave's
+        uint32_t key_lds, value_lds;
+    };
+    __device__ __forceinline__ Step step_of(int key_block, const Ids& key_ids, int value_block, const Ids& value_ids, int to) const {
+        Step s;
+        s.keys = key_block < to && !(kSplit && wave >= kKeyUnits);
+        s.values = value_block < to && !(kSplit && wave < kKeyUnits);
+        const int run = kKeyRun * wave, in_page = (1 << a.shift) - 1;
+        s.key = a.key + page_of(pick(key_ids, run / 16)) + ((key_block * kTileKeys + run) & in_page) * kKeyBytes;
+        s.value = a.value + (a.shift >= 6 ? page_of(value_ids.page[0]) + ((value_block * kTileKeys) & in_page) * kBytes
+                                          : page_of(pick(value_ids, value_chunk() * 4 / kValueChunks)));
+        s.key_lds = lds_of(key_block) + wave * kKeyLoads * 1024;
+        s.value_lds = lds_of(value_block) + kKeyTile + value_unit(0) * 1024;
+        return s;
+    }
+    __device__ __forceinline__ void load_keys(const Step& s, int i) const {
+        if (s.keys) dma16(s.key, key_off[i], s.key_lds + i * 1024);
+    }
+    __device__ __forceinline__ void load_values(const Step& s, int i) const {
+        if (s.values) dma16(s.value + value_off[i], s.value_lds + i * kChunkWaves * 1024);
+    }
+    __device__ __forceinline__ void load_all(const Step& s) const {
+#pragma unroll
+        for (int i = 0; i < kKeyLoads; ++i) load_keys(s, i);
+#pragma unroll
+        for (int i = 0; i < kValueLoads; ++i) load_values(s, i);
     }
 
     // First of the 8 consecutive keys of step s (of 4) that this lane holds scores of.
@@ -297,7 +326,7 @@ template <int kD, bool kF8> struct ChunkPass {
     // kAhead operands ahead of the products: one at a time, each is waited for in full (the
     // order is pinned because the compiler brings them together again).
     static constexpr int kAhead = 6;
-    template <bool kScores, bool kOutput> __device__ __forceinline__ void products(int block, v16f (&sc)[2], const v8h (&pf)[4]) {
+    template <bool kScores, bool kOutput> __device__ __forceinline__ void products(int block, v16f (&sc)[2], const v8h (&pf)[4], const Step& step) {
         constexpr int kPer = kF8 ? 2 : 1;  // products an operand's 16 bytes feed
         constexpr int kScoreReads = kScores ? 2 * kSteps / kPer : 0, kReads = kScoreReads + (kOutput ? 4 * kBlocks / kPer : 0);
         const uint8_t* kt = lds + buffer_of(block) * kBuffer;
@@ -332,13 +361,21 @@ template <int kD, bool kF8> struct ChunkPass {
                 }
             }
             if (i + kAhead < kReads) raw[i % kAhead] = read(i + kAhead);
+            if constexpr (kScores) {  // the step's loads, spread over the products
+                constexpr int kEvery = kReads / (kKeyLoads + kValueLoads);
+                const int n = i / kEvery;
+                if (i % kEvery == kEvery / 2 && n < kKeyLoads + kValueLoads) {
+                    if (n < kKeyLoads) load_keys(step, n);
+                    else load_values(step, n - kKeyLoads);
+                }
+            }
         }
         // the scores are next read by max3, before which the compiler places no wait for the MFMA
         if constexpr (kScores && !kOutput) asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    // Loads go out in steps: K(t + 3) and V(t + 2) while tile t is worked on.  Waits until
+    // Loads go out in steps: K(t + 3) and V(t + 2) among tile t's products.  Waits until
     // all but the last `steps` steps (of kLoads a wave) have arrived, which they do in order.
     template <int steps> __device__ __forceinline__ static void wait_steps(bool more) {
         if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(steps * kLoads) : "memory");
@@ -355,24 +392,24 @@ template <int kD, bool kF8> struct ChunkPass {
     //
     // Two waves share a SIMD (w and w + 4); the second four run half a period behind, so
     // that one's products (the scores of a tile and the output of the one before) run under
-    // the other's softmax and loads.  Buffers: K(t + 3) replaces K(t - 1) and V(t + 2)
-    // replaces V(t - 2) after the meeting that ends tile t's products, when the waves that
-    // are behind are at theirs: they read K(t) and V(t - 1).  The waves that are behind are
+    // the other's softmax.  Buffers: K(t + 3) replaces K(t - 1) and V(t + 2) replaces
+    // V(t - 2) during tile t's products, which read K(t) and V(t - 1); the other waves are
+    // at that tile's softmax, or at the softmax before.  The waves that are behind are
     // at their last products when the others go on to the next tiles' first loads, which
     // go to other buffers than V(to - 1).
     __device__ __forceinline__ void run(int from, int to, int& tick, Odd<kD, kChunkRows>& odd) {
         ring = (tick - from) & (kBuffers - 1);
         const bool behind = wave >= 4;
         uint32_t ok[3];  // pages of tiles b, b + 1, b + 2
+        Ids ids = tile_ids(from + 2), next = tile_ids(from + 3);  // of tiles b + 2 and b + 3
         {
-            const Ids v0 = value_ids(from), v1 = value_ids(from + 1);
-            ok[0] = pages_ok(v0);
-            ok[1] = pages_ok(v1);
-            issue_keys(from, key_id(from));
-            if (from + 1 < to) issue_keys(from + 1, key_id(from + 1));
-            issue_values(from, v0);
-            if (from + 2 < to) issue_keys(from + 2, key_id(from + 2));
-            if (from + 1 < to) issue_values(from + 1, v1);
+            const Ids first = tile_ids(from), second = tile_ids(from + 1);
+            ok[0] = pages_ok(first);
+            ok[1] = pages_ok(second);
+            Step s = step_of(from, first, to, first, to);
+            load_all(s);
+            load_all(step_of(from + 1, second, from, first, to));
+            load_all(step_of(from + 2, ids, from + 1, second, to));
         }
         wait_steps<2>(from + 2 < to);
         meet();
@@ -380,30 +417,32 @@ template <int kD, bool kF8> struct ChunkPass {
         const bool active = last >= 0;
         v16f sc[2];
         v8h pf[4];
-        int kid = key_id(from + 3);
-        Ids vid = value_ids(from + 2);
-        if (active) products<true, false>(from, sc, pf);
+        Step step = step_of(from + 3, next, from + 2, ids, to);
+        if (active) products<true, false>(from, sc, pf, step);
+        else load_all(step);
         for (int b = from; b < to; ++b) {
-            wait_steps<1>(b + 2 < to);
+            wait_steps<2>(b + 3 < to);
             const bool edge = b * kTileKeys < tile_full_lo || (b + 1) * kTileKeys > tile_full_hi || ok[0] != kAllPages;
             if (edge) tidy_values(b, ok[0], odd);
             meet();
-            if (b + 3 < to) issue_keys(b + 3, kid);
-            if (b + 2 < to) issue_values(b + 2, vid);
-            ok[2] = pages_ok(vid);
-            kid = key_id(b + 4);
-            vid = value_ids(b + 3);
+            ok[2] = pages_ok(ids);
+            ids = next;
+            next = tile_ids(b + 4);
             if (active) {
                 // a tile that none of the wave's rows sees has probabilities of zero and tidy values
                 if (edge && (b * kTileKeys < full_lo || (b + 1) * kTileKeys > full_hi || ok[0] != kAllPages)) mask(b, ok[0], sc);
                 soften(sc, pf);
             }
+            step = step_of(b + 4, next, b + 3, ids, to);
             meet();
             ok[0] = ok[1];
             ok[1] = ok[2];
-            if (b + 1 < to && active) products<true, true>(b + 1, sc, pf);
+            if (b + 1 < to) {
+                if (active) products<true, true>(b + 1, sc, pf, step);
+                else load_all(step);
+            }
         }
-        if (active) products<false, true>(to, sc, pf);
+        if (active) products<false, true>(to, sc, pf, step);
         tick += to - from;
         if (!behind) meet();
     }
@@ -454,6 +493,34 @@ template <int kD, bool kF8> __global__ __launch_bounds__(kChunkThreads, 2) void 
     pass.finish(true, nullptr, odd, odd.any != 0);
 }
 
+// A row tile's blocks among its sequence's: `tile` < 0 where a pair has blocks too many.
+struct Span {
+    int kvh, tile, first;      // first: the block of keys that the tile begins with
+    int at, blocks;            // the place in the span, and the span's length
+};
+__device__ __forceinline__ Span span_at(const PagedArgs& a, const RowTile& t, const Pairs& p, long long offset) {
+    Span s;
+    s.kvh = (int)(offset / p.per_head);
+    const int in_head = (int)(offset - s.kvh * p.per_head);
+    const int pair = p.pair ? in_head / p.pair : 0;
+    const bool middle = pair == p.tiles / 2;
+    s.tile = pair;
+    s.at = in_head - pair * p.pair;
+    s.blocks = chunk_blocks(a, t, s.tile, s.first);
+    if (!middle && s.at >= s.blocks) {
+        s.at -= s.blocks;
+        const int rest = p.pair - s.blocks;
+        s.tile = p.tiles - 1 - pair;
+        s.blocks = chunk_blocks(a, t, s.tile, s.first);
+        if (s.at >= s.blocks) {
+            s.at -= s.blocks;
+            s.blocks = rest - s.blocks;
+            s.tile = -1;
+        }
+    }
+    return s;
+}
+
 template <int kD, bool kF8>
 __global__ __launch_bounds__(kChunkThreads, 2) void paged_chunks_shares_kernel(PagedArgs a, Part<kD, kChunkRows>* slots, Join* joins) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[kBuffers * ChunkPass<kD, kF8>::kBuffer];
@@ -466,50 +533,61 @@ __global__ __launch_bounds__(kChunkThreads, 2) void paged_chunks_shares_kernel(P
     const auto blocks_of = [&](const RowTile& t) { return pairs_of(a, t).per_head * a.kv_heads; };
     if (!deal<kChunkThreads>(a, kChunkShares, kLeastChunkShare, index, blocks_of, share)) return;
 
-    int seq = share.seq, tick = 0;
-    long long at = share.from, offset = share.offset;  // offset: of `at` in the sequence's blocks
-    while (at < share.to) {
-        const RowTile t = wave_sequence(a, seq);
-        const Pairs p = pairs_of(a, t);
-        const long long all = p.per_head * a.kv_heads;
-        while (offset < all && at < share.to) {
-            const int kvh = (int)(offset / p.per_head);
-            const int in_head = (int)(offset - kvh * p.per_head);
-            const int pair = p.pair ? in_head / p.pair : 0;
-            const bool middle = pair == p.tiles / 2;
-            const int in_pair = in_head - pair * p.pair, pair_blocks = middle ? p.middle : p.pair;
-            int first_a, first_b = 0;
-            const int blocks_a = chunk_blocks(a, t, pair, first_a);
-            const int blocks_b = middle ? 0 : chunk_blocks(a, t, p.tiles - 1 - pair, first_b);
-            // the part of the item at `offset`: its first tile, its second, or what the pair has too many
-            const bool second = in_pair >= blocks_a;
-            const int b0 = second ? in_pair - blocks_a : in_pair, blocks = second ? blocks_b : blocks_a;
-            int n;
-            if (second && b0 >= blocks_b) {
-                n = pair_blocks - in_pair;
-                if (n > share.to - at) n = (int)(share.to - at);
-            } else {
-                n = share.to - at < blocks - b0 ? (int)(share.to - at) : blocks - b0;
-                const int tile = second ? p.tiles - 1 - pair : pair, first = (second ? first_b : first_a) + b0;
-                ChunkPass<kD, kF8> pass(a, lds, kvh);
-                pass.start(seq, t, tile);
-                pass.run(first, first + n, tick, odd);
+    // The beginning of the row tile that the share ends in comes first, then the rest in
+    // order: as shares are equal, the workgroups then stand at about the same keys at the
+    // same time, and find them in their L2.
+    int seq = share.last_seq, tick = 0;
+    RowTile t = wave_sequence(a, seq);
+    Pairs p = pairs_of(a, t);
+    const Span tail = span_at(a, t, p, share.last_offset);
+    const long long head = share.to - 1 - tail.at;  // where that row tile begins
+    const bool first_out = tail.at + 1 < tail.blocks && head > share.from;
+    long long at = first_out ? head : share.from, offset = first_out ? share.last_offset - tail.at : share.offset, to = share.to;
+    if (!first_out && seq != share.seq) {
+        seq = share.seq;
+        t = wave_sequence(a, seq);
+        p = pairs_of(a, t);
+    }
+    for (;;) {
+        const Span s = span_at(a, t, p, offset);
+        const int n = to - at < s.blocks - s.at ? (int)(to - at) : s.blocks - s.at;
+        if (s.tile >= 0) {
+            ChunkPass<kD, kF8> pass(a, lds, s.kvh);
+            pass.start(seq, t, s.tile);
+            pass.run(s.first + s.at, s.first + s.at + n, tick, odd);
+            __syncthreads();
+            const int which = at == share.from ? 0 : 1;
+            const bool any_odd = __builtin_amdgcn_readfirstlane((int)odd.any) != 0;
+            pass.finish(n == s.blocks, slots + 2 * index + which, odd, any_odd);
+            if (any_odd) {
                 __syncthreads();
-                const int which = at == share.from ? 0 : 1;
-                const bool any_odd = __builtin_amdgcn_readfirstlane((int)odd.any) != 0;
-                pass.finish(n == blocks, slots + 2 * index + which, odd, any_odd);
-                if (any_odd) {
-                    __syncthreads();
-                    odd.clear(kChunkThreads);
-                }
-                if (n != blocks && b0 == 0 && threadIdx.x == 0)
-                    joins[index] = {t.start, t.rows, kvh, tile * kChunkRows, (int)((at + blocks - 1) / share.size - index) + 1, which, {}};
+                odd.clear(kChunkThreads);
             }
-            at += n;
-            offset += n;
+            if (n != s.blocks && s.at == 0 && threadIdx.x == 0)
+                joins[index] = {t.start, t.rows, s.kvh, s.tile * kChunkRows, (int)((at + s.blocks - 1) / share.size - index) + 1, which, {}};
         }
-        ++seq;
-        offset = 0;
+        at += n;
+        offset += n;
+        if (at == share.to && to == share.to && first_out) {  // the beginning is done: the rest
+            to = head;
+            at = share.from;
+            offset = share.offset;
+            if (seq == share.seq) continue;
+            seq = share.seq;
+        } else if (at >= to) {
+            break;
+        } else if (offset < p.per_head * a.kv_heads) {
+            continue;
+        } else {
+            offset = 0;
+            do {
+                t = wave_sequence(a, ++seq);
+                p = pairs_of(a, t);
+            } while (p.per_head == 0);
+            continue;
+        }
+        t = wave_sequence(a, seq);
+        p = pairs_of(a, t);
     }
 }
 
