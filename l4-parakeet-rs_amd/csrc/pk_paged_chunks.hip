@@ -325,8 +325,8 @@ template <int kD, bool kF8> struct ChunkPass {
     // The scores of tile `block` and (or) the output of the tile before it, LDS reads
     // kAhead operands ahead of the products: one at a time, each is waited for in full (the
     // order is pinned because the compiler brings them together again).
-    static constexpr int kAhead = 6;
-    template <bool kScores, bool kOutput> __device__ __forceinline__ void products(int block, v16f (&sc)[2], const v8h (&pf)[4], const Step& step) {
+    static constexpr int kAhead = 4;
+    template <bool kScores, bool kOutput> __device__ __forceinline__ void products(int block, v16f (&sc)[2], const v8h (&pf)[4]) {
         constexpr int kPer = kF8 ? 2 : 1;  // products an operand's 16 bytes feed
         constexpr int kScoreReads = kScores ? 2 * kSteps / kPer : 0, kReads = kScoreReads + (kOutput ? 4 * kBlocks / kPer : 0);
         const uint8_t* kt = lds + buffer_of(block) * kBuffer;
@@ -342,6 +342,7 @@ template <int kD, bool kF8> struct ChunkPass {
             const int j = i - kScoreReads, d = l32 + 32 * (j / (4 / kPer)), s = j % (4 / kPer);
             return *(const uint4*)(vt + d * kValueBytes + ((2 * s + h) ^ value_swizzle(d)) * 16);
         };
+        __builtin_amdgcn_s_setprio(1);  // over the other wave's softmax
         if constexpr (kScores) sc[0] = sc[1] = v16f{};
         uint4 raw[kAhead];
 #pragma unroll
@@ -361,21 +362,14 @@ template <int kD, bool kF8> struct ChunkPass {
                 }
             }
             if (i + kAhead < kReads) raw[i % kAhead] = read(i + kAhead);
-            if constexpr (kScores) {  // the step's loads, spread over the products
-                constexpr int kEvery = kReads / (kKeyLoads + kValueLoads);
-                const int n = i / kEvery;
-                if (i % kEvery == kEvery / 2 && n < kKeyLoads + kValueLoads) {
-                    if (n < kKeyLoads) load_keys(step, n);
-                    else load_values(step, n - kKeyLoads);
-                }
-            }
         }
+        __builtin_amdgcn_s_setprio(0);
         // the scores are next read by max3, before which the compiler places no wait for the MFMA
         if constexpr (kScores && !kOutput) asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    // Loads go out in steps: K(t + 3) and V(t + 2) among tile t's products.  Waits until
+    // Loads go out in steps: K(t + 3) and V(t + 2) with tile t's softmax.  Waits until
     // all but the last `steps` steps (of kLoads a wave) have arrived, which they do in order.
     template <int steps> __device__ __forceinline__ static void wait_steps(bool more) {
         if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(steps * kLoads) : "memory");
@@ -392,11 +386,11 @@ template <int kD, bool kF8> struct ChunkPass {
     //
     // Two waves share a SIMD (w and w + 4); the second four run half a period behind, so
     // that one's products (the scores of a tile and the output of the one before) run under
-    // the other's softmax.  Buffers: K(t + 3) replaces K(t - 1) and V(t + 2) replaces
-    // V(t - 2) during tile t's products, which read K(t) and V(t - 1); the other waves are
-    // at that tile's softmax, or at the softmax before.  The waves that are behind are
-    // at their last products when the others go on to the next tiles' first loads, which
-    // go to other buffers than V(to - 1).
+    // the other's softmax and loads.  Buffers: K(t + 3) replaces K(t - 1) and V(t + 2)
+    // replaces V(t - 2) at tile t's softmax, when the other waves are at the products of
+    // that tile, which read K(t) and V(t - 1), or of the next.  The waves that are behind
+    // are at their last products when the others go on to the next tiles' first loads,
+    // which go to other buffers than V(to - 1).
     __device__ __forceinline__ void run(int from, int to, int& tick, Odd<kD, kChunkRows>& odd) {
         ring = (tick - from) & (kBuffers - 1);
         const bool behind = wave >= 4;
@@ -418,13 +412,13 @@ template <int kD, bool kF8> struct ChunkPass {
         v16f sc[2];
         v8h pf[4];
         Step step = step_of(from + 3, next, from + 2, ids, to);
-        if (active) products<true, false>(from, sc, pf, step);
-        else load_all(step);
+        if (active) products<true, false>(from, sc, pf);
         for (int b = from; b < to; ++b) {
-            wait_steps<2>(b + 3 < to);
+            wait_steps<1>(b + 2 < to);
             const bool edge = b * kTileKeys < tile_full_lo || (b + 1) * kTileKeys > tile_full_hi || ok[0] != kAllPages;
             if (edge) tidy_values(b, ok[0], odd);
             meet();
+            load_all(step);
             ok[2] = pages_ok(ids);
             ids = next;
             next = tile_ids(b + 4);
@@ -437,12 +431,9 @@ template <int kD, bool kF8> struct ChunkPass {
             meet();
             ok[0] = ok[1];
             ok[1] = ok[2];
-            if (b + 1 < to) {
-                if (active) products<true, true>(b + 1, sc, pf, step);
-                else load_all(step);
-            }
+            if (b + 1 < to && active) products<true, true>(b + 1, sc, pf);
         }
-        if (active) products<false, true>(to, sc, pf, step);
+        if (active) products<false, true>(to, sc, pf);
         tick += to - from;
         if (!behind) meet();
     }
