@@ -710,7 +710,7 @@ int32_t pk_page_plan(const int32_t* held, const int32_t* added, const int32_t* f
  * projection's rows) into their slots.  kind PK_CACHE_FP8 stores e4m3(x *
  * inverse_scale) (saturating; NaN stays NaN), PK_CACHE_FP16 the value itself.
  * A slot outside [0, pages * page_size) is skipped (-1: padding).  The slots of
- * one call must differ.  head_dim 64 or 128; keys, values and caches 16-byte
+ * one call must differ.  tokens <= 2^21, head_dim 64 or 128; keys, values and caches 16-byte
  * aligned, strides multiples of 8. */
 int32_t pk_paged_cache_write(int32_t kind, const uint16_t* key, int64_t key_stride, const uint16_t* value,
                              int64_t value_stride, const int32_t* slots, void* key_cache, void* value_cache,

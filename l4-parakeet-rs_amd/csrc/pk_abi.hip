@@ -995,8 +995,8 @@ int32_t pk_paged_cache_write(int32_t kind, const uint16_t* key, int64_t key_stri
     const int32_t shift = cache_shape(kind, kv_heads, head_dim, page_size, pages);
     if (shift < 0) return shift;
     const int64_t width = (int64_t)kv_heads * head_dim;
-    if (tokens < 0 || key_stride < width || value_stride < width || key_stride >= 1ll << 31 || value_stride >= 1ll << 31) {
-        set_error("cache write needs tokens >= 0 and strides of at least kv_heads * head_dim = %lld (tokens=%d strides %lld, %lld)",
+    if (tokens < 0 || tokens > 1 << 21 || key_stride < width || value_stride < width || key_stride >= 1ll << 31 || value_stride >= 1ll << 31) {
+        set_error("cache write needs 0 <= tokens <= 2^21 and strides of at least kv_heads * head_dim = %lld (tokens=%d strides %lld, %lld)",
                   (long long)width, tokens, (long long)key_stride, (long long)value_stride);
         return PK_E_SHAPE;
     }

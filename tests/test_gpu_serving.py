@@ -266,7 +266,7 @@ def test_plan_of_a_negative_page(pk):  # noqa: F811
 # ---- cache write ------------------------------------------------------------------------
 
 @pytest.mark.parametrize("tokens,kv,d,page", [(1, 1, 64, 16), (1, 8, 128, 16), (61, 8, 128, 16), (70, 3, 64, 32), (257, 2, 128, 64), (300, 1, 128, 256),
-                                              (513, 5, 64, 128), (1000, 8, 128, 32)])
+                                              (513, 5, 64, 128), (1000, 8, 128, 32), (1601, 2, 64, 16), (2047, 3, 128, 256), (3000, 8, 128, 64)])
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("order", ["runs", "shuffled", "offset"])
 def test_write(pk, tokens, kv, d, page, fp8, order):  # noqa: F811

@@ -76,7 +76,7 @@ def test_plan(want, kw):
 
 @pytest.mark.parametrize("want,kw", [
     (ARG, {"kind": 2}), (SHAPE, {"page_size": 48}), (SHAPE, {"kv_heads": 0}), (SHAPE, {"kv_heads": 257}), (SHAPE, {"head_dim": 96}),
-    (SHAPE, {"pages": 0}), (SHAPE, {"pages": 1 << 27}), (SHAPE, {"tokens": -1}), (SHAPE, {"key_stride": 1016}), (SHAPE, {"value_stride": 1 << 31}),
+    (SHAPE, {"pages": 0}), (SHAPE, {"pages": 1 << 27}), (SHAPE, {"tokens": -1}), (SHAPE, {"tokens": (1 << 21) + 1}), (SHAPE, {"key_stride": 1016}), (SHAPE, {"value_stride": 1 << 31}),
     (ARG, {"key": None}), (ARG, {"value": None}), (ARG, {"slots": None}), (ARG, {"key_cache": None}), (ARG, {"value_cache": None}),
     (ALIGN, {"key": P + 8}), (ALIGN, {"value_stride": 1028}), (ALIGN, {"value_cache": P + 8}), (ALIGN, {"slots": P + 2}),
 ])
