@@ -121,7 +121,8 @@ def weights(g, n, k):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 1, 128), (1, 16, 128), (2, 17, 256), (16, 33, 384), (1, 1030, 640), (3, 100, 1024), (5, 1024, 4096), (16, 4096, 1024),
-                                   (8, 250, 8192), (7, 40, 16384), (1, 15, 65536), (13, 5000, 512), (4, 3000, 4096), (16, 12321, 896)])
+                                   (8, 250, 8192), (7, 40, 16384), (1, 15, 65536), (13, 5000, 512), (4, 3000, 4096), (16, 12321, 896),
+                                   (2, 8191, 1152), (9, 8192, 1152), (5, 16383, 384), (16, 16384, 1280), (1, 20001, 128), (6, 300, 1920)])
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("fp32", [False, True])
 def test_gemv(pk, m, n, k, int8, fp32):  # noqa: F811
@@ -175,6 +176,19 @@ def test_gemv_against_the_linear(pk, int8):  # noqa: F811
         plain.close(lin, y, bound)
     else:  # each of the linear's weights is rounded to fp16
         plain.close(lin, y, bound + (x.double().abs() @ w.double().abs().t()) * 1.2 * plain.U16)
+
+
+@pytest.mark.parametrize("n,k", [(200, 512), (200, 1536), (200, 4096), (8200, 2560), (16400, 2560)])
+def test_gemv_result_does_not_depend_on_the_batch(pk, n, k):  # noqa: F811
+    g = gen(n + k)
+    q, scales, zeros = weights(g, n, k)
+    x = randn(g, 16, k)
+    out = torch.empty((16, n), device="cuda")
+    pk.gemv_int4g128(x, q, scales, zeros, None, out)
+    for m in (1, 7):
+        some = torch.empty((m, n), device="cuda")
+        pk.gemv_int4g128(x[9:9 + m], q, scales, zeros, None, some)
+        assert torch.equal(some, out[9:9 + m])
 
 
 def test_gemv_infinity_and_nan_rows_stay_in_their_row(pk):  # noqa: F811
