@@ -94,20 +94,23 @@ struct RowTile {
     int start, rows, length, first_pos;  // first_pos: position of the sequence's first new token
 };
 
-__device__ __forceinline__ RowTile sequence_of(const PagedArgs& a, int seq) {
-    int s = a.starts[seq], e = a.starts[seq + 1], len = a.lengths[seq];
+__device__ __forceinline__ RowTile sequence_of(const PagedArgs& a, int s, int e, int len) {
     s = s < 0 ? 0 : (s > a.tokens ? a.tokens : s);
     e = e < s ? s : (e > a.tokens ? a.tokens : e);
     const int most = a.max_pages << a.shift;
     len = len < 0 ? 0 : (len > most ? most : len);
     return {s, (e - s) * a.group, len, len - (e - s)};
 }
+__device__ __forceinline__ RowTile sequence_of(const PagedArgs& a, int seq) { return sequence_of(a, a.starts[seq], a.starts[seq + 1], a.lengths[seq]); }
+
+// What a launch does not write is read through the scalar cache where a whole wave needs it:
+// such loads do not wait behind the cache's, which return in order.
+typedef const __attribute__((address_space(4))) int* ScalarInts;
+__device__ __forceinline__ int scalar_at(const int* p, int index) { return ((ScalarInts)(uintptr_t)p)[__builtin_amdgcn_readfirstlane(index)]; }
 
 // The same for a sequence that the whole wave works on, in scalar registers.
 __device__ __forceinline__ RowTile wave_sequence(const PagedArgs& a, int seq) {
-    const RowTile t = sequence_of(a, seq);
-    return {__builtin_amdgcn_readfirstlane(t.start), __builtin_amdgcn_readfirstlane(t.rows), __builtin_amdgcn_readfirstlane(t.length),
-            __builtin_amdgcn_readfirstlane(t.first_pos)};
+    return sequence_of(a, scalar_at(a.starts, seq), scalar_at(a.starts, seq + 1), scalar_at(a.lengths, seq));
 }
 
 // Keys [lo, hi) that a query at `pos` sees.
@@ -131,20 +134,31 @@ __device__ __forceinline__ void store_row(const PagedArgs& a, const RowTile& t, 
 #pragma unroll
     for (int j = 0; j < kN / 2; ++j) w[j] = (uint32_t)f2h(v[2 * j] * inv) | ((uint32_t)f2h(v[2 * j + 1] * inv) << 16);
     if constexpr (kN == 8) *(uint4*)op = uint4{w[0], w[1], w[2], w[3]};
-    else *(uint2*)op = uint2{w[0], w[1]};
+    else if constexpr (kN == 4) *(uint2*)op = uint2{w[0], w[1]};
+    else *(uint32_t*)op = w[0];
 }
 
 // The work of all sequences in a row, in blocks of keys, dealt to `shares` workgroups in
-// equal contiguous shares: every workgroup (kThreads threads) sums the blocks of all
-// sequences and finds the sequences that its share begins and ends in.
+// contiguous shares that differ by one block at most, or of `least` blocks where there are
+// too few: every workgroup (kThreads threads) sums the blocks of all sequences and finds the
+// sequences that its share begins and ends in.
 struct Share {
-    long long from, to, size;  // its blocks, and the blocks of a full share
+    long long from, to, all;  // its blocks, and the blocks of all shares
     long long offset;          // blocks of `seq` before `from`
     long long last_offset;     // and of `last_seq` before `to` - 1
     int seq, last_seq;
 };
 
-template <int kThreads, class Blocks> __device__ __forceinline__ bool deal(const PagedArgs& a, int shares, int least, int index, Blocks blocks_of, Share& out) {
+template <int kShares, int kLeast> __device__ __forceinline__ long long share_begin(long long all, int index) {
+    if (all >= kShares * kLeast) return index * all / kShares;
+    return index * kLeast < all ? index * kLeast : all;
+}
+// The share that holds a block: the last one that begins at or before it.
+template <int kShares, int kLeast> __device__ __forceinline__ int share_of(long long all, long long block) {
+    return (int)(all >= kShares * kLeast ? ((block + 1) * kShares - 1) / all : block / kLeast);
+}
+
+template <int kThreads, int kShares, int kLeast, class Blocks> __device__ __forceinline__ bool deal(const PagedArgs& a, int index, Blocks blocks_of, Share& out) {
     __shared__ long long wave_total[kThreads / 64], found_offset[2];
     __shared__ int found_seq[2];
     const int per = (a.sequences + kThreads - 1) / kThreads, s0 = threadIdx.x * per;
@@ -161,12 +175,10 @@ template <int kThreads, class Blocks> __device__ __forceinline__ bool deal(const
     for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) end += wave_total[w];
     long long all = 0;
     for (int w = 0; w < kThreads / 64; ++w) all += wave_total[w];
-    all = uniform(all);
-    out.size = (all + shares - 1) / shares;
-    if (out.size < least) out.size = least;
-    out.from = index * out.size;
-    out.to = out.from + out.size < all ? out.from + out.size : all;
-    if (out.from >= all) return false;
+    out.all = all = uniform(all);
+    out.from = uniform(share_begin<kShares, kLeast>(all, index));
+    out.to = uniform(share_begin<kShares, kLeast>(all, index + 1));
+    if (out.from >= out.to) return false;
     const long long last = out.to - 1;
     if (end - mine <= last && out.from < end) {  // this thread's sequences hold blocks of the share
         long long at = end - mine;

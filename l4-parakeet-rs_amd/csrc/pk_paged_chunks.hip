@@ -134,9 +134,8 @@ template <int kD, bool kF8> struct ChunkPass {
         int page[4];
     };
     __device__ __forceinline__ int page_at(int key) const {
-        typedef const __attribute__((address_space(4))) int* ScalarTable;
         const int c = key >> a.shift;
-        return ((ScalarTable)(uintptr_t)table)[__builtin_amdgcn_readfirstlane(c > last_page ? last_page : c)];
+        return scalar_at(table, c > last_page ? last_page : c);
     }
     __device__ __forceinline__ Ids tile_ids(int block) const {
         const int k0 = block * kTileKeys;
@@ -522,7 +521,7 @@ __global__ __launch_bounds__(kChunkThreads, 2) void paged_chunks_shares_kernel(P
     if (threadIdx.x == 0) joins[index].count = 0;
     Share share;
     const auto blocks_of = [&](const RowTile& t) { return pairs_of(a, t).per_head * a.kv_heads; };
-    if (!deal<kChunkThreads>(a, kChunkShares, kLeastChunkShare, index, blocks_of, share)) return;
+    if (!deal<kChunkThreads, kChunkShares, kLeastChunkShare>(a, index, blocks_of, share)) return;
 
     // The beginning of the row tile that the share ends in comes first, then the rest in
     // order: as shares are equal, the workgroups then stand at about the same keys at the
@@ -555,7 +554,7 @@ __global__ __launch_bounds__(kChunkThreads, 2) void paged_chunks_shares_kernel(P
                 odd.clear(kChunkThreads);
             }
             if (n != s.blocks && s.at == 0 && threadIdx.x == 0)
-                joins[index] = {t.start, t.rows, s.kvh, s.tile * kChunkRows, (int)((at + s.blocks - 1) / share.size - index) + 1, which, {}};
+                joins[index] = {t.start, t.rows, s.kvh, s.tile * kChunkRows, share_of<kChunkShares, kLeastChunkShare>(share.all, at + s.blocks - 1) - index + 1, which, {}};
         }
         at += n;
         offset += n;
