@@ -1024,9 +1024,10 @@ static int32_t paged_shape(int32_t tokens, int32_t max_queries, int32_t sequence
         return PK_E_SHAPE;
     }
     if (tokens < 0 || tokens > 1 << 20 || max_queries < 0 || max_queries > tokens || sequences < 0 || sequences > 4096 || max_pages <= 0 ||
-        max_pages > (1 << 30) >> shift) {
-        set_error("paged attention needs tokens <= 2^20, max_queries <= tokens, sequences <= 4096 and max_pages * page_size <= 2^30 "
-                  "(tokens=%d max_queries=%d sequences=%d max_pages=%d)", tokens, max_queries, sequences, max_pages);
+        max_pages > (1 << 30) >> shift || (int64_t)max_queries * (heads / kv_heads) > 1 << 23) {
+        set_error("paged attention needs tokens <= 2^20, max_queries <= tokens, sequences <= 4096, max_pages * page_size <= 2^30 and "
+                  "max_queries * heads / kv_heads <= 2^23 (tokens=%d max_queries=%d sequences=%d max_pages=%d)", tokens, max_queries, sequences,
+                  max_pages);
         return PK_E_SHAPE;
     }
     return shift;

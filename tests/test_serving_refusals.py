@@ -94,6 +94,8 @@ def test_write(want, kw):
     (SHAPE, {"output_stride": 0}), (ARG, {"query": None}), (ARG, {"key_cache": None}), (ARG, {"value_cache": None}), (ARG, {"block_table": None}),
     (ARG, {"query_starts": None}), (ARG, {"key_lengths": None}), (ARG, {"output": None}), (ALIGN, {"query": P + 8}), (ALIGN, {"query_stride": 2052}),
     (ALIGN, {"output": P + 4}), (ALIGN, {"key_cache": P + 8}), (ALIGN, {"block_table": P + 2}), (ALIGN, {"workspace": P + 8}),
+    (ARG, {"workspace": None}), (ARG, {"workspace_bytes": 1000}), (ARG, {"max_queries": 1, "workspace": None}),
+    (SHAPE, {"tokens": 1 << 20, "max_queries": 1 << 20, "heads": 128}),
 ])
 def test_attention(want, kw):
     a = dict(kind=0, query=P, query_stride=2048, key_cache=P, value_cache=P, block_table=P, query_starts=P, key_lengths=P, output=P, output_stride=2048,
@@ -106,6 +108,8 @@ def test_attention(want, kw):
 def test_workspace_sizes_are_host_answers():
     assert pk.paged_attention_workspace_bytes(5, 5, 2, 16, 8, 128, 16, 400) >= 0
     assert pk.paged_attention_workspace_bytes(0, 0, 0, 16, 8, 128, 16, 400) >= 0
+    assert pk.paged_attention_workspace_bytes(5, 5, 2, 16, 8, 128, 16, 32) == 0  # tables of up to 512 keys need none
+    assert pk.paged_attention_workspace_bytes(5, 5, 2, 16, 8, 128, 16, 33) > 0
     with pytest.raises(pk.PkError):
         pk.paged_attention_workspace_bytes(5, 5, 2, 16, 8, 100, 16, 400)
 
