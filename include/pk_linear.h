@@ -31,7 +31,7 @@
  *     parts within a workgroup (pk_gemm_k_split reports 4) fold the group sums
  *     by parts, so their fp32 results are associated differently from the
  *     same rows' on a large grid (each part is exact; see pk_gemm_k_split).
- *     pk_paged_attention over long tables is another, see there.
+ *     pk_paged_attention is another, see there.
  */
 #ifndef PK_LINEAR_H
 #define PK_LINEAR_H
@@ -736,10 +736,10 @@ int32_t pk_paged_cache_write(int32_t kind, const uint16_t* key, int64_t key_stri
  * Scores, the running maximum and sum and the output's sum are fp32; scores
  * multiply fp16 queries with fp16 or e4m3 keys exactly, probabilities are
  * rounded to fp16 for the second product (their sum is not).
- * Results do not depend on the batch for tables of up to 512 keys.  Longer ones
- * are worked on in equal shares of the whole batch's keys, so where a row's sums
- * are cut, in fp32, depends on the other sequences' lengths.  The same call gives
- * the same bits.
+ * A row's fp32 sums are cut alike whatever stands beside it only for tables of
+ * up to 512 keys and the same kernel (max_queries * heads / kv_heads <= 16, or
+ * above): longer tables are worked on in equal shares of the whole batch's keys.
+ * The same call gives the same bits.
  * workspace: pk_paged_attention_workspace_bytes of device memory (16-byte
  * aligned), used by one call at a time; its content need not be kept or cleared
  * between calls. */
