@@ -736,9 +736,9 @@ int32_t pk_paged_cache_write(int32_t kind, const uint16_t* key, int64_t key_stri
  * Scores, the running maximum and sum and the output's sum are fp32; scores
  * multiply fp16 queries with fp16 or e4m3 keys exactly, probabilities are
  * rounded to fp16 for the second product (their sum is not).
- * A row's fp32 sums are cut alike whatever stands beside it only for tables of
- * up to 512 keys and the same kernel (max_queries * heads / kv_heads <= 16, or
- * above): longer tables are worked on in equal shares of the whole batch's keys.
+ * A row's fp32 sums are cut alike whatever stands beside it where a full table
+ * holds at most 384 KB of keys and values a kv head and max_queries * heads /
+ * kv_heads <= 32.  Larger work is dealt in equal shares of the whole batch's keys.
  * The same call gives the same bits.
  * workspace: pk_paged_attention_workspace_bytes of device memory (16-byte
  * aligned), used by one call at a time; its content need not be kept or cleared

@@ -279,6 +279,8 @@ template <int kD, int kN> __device__ __forceinline__ bool put_odd(const Odd<kD, 
 }
 
 // Short contexts: one workgroup for the keys of a (sequence, kv head, 16 rows).
+// A single token's 93 keys, 8 heads, fp16: 5.3 us, of which a launch is 2.5 and the rest the
+// chain length -> page id -> keys -> scores -> values -> the waves' join.
 constexpr int kDirectWaves = 4;
 
 template <int kD, bool kF8> __global__ __launch_bounds__(64 * kDirectWaves, 2) void paged_attention_rows_kernel(PagedArgs a) {
@@ -533,15 +535,30 @@ template <int kD> __global__ __launch_bounds__(kJoinGroups * kD / 4) void paged_
     }
 }
 
-// Whether one workgroup an item does: at most kDirectKeys keys each, by the table's width.
-constexpr int kDirectKeys = 512;
+// One launch, a workgroup an item, where a full table's keys and values of a kv head are few
+// bytes: a CU reads about 33 bytes a ns, while shares take 12 to 13 us however little there is
+// (one sequence, 8 kv heads of 128, e4m3: 900 keys 9.5 us against 13.0, 1900 14.5 and 13.1;
+// fp16: 448 keys 9.1, 900 16.6 and 12.5).  With many sequences it is ahead further up, since
+// workgroups that end early make room (64 of 1900 e4m3 keys: 34 us against 45).
+constexpr long long kDirectBytes = 384 << 10;
+// So do up to 32 rows of a kv head, in two tiles that read the same keys: one sequence of 24
+// rows, 448 keys, 7.3 us against 14.5 for a chunk's kernel, 64 of them of 1900 keys 65 and 95.
+// With four tiles the reading overtakes the gain (64 sequences of 48 rows, 1900 fp16 keys: 180
+// and 117).  Long tables (8 sequences of 24 rows, 12000 keys) take 115 in shares, 78 in chunks.
+constexpr int kDirectRows = 32;
+// A chunk's kernel divides even short tables: one sequence of 80 rows, 1900 keys, 37 us in
+// shares, 51 directly.
+constexpr int kChunkDirectKeys = 512;
 
-// From this many query rows a sequence on, chunks of 128 rows share their loads.
-constexpr int kChunksFrom = 17;
+static bool rows_directly(int head_dim, int key_bytes, long long keys, long long rows) {
+    return keys * head_dim * key_bytes * 2 <= kDirectBytes && rows <= kDirectRows;
+}
 
+// For either kind of cache: the fp16 one's, which is never less.
 size_t paged_attention_workspace(int head_dim, int page_shift, int max_pages, int max_rows) {
-    if ((long long)max_pages << page_shift <= kDirectKeys) return 0;
-    if (max_rows >= kChunksFrom) return paged_chunks_workspace(head_dim);
+    const long long keys = (long long)max_pages << page_shift;
+    if (rows_directly(head_dim, 2, keys, max_rows)) return 0;
+    if (max_rows > 16) return keys <= kChunkDirectKeys ? 0 : paged_chunks_workspace(head_dim);
     return 2 * kShares * (head_dim == 128 ? sizeof(Part<128, 16>) : sizeof(Part<64, 16>)) + kShares * sizeof(Join);
 }
 
@@ -559,9 +576,10 @@ template <int kD, bool kF8> static void launch_rows(const PagedArgs& a, bool dir
 }
 
 void launch_paged_attention(int kind, const PagedArgs& a, int head_dim, int max_queries, void* workspace, hipStream_t s) {
-    const bool direct = (long long)a.max_pages << a.shift <= kDirectKeys;
-    if (max_queries * a.group >= kChunksFrom) {
-        launch_paged_chunks(kind, a, head_dim, direct, max_queries, workspace, s);
+    const long long keys = (long long)a.max_pages << a.shift, rows = (long long)max_queries * a.group;
+    const bool direct = rows_directly(head_dim, kind == 1 ? 1 : 2, keys, rows);
+    if (rows > 16 && !direct) {
+        launch_paged_chunks(kind, a, head_dim, keys <= kChunkDirectKeys, max_queries, workspace, s);
         return;
     }
     if (head_dim == 128) {

@@ -18,11 +18,13 @@ def gen(seed):
 class Case:
     """Sequences of (new tokens, keys) over a shuffled cache; every place that no key fills holds NaN."""
 
+    wider = 0  # keys that the tables are wider than they need to be
+
     def __init__(self, shape, heads=4, kv=2, d=128, page=16, fp8=False, seed=1, spare_rows=3, peak=1.0):
         g = gen(seed)
         self.heads, self.kv, self.d, self.page, self.fp8 = heads, kv, d, page, fp8
         self.counts, self.lengths_ = [n for n, _ in shape], [length for _, length in shape]
-        columns = max(max(-(-length // page) for length in self.lengths_), 1) + 1
+        columns = max(max(-(-length // page) for length in self.lengths_), 1) + 1 + self.wider // page
         pages = sum(-(-length // page) for length in self.lengths_) + 3
         ids = torch.randperm(pages, generator=g, device="cuda").int()
         self.table = torch.full((len(shape), columns), 2 ** 30, dtype=torch.int32, device="cuda")  # never a page
@@ -70,6 +72,14 @@ class Case:
         plain.close(got[:tokens], want, bound, f"{self.counts} over {self.lengths_}, window ({left}, {right})")
         assert (got[tokens:] == 9).all()
         return got
+
+
+@pytest.fixture(autouse=True, params=[0, 6000])
+def tables(request):
+    """Everything with tables as wide as the longest sequence, and with wide ones, whose keys are dealt in shares."""
+    Case.wider = request.param
+    yield
+    Case.wider = 0
 
 
 @pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200, 255, 256, 257, 511, 513, 1000, 2049, 5000])

@@ -73,10 +73,12 @@ STEPS = [[5, 0, 7, 0], [1, 1, 1, 0], [0, 9, 1, 2], [1, 1, 1, 1], [12, 0, 0, 0], 
 
 
 @pytest.mark.parametrize("fp8", [False, True])
-@pytest.mark.parametrize("columns", [30, 40])
-def test_layer_steps(pk, fp8, columns):  # noqa: F811
-    """Each operator's output against the definition applied to what the one before it left (480 keys a table: one launch; 640: in shares)."""
-    layer = type("Sized", (Layer,), {"columns": columns})(pk, 4, fp8)
+@pytest.mark.parametrize("columns", [30, 250])
+@pytest.mark.parametrize("heads", [2, 4, 8])
+def test_layer_steps(pk, fp8, columns, heads):  # noqa: F811
+    """Each operator's output against the definition applied to what the one before it left (tables of 480 and of 4000 keys; 12, 24
+    and 48 rows a kv head)."""
+    layer = type("Sized", (Layer,), {"columns": columns, "heads": heads})(pk, 4, fp8)
     g, held = gen(8), [0] * 4
     for added in STEPS:
         layer.ask(added, g)

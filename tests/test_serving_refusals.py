@@ -108,8 +108,8 @@ def test_attention(want, kw):
 def test_workspace_sizes_are_host_answers():
     assert pk.paged_attention_workspace_bytes(5, 5, 2, 16, 8, 128, 16, 400) >= 0
     assert pk.paged_attention_workspace_bytes(0, 0, 0, 16, 8, 128, 16, 400) >= 0
-    assert pk.paged_attention_workspace_bytes(5, 5, 2, 16, 8, 128, 16, 32) == 0  # tables of up to 512 keys need none
-    assert pk.paged_attention_workspace_bytes(5, 5, 2, 16, 8, 128, 16, 33) > 0
+    for queries, kv, pages, none in ((5, 8, 48, True), (5, 8, 49, False), (5, 4, 48, True), (5, 2, 32, True), (5, 2, 33, False)):  # 10, 20, 40 rows
+        assert (pk.paged_attention_workspace_bytes(5, queries, 2, 16, kv, 128, 16, pages) == 0) is none
     with pytest.raises(pk.PkError):
         pk.paged_attention_workspace_bytes(5, 5, 2, 16, 8, 100, 16, 400)
 
