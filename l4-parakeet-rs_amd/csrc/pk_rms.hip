@@ -4,7 +4,8 @@
 //   scale = max|y| / 448 (INT8: / 127),  q = e4m3(y / scale) (INT8: rne).
 // h, the sum of squares and y stay in fp32: the only roundings are the stored
 // residual stream's and the codes'.  A row is read once and held in registers
-// between its two reductions.
+// between its two reductions.  Bound by HBM: 45000 x 1024 with a residual in and
+// out, e4m3 (323 MB), 59 us, 5.5 TB/s; one row 2.7 us, about a launch.
 #include "pk_kernels.hpp"
 
 namespace pk {
@@ -122,6 +123,9 @@ template <bool kInt8>
 static void launch_rms(const uint16_t* in, const uint16_t* residual, const uint16_t* w, uint16_t* r_out, uint8_t* out, float* scales,
                        int rows, int width, float eps, hipStream_t s) {
     const unsigned waves = (unsigned)((rows + 3) / 4);
+    // A wave a row up to 1024 features: 45000 rows take 60 us, with a workgroup each 85 (one row
+    // 3.0 and 2.7).  Above, a workgroup: 12000 x 2048 35 us against 38 for waves, x 4096 64 and 76,
+    // one row of 4096 3.3 and 6.5.
 #define PK_RMS(lanes, chunks, grid) \
     rms_norm_quantize_kernel<kInt8, lanes, chunks><<<grid, 256, 0, s>>>(in, residual, w, r_out, out, scales, rows, width, eps)
     if (width <= 512) PK_RMS(64, 1, waves);
