@@ -37,9 +37,11 @@ __device__ __forceinline__ int chunk_blocks(const PagedArgs& a, const RowTile& t
 }
 
 // With a causal mask the row tiles of a sequence differ in length; tile j and tile n - 1 -
-// j together hardly do (their blocks are concave in j), so they are dealt as one item of
-// `pair` blocks, the most any pair has; the middle tile of an odd number is an item by
-// itself.
+// j together hardly do (their keys are concave in j, and the blocks of a tile less than two
+// more than its keys), so they are dealt as one item of `pair` blocks, at least what any pair
+// has; the middle tile of an odd number is an item by itself.  Keys are not concave where the
+// first rows stand before key 0 and see nothing (more new tokens than keys): a pair then has
+// room for two tiles of all keys.
 struct Pairs {
     int tiles, pair, middle;
     long long per_head;
@@ -51,7 +53,9 @@ __device__ __forceinline__ Pairs pairs_of(const PagedArgs& a, const RowTile& t) 
     int first;
     const int mid = chunk_blocks(a, t, p.tiles / 2, first);
     if (p.tiles & 1) p.middle = mid;
-    if (p.tiles > 1) p.pair = mid + chunk_blocks(a, t, (p.tiles - 1) / 2, first) + 2;  // + 2: blocks are whole
+    const int all = (t.length + kTileKeys - 1) / kTileKeys;
+    if (p.tiles > 1 && a.right >= 0 && t.first_pos + a.right + 1 < 0) p.pair = 2 * (all > 1 ? all : 1);
+    else if (p.tiles > 1) p.pair = mid + chunk_blocks(a, t, (p.tiles - 1) / 2, first) + 3;
     p.per_head = (long long)(p.tiles / 2) * p.pair + p.middle;
     return p;
 }

@@ -146,6 +146,16 @@ def test_rows_that_see_nothing_are_zero(pk, fp8):  # noqa: F811
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("left,right", [(-1, 0), (150, 20)])
+def test_long_chunks_of_more_tokens_than_keys(pk, fp8, left, right):  # noqa: F811
+    """Most row tiles see nothing, the last ones several tiles of keys."""
+    c = Case([(1500, 1500), (3, 80), (900, 950)], fp8=fp8, seed=25, page=32)
+    c.lengths[0], c.lengths[2] = 400, 700
+    got = c.check(pk, left, right)
+    assert not got[:1000].any() and got[1400:1500].any()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("n", [6, 50])
 def test_infinities_and_nan_in_unseen_keys(pk, fp8, n):  # noqa: F811
     """A later token's key and value are not seen by the earlier ones of the chunk, whatever they hold."""
