@@ -660,7 +660,8 @@ int32_t pk_pack_position_heads(const uint16_t* input, uint16_t* output, void* st
  * A row of zeros has scale 1 (also with epsilon 0); a row whose y holds an
  * infinity or a NaN has scale NaN and codes 0x7f (INT8: 0).  The rows feed
  * pk_linear_fp8_dyn, pk_linear_int8_dyn, pk_linear_int4g128_a8 and
- * pk_gemv_int4g128_a8.  Rows and weight 16-byte, output 8-byte aligned. */
+ * pk_gemv_int4g128_a8.  Rows and weight 16-byte, output 8-byte aligned; output,
+ * scales and a residual_out of its own overlap nothing else. */
 int32_t pk_rms_norm_quantize(int32_t kind, const uint16_t* input, const uint16_t* residual, const uint16_t* weight,
                              uint16_t* residual_out, void* output, float* scales, int32_t rows, int32_t width,
                              float epsilon, void* stream);
@@ -671,8 +672,8 @@ int32_t pk_rms_norm_quantize(int32_t kind, const uint16_t* input, const uint16_t
  * The levels q - z (weight_zeros whole numbers 0..15) multiply exactly and the
  * scale is applied to the group's sum in fp32, where pk_linear_int4g128 rounds
  * each dequantized weight to fp16 first.  The INT8 form's group sums are exact.
- * n free, k % 128 == 0 up to 65536; input and weight_q 16-byte aligned, bias may
- * be NULL; fp16 or fp32 output [m x n]. */
+ * n up to 2^30, k % 128 == 0 up to 65536; input and weight_q 16-byte aligned, bias
+ * may be NULL; fp16 or fp32 output [m x n], apart from every input. */
 int32_t pk_gemv_int4g128(const uint16_t* input, const uint32_t* weight_q, const uint16_t* weight_scales,
                          const uint16_t* weight_zeros, const float* bias, void* output, int32_t output_fp32, int32_t m,
                          int32_t n, int32_t k, void* stream);
@@ -739,7 +740,7 @@ int32_t pk_paged_cache_write(int32_t kind, const uint16_t* key, int64_t key_stri
  * A row's fp32 sums are cut alike whatever stands beside it where a full table
  * holds at most 384 KB of keys and values a kv head and max_queries * heads /
  * kv_heads <= 32.  Larger work is dealt in equal shares of the whole batch's keys.
- * The same call gives the same bits.
+ * The same call gives the same bits.  output and workspace overlap nothing else.
  * workspace: pk_paged_attention_workspace_bytes of device memory (16-byte
  * aligned), used by one call at a time; its content need not be kept or cleared
  * between calls. */

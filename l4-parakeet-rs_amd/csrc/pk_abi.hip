@@ -904,14 +904,22 @@ int32_t pk_rms_norm_quantize(int32_t kind, const uint16_t* input, const uint16_t
         set_error("residual_out may be input or residual itself; other overlaps of the norm's rows are refused");
         return PK_E_ARG;
     }
+    const size_t w = 2 * (size_t)width, r = 4 * (size_t)rows;
+    if (overlap(weight, w, residual_out, 2 * n) || overlap(weight, w, output, n) || overlap(scales, r, weight, w) ||
+        overlap(scales, r, input, 2 * n) || overlap(scales, r, residual, 2 * n) || overlap(scales, r, residual_out, 2 * n) ||
+        overlap(scales, r, output, n)) {
+        set_error("the norm's weight and scales must not overlap its rows");
+        return PK_E_ARG;
+    }
     launch_rms_norm_quantize(kind, input, residual, weight, residual_out, output, scales, rows, width, epsilon, STREAM);
     return check_launch("rms_norm_quantize");
 }
 
 static int32_t gemv(const void* input, const float* input_scales, const uint32_t* q, const uint16_t* scales, const uint16_t* zeros,
                     const float* bias, void* output, int32_t output_fp32, int32_t m, int32_t n, int32_t k, void* stream) {
-    if (m < 0 || m > 16 || n < 0 || k <= 0 || k % 128 || k > 65536) {
-        set_error("int4g128 gemv needs m <= 16 and k %% 128 == 0 up to 65536 (m=%d n=%d k=%d); pk_linear_int4g128 takes more rows", m, n, k);
+    if (m < 0 || m > 16 || n < 0 || n > 1 << 30 || k <= 0 || k % 128 || k > 65536) {
+        set_error("int4g128 gemv needs m <= 16, n <= 2^30 and k %% 128 == 0 up to 65536 (m=%d n=%d k=%d); pk_linear_int4g128 takes more rows",
+                  m, n, k);
         return PK_E_SHAPE;
     }
     if (m == 0 || n == 0) return PK_OK;
@@ -922,6 +930,13 @@ static int32_t gemv(const void* input, const float* input_scales, const uint32_t
         misaligned(input_scales, 4) || misaligned(output, output_fp32 ? 4 : 2)) {
         set_error("gemv input and weight_q must be 16-byte aligned, the others as their types");
         return PK_E_ALIGN;
+    }
+    const size_t out = (size_t)m * n * (output_fp32 ? 4 : 2), groups = (size_t)n * (k / 128) * 2;
+    if (overlap(output, out, input, (size_t)m * k * (input_scales ? 1 : 2)) || overlap(output, out, input_scales, 4 * (size_t)m) ||
+        overlap(output, out, q, (size_t)n * k / 2) || overlap(output, out, scales, groups) || overlap(output, out, zeros, groups) ||
+        overlap(output, out, bias, 4 * (size_t)n)) {
+        set_error("gemv output overlaps an input");
+        return PK_E_ARG;
     }
     launch_gemv_g128(input, input_scales, q, scales, zeros, bias, output, output_fp32 != 0, m, n, k, STREAM);
     return check_launch("gemv_int4g128");

@@ -548,7 +548,7 @@ def _row_stride(what, name, t):
     step, head, one = t.stride()
     if one != 1 or (heads > 1 and head != head_dim):
         raise ValueError(f"{what}: {name} must hold each token's heads contiguously")
-    return step if tokens > 1 else max(step, heads * head_dim)
+    return step if tokens > 1 else heads * head_dim
 
 
 def paged_cache_write(key, value, slots, key_cache, value_cache, key_inverse_scale=1.0, value_inverse_scale=1.0, stream=None):

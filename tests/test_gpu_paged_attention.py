@@ -233,6 +233,18 @@ def test_output_as_a_slice(pk):  # noqa: F811
     assert torch.equal(wide[:4, 2:6], want[:4]) and (wide[:, :2] == 4).all() and (wide[:, 6] == 4).all() and (wide[4:] == 4).all()
 
 
+def test_one_token_whatever_its_stride(pk):  # noqa: F811
+    """A single token's stride leads nowhere."""
+    c = Case([(1, 100)], seed=26, spare_rows=0)
+    wide = torch.zeros((1, 4 * 128 + 5), dtype=torch.float16, device="cuda")
+    wide[:, :512] = c.q.reshape(1, 512)
+    out = torch.full((1, 517), 4.0, dtype=torch.float16, device="cuda")
+    c.q = wide[:, :512].unflatten(1, (4, 128))
+    c.run(pk, out=out[:, :512].unflatten(1, (4, 128)))
+    want = c.check(pk)
+    assert torch.equal(out[:, :512], want.reshape(1, 512)) and (out[:, 512:] == 4).all()
+
+
 def test_twice_the_same_bits(pk):  # noqa: F811
     c = Case([(1, 3000), (50, 800), (1, 40)], heads=8, kv=2, seed=23)
     first = c.run(pk).clone()

@@ -31,6 +31,8 @@ def norm(**kw):
     (ARG, {"output": None}), (ARG, {"scales": None}), (ALIGN, {"input": P + 8}), (ALIGN, {"residual": P + (1 << 21) + 2}),
     (ALIGN, {"output": P + (1 << 24) + 4}), (ALIGN, {"scales": P + (1 << 25) + 2}), (ARG, {"residual_out": P + 2048}),
     (ARG, {"residual_out": P + (1 << 21) + 2048}), (ARG, {"output": P}), (ARG, {"output": P + (1 << 23)}),
+    (ARG, {"residual_out": P + (1 << 22)}), (ARG, {"output": P + (1 << 22)}), (ARG, {"scales": P + (1 << 22) + 4}), (ARG, {"scales": P}),
+    (ARG, {"scales": P + (1 << 21)}), (ARG, {"scales": P + (1 << 23)}), (ARG, {"scales": P + (1 << 24) + 4092}),
 ])
 def test_norm(want, kw):
     assert norm(**kw) == want
@@ -40,10 +42,12 @@ def test_norm(want, kw):
     (SHAPE, {"m": 17}), (SHAPE, {"m": -1}), (SHAPE, {"n": -1}), (SHAPE, {"k": 0}), (SHAPE, {"k": 192}), (SHAPE, {"k": 65664}),
     (ARG, {"input": None}), (ARG, {"q": None}), (ARG, {"scales": None}), (ARG, {"zeros": None}), (ARG, {"output": None}),
     (ALIGN, {"input": P + 2}), (ALIGN, {"q": P + 4}), (ALIGN, {"scales": P + 1}), (ALIGN, {"output": P + 2}), (ALIGN, {"bias": P + 2}),
+    (SHAPE, {"n": (1 << 30) + 1}), (ARG, {"output": P + (1 << 16)}), (ARG, {"output": P + (2 << 16) + 64 * 128 - 4}), (ARG, {"output": P + (3 << 16) + 252}),
+    (ARG, {"output": P + (4 << 16)}), (ARG, {"output": P + (5 << 16) - 252}),
 ])
 @pytest.mark.parametrize("int8", [False, True])
 def test_gemv(want, kw, int8):
-    a = dict(input=P, q=P, scales=P, zeros=P, bias=P, output=P, fp32=1, m=1, n=64, k=256)
+    a = dict(input=P + (1 << 16), q=P + (2 << 16), scales=P + (3 << 16), zeros=P + (4 << 16), bias=P + (5 << 16), output=P, fp32=1, m=1, n=64, k=256)
     a.update(kw)
     if int8:
         a = {"input": a.pop("input"), "input_scales": P, **a}
