@@ -147,14 +147,8 @@ template <int kD, bool kF8> struct ChunkPass {
     }
     __device__ __forceinline__ Ids tile_ids(int block) const {
         const int k0 = block * kTileKeys;
-        Ids r;
-        r.page[0] = r.page[1] = r.page[2] = r.page[3] = page_at(k0);
-        if (a.shift < 6) {  // else a tile lies in one page
-            r.page[1] = page_at(k0 + 16);
-            r.page[2] = page_at(k0 + 32);
-            r.page[3] = page_at(k0 + 48);
-        }
-        return r;
+        // also where a tile lies in one page: copies would be waited for right here
+        return {{page_at(k0), page_at(k0 + 16), page_at(k0 + 32), page_at(k0 + 48)}};
     }
     // Of one of the groups, chosen by the wave or by a lane.
     __device__ __forceinline__ static int pick(const Ids& id, int group) {
