@@ -106,7 +106,10 @@ __device__ __forceinline__ RowTile sequence_of(const PagedArgs& a, int seq) { re
 // What a launch does not write is read through the scalar cache where a whole wave needs it:
 // such loads do not wait behind the cache's, which return in order.
 typedef const __attribute__((address_space(4))) int* ScalarInts;
-__device__ __forceinline__ int scalar_at(const int* p, int index) { return ((ScalarInts)(uintptr_t)p)[__builtin_amdgcn_readfirstlane(index)]; }
+__device__ __forceinline__ int scalar_at(const int* p, int index) {  // 0 <= index < 2^30: the byte offset is one register
+    typedef const __attribute__((address_space(4))) uint8_t* ScalarBytes;
+    return *(ScalarInts)((ScalarBytes)(uintptr_t)p + (uint32_t)(__builtin_amdgcn_readfirstlane(index) << 2));
+}
 
 // The same for a sequence that the whole wave works on, in scalar registers.
 __device__ __forceinline__ RowTile wave_sequence(const PagedArgs& a, int seq) {

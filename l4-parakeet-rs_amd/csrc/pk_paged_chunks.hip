@@ -286,13 +286,21 @@ template <int kD, bool kF8> struct ChunkPass {
                 if (!(seen >> j & 1u)) sc[s >> 1][8 * (s & 1) + j] = kNegInf;
         }
     }
-    // The largest of three, in one instruction: the compiler's own form of it first passes
-    // products of the MFMA through another maximum each, for signalling NaN.  (A NaN among
-    // the scores comes through the exponentials.)
-    __device__ __forceinline__ static float max3(float x, float y, float z) {
-        float r;
-        asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
-        return r;
+    // The largest of the scores and m, three at once: the compiler's own form of it first
+    // passes products of the MFMA through another maximum each, for signalling NaN (a NaN among
+    // the scores comes through the exponentials), and between asms of one it places a wait.
+    __device__ __forceinline__ static float max3(float m, const v16f& x, const v16f& y) {
+        asm("v_max3_f32 %0, %0, %1, %9\n\tv_max3_f32 %0, %0, %2, %10\n\tv_max3_f32 %0, %0, %3, %11\n\tv_max3_f32 %0, %0, %4, %12\n\t"
+            "v_max3_f32 %0, %0, %5, %13\n\tv_max3_f32 %0, %0, %6, %14\n\tv_max3_f32 %0, %0, %7, %15\n\tv_max3_f32 %0, %0, %8, %16"
+            : "+v"(m)
+            : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]), "v"(y[0]), "v"(y[1]), "v"(y[2]), "v"(y[3]),
+              "v"(y[4]), "v"(y[5]), "v"(y[6]), "v"(y[7]));
+        asm("v_max3_f32 %0, %0, %1, %9\n\tv_max3_f32 %0, %0, %2, %10\n\tv_max3_f32 %0, %0, %3, %11\n\tv_max3_f32 %0, %0, %4, %12\n\t"
+            "v_max3_f32 %0, %0, %5, %13\n\tv_max3_f32 %0, %0, %6, %14\n\tv_max3_f32 %0, %0, %7, %15\n\tv_max3_f32 %0, %0, %8, %16"
+            : "+v"(m)
+            : "v"(x[8]), "v"(x[9]), "v"(x[10]), "v"(x[11]), "v"(x[12]), "v"(x[13]), "v"(x[14]), "v"(x[15]), "v"(y[8]), "v"(y[9]), "v"(y[10]),
+              "v"(y[11]), "v"(y[12]), "v"(y[13]), "v"(y[14]), "v"(y[15]));
+        return m;
     }
     // Scores are taken relative to a running maximum that is only raised where a row's
     // falls kSlack short (factors of two): probabilities up to 2^8 are as exact in fp16 and
@@ -300,11 +308,7 @@ template <int kD, bool kF8> struct ChunkPass {
     static constexpr float kSlack = 8.0f;
     // Scores -> probabilities as operands; the sums so far are scaled to the new maximum.
     __device__ __forceinline__ void soften(const v16f (&sc)[2], v8h (&pf)[4]) {
-        float m = max3(sc[0][0], sc[0][1], sc[1][0]);
-        m = max3(m, sc[1][1], kNegInf);
-#pragma unroll
-        for (int j = 2; j < 16; ++j) m = max3(m, sc[0][j], sc[1][j]);
-        m = max_level(m, 32);
+        const float m = max_level(max3(kNegInf, sc[0], sc[1]), 32);
         const bool far = (m - top) * scale > kSlack;  // also from -inf; false while nothing is seen
         if (__any(far)) {
             const float keep = far ? __builtin_amdgcn_exp2f((top - m) * scale) : 1.0f;
