@@ -383,6 +383,7 @@ __global__ __launch_bounds__(64 * kShareWaves, 8 / kShareWaves) void paged_atten
         return (long long)item_blocks<kSpan>(a, t, first) * items_of(a, t);
     };
     if (!deal<64 * kShareWaves, kShares, kLeastShare>(a, blockIdx.x, blocks_of, share)) return;
+    __syncthreads();  // `odd` is clear
 
     Pass pass(a);
     // The run behind the current one: its first tile's pages are asked for at the current one's

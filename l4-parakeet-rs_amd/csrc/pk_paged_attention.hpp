@@ -161,7 +161,38 @@ template <int kShares, int kLeast> __device__ __forceinline__ int share_of(long 
     return (int)(all >= kShares * kLeast ? ((block + 1) * kShares - 1) / all : block / kLeast);
 }
 
+__device__ __forceinline__ long long lane_value(long long v, int lane) {
+    return (long long)((unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+                       (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
+}
+
+// Up to 64 sequences: one a lane, each wave for itself (one sequence of 1900 e4m3 keys 12.4 us
+// against 12.8 through LDS, 16 of them 19.7 and 20.2).
+template <int kShares, int kLeast, class Blocks> __device__ __forceinline__ bool deal_wave(const PagedArgs& a, int index, Blocks blocks_of, Share& out) {
+    const int lane = threadIdx.x & 63;
+    const long long mine = lane < a.sequences ? blocks_of(sequence_of(a, lane)) : 0;
+    long long end = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const long long up = __shfl_up(end, off, 64);
+        if (lane >= off) end += up;
+    }
+    const long long all = lane_value(end, 63);
+    out.all = all;
+    out.from = uniform(share_begin<kShares, kLeast>(all, index));
+    out.to = uniform(share_begin<kShares, kLeast>(all, index + 1));
+    if (out.from >= out.to) return false;
+    const long long at = end - mine, last = out.to - 1;
+    out.seq = __builtin_ctzll(__ballot(at <= out.from && out.from < end));
+    out.last_seq = __builtin_ctzll(__ballot(at <= last && last < end));
+    out.offset = out.from - lane_value(at, out.seq);
+    out.last_offset = last - lane_value(at, out.last_seq);
+    return true;
+}
+
+// (No barrier with up to 64 sequences.)
 template <int kThreads, int kShares, int kLeast, class Blocks> __device__ __forceinline__ bool deal(const PagedArgs& a, int index, Blocks blocks_of, Share& out) {
+    if (a.sequences <= 64) return deal_wave<kShares, kLeast>(a, index, blocks_of, out);
     __shared__ long long wave_total[kThreads / 64], found_offset[2];
     __shared__ int found_seq[2];
     const int per = (a.sequences + kThreads - 1) / kThreads, s0 = threadIdx.x * per;
