@@ -539,9 +539,12 @@ template <int kD> __global__ __launch_bounds__(kJoinGroups * kD / 4) void paged_
 // One launch, a workgroup an item, where a full table's keys and values of a kv head are few
 // bytes: a CU reads about 33 bytes a ns, while shares take 12 to 13 us however little there is
 // (one sequence, 8 kv heads of 128, e4m3: 900 keys 9.5 us against 13.0, 1900 14.5 and 13.1;
-// fp16: 448 keys 9.1, 900 16.6 and 12.5).  With many sequences it is ahead further up, since
-// workgroups that end early make room (64 of 1900 e4m3 keys: 34 us against 45).
-constexpr long long kDirectBytes = 384 << 10;
+// fp16: 448 keys 9.1, 900 16.6 and 12.5).  With kManyItems it is ahead further up, since
+// workgroups that end early make room: 16 sequences of 1900 e4m3 keys 16 us against 20, 64 of
+// them 34 and 44, 200 83 and 103, 64 of 900 fp16 keys 48 and 52.  Four times as far (200 of
+// 4000) it is still 164 and 174 us, but a lone long sequence among idle ones waits for one CU.
+constexpr long long kDirectBytes = 384 << 10, kDirectBytesMany = 512 << 10;
+constexpr long long kManyItems = 128;
 // So do up to 32 rows of a kv head, in two tiles that read the same keys: one sequence of 24
 // rows, 448 keys, 7.3 us against 14.5 for a chunk's kernel, 64 of them of 1900 keys 65 and 95.
 // With four tiles the reading overtakes the gain (64 sequences of 48 rows, 1900 fp16 keys: 180
@@ -551,14 +554,14 @@ constexpr int kDirectRows = 32;
 // shares, 51 directly.
 constexpr int kChunkDirectKeys = 512;
 
-static bool rows_directly(int head_dim, int key_bytes, long long keys, long long rows) {
-    return keys * head_dim * key_bytes * 2 <= kDirectBytes && rows <= kDirectRows;
+static bool rows_directly(int head_dim, int key_bytes, long long keys, long long rows, long long items) {
+    return keys * head_dim * key_bytes * 2 <= (items >= kManyItems ? kDirectBytesMany : kDirectBytes) && rows <= kDirectRows;
 }
 
-// For either kind of cache: the fp16 one's, which is never less.
+// Enough for either kind of cache and for any smaller call: fewer sequences, queries or pages.
 size_t paged_attention_workspace(int head_dim, int page_shift, int max_pages, int max_rows) {
     const long long keys = (long long)max_pages << page_shift;
-    if (rows_directly(head_dim, 2, keys, max_rows)) return 0;
+    if (rows_directly(head_dim, 2, keys, max_rows, 0)) return 0;
     if (max_rows > 16) return keys <= kChunkDirectKeys ? 0 : paged_chunks_workspace(head_dim);
     return 2 * kShares * (head_dim == 128 ? sizeof(Part<128, 16>) : sizeof(Part<64, 16>)) + kShares * sizeof(Join);
 }
@@ -578,7 +581,7 @@ template <int kD, bool kF8> static void launch_rows(const PagedArgs& a, bool dir
 
 void launch_paged_attention(int kind, const PagedArgs& a, int head_dim, int max_queries, void* workspace, hipStream_t s) {
     const long long keys = (long long)a.max_pages << a.shift, rows = (long long)max_queries * a.group;
-    const bool direct = rows_directly(head_dim, kind == 1 ? 1 : 2, keys, rows);
+    const bool direct = rows_directly(head_dim, kind == 1 ? 1 : 2, keys, rows, (long long)a.sequences * a.kv_heads);
     if (rows > 16 && !direct) {
         launch_paged_chunks(kind, a, head_dim, keys <= kChunkDirectKeys, max_queries, workspace, s);
         return;

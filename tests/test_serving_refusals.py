@@ -114,6 +114,18 @@ def test_workspace_sizes_are_host_answers():
     assert pk.paged_attention_workspace_bytes(0, 0, 0, 16, 8, 128, 16, 400) >= 0
     for queries, kv, pages, none in ((5, 8, 48, True), (5, 8, 49, False), (5, 4, 48, True), (5, 2, 32, True), (5, 2, 33, False)):  # 10, 20, 40 rows
         assert (pk.paged_attention_workspace_bytes(5, queries, 2, 16, kv, 128, 16, pages) == 0) is none
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("page", [16, 256])
+def test_workspace_sizes_hold_for_smaller_calls(head_dim, page):
+    """A workspace for the largest step serves every step with fewer queries, sequences or pages."""
+    queries, sequences, pages = (1, 2, 4, 8, 16, 40, 300), (1, 15, 16, 64, 4096), [n for n in (1, 2, 3, 4, 6, 20, 32, 33, 48, 49, 64, 96, 97, 200, 4000)]
+    size = lambda q, s, p: pk.paged_attention_workspace_bytes(4096, q, s, 32, 8, head_dim, page, p)  # noqa: E731
+    for axis, line in ((0, queries), (1, sequences), (2, pages)):
+        for at in ((8, 16, 40), (40, 16, 33), (1, 1, 200), (300, 64, 4000), (4, 16, 3)):
+            sizes = [size(*(at[:axis] + (x,) + at[axis + 1:])) for x in line]
+            assert sizes == sorted(sizes), (axis, at)
     with pytest.raises(pk.PkError):
         pk.paged_attention_workspace_bytes(5, 5, 2, 16, 8, 100, 16, 400)
 
