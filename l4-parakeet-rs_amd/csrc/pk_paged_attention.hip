@@ -25,13 +25,15 @@ struct Rows {
 
 // One wave's pass over key tiles for 16 query rows.  Loads are issued a stage ahead: the
 // next tile's keys before the softmax, its values behind the products, and page ids two
-// tiles ahead, since loads return in order.
-template <int kD, bool kF8, int kWaves> struct RowPass {
+// tiles ahead.
+constexpr int kRowWaves = 4;  // of a workgroup; a CU holds two of them
+
+template <int kD, bool kF8> struct RowPass {
     static constexpr int kSteps = kD / 32, kBlocks = kD / 16;  // MFMA steps of S over features, feature blocks of O
     static constexpr int kU = kF8 ? 2 : 1, kKeys = 32 * kU;    // 16 bytes of a value row hold 8 * kU keys; keys a wave tile
     static constexpr int kBytes = kF8 ? 1 : 2;
     static constexpr int kLoads = kSteps / kU;                 // 16-byte loads of a key row
-    static constexpr int kSpan = kWaves * kKeys;               // keys that the waves take at once
+    static constexpr int kSpan = kRowWaves * kKeys;            // keys that the waves take at once
 
     // The pages of a tile, by 16 keys, in scalar registers: their loads go through the scalar
     // cache, out of the way of the cache's, which return in order.
@@ -235,12 +237,12 @@ template <int kD, bool kF8, int kWaves> struct RowPass {
 };
 
 // What the waves hold of 16 rows, side by side in LDS.
-template <int kD, int kWaves> struct Parts {
-    float acc[kWaves][16][kD + 4];
-    float top[kWaves][16], total[kWaves][16];
+template <int kD> struct Parts {
+    float acc[kRowWaves][16][kD + 4];
+    float top[kRowWaves][16], total[kRowWaves][16];
 };
 
-template <int kD, bool kF8, int kWaves> __device__ __forceinline__ void to_lds(RowPass<kD, kF8, kWaves>& pass, Parts<kD, kWaves>& parts) {
+template <int kD, bool kF8> __device__ __forceinline__ void to_lds(RowPass<kD, kF8>& pass, Parts<kD>& parts) {
     const int wave = threadIdx.x >> 6;
     const float total = add_level(add_level(pass.total, 16), 32);
 #pragma unroll
@@ -252,16 +254,16 @@ template <int kD, bool kF8, int kWaves> __device__ __forceinline__ void to_lds(R
 }
 
 // Row r of the joined waves: its maximum and sum, and kN features from d0 on.
-template <int kD, int kWaves, int kN> __device__ __forceinline__ void join(const Parts<kD, kWaves>& parts, int r, int d0, float& best, float& total, float (&v)[kN]) {
+template <int kD, int kN> __device__ __forceinline__ void join(const Parts<kD>& parts, int r, int d0, float& best, float& total, float (&v)[kN]) {
     best = parts.top[0][r];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) best = __builtin_fmaxf(best, parts.top[w][r]);
+    for (int w = 1; w < kRowWaves; ++w) best = __builtin_fmaxf(best, parts.top[w][r]);
     const float base = best == kNegInf ? 0.0f : best;
     total = 0.0f;
 #pragma unroll
     for (int j = 0; j < kN; ++j) v[j] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kRowWaves; ++w) {
         const float f = __builtin_amdgcn_exp2f(parts.top[w][r] - base);
         total += parts.total[w][r] * f;
 #pragma unroll
@@ -281,14 +283,12 @@ template <int kD, int kN> __device__ __forceinline__ bool put_odd(const Odd<kD, 
 // Short contexts: one workgroup for the keys of a (sequence, kv head, 16 rows).
 // A single token's 93 keys, 8 heads, fp16: 5.3 us, of which a launch is 2.5 and the rest the
 // chain length -> page id -> keys -> scores -> values -> the waves' join.
-constexpr int kDirectWaves = 4;
-
-template <int kD, bool kF8> __global__ __launch_bounds__(64 * kDirectWaves, 2) void paged_attention_rows_kernel(PagedArgs a) {
-    constexpr int kN = kD / (4 * kDirectWaves);
-    using Pass = RowPass<kD, kF8, kDirectWaves>;
-    __shared__ Parts<kD, kDirectWaves> parts;
+template <int kD, bool kF8> __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_attention_rows_kernel(PagedArgs a) {
+    constexpr int kN = kD / (4 * kRowWaves);
+    using Pass = RowPass<kD, kF8>;
+    __shared__ Parts<kD> parts;
     __shared__ Odd<kD, 16> odd;
-    odd.clear(64 * kDirectWaves);
+    odd.clear(64 * kRowWaves);
     __syncthreads();
     const Rows w = {wave_sequence(a, blockIdx.z), (int)blockIdx.z, (int)blockIdx.x, (int)blockIdx.y * 16};
     if (w.row0 >= w.t.rows) return;
@@ -302,7 +302,7 @@ template <int kD, bool kF8> __global__ __launch_bounds__(64 * kDirectWaves, 2) v
     pass.run(w, k0, end, odd, false, w, 0, {});
     to_lds(pass, parts);
     __syncthreads();
-    const int r = threadIdx.x / (4 * kDirectWaves), d0 = threadIdx.x % (4 * kDirectWaves) * kN;
+    const int r = threadIdx.x / (4 * kRowWaves), d0 = threadIdx.x % (4 * kRowWaves) * kN;
     if (r > w.last()) return;
     float best, total, v[kN];
     join(parts, r, d0, best, total, v);
@@ -324,7 +324,6 @@ template <int kD, bool kF8> __global__ __launch_bounds__(64 * kDirectWaves, 2) v
 // them alike.  More, smaller shares even that out but pay more beginnings and parts: 1024 take
 // 102 and 116 us, 2048 110 and 123.  One sequence of 131072 fp16 keys, 2 kv heads (134 MB): 31
 // us, of which 5 are the way to the first keys.
-constexpr int kShareWaves = 4;
 constexpr int kShares = 512;  // two workgroups on each of 256 CUs
 constexpr int kLeastShare = 2;  // one sequence of 1900 e4m3 keys 13.1 us; with 1 14.7, with 4 15.4
 
@@ -369,20 +368,20 @@ struct ShareRun {
 };
 
 template <int kD, bool kF8>
-__global__ __launch_bounds__(64 * kShareWaves, 8 / kShareWaves) void paged_attention_shares_kernel(PagedArgs a, Part<kD, 16>* slots, Join* joins) {
-    constexpr int kN = kD / (4 * kShareWaves);
-    using Pass = RowPass<kD, kF8, kShareWaves>;
+__global__ __launch_bounds__(64 * kRowWaves, 2) void paged_attention_shares_kernel(PagedArgs a, Part<kD, 16>* slots, Join* joins) {
+    constexpr int kN = kD / (4 * kRowWaves);
+    using Pass = RowPass<kD, kF8>;
     constexpr int kSpan = Pass::kSpan;
-    __shared__ Parts<kD, kShareWaves> parts;
+    __shared__ Parts<kD> parts;
     __shared__ Odd<kD, 16> odd;
-    odd.clear(64 * kShareWaves);
+    odd.clear(64 * kRowWaves);
     if (threadIdx.x == 0) joins[blockIdx.x].count = 0;
     Share share;
     const auto blocks_of = [&](const RowTile& t) {
         int first;
         return (long long)item_blocks<kSpan>(a, t, first) * items_of(a, t);
     };
-    if (!deal<64 * kShareWaves, kShares, kLeastShare>(a, blockIdx.x, blocks_of, share)) return;
+    if (!deal<64 * kRowWaves, kShares, kLeastShare>(a, blockIdx.x, blocks_of, share)) return;
     __syncthreads();  // `odd` is clear
 
     Pass pass(a);
@@ -401,7 +400,7 @@ __global__ __launch_bounds__(64 * kShareWaves, 8 / kShareWaves) void paged_atten
     tiles();
     pass.open(next.w, k0);
 
-    const int r = threadIdx.x / (4 * kShareWaves), d0 = threadIdx.x % (4 * kShareWaves) * kN;
+    const int r = threadIdx.x / (4 * kRowWaves), d0 = threadIdx.x % (4 * kRowWaves) * kN;
     for (bool more = true; more;) {
         const ShareRun now = next;
         const int now_k0 = k0, now_end = end;
@@ -425,10 +424,7 @@ __global__ __launch_bounds__(64 * kShareWaves, 8 / kShareWaves) void paged_atten
             const long long at = share.to - now.left;
             Part<kD, 16>& slot = slots[2 * blockIdx.x + (at == share.from ? 0 : 1)];
 #pragma unroll
-            for (int j = 0; j < kN; j += kN < 4 ? 2 : 4) {
-                if constexpr (kN < 4) *(float2*)&slot.acc[r][d0 + j] = float2{v[j], v[j + 1]};
-                else *(v4f*)&slot.acc[r][d0 + j] = v4f{v[j], v[j + 1], v[j + 2], v[j + 3]};
-            }
+            for (int j = 0; j < kN; j += 4) *(v4f*)&slot.acc[r][d0 + j] = v4f{v[j], v[j + 1], v[j + 2], v[j + 3]};
             if (d0 == 0) {
                 slot.top[r] = best;
                 slot.total[r] = total;
@@ -439,7 +435,7 @@ __global__ __launch_bounds__(64 * kShareWaves, 8 / kShareWaves) void paged_atten
         }
         if (any_odd) {
             __syncthreads();
-            odd.clear(64 * kShareWaves);
+            odd.clear(64 * kRowWaves);
             __syncthreads();
         }
     }
@@ -570,12 +566,12 @@ template <int kD, bool kF8> static void launch_rows(const PagedArgs& a, bool dir
     const unsigned rows = (unsigned)(max_queries * a.group);
     if (direct) {
         const dim3 grid((unsigned)a.kv_heads, (rows + 15) / 16, (unsigned)a.sequences);
-        paged_attention_rows_kernel<kD, kF8><<<grid, 64 * kDirectWaves, 0, s>>>(a);
+        paged_attention_rows_kernel<kD, kF8><<<grid, 64 * kRowWaves, 0, s>>>(a);
         return;
     }
     auto* slots = (Part<kD, 16>*)workspace;
     Join* joins = (Join*)(slots + 2 * kShares);
-    paged_attention_shares_kernel<kD, kF8><<<kShares, 64 * kShareWaves, 0, s>>>(a, slots, joins);
+    paged_attention_shares_kernel<kD, kF8><<<kShares, 64 * kRowWaves, 0, s>>>(a, slots, joins);
     paged_attention_join_kernel<kD><<<dim3(kShares / kJoinGroups, rows < 16 ? rows : 16), kJoinGroups * kD / 4, 0, s>>>(a, slots, joins);
 }
 

@@ -137,8 +137,7 @@ __device__ __forceinline__ void store_row(const PagedArgs& a, const RowTile& t, 
 #pragma unroll
     for (int j = 0; j < kN / 2; ++j) w[j] = (uint32_t)f2h(v[2 * j] * inv) | ((uint32_t)f2h(v[2 * j + 1] * inv) << 16);
     if constexpr (kN == 8) *(uint4*)op = uint4{w[0], w[1], w[2], w[3]};
-    else if constexpr (kN == 4) *(uint2*)op = uint2{w[0], w[1]};
-    else *(uint32_t*)op = w[0];
+    else *(uint2*)op = uint2{w[0], w[1]};
 }
 
 // The work of all sequences in a row, in blocks of keys, dealt to `shares` workgroups in
