@@ -271,13 +271,11 @@ template <int kD, int kN> __device__ __forceinline__ void join(const Parts<kD>& 
     }
 }
 
-template <int kD, int kN> __device__ __forceinline__ bool put_odd(const Odd<kD, 16>& odd, int r, int d0, float (&v)[kN]) {
-    const bool any = __builtin_amdgcn_readfirstlane((int)odd.any) != 0;
+template <int kD, int kN> __device__ __forceinline__ void put_odd(const Odd<kD, 16>& odd, bool any, int r, int d0, float (&v)[kN]) {
     if (__builtin_expect(any, 0)) {
 #pragma unroll
         for (int j = 0; j < kN; ++j) v[j] = odd.put(v[j], r, d0 + j);
     }
-    return any;
 }
 
 // Short contexts: one workgroup for the keys of a (sequence, kv head, 16 rows).
@@ -306,7 +304,7 @@ template <int kD, bool kF8> __global__ __launch_bounds__(64 * kRowWaves, 2) void
     if (r > w.last()) return;
     float best, total, v[kN];
     join(parts, r, d0, best, total, v);
-    put_odd(odd, r, d0, v);
+    put_odd(odd, odd.any != 0, r, d0, v);
     store_row<kN>(a, w.t, w.kvh, w.row0 + r, kD, d0, total, v);
 }
 
@@ -412,12 +410,15 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_attention_shares_kern
         }
         pass.clear();
         pass.run(now.w, now_k0, now_end, odd, more, next.w, k0, id);
-        __syncthreads();  // the previous item's parts are read
+        __syncthreads();  // the previous item's parts are read, and what this one's values hold is noted
+        // Between the barriers no wave is in a run: all waves find the same here, and take the
+        // same way to the next run, whose values are noted only after that.
+        const bool any_odd = __builtin_amdgcn_readfirstlane((int)odd.any) != 0;
         to_lds(pass, parts);
         __syncthreads();
         float best, total, v[kN];
         join(parts, r, d0, best, total, v);
-        const bool any_odd = put_odd(odd, r, d0, v);
+        put_odd(odd, any_odd, r, d0, v);
         if (now.n == now.blocks) {
             if (r <= now.w.last()) store_row<kN>(a, now.w.t, now.w.kvh, now.w.row0 + r, kD, d0, total, v);
         } else {
