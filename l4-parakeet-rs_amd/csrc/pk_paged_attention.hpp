@@ -3,6 +3,7 @@
 #pragma once
 
 #include "pk_kernels.hpp"
+#include "pk_paged_deal.hpp"
 
 namespace pk {
 
@@ -89,11 +90,6 @@ template <int kD, int kRows> struct Odd {
     }
 };
 
-// One sequence's view for a tile of 16 query rows.
-struct RowTile {
-    int start, rows, length, first_pos;  // first_pos: position of the sequence's first new token
-};
-
 __device__ __forceinline__ RowTile sequence_of(const PagedArgs& a, int s, int e, int len) {
     s = s < 0 ? 0 : (s > a.tokens ? a.tokens : s);
     e = e < s ? s : (e > a.tokens ? a.tokens : e);
@@ -116,13 +112,6 @@ __device__ __forceinline__ RowTile wave_sequence(const PagedArgs& a, int seq) {
     return sequence_of(a, scalar_at(a.starts, seq), scalar_at(a.starts, seq + 1), scalar_at(a.lengths, seq));
 }
 
-// Keys [lo, hi) that a query at `pos` sees.
-__device__ __forceinline__ void window(const PagedArgs& a, int pos, int length, int& lo, int& hi) {
-    lo = a.left < 0 || pos < a.left ? 0 : pos - a.left;
-    hi = a.right < 0 || length - pos <= a.right ? length : pos + a.right + 1;
-    if (hi < 0) hi = 0;
-}
-
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 __device__ __forceinline__ long long uniform(long long v) {
@@ -140,25 +129,14 @@ __device__ __forceinline__ void store_row(const PagedArgs& a, const RowTile& t, 
     else *(uint2*)op = uint2{w[0], w[1]};
 }
 
-// The work of all sequences in a row, in blocks of keys, dealt to `shares` workgroups in
-// contiguous shares that differ by one block at most, or of `least` blocks where there are
-// too few: every workgroup (kThreads threads) sums the blocks of all sequences and finds the
-// sequences that its share begins and ends in.
+// A workgroup's share of the work: every workgroup (kThreads threads) sums the blocks of all
+// sequences and finds the sequences that its share begins and ends in.
 struct Share {
     long long from, to, all;  // its blocks, and the blocks of all shares
     long long offset;          // blocks of `seq` before `from`
     long long last_offset;     // and of `last_seq` before `to` - 1
     int seq, last_seq;
 };
-
-template <int kShares, int kLeast> __device__ __forceinline__ long long share_begin(long long all, int index) {
-    if (all >= kShares * kLeast) return index * all / kShares;
-    return index * kLeast < all ? index * kLeast : all;
-}
-// The share that holds a block: the last one that begins at or before it.
-template <int kShares, int kLeast> __device__ __forceinline__ int share_of(long long all, long long block) {
-    return (int)(all >= kShares * kLeast ? ((block + 1) * kShares - 1) / all : block / kLeast);
-}
 
 __device__ __forceinline__ long long lane_value(long long v, int lane) {
     return (long long)((unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |

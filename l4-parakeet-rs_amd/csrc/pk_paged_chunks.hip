@@ -21,47 +21,12 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 
 namespace pk {
 
-constexpr int kChunkWaves = 8, kChunkThreads = 64 * kChunkWaves, kChunkRows = 32 * kChunkWaves;
-constexpr int kTileKeys = 64, kBuffers = 4;
+constexpr int kChunkWaves = 8, kChunkThreads = 64 * kChunkWaves, kBuffers = 4;
+static_assert(kChunkRows == 32 * kChunkWaves);
 constexpr int kChunkShares = 256;  // a workgroup on each of 256 CUs
 // Fewer blocks a share than this are more parts to join than work: 100 tokens over 3000 keys, 8 kv
 // heads of 4: 47 us, with one block at least 117, with twelve 52; 24 rows over 1900 keys 25, 41, 34.
 constexpr int kLeastChunkShare = 4;
-
-// Blocks (tiles of keys) that the rows of one row tile see, from block `first` on.
-__device__ __forceinline__ int chunk_blocks(const PagedArgs& a, const RowTile& t, int tile, int& first) {
-    const int r0 = tile * kChunkRows, r1 = r0 + kChunkRows < t.rows ? r0 + kChunkRows - 1 : t.rows - 1;
-    int lo, hi, none;
-    window(a, t.first_pos + r0 / a.group, t.length, lo, none);
-    window(a, t.first_pos + r1 / a.group, t.length, none, hi);
-    first = lo / kTileKeys;
-    const int n = (hi + kTileKeys - 1) / kTileKeys - first;
-    return n > 0 ? n : 1;
-}
-
-// With a causal mask the row tiles of a sequence differ in length; tile j and tile n - 1 -
-// j together hardly do (their keys are concave in j, and the blocks of a tile less than two
-// more than its keys), so they are dealt as one item of `pair` blocks, at least what any pair
-// has; the middle tile of an odd number is an item by itself.  Keys are not concave where the
-// first rows stand before key 0 and see nothing (more new tokens than keys): a pair then has
-// room for two tiles of all keys.
-struct Pairs {
-    int tiles, pair, middle;
-    long long per_head;
-};
-__device__ __forceinline__ Pairs pairs_of(const PagedArgs& a, const RowTile& t) {
-    Pairs p{};
-    p.tiles = (t.rows + kChunkRows - 1) / kChunkRows;
-    if (p.tiles == 0) return p;
-    int first;
-    const int mid = chunk_blocks(a, t, p.tiles / 2, first);
-    if (p.tiles & 1) p.middle = mid;
-    const int all = (t.length + kTileKeys - 1) / kTileKeys;
-    if (p.tiles > 1 && a.right >= 0 && t.first_pos + a.right + 1 < 0) p.pair = 2 * (all > 1 ? all : 1);
-    else if (p.tiles > 1) p.pair = mid + chunk_blocks(a, t, (p.tiles - 1) / 2, first) + 3;
-    p.per_head = (long long)(p.tiles / 2) * p.pair + p.middle;
-    return p;
-}
 
 template <int kD, bool kF8> struct ChunkPass {
     static constexpr int kBytes = kF8 ? 1 : 2;
@@ -490,34 +455,6 @@ template <int kD, bool kF8> __global__ __launch_bounds__(kChunkThreads, 2) void 
     pass.run(first, first + blocks, tick, odd);
     __syncthreads();
     pass.finish(true, nullptr, odd, odd.any != 0);
-}
-
-// A row tile's blocks among its sequence's: `tile` < 0 where a pair has blocks too many.
-struct Span {
-    int kvh, tile, first;      // first: the block of keys that the tile begins with
-    int at, blocks;            // the place in the span, and the span's length
-};
-__device__ __forceinline__ Span span_at(const PagedArgs& a, const RowTile& t, const Pairs& p, long long offset) {
-    Span s;
-    s.kvh = (int)(offset / p.per_head);
-    const int in_head = (int)(offset - s.kvh * p.per_head);
-    const int pair = p.pair ? in_head / p.pair : 0;
-    const bool middle = pair == p.tiles / 2;
-    s.tile = pair;
-    s.at = in_head - pair * p.pair;
-    s.blocks = chunk_blocks(a, t, s.tile, s.first);
-    if (!middle && s.at >= s.blocks) {
-        s.at -= s.blocks;
-        const int rest = p.pair - s.blocks;
-        s.tile = p.tiles - 1 - pair;
-        s.blocks = chunk_blocks(a, t, s.tile, s.first);
-        if (s.at >= s.blocks) {
-            s.at -= s.blocks;
-            s.blocks = rest - s.blocks;
-            s.tile = -1;
-        }
-    }
-    return s;
 }
 
 template <int kD, bool kF8>
