@@ -119,6 +119,10 @@ __global__ __launch_bounds__(256) void rms_norm_quantize_kernel(const uint16_t* 
     if (lane == 0) scales[row] = scale;
 }
 
+// A launch has fewer than 2^32 threads in a dimension (a larger grid wraps, without an
+// error): more rows than this, of 64 or 256 threads, go in several launches.
+constexpr int kMostRows = 1 << 23;
+
 template <bool kInt8>
 static void launch_rms(const uint16_t* in, const uint16_t* residual, const uint16_t* w, uint16_t* r_out, uint8_t* out, float* scales,
                        int rows, int width, float eps, hipStream_t s) {
@@ -139,8 +143,18 @@ static void launch_rms(const uint16_t* in, const uint16_t* residual, const uint1
 
 void launch_rms_norm_quantize(int kind, const uint16_t* in, const uint16_t* residual, const uint16_t* w, uint16_t* r_out, void* out,
                               float* scales, int rows, int width, float eps, hipStream_t s) {
-    if (kind == 1) launch_rms<true>(in, residual, w, r_out, (uint8_t*)out, scales, rows, width, eps, s);
-    else launch_rms<false>(in, residual, w, r_out, (uint8_t*)out, scales, rows, width, eps, s);
+    for (int done = 0; rows > 0; done = kMostRows) {
+        const size_t skip = (size_t)done * width;
+        in += skip;
+        if (residual) residual += skip;
+        if (r_out) r_out += skip;
+        out = (uint8_t*)out + skip;
+        scales += done;
+        const int part = rows < kMostRows ? rows : kMostRows;
+        if (kind == 1) launch_rms<true>(in, residual, w, r_out, (uint8_t*)out, scales, part, width, eps, s);
+        else launch_rms<false>(in, residual, w, r_out, (uint8_t*)out, scales, part, width, eps, s);
+        rows -= part;
+    }
 }
 
 }  // namespace pk
