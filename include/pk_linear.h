@@ -672,7 +672,7 @@ int32_t pk_rms_norm_quantize(int32_t kind, const uint16_t* input, const uint16_t
  * The levels q - z (weight_zeros whole numbers 0..15) multiply exactly and the
  * scale is applied to the group's sum in fp32, where pk_linear_int4g128 rounds
  * each dequantized weight to fp16 first.  The INT8 form's group sums are exact.
- * n up to 2^30, k % 128 == 0 up to 65536; input and weight_q 16-byte aligned, bias
+ * n below 2^29, k % 128 == 0 up to 65536; input and weight_q 16-byte aligned, bias
  * may be NULL; fp16 or fp32 output [m x n], apart from every input. */
 int32_t pk_gemv_int4g128(const uint16_t* input, const uint32_t* weight_q, const uint16_t* weight_scales,
                          const uint16_t* weight_zeros, const float* bias, void* output, int32_t output_fp32, int32_t m,

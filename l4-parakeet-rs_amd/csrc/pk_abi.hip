@@ -917,8 +917,9 @@ int32_t pk_rms_norm_quantize(int32_t kind, const uint16_t* input, const uint16_t
 
 static int32_t gemv(const void* input, const float* input_scales, const uint32_t* q, const uint16_t* scales, const uint16_t* zeros,
                     const float* bias, void* output, int32_t output_fp32, int32_t m, int32_t n, int32_t k, void* stream) {
-    if (m < 0 || m > 16 || n < 0 || n > 1 << 30 || k <= 0 || k % 128 || k > 65536) {
-        set_error("int4g128 gemv needs m <= 16, n <= 2^30 and k %% 128 == 0 up to 65536 (m=%d n=%d k=%d); pk_linear_int4g128 takes more rows",
+    // 64 rows a workgroup of 512 threads: 2^29 rows would be 2^32 threads, and such a grid wraps without an error
+    if (m < 0 || m > 16 || n < 0 || n >= 1 << 29 || k <= 0 || k % 128 || k > 65536) {
+        set_error("int4g128 gemv needs m <= 16, n < 2^29 and k %% 128 == 0 up to 65536 (m=%d n=%d k=%d); pk_linear_int4g128 takes more rows",
                   m, n, k);
         return PK_E_SHAPE;
     }
