@@ -108,8 +108,9 @@ __global__ __launch_bounds__(256) void page_plan_kernel(const int* __restrict__ 
     }
     __syncthreads();
 
-    const int at = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
-    for (int i = at; i < requests; i += step) {
+    // unsigned: behind the last of 2^31 - 1 slots the next index is still one that ends the loop
+    const uint32_t at = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
+    for (uint32_t i = at; i < (uint32_t)requests; i += step) {
         starts[i + 1] = status ? 0 : ends[i];
         lengths[i] = status ? held[i] : held[i] + added[i];
     }
@@ -120,17 +121,17 @@ __global__ __launch_bounds__(256) void page_plan_kernel(const int* __restrict__ 
         info[2] = status;
         info[3] = 0;
     }
-    for (int i = at; i < n_pages; i += step) {
-        const int r = owner_of(page_ends, requests, i);
+    for (uint32_t i = at; i < (uint32_t)n_pages; i += step) {
+        const int r = owner_of(page_ends, requests, (int)i);
         const int have = (held[r] + round) >> shift;
-        table[(size_t)r * max_pages + have + i - (r ? page_ends[r - 1] : 0)] = free_pages[begin + i];
+        table[(size_t)r * max_pages + have + (int)i - (r ? page_ends[r - 1] : 0)] = free_pages[begin + (int)i];
     }
-    for (int t = at; t < capacity; t += step) {
+    for (uint32_t t = at; t < (uint32_t)capacity; t += step) {
         int slot = -1, pos = 0;
-        if (t < n_tokens) {
-            const int r = owner_of(ends, requests, t);
+        if (t < (uint32_t)n_tokens) {
+            const int r = owner_of(ends, requests, (int)t);
             const int h = held[r], have = (int)(((long long)h + round) >> shift);
-            pos = h + t - (r ? ends[r - 1] : 0);
+            pos = h + (int)t - (r ? ends[r - 1] : 0);
             const int page = pos >> shift;
             // a page of this step is read from the free list: the table entry is another workgroup's to write
             const int id = page < have ? table[(size_t)r * max_pages + page] : free_pages[begin + (r ? page_ends[r - 1] : 0) + page - have];
@@ -146,7 +147,7 @@ void launch_page_plan(const int* held, const int* added, const int* free_pages, 
                       int* starts, int* lengths, int* slots, int* positions, int* info, int requests, int max_pages, int page_shift,
                       int capacity, hipStream_t s) {
     const int work = capacity > requests ? capacity : requests;
-    const int grid = work <= 256 ? 1 : (work + 255) / 256 < 256 ? (work + 255) / 256 : 256;
+    const int grid = work > 65536 - 256 ? 256 : (work > 256 ? (work + 255) / 256 : 1);
     const auto launch = [&](auto kernel) {
         kernel<<<grid, 256, (size_t)requests * 8, s>>>(held, added, free_pages, free_range, free_capacity, table, starts, lengths, slots, positions,
                                                        info, requests, max_pages, page_shift, capacity);

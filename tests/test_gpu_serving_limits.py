@@ -23,3 +23,19 @@ def test_norm_of_more_rows_than_a_launch_has_threads_for(pk, int8):  # noqa: F81
     pk.rms_norm_quantize(int(int8), many, many, w, h, out, scales, 1e-5)
     assert torch.equal(scales, want_scales.repeat(times)[:rows])
     assert torch.equal(out, want.repeat(times, 1)[:rows]) and torch.equal(h, want_h.repeat(times, 1)[:rows])
+
+
+def test_plan_of_the_most_slots(pk):  # noqa: F811
+    """2^31 - 1 slots: those behind the last token are -1 up to the end, and nothing behind them is written."""
+    capacity = 2**31 - 1
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    held, added, free, table = i32(5, 0, 20), i32(3, 0, 40), i32(*range(100, 110)), torch.full((3, 4), 7, dtype=torch.int32, device="cuda")
+    starts, lengths, info = torch.empty(4, dtype=torch.int32, device="cuda"), torch.empty(3, dtype=torch.int32, device="cuda"), i32(9, 9, 9, 9)
+    slots = torch.full((capacity + 1,), 5, dtype=torch.int32, device="cuda")
+    pk.page_plan(held, added, free, i32(0, 10), table, starts, lengths, slots[:capacity], None, info, 16)
+    assert info.tolist() == [43, 2, 0, 0] and lengths.tolist() == [8, 0, 60] and starts.tolist() == [0, 3, 3, 43]
+    assert slots[:3].tolist() == [7 * 16 + 5, 7 * 16 + 6, 7 * 16 + 7] and slots[3:43].tolist() == [
+        page * 16 + i for page, i in [(7, j) for j in range(4, 16)] + [(100, j) for j in range(16)] + [(101, j) for j in range(12)]]
+    for part in slots[43:capacity].split(1 << 28):
+        assert (part == -1).all()
+    assert slots[capacity] == 5
