@@ -275,7 +275,10 @@ template <int kD, bool kF8> struct ChunkPass {
     // fp32 as those up to 1, and the output so far is rarely rescaled.
     static constexpr float kSlack = 8.0f;
     // Scores -> probabilities as operands; the sums so far are scaled to the new maximum.
-    __device__ __forceinline__ void soften(const v16f (&sc)[2], v8h (&pf)[4]) {
+    // Scaling and subtraction are one step, in which the rounding of the scaled maximum, half a
+    // step of its own, becomes a factor of all probabilities: harmless up to 2^20, far outside
+    // fp16 from 2^28 on.  With kCareful the subtraction, exact near the maximum, comes first.
+    template <bool kCareful> __device__ __forceinline__ void soften(const v16f (&sc)[2], v8h (&pf)[4]) {
         const float m = max_level(max3(kNegInf, sc[0], sc[1]), 32);
         const bool far = (m - top) * scale > kSlack;  // also from -inf; false while nothing is seen
         if (__any(far)) {
@@ -285,12 +288,13 @@ template <int kD, bool kF8> struct ChunkPass {
 #pragma unroll
             for (int c = 0; c < kBlocks; ++c) acc[c] = acc[c] * keep;
         }
-        const float base = top == kNegInf ? 0.0f : top * scale;
+        const float from = top == kNegInf ? 0.0f : top, base = from * scale;
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[s >> 1][8 * (s & 1) + j], scale, -base));
+                const float score = sc[s >> 1][8 * (s & 1) + j];
+                const float p = __builtin_amdgcn_exp2f(kCareful ? (score - from) * scale : __builtin_fmaf(score, scale, -base));
                 total += p;
                 pf[s][j] = (_Float16)p;
             }
@@ -364,7 +368,7 @@ template <int kD, bool kF8> struct ChunkPass {
     // that tile, which read K(t) and V(t - 1), or of the next.  The waves that are behind
     // are at their last products when the others go on to the next tiles' first loads,
     // which go to other buffers than V(to - 1).
-    __device__ __forceinline__ void run(int from, int to, int& tick, Odd<kD, kChunkRows>& odd) {
+    template <bool kCareful> __device__ __forceinline__ void run(int from, int to, int& tick, Odd<kD, kChunkRows>& odd) {
         ring = (tick - from) & (kBuffers - 1);
         const bool behind = wave >= 4;
         uint32_t ok[3];  // pages of tiles b, b + 1, b + 2
@@ -398,7 +402,7 @@ template <int kD, bool kF8> struct ChunkPass {
             if (active) {
                 // a tile that none of the wave's rows sees has probabilities of zero and tidy values
                 if (edge && (b * kTileKeys < full_lo || (b + 1) * kTileKeys > full_hi || ok[0] != kAllPages)) mask(b, ok[0], sc);
-                soften(sc, pf);
+                soften<kCareful>(sc, pf);
             }
             step = step_of(b + 4, next, b + 3, ids, to);
             meet();
@@ -409,6 +413,34 @@ template <int kD, bool kF8> struct ChunkPass {
         if (active) products<false, true>(to, sc, pf);
         tick += to - from;
         if (!behind) meet();
+    }
+
+    // Whether a row of this wave may have come out wrong in a run without care: its maximum is
+    // large, or its sums are not finite (early probabilities may have been too large for fp16).
+    __device__ __forceinline__ bool doubtful() const {
+        v16f sums = acc[0];
+#pragma unroll
+        for (int c = 1; c < kBlocks; ++c) sums += acc[c];
+#pragma unroll
+        for (int n = 8; n > 0; n >>= 1)
+#pragma unroll
+            for (int j = 0; j < n; ++j) sums[j] += sums[j + n];
+        const bool far = top != kNegInf && !(__builtin_fabsf(top * scale) < (float)(1 << 20));
+        return last >= 0 && __any(far || !(__builtin_fabsf(sums[0] + total) < __builtin_inff()));
+    }
+    // A row tile's tiles [from, to), all of them read by all waves at the end.  Where a wave has
+    // doubts all start again, with care: it costs a second pass, and only these calls.
+    __device__ __forceinline__ void attend(int seq, const RowTile& rows, int tile, int from, int to, int& tick, Odd<kD, kChunkRows>& odd, int& again) {
+        start(seq, rows, tile);
+        run<false>(from, to, tick, odd);
+        if (doubtful()) again = 1;
+        __syncthreads();
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(again) != 0, 0)) {
+            start(seq, rows, tile);
+            run<true>(from, to, tick, odd);  // (its first barrier stands behind all reads of `again`)
+            if (threadIdx.x == 0) again = 0;
+            __syncthreads();
+        }
     }
 
     // The lane's row (unless it repeats the last) of the output, or of a part.
@@ -444,16 +476,16 @@ template <int kD, bool kF8> struct ChunkPass {
 template <int kD, bool kF8> __global__ __launch_bounds__(kChunkThreads, 2) void paged_chunks_direct_kernel(PagedArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[kBuffers * ChunkPass<kD, kF8>::kBuffer];
     __shared__ Odd<kD, kChunkRows> odd;
+    __shared__ int again;
     odd.clear(kChunkThreads);
+    if (threadIdx.x == 0) again = 0;
     const int kvh = blockIdx.x, seq = blockIdx.z, tile = blockIdx.y;
     const RowTile t = wave_sequence(a, seq);
     if (tile * kChunkRows >= t.rows) return;
     int first, tick = 0;
     const int blocks = chunk_blocks(a, t, tile, first);
     ChunkPass<kD, kF8> pass(a, lds, kvh);
-    pass.start(seq, t, tile);
-    pass.run(first, first + blocks, tick, odd);
-    __syncthreads();
+    pass.attend(seq, t, tile, first, first + blocks, tick, odd, again);
     pass.finish(true, nullptr, odd, odd.any != 0);
 }
 
@@ -461,7 +493,9 @@ template <int kD, bool kF8>
 __global__ __launch_bounds__(kChunkThreads, 2) void paged_chunks_shares_kernel(PagedArgs a, Part<kD, kChunkRows>* slots, Join* joins) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[kBuffers * ChunkPass<kD, kF8>::kBuffer];
     __shared__ Odd<kD, kChunkRows> odd;
+    __shared__ int again;
     odd.clear(kChunkThreads);
+    if (threadIdx.x == 0) again = 0;
     // neighbouring shares read the same keys: they go to one XCD's L2
     const int index = (blockIdx.x & 7) * (kChunkShares / 8) + (blockIdx.x >> 3);
     if (threadIdx.x == 0) joins[index].count = 0;
@@ -489,9 +523,7 @@ __global__ __launch_bounds__(kChunkThreads, 2) void paged_chunks_shares_kernel(P
         const int n = to - at < s.blocks - s.at ? (int)(to - at) : s.blocks - s.at;
         if (s.tile >= 0) {
             ChunkPass<kD, kF8> pass(a, lds, s.kvh);
-            pass.start(seq, t, s.tile);
-            pass.run(s.first + s.at, s.first + s.at + n, tick, odd);
-            __syncthreads();
+            pass.attend(seq, t, s.tile, s.first + s.at, s.first + s.at + n, tick, odd, again);
             const int which = at == share.from ? 0 : 1;
             const bool any_odd = __builtin_amdgcn_readfirstlane((int)odd.any) != 0;
             pass.finish(n == s.blocks, slots + 2 * index + which, odd, any_odd);

@@ -1,0 +1,58 @@
+"""Paged attention over keys and values made so that each answer is known in closed form."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_parity import pk  # noqa: E402, F401
+from test_gpu_paged_attention import Case  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+STEP = 32  # every 32nd key is a strong one: each wave and each part of the keys has some
+
+# one launch; shares of several sequences' keys; chunks directly and in shares
+SHAPES = [([(1, 700)], 0), ([(1, 700), (2, 300)], 6000), ([(1, 2500)] * 130, 0), ([(40, 500)], 0), ([(40, 3001), (77, 2000)] * 20, 6000)]
+
+
+def put(c, key_or_value, r, token, feature, x, scale):
+    """Feature `feature` of tokens `token` (a slice) of sequence r, all kv heads."""
+    cache = c.key if key_or_value == "key" else c.value.transpose(2, 3)
+    at = torch.arange(c.lengths_[r], device="cuda")[token]
+    x = torch.tensor(x / scale, device="cuda")
+    cache[c.table[r].long()[at // c.page], :, at % c.page, feature] = x.to(torch.float8_e4m3fn).view(torch.uint8) if c.fp8 else x.half()
+
+
+def strong_and_weak(shape, wider, fp8, far):
+    """Every STEP-th key has score `far` and value 1 in feature 1, the others score 0 and value 128 in feature 0; (case, scale)."""
+    Case.wider = wider
+    try:
+        c = Case(shape, heads=2, kv=1, d=128, fp8=fp8, seed=5)
+    finally:
+        Case.wider = 0
+    c.key.zero_()
+    c.value.zero_()
+    c.q.zero_()
+    c.q[:, :, 0] = 8
+    for r in range(len(shape)):
+        put(c, "key", r, slice(0, None, STEP), 0, 8 * c.key_scale, c.key_scale)
+        put(c, "value", r, slice(0, None), 0, 128.0, c.value_scale)
+        put(c, "value", r, slice(0, None, STEP), 0, 0.0, c.value_scale)
+        put(c, "value", r, slice(0, None, STEP), 1, 1.0, c.value_scale)
+    return c, far / (64 * c.key_scale)
+
+
+@pytest.mark.parametrize("shape,wider", SHAPES)
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("far", [3e5, 1e7, 1e9, 1e12, 1e20, -1e9])
+def test_huge_scores(pk, shape, wider, fp8, far):  # noqa: F811
+    """Scores whose fp32 steps are larger than 1: equal ones still share the sum equally, the others have none of it."""
+    c, _ = strong_and_weak(shape, wider, fp8, 1.0)
+    c.q[:, :, 0] = 7
+    for r in range(len(shape)):
+        put(c, "key", r, slice(0, None, STEP), 0, 9 * c.key_scale, c.key_scale)
+    got = c.run(pk, scale=far / (63 * c.key_scale))[:sum(c.counts)]
+    if far > 0:
+        assert (got[:, :, 1] == 1).all() and not got[:, :, 0].any() and not got[:, :, 2:].any()
+    else:  # the strong keys are the weak ones then; the first of a sequence's keys is a strong one
+        alone = torch.tensor([length - n + i == 0 for n, length in shape for i in range(n)], device="cuda")
+        assert not got[~alone][:, :, 1:].any() and (got[~alone][:, :, 0] == 128).all() and (got[alone][:, :, 1] == 1).all()
