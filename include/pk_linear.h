@@ -736,7 +736,8 @@ int32_t pk_paged_cache_write(int32_t kind, const uint16_t* key, int64_t key_stri
  * tokens <= 2^20, sequences <= 4096, max_queries * heads / kv_heads <= 2^23.
  * Scores, the running maximum and sum and the output's sum are fp32; scores
  * multiply fp16 queries with fp16 or e4m3 keys exactly, probabilities are
- * rounded to fp16 for the second product (their sum is not).
+ * rounded to fp16 for the second product (their sum is not), which keeps those
+ * down to 2^-21 of a row's largest to full precision and those down to 2^-31.
  * A row's fp32 sums are cut alike whatever stands beside it where a full table
  * holds at most 384 KB of keys and values a kv head (512 KB with sequences *
  * kv_heads >= 128) and max_queries * heads / kv_heads <= 32.  Larger work is dealt in equal shares of the whole batch's keys.

@@ -27,6 +27,11 @@ struct Rows {
 // next tile's keys before the softmax, its values behind the products, and page ids two
 // tiles ahead.
 constexpr int kRowWaves = 4;  // of a workgroup; a CU holds two of them
+// The largest probability is 2^kLift, not 1 (the division by the sum takes it out again): fp16
+// then holds those down to 2^-29 of it to full precision and down to 2^-39 at all, where 2^-14
+// and 2^-24 left out small ones that the sum counts and that are many in a long context.
+// 2^15 times a value of 65504 and 2^30 keys stays far inside fp32.
+constexpr float kLift = 15.0f;
 
 template <int kD, bool kF8> struct RowPass {
     static constexpr int kSteps = kD / 32, kBlocks = kD / 16;  // MFMA steps of S over features, feature blocks of O
@@ -195,7 +200,7 @@ template <int kD, bool kF8> struct RowPass {
             v8h pf[kU];
 #pragma unroll
             for (int j = 0; j < 8 * kU; ++j) {
-                p[j] = __builtin_amdgcn_exp2f(p[j] - base);
+                p[j] = __builtin_amdgcn_exp2f((p[j] - base) + kLift);  // in this order: base - kLift would be rounded
                 sum += p[j];
                 pf[j >> 3][j & 7] = (_Float16)p[j];
             }

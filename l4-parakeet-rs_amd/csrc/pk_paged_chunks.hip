@@ -271,9 +271,11 @@ template <int kD, bool kF8> struct ChunkPass {
         return m;
     }
     // Scores are taken relative to a running maximum that is only raised where a row's
-    // falls kSlack short (factors of two): probabilities up to 2^8 are as exact in fp16 and
-    // fp32 as those up to 1, and the output so far is rarely rescaled.
-    static constexpr float kSlack = 8.0f;
+    // falls kSlack short (factors of two), so that the output so far is rarely rescaled.
+    // Probabilities are 2^kLift at that maximum and at most 2^15: fp16 then holds those down to
+    // 2^-21 of it to full precision and down to 2^-31 at all, so that the sum counts no small
+    // ones that the output leaves out.
+    static constexpr float kSlack = 8.0f, kLift = 15.0f - kSlack;
     // Scores -> probabilities as operands; the sums so far are scaled to the new maximum.
     // Scaling and subtraction are one step, in which the rounding of the scaled maximum, half a
     // step of its own, becomes a factor of all probabilities: harmless up to 2^20, far outside
@@ -288,13 +290,13 @@ template <int kD, bool kF8> struct ChunkPass {
 #pragma unroll
             for (int c = 0; c < kBlocks; ++c) acc[c] = acc[c] * keep;
         }
-        const float from = top == kNegInf ? 0.0f : top, base = from * scale;
+        const float from = top == kNegInf ? 0.0f : top, base = from * scale - kLift;
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float score = sc[s >> 1][8 * (s & 1) + j];
-                const float p = __builtin_amdgcn_exp2f(kCareful ? (score - from) * scale : __builtin_fmaf(score, scale, -base));
+                const float p = __builtin_amdgcn_exp2f(kCareful ? (score - from) * scale + kLift : __builtin_fmaf(score, scale, -base));
                 total += p;
                 pf[s][j] = (_Float16)p;
             }

@@ -1,8 +1,12 @@
-"""Paged attention over keys and values made so that each answer is known in closed form."""
+"""Paged attention over keys and values made so that each answer is known in closed form: probabilities far below the
+largest one, scores of any size."""
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
+import serving_plain as plain  # noqa: E402
 from test_gpu_parity import pk  # noqa: E402, F401
 from test_gpu_paged_attention import Case  # noqa: E402
 
@@ -39,6 +43,30 @@ def strong_and_weak(shape, wider, fp8, far):
         put(c, "value", r, slice(0, None, STEP), 0, 0.0, c.value_scale)
         put(c, "value", r, slice(0, None, STEP), 1, 1.0, c.value_scale)
     return c, far / (64 * c.key_scale)
+
+
+@pytest.mark.parametrize("shape,wider", SHAPES)
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("far", [10.0, 14.5, 16.3, 17.6, 19.5])
+def test_many_small_probabilities(pk, shape, wider, fp8, far):  # noqa: F811
+    """Keys whose probability is e^-19 of the largest are not left out of the output, however many there are."""
+    c, scale = strong_and_weak(shape, wider, fp8, far)
+    got = c.run(pk, scale=scale).double().cpu()
+    # two roundings to fp16 (probability and output); scores of up to 28 factors of two with four roundings; sums over at
+    # most 64 products a step and, for these shapes, 200 steps, waves and parts, some of which truncate.  fp16 has no step
+    # below 2^-24: next to a largest probability of 2^7 at least, each is also off by up to 2^-25 / 2^7 of that one, all
+    # equal ones to the same side
+    rel, each = 2 * plain.U16 + (4 * 28 + 2 * 264) * plain.U32, 2.0**-32
+    for r, (n, length) in enumerate(shape):
+        for i in range(n):
+            seen = length - n + i + 1
+            strong = -(-seen // STEP)
+            weak = (seen - strong) * math.exp(-far)
+            row = got[sum(c.counts[:r]) + i]
+            for feature, want in ((0, 128 * weak / (strong + weak)), (1, strong / (strong + weak))):
+                bound = want * rel + plain.TINY16 + 128 * (seen - strong) * each / (strong + weak)
+                assert ((row[:, feature] - want).abs() <= bound).all(), (r, i, feature, row[:, feature], want, bound)
+            assert not row[:, 2:].any()
 
 
 @pytest.mark.parametrize("shape,wider", SHAPES)
