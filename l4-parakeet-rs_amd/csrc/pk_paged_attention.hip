@@ -194,7 +194,7 @@ template <int kD, bool kF8> struct RowPass {
             m = max_level(max_level(m, 16), 32);
             const float new_top = __builtin_fmaxf(top, m);
             const float base = new_top == kNegInf ? 0.0f : new_top;
-            const float keep = __builtin_amdgcn_exp2f(top - base);
+            const float keep = weight_of(top - base);
             top = new_top;
             float sum = 0.0f;
             v8h pf[kU];
@@ -207,7 +207,15 @@ template <int kD, bool kF8> struct RowPass {
             total = total * keep + sum;
 #pragma unroll
             for (int c = 0; c < kBlocks; ++c) acc[c] = acc[c] * keep;
-            if (!whole) {
+            // a probability that is zero in fp16, while all rows see all keys
+            bool faint = false;
+            if constexpr (!kF8) {
+                float least = p[0];
+#pragma unroll
+                for (int j = 1; j < 8; ++j) least = __builtin_fminf(least, p[j]);
+                faint = __any(least <= 0x1p-25f);
+            }
+            if (!whole || faint) {
                 // keys that do not exist hold anything: their values are taken as zero
                 constexpr int kPerWord = 4 / kBytes;
                 uint32_t there_mask[4];
@@ -222,7 +230,7 @@ template <int kD, bool kF8> struct RowPass {
                     vraw[c].y &= there_mask[1];
                     vraw[c].z &= there_mask[2];
                     vraw[c].w &= there_mask[3];
-                    odd.template take<kF8>(vraw[c], 16 * c + l16, mine, [&](int r, int& from, int& to) {
+                    odd.template take<kF8>(vraw[c], 16 * c + l16, mine, whole, [&](int r, int& from, int& to) {
                         from = lo;  // lane r < 16 has row r
                         to = r <= w.last() ? hi : lo;
                     });
@@ -269,7 +277,7 @@ template <int kD, int kN> __device__ __forceinline__ void join(const Parts<kD>& 
     for (int j = 0; j < kN; ++j) v[j] = 0.0f;
 #pragma unroll
     for (int w = 0; w < kRowWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(parts.top[w][r] - base);
+        const float f = weight_of(parts.top[w][r] - base);
         total += parts.total[w][r] * f;
 #pragma unroll
         for (int j = 0; j < kN; ++j) v[j] += parts.acc[w][r][d0 + j] * f;
@@ -476,13 +484,13 @@ __device__ __forceinline__ void join_parts(const Part<kD, 16>* first, const Join
         float new_top = top;
 #pragma unroll
         for (int j = 0; j < kDeep; ++j) new_top = __builtin_fmaxf(new_top, tops[j]);
-        const float base = new_top == kNegInf ? 0.0f : new_top, keep = __builtin_amdgcn_exp2f(top - base);
+        const float base = new_top == kNegInf ? 0.0f : new_top, keep = weight_of(top - base);
         top = new_top;
         total *= keep;
         v = v * keep;
 #pragma unroll
         for (int j = 0; j < kDeep; ++j) {
-            const float f = __builtin_amdgcn_exp2f(tops[j] - base);
+            const float f = weight_of(tops[j] - base);
             if (i + j * step >= job.count) continue;  // no part twice, not even with weight 0: it may hold a NaN
             total += totals[j] * f;
             v = v + accs[j] * f;
@@ -528,7 +536,7 @@ template <int kD> __global__ __launch_bounds__(kJoinGroups * kD / 4) void paged_
             v = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int w = 0; w < kJoinGroups; ++w) {
-                const float f = __builtin_amdgcn_exp2f(part_top[w] - base);
+                const float f = weight_of(part_top[w] - base);
                 total += part_total[w] * f;
                 v = v + *(const v4f*)&part_acc[w][4 * lane] * f;
             }

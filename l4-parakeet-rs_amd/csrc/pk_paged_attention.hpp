@@ -9,6 +9,10 @@ namespace pk {
 
 constexpr float kNegInf = -__builtin_inff();
 
+// The weight of sums whose maximum is `below` (factors of two) under the new one: not zero, which
+// would make NaN of an infinity among them; sums of 2^61 at most vanish all the same.
+__device__ __forceinline__ float weight_of(float below) { return __builtin_fmaxf(__builtin_amdgcn_exp2f(below), 0x1p-126f); }
+
 // Eight cache values of an operand -> fp16 (e4m3 values are exact in fp16).
 template <bool kF8> __device__ __forceinline__ v8h operand(const uint4& raw, int half) {
     if constexpr (kF8) {
@@ -41,11 +45,16 @@ template <bool kF8> __device__ __forceinline__ uint32_t odd_cleared(uint32_t w) 
     if constexpr (kF8) return w & ~((((w & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 0xffu);
     else return w & ~(((((w & 0x7c007c00u) + 0x04000400u) >> 15) & 0x00010001u) * 0xffffu);
 }
+// All ones in the halves of a word of fp16 values that are infinities.
+__device__ __forceinline__ uint32_t infinite(uint32_t w) {
+    return ((w & 0x7fffu) == 0x7c00u ? 0xffffu : 0u) | ((w & 0x7fff0000u) == 0x7c000000u ? 0xffff0000u : 0u);
+}
 
 // Infinities and NaN in values: a product with the zero of a masked key would spoil rows
 // that do not see that key.  At the edges of the rows' keys they are therefore taken out
 // of the operands, and which outputs they belong to (those of the rows that do see the
-// key) is noted in LDS, for the end.  Rare, and kept out of the way of everything else.
+// key) is noted in LDS, for the end; so are infinities where a probability is one that fp16
+// rounds to zero, of which they would make NaN.  Rare, and kept out of the way of everything else.
 template <int kD, int kRows> struct Odd {
     static constexpr int kWords = (kRows + 31) / 32;
     uint32_t any;
@@ -56,9 +65,12 @@ template <int kD, int kRows> struct Odd {
         if (threadIdx.x == 0) any = 0;
     }
     // 16 bytes of values of feature d from key `key` on, a lane; window(r, lo, hi): the keys that row r of this lane sees.
-    template <bool kF8, class Window> __device__ __forceinline__ void take(uint4& raw, int d, int key, Window window) {
+    // inside: all rows see these keys, and a NaN may stay (so may all of e4m3, which has no infinity).
+    template <bool kF8, class Window> __device__ __forceinline__ void take(uint4& raw, int d, int key, bool inside, Window window) {
+        if (kF8 && inside) return;
         const int lane = threadIdx.x & 63;
         unsigned long long todo = __ballot(not_finite<kF8>(raw) != 0);
+        if (inside && todo) todo = __ballot((infinite(raw.x) | infinite(raw.y) | infinite(raw.z) | infinite(raw.w)) != 0);
         while (__builtin_expect(todo != 0, 0)) {
             const int from = __builtin_ctzll(todo);
             todo &= todo - 1;
@@ -72,6 +84,7 @@ template <int kD, int kRows> struct Odd {
                 const uint32_t v = kF8 ? word >> (8 * (j & 3)) & 0xffu : word >> (16 * (j & 1)) & 0xffffu;
                 if (kF8 ? (v & 0x7fu) != 0x7fu : (v & 0x7c00u) != 0x7c00u) continue;
                 const int kind = kF8 || v & 0x3ffu ? 0 : (v >> 15 ? 2 : 1);
+                if (inside && kind == 0) continue;
                 for (int r = lane; r < kRows; r += 64) {
                     int lo, hi;
                     window(r, lo, hi);
@@ -80,7 +93,8 @@ template <int kD, int kRows> struct Odd {
                 if (lane == 0) any = 1;
             }
         }
-        raw = uint4{odd_cleared<kF8>(raw.x), odd_cleared<kF8>(raw.y), odd_cleared<kF8>(raw.z), odd_cleared<kF8>(raw.w)};
+        if (inside) raw = uint4{raw.x & ~infinite(raw.x), raw.y & ~infinite(raw.y), raw.z & ~infinite(raw.z), raw.w & ~infinite(raw.w)};
+        else raw = uint4{odd_cleared<kF8>(raw.x), odd_cleared<kF8>(raw.y), odd_cleared<kF8>(raw.z), odd_cleared<kF8>(raw.w)};
     }
     // What row r's sum of feature d becomes.
     __device__ __forceinline__ float put(float v, int r, int d) const {

@@ -219,7 +219,8 @@ template <int kD, bool kF8> struct ChunkPass {
 
     // The values that this wave loaded of a tile at an edge of some row's keys: those of keys
     // that do not exist hold anything and are cleared, infinities and NaN are taken out.
-    __device__ __forceinline__ void tidy_values(int block, uint32_t ok, Odd<kD, kChunkRows>& odd) const {
+    // kInside: of a tile that all rows see, infinities only.
+    template <bool kInside> __device__ __forceinline__ void tidy_values(int block, uint32_t ok, Odd<kD, kChunkRows>& odd) const {
         if (kSplit && wave < kKeyUnits) return;
         uint8_t* vt = lds + buffer_of(block) * kBuffer + kKeyTile + here(lane) * 16;
         const int chunk = here(value_chunk()), key = block * kTileKeys + chunk * (16 / kBytes), there = ok >> chunk & 1u ? t.length - key : 0;
@@ -240,7 +241,7 @@ template <int kD, bool kF8> struct ChunkPass {
                 w[j] &= n >= kPerWord ? 0xffffffffu : (n <= 0 ? 0u : (1u << (8 * kBytes * n)) - 1u);
             }
             uint4 now{w[0], w[1], w[2], w[3]};
-            odd.template take<kF8>(now, value_unit(i) * (64 / kValueChunks) + here(lane) / kValueChunks, key, seen);
+            odd.template take<kF8>(now, value_unit(i) * (64 / kValueChunks) + here(lane) / kValueChunks, key, kInside, seen);
             *p = now;
         }
     }
@@ -275,11 +276,11 @@ template <int kD, bool kF8> struct ChunkPass {
     // Probabilities are 2^kLift at that maximum and at most 2^15: fp16 then holds those down to
     // 2^-21 of it to full precision and down to 2^-31 at all, so that the sum counts no small
     // ones that the output leaves out.
-    static constexpr float kSlack = 8.0f, kLift = 15.0f - kSlack;
+    static constexpr float kSlack = 8.0f, kLift = 15.0f - kSlack, kHuge = 1 << 20;
     // Scores -> probabilities as operands; the sums so far are scaled to the new maximum.
     // Scaling and subtraction are one step, in which the rounding of the scaled maximum, half a
     // step of its own, becomes a factor of all probabilities: harmless up to 2^20, far outside
-    // fp16 from 2^28 on.  With kCareful the subtraction, exact near the maximum, comes first.
+    // fp16 from 2^28 on.  With kCareful the subtraction, exact near the maximum, comes first there.
     template <bool kCareful> __device__ __forceinline__ void soften(const v16f (&sc)[2], v8h (&pf)[4]) {
         const float m = max_level(max3(kNegInf, sc[0], sc[1]), 32);
         const bool far = (m - top) * scale > kSlack;  // also from -inf; false while nothing is seen
@@ -291,12 +292,13 @@ template <int kD, bool kF8> struct ChunkPass {
             for (int c = 0; c < kBlocks; ++c) acc[c] = acc[c] * keep;
         }
         const float from = top == kNegInf ? 0.0f : top, base = from * scale - kLift;
+        const bool huge = kCareful && !(__builtin_fabsf(base) < kHuge);
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float score = sc[s >> 1][8 * (s & 1) + j];
-                const float p = __builtin_amdgcn_exp2f(kCareful ? (score - from) * scale + kLift : __builtin_fmaf(score, scale, -base));
+                const float p = __builtin_amdgcn_exp2f(huge ? (score - from) * scale + kLift : __builtin_fmaf(score, scale, -base));
                 total += p;
                 pf[s][j] = (_Float16)p;
             }
@@ -395,7 +397,8 @@ template <int kD, bool kF8> struct ChunkPass {
         for (int b = from; b < to; ++b) {
             wait_steps<1>(b + 2 < to);
             const bool edge = b * kTileKeys < tile_full_lo || (b + 1) * kTileKeys > tile_full_hi || ok[0] != kAllPages;
-            if (edge) tidy_values(b, ok[0], odd);
+            if (edge) tidy_values<false>(b, ok[0], odd);
+            else if constexpr (kCareful && !kF8) tidy_values<true>(b, ok[0], odd);
             meet();
             load_all(step);
             ok[2] = pages_ok(ids);
@@ -418,7 +421,8 @@ template <int kD, bool kF8> struct ChunkPass {
     }
 
     // Whether a row of this wave may have come out wrong in a run without care: its maximum is
-    // large, or its sums are not finite (early probabilities may have been too large for fp16).
+    // large, or its sums are not finite (a value was infinite, or early probabilities were too
+    // large for fp16).
     __device__ __forceinline__ bool doubtful() const {
         v16f sums = acc[0];
 #pragma unroll
@@ -427,7 +431,7 @@ template <int kD, bool kF8> struct ChunkPass {
         for (int n = 8; n > 0; n >>= 1)
 #pragma unroll
             for (int j = 0; j < n; ++j) sums[j] += sums[j + n];
-        const bool far = top != kNegInf && !(__builtin_fabsf(top * scale) < (float)(1 << 20));
+        const bool far = top != kNegInf && !(__builtin_fabsf(top * scale - kLift) < kHuge);
         return last >= 0 && __any(far || !(__builtin_fabsf(sums[0] + total) < __builtin_inff()));
     }
     // A row tile's tiles [from, to), all of them read by all waves at the end.  Where a wave has
@@ -582,7 +586,7 @@ template <int kD> __global__ __launch_bounds__(16 * kD / 4) void paged_chunks_jo
             const Part<kD, kChunkRows>& slot = first[2 * i + (i == 0 ? job.first_slot : 0)];
             const float new_top = __builtin_fmaxf(top, slot.top[r]);
             const float base = new_top == kNegInf ? 0.0f : new_top;
-            const float f = __builtin_amdgcn_exp2f(slot.top[r] - base), keep = __builtin_amdgcn_exp2f(top - base);
+            const float f = weight_of(slot.top[r] - base), keep = weight_of(top - base);
             total = total * keep + slot.total[r] * f;
             v = v * keep + *(const v4f*)&slot.acc[r][4 * lane] * f;
             top = new_top;
@@ -604,7 +608,7 @@ template <int kD> __global__ __launch_bounds__(16 * kD / 4) void paged_chunks_jo
             v = v4f{};
 #pragma unroll
             for (int w = 0; w < 16; ++w) {
-                const float f = __builtin_amdgcn_exp2f(part_top[w] - base);
+                const float f = weight_of(part_top[w] - base);
                 total += part_total[w] * f;
                 v = v + *(const v4f*)&part_acc[w][4 * lane] * f;
             }

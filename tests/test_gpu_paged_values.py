@@ -1,5 +1,5 @@
 """Paged attention over keys and values made so that each answer is known in closed form: probabilities far below the
-largest one, scores of any size."""
+largest one, infinities among them, scores of any size."""
 import math
 
 import pytest
@@ -84,3 +84,28 @@ def test_huge_scores(pk, shape, wider, fp8, far):  # noqa: F811
     else:  # the strong keys are the weak ones then; the first of a sequence's keys is a strong one
         alone = torch.tensor([length - n + i == 0 for n, length in shape for i in range(n)], device="cuda")
         assert not got[~alone][:, :, 1:].any() and (got[~alone][:, :, 0] == 128).all() and (got[alone][:, :, 1] == 1).all()
+
+
+@pytest.mark.parametrize("shape,wider", SHAPES)
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("far,lone", [(60.0, False), (300.0, False), (300.0, True)])
+def test_infinity_of_a_tiny_probability(pk, shape, wider, fp8, far, lone):  # noqa: F811
+    """A seen infinity (e4m3: NaN) reaches the rows that see it, the others not, however small its probability and wherever it
+    stands; with a lone strong key the parts of the keys that do not hold it have a weight below fp32's smallest."""
+    c, scale = strong_and_weak(shape, wider, fp8, far)
+    if lone:
+        for r in range(len(shape)):
+            put(c, "key", r, slice(STEP, None, STEP), 0, 0.0, c.key_scale)
+    clean = c.run(pk, scale=scale).clone()
+    places = [(0, 5, 7, 1), (0, 131, 8, 2), (len(shape) - 1, 70, 9, 1), (len(shape) - 1, 201, 7, 2), (len(shape) // 2, shape[len(shape) // 2][1] - 2, 10, 1)]
+    for r, token, feature, kind in places:
+        p, off = int(c.table[r, token // c.page]), token % c.page
+        c.value[p, :, feature, off] = 0x7F if fp8 else (0.0, float("inf"), float("-inf"))[kind]
+    got = c.run(pk, scale=scale)
+    want = clean.clone()
+    for r, token, feature, kind in places:
+        n, length = shape[r]
+        first = max(0, token - (length - n))  # first row that sees it
+        rows = want[sum(c.counts[:r]) + first:sum(c.counts[:r + 1])]
+        rows[:, :, feature] += float("nan") if fp8 else (0.0, float("inf"), float("-inf"))[kind]  # both: NaN
+    plain.close(got, want.double(), torch.zeros_like(want, dtype=torch.float64))
