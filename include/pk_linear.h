@@ -738,9 +738,11 @@ int32_t pk_paged_cache_write(int32_t kind, const uint16_t* key, int64_t key_stri
  * multiply fp16 queries with fp16 or e4m3 keys exactly, probabilities are
  * rounded to fp16 for the second product (their sum is not), which keeps those
  * down to 2^-21 of a row's largest to full precision and those down to 2^-31.
- * A row's fp32 sums are cut alike whatever stands beside it where a full table
- * holds at most 384 KB of keys and values a kv head (512 KB with sequences *
- * kv_heads >= 128) and max_queries * heads / kv_heads <= 32.  Larger work is dealt in equal shares of the whole batch's keys.
+ * A row's fp32 sums are cut alike, and its bits the same, whatever stands beside
+ * it where a full table holds at most 384 KB of keys and values a kv head and
+ * max_queries * heads / kv_heads <= 32; with sequences * kv_heads >= 128 that
+ * holds up to 512 KB, among such calls.  Larger work is dealt in equal shares of
+ * the whole batch's keys.
  * The same call gives the same bits.  output and workspace overlap nothing else.
  * workspace: pk_paged_attention_workspace_bytes (enough also for calls with fewer
  * queries, sequences or pages, and for both kinds) of device memory (16-byte

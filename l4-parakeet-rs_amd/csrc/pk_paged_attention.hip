@@ -306,7 +306,7 @@ template <int kD, bool kF8> __global__ __launch_bounds__(64 * kRowWaves, 2) void
     Pass pass(a);
     int lo, hi, k0, end;
     pass.reach(w, lo, hi);
-    lo &= ~(Pass::kKeys - 1);
+    lo &= ~(Pass::kSpan - 1);  // a wave's tiles are the same keys whichever row comes first
     pass.tiles(w, lo, hi > lo ? hi : lo + 1, k0, end);
     pass.clear();
     pass.open(w, k0);

@@ -1,5 +1,5 @@
 """Paged attention over keys and values made so that each answer is known in closed form: probabilities far below the
-largest one, infinities among them, scores of any size."""
+largest one, infinities among them, scores of any size; and the same token in different company."""
 import math
 
 import pytest
@@ -109,3 +109,36 @@ def test_infinity_of_a_tiny_probability(pk, shape, wider, fp8, far, lone):  # no
         rows = want[sum(c.counts[:r]) + first:sum(c.counts[:r + 1])]
         rows[:, :, feature] += float("nan") if fp8 else (0.0, float("inf"), float("-inf"))[kind]  # both: NaN
     plain.close(got, want.double(), torch.zeros_like(want, dtype=torch.float64))
+
+
+@pytest.mark.parametrize("left", [-1, 40, 130, 300])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_row_in_other_company(pk, left, fp8):  # noqa: F811
+    """In a table that takes one launch a token's bits are the same alone, behind others of its chunk, and among other sequences."""
+    together = Case([(4, 420), (3, 700), (2, 5)], heads=8, kv=2, fp8=fp8, seed=9)
+    got = together.run(pk, left=left)
+    for r, (n, length) in enumerate([(4, 420), (3, 700), (2, 5)]):
+        for i in range(n):
+            at = sum(together.counts[:r]) + i
+            q, out = together.q[at:at + 1].contiguous(), torch.empty((1, 8, 128), dtype=torch.float16, device="cuda")
+            pk.paged_attention(q, together.key, together.value, together.table[r:r + 1], torch.tensor([0, 1], dtype=torch.int32, device="cuda"),
+                               torch.tensor([length - n + i + 1], dtype=torch.int32, device="cuda"), out, None, max_queries=1, left=left,
+                               key_scale=together.key_scale, value_scale=together.value_scale)
+            assert torch.equal(out[0], got[at]), (r, i)
+
+
+@pytest.mark.parametrize("shape,wider", SHAPES)
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("far", [3e5, 1e7, 1e9, 1e12, 1e20, -1e9])
+def test_huge_scores(pk, shape, wider, fp8, far):  # noqa: F811
+    """Scores whose fp32 steps are larger than 1: equal ones still share the sum equally, the others have none of it."""
+    c, _ = strong_and_weak(shape, wider, fp8, 1.0)
+    c.q[:, :, 0] = 7
+    for r in range(len(shape)):
+        put(c, "key", r, slice(0, None, STEP), 0, 9 * c.key_scale, c.key_scale)
+    got = c.run(pk, scale=far / (63 * c.key_scale))[:sum(c.counts)]
+    if far > 0:
+        assert (got[:, :, 1] == 1).all() and not got[:, :, 0].any() and not got[:, :, 2:].any()
+    else:  # the strong keys are the weak ones then; the first of a sequence's keys is a strong one
+        alone = torch.tensor([length - n + i == 0 for n, length in shape for i in range(n)], device="cuda")
+        assert not got[~alone][:, :, 1:].any() and (got[~alone][:, :, 0] == 128).all() and (got[alone][:, :, 1] == 1).all()
