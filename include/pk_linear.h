@@ -712,8 +712,8 @@ int32_t pk_page_plan(const int32_t* held, const int32_t* added, const int32_t* f
  * projection's rows) into their slots.  kind PK_CACHE_FP8 stores e4m3(x *
  * inverse_scale) (saturating; NaN stays NaN), PK_CACHE_FP16 the value itself.
  * A slot outside [0, pages * page_size) is skipped (-1: padding).  The slots of
- * one call must differ.  tokens <= 2^21, head_dim 64 or 128; keys, values and caches 16-byte
- * aligned, strides multiples of 8. */
+ * one call must differ; the caches overlap no other array.  tokens <= 2^21,
+ * head_dim 64 or 128; keys, values and caches 16-byte aligned, strides multiples of 8. */
 int32_t pk_paged_cache_write(int32_t kind, const uint16_t* key, int64_t key_stride, const uint16_t* value,
                              int64_t value_stride, const int32_t* slots, void* key_cache, void* value_cache,
                              int32_t tokens, int32_t kv_heads, int32_t head_dim, int32_t page_size, int32_t pages,
@@ -743,7 +743,9 @@ int32_t pk_paged_cache_write(int32_t kind, const uint16_t* key, int64_t key_stri
  * max_queries * heads / kv_heads <= 32; with sequences * kv_heads >= 128 that
  * holds up to 512 KB, among such calls.  Larger work is dealt in equal shares of
  * the whole batch's keys.
- * The same call gives the same bits.  output and workspace overlap nothing else.
+ * The same call gives the same bits.  output may be query itself (with its
+ * stride); it and the workspace overlap nothing else, row by row: slices of one
+ * array's rows may lie between each other.
  * workspace: pk_paged_attention_workspace_bytes (enough also for calls with fewer
  * queries, sequences or pages, and for both kinds) of device memory (16-byte
  * aligned), used by one call at a time; its content need not be kept or cleared

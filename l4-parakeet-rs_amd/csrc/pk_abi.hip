@@ -8,6 +8,7 @@
 
 #include "../../include/pk_linear.h"
 #include "pk_kernels.hpp"
+#include "pk_overlap.hpp"
 
 namespace pk {
 
@@ -871,10 +872,6 @@ int32_t pk_pack_position_heads(const uint16_t* input, uint16_t* output, void* st
 
 // ---- a decoder layer's serving step -------------------------------------------------
 
-static bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
-    return a && b && (const char*)a < (const char*)b + b_bytes && (const char*)b < (const char*)a + a_bytes;
-}
-
 static int page_shift(int32_t page_size) {  // log2 of 16, 32, ..., 256; -1 otherwise
     for (int s = 4; s <= 8; ++s)
         if (page_size == 1 << s) return s;
@@ -1025,6 +1022,13 @@ int32_t pk_paged_cache_write(int32_t kind, const uint16_t* key, int64_t key_stri
         set_error("keys, values and caches must be 16-byte aligned, strides multiples of 8, slots 4-byte aligned");
         return PK_E_ALIGN;
     }
+    const int64_t cache = ((int64_t)pages << shift) * width * (kind == PK_CACHE_FP8 ? 1 : 2);
+    const RowSet new_rows[] = {{key, 2 * key_stride, 2 * width, tokens}, {value, 2 * value_stride, 2 * width, tokens}};
+    const void* caches[] = {key_cache, value_cache};
+    bool meet = overlap(key_cache, cache, value_cache, cache);
+    for (const void* c : caches)
+        meet = meet || overlap(c, cache, slots, 4 * (size_t)tokens) || overlap(new_rows[0], c, cache) || overlap(new_rows[1], c, cache);
+    if (meet) { set_error("paged_cache_write: a cache overlaps another array"); return PK_E_ARG; }
     launch_paged_cache_write(kind, key, value, key_stride, value_stride, slots, key_cache, value_cache, tokens, kv_heads, head_dim, shift,
                              pages, key_inverse_scale, value_inverse_scale, STREAM);
     return check_launch("paged_cache_write");
@@ -1085,6 +1089,18 @@ int32_t pk_paged_attention(int32_t kind, const uint16_t* query, int64_t query_st
     const int64_t wanted = pk_paged_attention_workspace_bytes(tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, max_pages);
     if (wanted > 0 && (!need(workspace, "workspace") || workspace_bytes < (uint64_t)wanted)) {
         if (workspace) set_error("paged attention needs %lld bytes of workspace, got %llu", (long long)wanted, (unsigned long long)workspace_bytes);
+        return PK_E_ARG;
+    }
+    const int64_t cache_bytes = ((int64_t)pages << shift) * kv_heads * head_dim * (kind == PK_CACHE_FP8 ? 1 : 2);
+    const RowSet q{query, 2 * query_stride, 2 * width, tokens}, o{output, 2 * output_stride, 2 * width, tokens};
+    const bool in_place = query == output && (query_stride == output_stride || tokens == 1);
+    const struct { const void* p; int64_t bytes; } read[] = {
+        {key_cache, cache_bytes}, {value_cache, cache_bytes}, {block_table, (int64_t)sequences * max_pages * 4},
+        {query_starts, (int64_t)sequences * 4 + 4}, {key_lengths, (int64_t)sequences * 4}};
+    bool meet = (!in_place && overlap(q, o)) || overlap(q, workspace, wanted) || overlap(o, workspace, wanted);
+    for (const auto& r : read) meet = meet || overlap(o, r.p, r.bytes) || (wanted > 0 && overlap(workspace, wanted, r.p, r.bytes));
+    if (meet) {
+        set_error("paged attention: output and workspace must not overlap other arrays (output may be query itself)");
         return PK_E_ARG;
     }
     PagedArgs a{};

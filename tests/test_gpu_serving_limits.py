@@ -4,6 +4,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from test_gpu_parity import pk  # noqa: E402, F401
+from test_gpu_paged_attention import Case  # noqa: E402
 from test_gpu_serving import randn, gen  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -39,3 +40,23 @@ def test_plan_of_the_most_slots(pk):  # noqa: F811
     for part in slots[43:capacity].split(1 << 28):
         assert (part == -1).all()
     assert slots[capacity] == 5
+
+
+@pytest.mark.parametrize("shape,wider", [([(1, 300), (4, 90)], 0), ([(1, 900), (2, 3000)], 6000), ([(40, 700), (90, 300)], 6000), ([(40, 400), (3, 3)], 0)])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_attention_in_place_and_between(pk, shape, wider, fp8):  # noqa: F811
+    """The output may take the queries' place, or lie between them in the same rows."""
+    Case.wider = wider
+    try:
+        c = Case(shape, heads=4, kv=2, fp8=fp8, seed=41)
+    finally:
+        Case.wider = 0
+    tokens = sum(c.counts)
+    want = c.check(pk)[:tokens].clone()
+    wide = torch.full((c.q.shape[0], 9, 128), 3.0, dtype=torch.float16, device="cuda")
+    wide[:, 1:5] = c.q
+    c.q = wide[:, 1:5]
+    c.run(pk, out=wide[:, 5:])
+    assert torch.equal(wide[:tokens, 5:], want) and (wide[tokens:, 5:] == 3).all() and (wide[:, 0] == 3).all()
+    c.run(pk, out=c.q)
+    assert torch.equal(wide[:tokens, 1:5], want) and torch.equal(wide[:tokens, 5:], want) and (wide[:, 0] == 3).all()
