@@ -4,6 +4,7 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <cmath>
 #include <string>
 
 #include "../../include/pk_linear.h"
@@ -1076,6 +1077,11 @@ int32_t pk_paged_attention(int32_t kind, const uint16_t* query, int64_t query_st
                   (long long)query_stride, (long long)output_stride);
         return PK_E_SHAPE;
     }
+    const float scale_log2 = scale * (kind == PK_CACHE_FP8 ? key_scale : 1.0f) * 1.4426950408889634f;
+    if (!std::isfinite(scale_log2)) {
+        set_error("paged attention needs a finite scale, got %g (key scale %g)", (double)scale, (double)key_scale);
+        return PK_E_ARG;
+    }
     if (tokens == 0 || max_queries == 0 || sequences == 0) return PK_OK;
     if (!need(query, "query") || !need(key_cache, "key_cache") || !need(value_cache, "value_cache") || !need(block_table, "block_table") ||
         !need(query_starts, "query_starts") || !need(key_lengths, "key_lengths") || !need(output, "output"))
@@ -1122,7 +1128,7 @@ int32_t pk_paged_attention(int32_t kind, const uint16_t* query, int64_t query_st
     a.max_pages = max_pages;
     a.left = left < 0 ? -1 : left;
     a.right = right < 0 || right > 1 << 30 ? -1 : right;
-    a.scale_log2 = scale * (kind == PK_CACHE_FP8 ? key_scale : 1.0f) * 1.4426950408889634f;
+    a.scale_log2 = scale_log2;
     a.value_scale = kind == PK_CACHE_FP8 ? value_scale : 1.0f;
     launch_paged_attention(kind, a, head_dim, max_queries, workspace, STREAM);
     return check_launch("paged_attention");

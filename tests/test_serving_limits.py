@@ -87,3 +87,14 @@ def test_overlaps_by_rows(tmp_path):
         assert fn(s, w, n, at, s2, w2, n2) == meet + 2 * one, (s, w, n, at, s2, w2, n2)
         seen[meet] += 1
     assert min(seen) > 5000
+
+
+@pytest.mark.parametrize("kind,kw", [(0, {"scale": float("nan")}), (1, {"scale": float("inf")}), (1, {"key_scale": float("nan")}),
+                                     (1, {"scale": 1e30, "key_scale": -1e30})])
+def test_attention_needs_a_finite_scale(kind, kw):
+    """Chunks took a NaN for 0, so that all keys counted alike."""
+    a = dict(kind=kind, query=P, query_stride=2048, key_cache=P, value_cache=P, block_table=P, query_starts=P, key_lengths=P, output=P, output_stride=2048,
+             tokens=0, max_queries=0, sequences=2, heads=16, kv_heads=8, head_dim=128, page_size=16, pages=10, max_pages=400, left=-1, right=0, scale=0.1,
+             key_scale=1.0, value_scale=1.0, workspace=P, workspace_bytes=1 << 40)
+    a.update(kw)
+    assert status("pk_paged_attention", *a.values()) == ARG and b"finite" in pk.lib.pk_last_error()
