@@ -409,7 +409,9 @@ def launch_decode(encoder_projection, frames, lstm, projection, joint, tokens, r
 #
 # These calls take their sizes from the tensors, so they check what they are given: a
 # single token's step is a few microseconds of GPU time, so the checks are one plain
-# condition each, and only a call that fails it is looked at again to say why.
+# condition each, and only a call that fails it is looked at again to say why.  ctypes
+# cuts integers to 32 bits without a word, so sizes are checked here: `(a | b) >> 31` is
+# not 0 where one of them is negative or 2^31 or more.
 
 NORM_FP8, NORM_INT8 = 0, 1
 CACHE_FP16, CACHE_FP8 = 0, 1
@@ -449,7 +451,7 @@ def _refuse(what, device, *tensors):
             raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
         if dense and not t.is_contiguous():
             raise ValueError(f"{what}: {name} must be contiguous")
-    raise ValueError(f"{what}: the tensors do not fit together")
+    raise ValueError(f"{what}: the tensors do not fit together, or a size is not one of 32 bits")
 
 
 def _done(name, status):
@@ -467,7 +469,7 @@ def rms_norm_quantize(kind, input, residual, weight, residual_out, output, scale
     rows, width = shape
     codes = (torch.int8,) if kind == NORM_INT8 else (torch.uint8, torch.float8_e4m3fn)
     if not (input.dtype is f16 and weight.dtype is f16 and output.dtype in codes and scales.dtype is torch.float32 and output.shape == shape
-            and weight.shape == (width,) and scales.shape == (rows,) and input.is_contiguous() and weight.is_contiguous() and output.is_contiguous()
+            and not (rows | width | kind) >> 31 and weight.shape == (width,) and scales.shape == (rows,) and input.is_contiguous() and weight.is_contiguous() and output.is_contiguous()
             and scales.is_contiguous() and input.get_device() == weight.get_device() == output.get_device() == scales.get_device() == device
             and all(t is None or (t.dtype is f16 and t.shape == shape and t.is_contiguous() and t.get_device() == device)
                     for t in (residual, residual_out))):
@@ -486,7 +488,7 @@ def _gemv(name, input, input_scales, weight_q, weight_scales, weight_zeros, bias
     f16, f32, groups = torch.float16, torch.float32, (n, k // 128)
     row_type, words, outs = f16 if input_scales is None else torch.int8, (torch.int32, torch.uint32), (f16, f32)
     if not (input.dtype is row_type and weight_q.dtype in words and weight_scales.dtype is f16 and weight_zeros.dtype is f16 and output.dtype in outs
-            and weight_q.shape == (n, k // 8) and weight_scales.shape == groups and weight_zeros.shape == groups and output.shape == (m, n)
+            and not (n | k) >> 31 and weight_q.shape == (n, k // 8) and weight_scales.shape == groups and weight_zeros.shape == groups and output.shape == (m, n)
             and input.is_contiguous() and weight_q.is_contiguous() and weight_scales.is_contiguous() and weight_zeros.is_contiguous()
             and output.is_contiguous()
             and input.get_device() == weight_q.get_device() == weight_scales.get_device() == weight_zeros.get_device() == output.get_device() == device
@@ -527,7 +529,7 @@ def page_plan(held, added, free_pages, free_range, block_table, query_starts, ke
     arrays = (held, added, free_pages, free_range, block_table, query_starts, key_lengths, slots, info)
     if not (all(t.dtype is i32 and t.get_device() == device and t.is_contiguous() for t in arrays) and held.shape == one and added.shape == one
             and key_lengths.shape == one and query_starts.shape == (requests + 1,) and free_range.shape == (2,) and info.shape == (4,)
-            and free_pages.dim() == slots.dim() == 1
+            and free_pages.dim() == slots.dim() == 1 and not (max_pages | capacity | free_pages.numel() | page_size) >> 31
             and (positions is None or (positions.dtype is i32 and positions.shape == slots.shape and positions.get_device() == device
                                        and positions.is_contiguous()))):
         i32 = (i32,)
@@ -575,6 +577,8 @@ def paged_cache_write(key, value, slots, key_cache, value_cache, key_inverse_sca
 
 def paged_attention_workspace_bytes(tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, max_pages):
     """Bytes of workspace that paged_attention needs for these sizes (host only)."""
+    if (tokens | max_queries | sequences | heads | kv_heads | head_dim | page_size | max_pages) >> 31:
+        raise ValueError("paged_attention_workspace_bytes: a size is negative or 2^31 and more")
     size = lib.pk_paged_attention_workspace_bytes(tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, max_pages)
     _done("pk_paged_attention_workspace_bytes", size)
     return size
@@ -594,7 +598,7 @@ def paged_attention(query, key_cache, value_cache, block_table, query_starts, ke
     f16, i32, kind, kinds = torch.float16, torch.int32, key_cache.dtype, (torch.float16, torch.uint8, torch.float8_e4m3fn)
     transposed = (pages, kv_heads, head_dim, page_size)
     if not (kind in kinds and value_cache.dtype is kind and query.dtype is f16 and output.dtype is f16 and value_cache.shape == transposed
-            and rows[2] == head_dim and output.shape == rows and query_starts.shape == (sequences + 1,) and key_lengths.shape == (sequences,)
+            and rows[2] == head_dim and output.shape == rows and not (max_queries | max_pages | sequences) >> 31 and query_starts.shape == (sequences + 1,) and key_lengths.shape == (sequences,)
             and key_cache.is_contiguous() and value_cache.is_contiguous()
             and key_cache.get_device() == value_cache.get_device() == query.get_device() == output.get_device() == device
             and all(t.dtype is i32 and t.is_contiguous() and t.get_device() == device for t in (block_table, query_starts, key_lengths))
@@ -604,6 +608,8 @@ def paged_attention(query, key_cache, value_cache, block_table, query_starts, ke
                 ("query", query, (f16,), (tokens, heads, head_dim), False), ("output", output, (f16,), (tokens, heads, head_dim), False),
                 ("block_table", block_table, i32, None, True), ("query_starts", query_starts, i32, (sequences + 1,), True),
                 ("key_lengths", key_lengths, i32, (sequences,), True), ("workspace", workspace, (torch.uint8,), None, True))
+    if (left + (1 << 31) | right + (1 << 31)) >> 32:  # further than any key
+        left, right = (-1 if (x + (1 << 31)) >> 32 else x for x in (left, right))
     _done("pk_paged_attention", lib.pk_paged_attention(
         CACHE_FP16 if kind is f16 else CACHE_FP8, query.data_ptr(), _row_stride("paged_attention", "query", query), key_cache.data_ptr(),
         value_cache.data_ptr(), block_table.data_ptr(), query_starts.data_ptr(), key_lengths.data_ptr(), output.data_ptr(),

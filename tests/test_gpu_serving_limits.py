@@ -60,3 +60,43 @@ def test_attention_in_place_and_between(pk, shape, wider, fp8):  # noqa: F811
     assert torch.equal(wide[:tokens, 5:], want) and (wide[tokens:, 5:] == 3).all() and (wide[:, 0] == 3).all()
     c.run(pk, out=c.q)
     assert torch.equal(wide[:tokens, 1:5], want) and torch.equal(wide[:tokens, 5:], want) and (wide[:, 0] == 3).all()
+
+
+def test_integers_beyond_32_bits(pk):  # noqa: F811
+    """No size and no window is cut to its low 32 bits."""
+    big = 1 << 32
+    c = Case([(3, 100), (1, 40)], seed=42)
+    want, ws = c.run(pk).clone(), c.workspace(pk)
+    for left, right in ((big + 5, 0), (-1, 0), (-big + 5, 0), (1 << 31, 0), ((1 << 31) - 1, 0)):
+        assert torch.equal(c.run(pk, left=left, right=right, workspace=ws), want), (left, right)
+    free = c.run(pk, left=-1, right=-1).clone()
+    for right in (big, 1 << 31, -big, (1 << 31) - 1):
+        assert torch.equal(c.run(pk, left=-1, right=right), free)
+    with pytest.raises(ValueError):
+        c.run(pk, max_queries=big + 3)
+    with pytest.raises(ValueError):
+        pk.paged_attention_workspace_bytes(big + 5, 5, 2, 16, 8, 128, 16, 400)
+    with pytest.raises(pk.PkError):
+        c.run(pk, max_queries=c.q.shape[0] + 1)  # more than there are
+    wide = torch.empty((2, big + 8), dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        pk.paged_attention(c.q, c.key, c.value, wide, c.starts, c.lengths, c.out, ws, max_queries=3)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    plan = lambda free, table, slots, page: pk.page_plan(i32(1, 2), i32(1, 1), free, i32(0, 4), table, i32(0, 0, 0), i32(0, 0), slots, None,  # noqa: E731
+                                                         i32(0, 0, 0, 0), page)
+    few, table = i32(1, 2, 3, 4), torch.zeros((2, 3), dtype=torch.int32, device="cuda")
+    plan(few, table, i32(0, 0), 16)
+    for bad in ((few, wide, i32(0, 0), 16), (few, table, wide.view(-1)[:big + 2], 16), (wide.view(-1)[:big + 2], table, i32(0, 0), 16),
+                (few, table, i32(0, 0), big + 16)):
+        with pytest.raises(ValueError):
+            plan(*bad)
+    del wide
+    rows = torch.empty((big + 2, 8), dtype=torch.uint8, device="cuda")
+    x = torch.empty((big + 2, 8), dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError):
+        pk.rms_norm_quantize(0, x, None, x[0], None, rows, torch.empty(big + 2, device="cuda"), 1e-5)
+    del x, rows
+    x, q = torch.empty((1, big + 128), dtype=torch.float16, device="cuda"), torch.empty((1, big // 8 + 16), dtype=torch.int32, device="cuda")
+    s = torch.empty((1, big // 128 + 1), dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError):
+        pk.gemv_int4g128(x, q, s, s, None, torch.empty((1, 1), device="cuda"))
