@@ -16,12 +16,13 @@ def blocks(case, left=-1, right=0):
     """Blocks that the batch is cut into, at least: keys of a (sequence, kv head, 16 rows) by 128 (e4m3: 256), or of a chunk's
     256 rows by 64."""
     group, total = case.heads // case.kv, 0
+    few = case.most * group <= 16  # (in a wide table)
     for n, length in zip(case.counts, case.lengths_):
-        for first in range(0, n * group, 16 if case.most * group <= 16 else 256):
-            last = min(first + (16 if case.most * group <= 16 else 256), n * group) - 1
+        for first in range(0, n * group, 16 if few else 256):
+            last = min(first + (16 if few else 256), n * group) - 1
             lo = max(0, length - n + first // group - left) if left >= 0 else 0
             hi = min(length, length - n + last // group + right + 1) if right >= 0 else length
-            keys = 64 if case.most * group > 32 else (256 if case.fp8 else 128)
+            keys = (256 if case.fp8 else 128) if few else 64
             total += (-(-hi // keys) - lo // keys) * case.kv
     return total
 
@@ -67,7 +68,7 @@ DEALT = [(ONE, 8, 4, (-1, 0)), (STREAMS, 8, 4, (-1, 0)), (FEW, 8, 4, (-1, 0)), (
 
 def dealt(shape, heads, kv, window, fp8):
     c = Case(shape, heads=heads, kv=kv, d=128, page=64, fp8=fp8, seed=7)
-    shares, least = FEW_ROWS if c.most * heads // kv <= 32 else CHUNKS
+    shares, least = FEW_ROWS if c.most * heads // kv <= 16 else CHUNKS
     assert blocks(c, *window) > shares * least
     return c
 
