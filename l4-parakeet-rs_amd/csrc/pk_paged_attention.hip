@@ -224,16 +224,22 @@ template <int kD, bool kF8> struct RowPass {
                     const int n = there - i * kPerWord;  // keys of this word that exist
                     there_mask[i] = n >= kPerWord ? 0xffffffffu : (n <= 0 ? 0u : (1u << (8 * kBytes * n)) - 1u);
                 }
+                uint32_t any = 0;  // (one look for all of them: the code for each stays out of the way)
 #pragma unroll
                 for (int c = 0; c < kBlocks; ++c) {
                     vraw[c].x &= there_mask[0];
                     vraw[c].y &= there_mask[1];
                     vraw[c].z &= there_mask[2];
                     vraw[c].w &= there_mask[3];
-                    odd.template take<kF8>(vraw[c], 16 * c + l16, mine, whole, [&](int r, int& from, int& to) {
-                        from = lo;  // lane r < 16 has row r
-                        to = r <= w.last() ? hi : lo;
-                    });
+                    any |= not_finite<kF8>(vraw[c]);
+                }
+                if (__builtin_expect(__any(any != 0), 0)) {
+#pragma unroll
+                    for (int c = 0; c < kBlocks; ++c)
+                        odd.template take<kF8>(vraw[c], 16 * c + l16, mine, whole, [&](int r, int& from, int& to) {
+                            from = lo;  // lane r < 16 has row r
+                            to = r <= w.last() ? hi : lo;
+                        });
                 }
             }
 #pragma unroll

@@ -229,6 +229,7 @@ template <int kD, bool kF8> struct ChunkPass {
             from = to = 0;
             if (tile_row0 + r < t.rows) window(a, t.first_pos + (tile_row0 + r) / a.group, t.length, from, to);
         };
+        uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < kValueLoads; ++i) {
             uint4* p = (uint4*)(vt + value_unit(i) * 1024);
@@ -240,9 +241,17 @@ template <int kD, bool kF8> struct ChunkPass {
                 const int n = there - j * kPerWord;  // keys of this word that exist
                 w[j] &= n >= kPerWord ? 0xffffffffu : (n <= 0 ? 0u : (1u << (8 * kBytes * n)) - 1u);
             }
-            uint4 now{w[0], w[1], w[2], w[3]};
-            odd.template take<kF8>(now, value_unit(i) * (64 / kValueChunks) + here(lane) / kValueChunks, key, kInside, seen);
-            *p = now;
+            *p = uint4{w[0], w[1], w[2], w[3]};
+            any |= not_finite<kF8>(*p);
+        }
+        if (__builtin_expect(__any(any != 0), 0)) {
+#pragma unroll
+            for (int i = 0; i < kValueLoads; ++i) {
+                uint4* p = (uint4*)(vt + value_unit(i) * 1024);
+                uint4 now = *p;
+                odd.template take<kF8>(now, value_unit(i) * (64 / kValueChunks) + here(lane) / kValueChunks, key, kInside, seen);
+                *p = now;
+            }
         }
     }
 
