@@ -181,7 +181,9 @@ static void launch_gemv_type(const void* x, const float* xs, const uint32_t* q, 
     // exist: 64 rows each where that still gives every CU one, 32 where those do.  With k = 8192,
     // one INT8 row: n = 16384 takes 17.3 us with 64 rows, 17.5 with 32 and 19.0 with 16 (16 fp16
     // rows: 22.6, 29.3, 46.6); n = 8192, k = 4096 the other way round 9.4 and 7.0, 6.9 (16 rows:
-    // 10.1, 7.5, 8.9).
+    // 10.1, 7.5, 8.9).  Between the two, with k = 8192, 64 rows would already be ahead: one INT8 row
+    // 16.3 us against 16.6 at n = 10000, 16.7 and 16.9 at 14000, 16 fp16 rows 21.9 and 28.5, 22.7
+    // and 28.9; n = 8192 takes 16.1 and 11.8, 21.5 and 16.7.
     if (n >= 64 * kGemvWorkgroups) launch(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
     else if (n >= 32 * kGemvWorkgroups) launch(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
     // Few weight rows: the waves' number of turns counts.  One row, 1024 x 4096: 5.2 us with one

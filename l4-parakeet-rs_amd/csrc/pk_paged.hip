@@ -307,7 +307,9 @@ template <int kD, bool kF8> __global__ __launch_bounds__(256) void paged_cache_w
 
 // Fewer tokens than this are mostly single ones, and too few tiles to fill the GPU (8 heads of
 // 128, one prompt, e4m3 / fp16: 1024 tokens 8.3 / 9.7 us against 9.7 / 8.2 for tiles, 2048 15.3 /
-// 15.8 against 11.2 / 10.2, 16000 117 / 130 against 28 / 38, 3.5 TB/s).
+// 15.8 against 11.2 / 10.2, 16000 117 / 130 against 28 / 38, 3.5 TB/s).  What tiles are short of
+// a copy's rate is a chain: a border's slot, then the rows, then the stores, in workgroups that
+// the GPU holds hardly more than once over, so that reading and writing barely overlap.
 constexpr int kTileTokens = 1536;
 
 template <int kD, bool kF8> static void launch_write(const WriteArgs& a, hipStream_t s) {

@@ -298,7 +298,7 @@ template <int kD, int kN> __device__ __forceinline__ void put_odd(const Odd<kD, 
 }
 
 // Short contexts: one workgroup for the keys of a (sequence, kv head, 16 rows).
-// A single token's 93 keys, 8 heads, fp16: 5.3 us, of which a launch is 2.5 and the rest the
+// A single token's 93 keys, 8 heads, fp16: 4.7 us, of which a launch is 2.5 and the rest the
 // chain length -> page id -> keys -> scores -> values -> the waves' join.
 template <int kD, bool kF8> __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_attention_rows_kernel(PagedArgs a) {
     constexpr int kN = kD / (4 * kRowWaves);
@@ -342,7 +342,7 @@ template <int kD, bool kF8> __global__ __launch_bounds__(64 * kRowWaves, 2) void
 // 102 and 116 us, 2048 110 and 123.  One sequence of 131072 fp16 keys, 2 kv heads (134 MB): 31
 // us, of which 5 are the way to the first keys.
 constexpr int kShares = 512;  // two workgroups on each of 256 CUs
-constexpr int kLeastShare = 2;  // one sequence of 1900 e4m3 keys 13.1 us; with 1 14.7, with 4 15.4
+constexpr int kLeastShare = 2;  // one sequence of 1900 e4m3 keys 11.9 us; with 1 13.5, with 4 14.3
 
 // Blocks of one item of a sequence (0: the sequence has no rows) and its first block.
 template <int kSpan> __device__ __forceinline__ int item_blocks(const PagedArgs& a, const RowTile& t, int& first) {
@@ -553,16 +553,18 @@ template <int kD> __global__ __launch_bounds__(kJoinGroups * kD / 4) void paged_
 }
 
 // One launch, a workgroup an item, where a full table's keys and values of a kv head are few
-// bytes: a CU reads about 33 bytes a ns, while shares take 12 to 13 us however little there is
-// (one sequence, 8 kv heads of 128, e4m3: 900 keys 9.5 us against 13.0, 1900 14.5 and 13.1;
-// fp16: 448 keys 9.1, 900 16.6 and 12.5).  With kManyItems it is ahead further up, since
-// workgroups that end early make room: 16 sequences of 1900 e4m3 keys 16 us against 20, 64 of
-// them 34 and 44, 200 83 and 103, 64 of 900 fp16 keys 48 and 52.  Four times as far (200 of
-// 4000) it is still 164 and 174 us, but a lone long sequence among idle ones waits for one CU.
+// bytes: a CU reads about 33 bytes a ns, while shares take 12 us however little there is
+// (one sequence, 8 kv heads of 128, e4m3: 900 keys 9.2 us against 11.8, 1900 14.2 and 12.0;
+// fp16: 448 keys 9.1 and 11.5, 900 16.3 and 11.7).  With kManyItems it is ahead further up, since
+// workgroups that end early make room: 16 sequences of 1900 e4m3 keys 15.5 us against 19.5, 64 of
+// them 49 and 54, 200 146 and 157, 64 of 900 fp16 keys 48 and 53.  Four times as far (200 of
+// 4000) it is still 297 and 305 us, but a lone long sequence among idle ones waits for one CU.
+// The table's width decides, not the lengths, which the host does not know: a short sequence in
+// a wide table takes shares (93 keys 12.3 us).
 constexpr long long kDirectBytes = 384 << 10, kDirectBytesMany = 512 << 10;
 constexpr long long kManyItems = 128;
 // So do up to 32 rows of a kv head, in two tiles that read the same keys: one sequence of 24
-// rows, 448 keys, 7.3 us against 14.5 for a chunk's kernel, 64 of them of 1900 keys 65 and 95.
+// rows, 448 keys, 9.9 us against 14.7 for a chunk's kernel, 64 of them of 1900 keys 62 and 92.
 // With four tiles the reading overtakes the gain (64 sequences of 48 rows, 1900 fp16 keys: 180
 // and 117).  Long tables (8 sequences of 24 rows, 12000 keys) take 115 in shares, 78 in chunks.
 constexpr int kDirectRows = 32;

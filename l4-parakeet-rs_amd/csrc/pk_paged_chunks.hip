@@ -3,18 +3,24 @@
 // The same two products as for few rows (S^T = K Q^T, O^T = V^T P^T, probabilities in
 // registers), on 32 x 32 x 16 MFMAs.  The eight waves share 64-key tiles of keys and
 // values in LDS, which the loads fill directly, three tiles ahead of the one that is
-// multiplied (four buffers, one barrier a tile).  Tile rows are whole key or value rows
+// multiplied (four buffers, two barriers a tile).  Tile rows are whole key or value rows
 // whose 16-byte chunks are XOR-swizzled at the source, since such loads write LDS in lane
 // order.
 //
-// Bound by the softmax's vector instructions next to the MFMAs: 32 scores a lane and
-// tile, each a maximum, a fused scale and subtraction, an exponential, a sum and half a
-// conversion; the running output is only rescaled on tiles that raise some row's maximum.
-// 4 sequences of up to 777 new tokens over up to 12007 fp16 keys, 32 / 8 heads of 128:
-// 760-790 TFLOP/s with the joins (a library product of fp16 8192^3: 1431).  Of about 3470
-// cycles a tile (of two waves a SIMD) the products take 1290 and the softmax 1500 to 1650,
-// which is as many instructions as a wave can issue in it; the clock is at 1.9 GHz then.
-// A run of tiles begins and ends with 9 us of loads and stores that nothing covers.
+// Probabilities are fp16, which the matrix instructions multiply; fp32 ones run at a
+// sixteenth of the rate.
+//
+// Bound by the vector instructions next to the MFMAs: 32 scores a lane and tile, each a
+// maximum, a fused scale and subtraction, an exponential, a sum and half a conversion, about
+// 130 of some 230; the others are addresses and bookkeeping.  The running output is only
+// rescaled on tiles that raise some row's maximum.  4 sequences of up to 777 new tokens over
+// up to 12007 fp16 keys, 32 / 8 heads of 128: 770 to 920 TFLOP/s with the joins, by the
+// lengths (135 to 342 GFLOP; equal lengths 960; a library product of fp16 8192^3 1431).  Of
+// about 3470 cycles a tile (of two waves a SIMD) the products take 1290, the softmax with the
+// next loads 1500 to 1650, and 820 are waits at the two barriers; the clock is at 1.9 GHz then.
+// A run of tiles begins and ends with 9 us of loads and stores that nothing covers.  The same
+// with e4m3 keys 970 TFLOP/s, with heads of 64 740 (half the products for the same softmax;
+// e4m3 700), and with a window of 145 keys 59 us for 7.4 GFLOP: most tiles lie at an edge.
 #include "pk_paged_attention.hpp"
 
 typedef float v16f __attribute__((ext_vector_type(16)));
