@@ -729,7 +729,8 @@ int32_t pk_paged_cache_write(int32_t kind, const uint16_t* key, int64_t key_stri
  * key_scale * q.k) * value_scale * v over the seen keys; heads / kv_heads query
  * heads in order share a kv head.  The scales of the cache apply to PK_CACHE_FP8
  * only; scale * key_scale is finite.  A query that sees no key gives zeros; infinities and NaN in keys and
- * values that a query does not see do not reach it.  Keys of a page id outside
+ * values that a query does not see do not reach it; an infinite value that it
+ * sees does, however small its probability.  Keys of a page id outside
  * [0, pages) count as not there; lengths beyond max_pages * page_size are cut.
  * Rows of output outside the sequences' ranges stay as they were.  max_queries
  * (<= tokens) is at least the largest n (rows of longer chunks may be left out),
