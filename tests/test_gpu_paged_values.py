@@ -142,3 +142,28 @@ def test_huge_scores(pk, shape, wider, fp8, far):  # noqa: F811
     else:  # the strong keys are the weak ones then; the first of a sequence's keys is a strong one
         alone = torch.tensor([length - n + i == 0 for n, length in shape for i in range(n)], device="cuda")
         assert not got[~alone][:, :, 1:].any() and (got[~alone][:, :, 0] == 128).all() and (got[alone][:, :, 1] == 1).all()
+
+
+@pytest.mark.parametrize("shape,wider", SHAPES)
+def test_replays_over_changing_values(pk, shape, wider):  # noqa: F811
+    """A replayed call over values that are finite, then infinite somewhere, then huge in their scores, then finite again equals
+    the eager call each time."""
+    c, _ = strong_and_weak(shape, wider, False, 60.0)
+    ws, clean, query = c.workspace(pk), c.value.clone(), c.q.clone()
+    scale = 60.0 / 64
+    c.run(pk, scale=scale, workspace=ws)
+    torch.cuda.synchronize()
+    graph, out = torch.cuda.CUDAGraph(), torch.full_like(c.out, 7.0)
+    with torch.cuda.graph(graph):
+        c.run(pk, scale=scale, workspace=ws, out=out)
+    for turn in range(5):
+        c.value.copy_(clean)
+        c.q.copy_(query * (1 if turn != 2 else 8000))
+        if turn in (1, 3):
+            for r in range(0, len(shape), 7):
+                c.value[c.table[r, 5].long(), :, 40 + turn, 3] = float("inf")
+        out.fill_(7.0)
+        graph.replay()
+        want = c.run(pk, scale=scale, out=torch.full_like(c.out, 7.0))
+        assert torch.equal(out.isinf(), want.isinf()) and torch.equal(out.nan_to_num(), want.nan_to_num()) and not out.isnan().any()
+        assert bool(out.isinf().any()) == (turn in (1, 3))

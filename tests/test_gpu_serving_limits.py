@@ -100,3 +100,54 @@ def test_integers_beyond_32_bits(pk):  # noqa: F811
     s = torch.empty((1, big // 128 + 1), dtype=torch.float16, device="cuda")
     with pytest.raises(ValueError):
         pk.gemv_int4g128(x, q, s, s, None, torch.empty((1, 1), device="cuda"))
+
+
+@pytest.mark.parametrize("heads,kv,shape", [(1024, 1, [(1, 100), (3, 50)]), (256, 256, [(1, 70), (2, 33)]), (1024, 256, [(2, 40)]), (1024, 64, [(1, 900)])])
+@pytest.mark.parametrize("wider", [0, 6000])
+def test_attention_of_the_most_heads(pk, heads, kv, shape, wider):  # noqa: F811
+    Case.wider = wider
+    try:
+        Case(shape, heads=heads, kv=kv, d=64, seed=43).check(pk)
+    finally:
+        Case.wider = 0
+
+
+@pytest.mark.parametrize("columns", [1, 40])
+@pytest.mark.parametrize("n", [1, 256])
+def test_attention_of_the_most_sequences_and_tokens(pk, columns, n):  # noqa: F811
+    """4096 sequences, 2^20 tokens: with equal scores each row is the average of the keys it sees, all in the sequence's one page."""
+    sequences, page, d = 4096, 256, 64
+    tokens = sequences * n
+    g = gen(44)
+    key = torch.zeros((sequences, 1, page, d), dtype=torch.float16, device="cuda")
+    value = torch.randint(-8, 9, (sequences, 1, d, page), generator=g, device="cuda").half()  # sums and their averages are exact in fp32
+    ids = torch.randperm(sequences, generator=g, device="cuda")
+    table = torch.full((sequences, columns), -1, dtype=torch.int32, device="cuda")
+    table[:, 0] = ids
+    lengths = torch.full((sequences,), page, dtype=torch.int32, device="cuda")
+    if n == 1:
+        lengths = torch.randint(1, page + 1, (sequences,), generator=g, device="cuda").int()
+    starts = torch.arange(sequences + 1, device="cuda").int() * n
+    q = randn(g, tokens, 1, d)
+    out = torch.full_like(q, 9)
+    size = pk.paged_attention_workspace_bytes(tokens, n, sequences, 1, 1, d, page, columns)
+    pk.paged_attention(q, key, value, table, starts, lengths, out, torch.empty(size, dtype=torch.uint8, device="cuda"), max_queries=n)
+    v = value[ids, 0].float().cumsum(2).transpose(1, 2)  # [sequence, keys, feature]
+    seen = torch.arange(1, page + 1, device="cuda").float()
+    want = v / seen[:, None] if n > 1 else (v / seen[:, None])[torch.arange(sequences, device="cuda"), lengths.long() - 1][:, None]
+    # two roundings in fp32 and one to fp16
+    off = (out.view(sequences, n, d).float() - want).abs() - want.abs() * (2.0**-11 + 2.0**-20) - 2.0**-24
+    assert off.max() <= 0
+
+
+def test_write_of_the_most_tokens(pk):  # noqa: F811
+    tokens, page, d = 1 << 21, 128, 64
+    g = gen(45)
+    rows = randn(g, tokens, 2, d)
+    pages = tokens // page
+    ids = torch.randperm(pages, generator=g, device="cuda")
+    slots = (ids[:, None] * page + torch.arange(page, device="cuda")).view(-1).int()
+    key, value = torch.zeros((pages, 1, page, d), dtype=torch.float16, device="cuda"), torch.zeros((pages, 1, d, page), dtype=torch.float16, device="cuda")
+    pk.paged_cache_write(rows[:, :1], rows[:, 1:], slots, key, value)
+    assert torch.equal(key[ids, 0].view(tokens, d), rows[:, 0])
+    assert torch.equal(value[ids, 0].transpose(1, 2).reshape(tokens, d), rows[:, 1])
