@@ -761,6 +761,146 @@ int32_t pk_paged_attention(int32_t kind, const uint16_t* query, int64_t query_st
                            float scale, float key_scale, float value_scale, void* workspace,
                            uint64_t workspace_bytes, void* stream);
 
+/* ---- between projection and cache, and behind the logits, of a step -------------
+ * No reference counterpart.  Inference only. */
+
+#define PK_ROTARY_PLAIN 0
+#define PK_ROTARY_LINEAR 1
+#define PK_ROTARY_BASE 2
+#define PK_ROTARY_BANDS 3
+#define PK_ROTARY_RAMP 4
+
+/* Frequencies of rotary positions (host only, host memory): pair i of rotary_dim /
+ * 2 turns by f_i = base^(-2 i / rotary_dim) radians a position, frequencies[i] =
+ * f_i / (2 pi) * 2^64.  scaling, for contexts longer than the `original` positions a
+ * model was trained on, by factor (>= 1):
+ *   PLAIN   f_i (the other arguments are not looked at),
+ *   LINEAR  f_i / factor,
+ *   BASE    base * factor^(rotary_dim / (rotary_dim - 2)) in place of base,
+ *   BANDS   f_i (k + (1 - k) / factor), k = (n_i - low) / (high - low) within
+ *           [0, 1], n_i = original f_i / (2 pi) the turns over those positions,
+ *   RAMP    the same with 1 - k = (i - first) / (last - first) within [0, 1]: first
+ *           and last are the (fractional) pairs of `high` turns, rounded down, and of
+ *           `low` turns, rounded up, within 0 and rotary_dim - 1.
+ * rotary_dim % 16 == 0 up to 256, 1 < base <= 1e12, 1 <= factor <= 1e6, 0 < low < high. */
+int32_t pk_rotary_frequencies(int32_t scaling, int32_t rotary_dim, double base, double factor, double low, double high,
+                              int32_t original, uint64_t* frequencies);
+
+/* Norm of each head and its rotation by position, in one pass over queries
+ * [tokens x heads x head_dim] and keys [tokens x kv_heads x head_dim] (fp16, rows
+ * query_stride / key_stride elements apart, so both may be slices of one
+ * projection's rows): y = x / sqrt(mean(x^2) + epsilon) * weight over a head's
+ * features (query_weight, key_weight [head_dim]; NULL: y = x), then the pairs
+ * (y_i, y_{i + rotary_dim / 2}), or with interleaved (y_2i, y_{2i + 1}), turn by
+ * positions[t] * frequencies[i]: (u, v) -> amplitude * (u cos - v sin, v cos + u
+ * sin).  Features from rotary_dim on do not turn (nor are multiplied by amplitude).
+ * y is not rounded in between and phases are exact at any position.
+ * head_dim % 16 == 0 from 32 to 256, rotary_dim % 16 == 0 from 0 to head_dim (0: norms
+ * alone; positions and frequencies may be NULL), kv_heads 0: queries alone (key and
+ * key_out may be NULL).  The outputs may be query and key themselves (with their
+ * strides) and overlap nothing else.  A head of zeros stays zeros, also with epsilon 0.
+ * tokens <= 2^21, rows and weights 16-byte, frequencies 8-byte aligned, strides
+ * multiples of 8, 0 <= epsilon <= 1. */
+int32_t pk_head_norm_rotary(const uint16_t* query, int64_t query_stride, const uint16_t* key, int64_t key_stride,
+                            const uint16_t* query_weight, const uint16_t* key_weight, const int32_t* positions,
+                            const uint64_t* frequencies, uint16_t* query_out, int64_t query_out_stride, uint16_t* key_out,
+                            int64_t key_out_stride, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                            int32_t rotary_dim, int32_t interleaved, float amplitude, float epsilon, void* stream);
+
+/* pk_head_norm_rotary and pk_paged_cache_write in one launch: keys go into their
+ * slots instead of key_out, and values [tokens x kv_heads x head_dim] beside them.
+ * PK_CACHE_FP8 stores e4m3(y * key_inverse_scale) of the unrounded key (the two calls
+ * round it to fp16 first).  Of a token whose slot is outside [0, pages * page_size)
+ * nothing is written, its row of query_out included.  head_dim 64 or 128, kv_heads
+ * 1..256; the rest as in those two calls. */
+int32_t pk_head_norm_rotary_write(int32_t kind, const uint16_t* query, int64_t query_stride, const uint16_t* key,
+                                  int64_t key_stride, const uint16_t* value, int64_t value_stride,
+                                  const uint16_t* query_weight, const uint16_t* key_weight, const int32_t* positions,
+                                  const int32_t* slots, const uint64_t* frequencies, uint16_t* query_out,
+                                  int64_t query_out_stride, void* key_cache, void* value_cache, int32_t tokens,
+                                  int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t rotary_dim,
+                                  int32_t interleaved, float amplitude, float epsilon, int32_t page_size, int32_t pages,
+                                  float key_inverse_scale, float value_inverse_scale, void* stream);
+
+#define PK_LOGITS_FP16 0
+#define PK_LOGITS_FP32 1
+
+/* A step of beam search: of the candidates (beam b, token t) of each sequence, with
+ *   score(b, t) = scores[b] + logits[b, t] - log(sum over t of exp(logits[b, t])),
+ * the `choices` best, best first; equal scores: the lowest b * vocab + t.  logits
+ * [sequences * beams x vocab] with rows logits_stride elements apart, scores
+ * [sequences x beams].  ended [sequences x beams] (bytes, may be NULL): such a beam has one
+ * candidate, end_token with its own score, and its logits are not read.  A logit of
+ * -infinity is no candidate; a beam whose score is not finite, or whose logits hold a
+ * NaN or +infinity or are all -infinity, has none.
+ * Written are [sequences x choices] scores (fp32), tokens, parents (the row sequence *
+ * beams + b) and out_ended (the parent had ended, or the token is end_token; may be
+ * NULL); where candidates run out score -infinity, token -1, parent -1, ended 0.
+ * end_token in [0, vocab), or -1: none (ended is NULL then).  Sums and scores are compared in 64
+ * bits, terms of the sums are fp32.  sequences <= 4096, beams <= 32, choices <= 64,
+ * vocab <= 2^20.  logits as their type aligned, workspace (16-byte aligned) of
+ * pk_beam_select_workspace_bytes (enough also for fewer sequences, beams, tokens and
+ * choices), used by one call at a time, need not be kept; outputs and workspace
+ * overlap nothing else. */
+int64_t pk_beam_select_workspace_bytes(int32_t sequences, int32_t beams, int32_t vocab, int32_t choices);
+int32_t pk_beam_select(int32_t kind, const void* logits, int64_t logits_stride, const float* scores,
+                       const uint8_t* ended, float* out_scores, int32_t* out_tokens, int32_t* out_parents,
+                       uint8_t* out_ended, int32_t sequences, int32_t beams, int32_t vocab, int32_t choices,
+                       int32_t end_token, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Rows of a state in their beams' new order: output[s, b] = state[parents[s, b]] for
+ * [sequences x beams] rows of row_bytes bytes; parents are rows of the same sequence
+ * (sequence * beams + beam); with any other (-1) the row of output stays as it was.  output may
+ * be state itself, and overlaps nothing else.  sequences <= 4096, beams <= 32,
+ * row_bytes <= 2^32.  Fastest where the addresses and row_bytes are multiples of 16. */
+int32_t pk_beam_reorder(const void* state, const int32_t* parents, void* output, int32_t sequences, int32_t beams,
+                        int64_t row_bytes, void* stream);
+
+/* Pages that follow their beams: row r of the new tables is a child of row parents[r]
+ * of the old ones (any row; -1: none, the row is empty), with the same length and pages,
+ *   new_lengths[r] = lengths[parents[r]] (0),  new_table[r, c] = block_table[parents[r], c],
+ * but for a page that is not full (lengths % page_size != 0): the parent's lowest child
+ * keeps it, and each other child takes a page of its own from free_pages[free_range[0]
+ * ..), in row order, and copies[r] = {the parent's page, that page} ({-1, -1} where
+ * nothing is to be copied; pk_paged_cache_copy copies them).  freed [pages] lists, in
+ * ascending order, the pages that rows listed and no row does any more, but for those
+ * with held[page] != 0 (bytes, may be NULL: pages that something else has, say a cache
+ * of prompts).  A row of length n has its first ceil(n / page_size) entries; entries
+ * of new_table and freed behind the last stay as they were.  Page ids outside [0,
+ * pages) are passed on and neither copied nor given back.
+ * info [4]: {rows with a parent, pages taken, status, pages given back}; status is 1 (too
+ * few free pages) or 8 (a parent outside [-1, rows), a negative length or one beyond
+ * max_pages pages, or a negative free_range[0]); if it is not 0, the new tables and
+ * lengths are the old ones, and nothing is taken, copied or given back.
+ * pk_page_keep moves the free list behind a fork, or behind a plan, that is kept.
+ * Nothing that is read is changed; what is written overlaps nothing else.  rows <=
+ * 4096, max_pages * page_size <= 2^30, pages * page_size < 2^31.  workspace (16-byte
+ * aligned) of pk_page_fork_workspace_bytes (enough also for fewer rows, columns and
+ * pages), used by one call at a time, need not be kept. */
+int64_t pk_page_fork_workspace_bytes(int32_t rows, int32_t max_pages, int32_t pages);
+int32_t pk_page_fork(const int32_t* parents, const int32_t* block_table, const int32_t* lengths,
+                     const int32_t* free_pages, const int32_t* free_range, int32_t free_capacity, const uint8_t* held,
+                     int32_t* new_table, int32_t* new_lengths, int32_t* copies, int32_t* freed, int32_t* info,
+                     int32_t rows, int32_t max_pages, int32_t page_size, int32_t pages, void* workspace,
+                     uint64_t workspace_bytes, void* stream);
+
+/* The free list behind a step that is kept: free_range[0] += info[1] - info[3], and the
+ * info[3] pages of freed stand in front of the list, free_pages[free_range[0] ..).
+ * info as pk_page_fork or (freed NULL) pk_page_plan wrote it; nothing happens where its status is
+ * not 0.  A list in front of which there is no room for all (its pages never came from
+ * it) takes the first ones. */
+int32_t pk_page_keep(const int32_t* info, const int32_t* freed, int32_t* free_pages, int32_t* free_range,
+                     int32_t free_capacity, void* stream);
+
+/* Copies of pages: for each pair {source, destination} of copies [count x 2], the keys
+ * and values of page source into page destination, in each of `layers` layers
+ * (key_cache and value_cache [layers x pages x page_bytes]).  Pairs with a page outside
+ * [0, pages) are skipped.  No destination is a source, or a destination twice.
+ * count <= 65535, layers <= 4096, page_bytes % 16 == 0 up to 2^24, pages < 2^31 / 16; the caches are
+ * 16-byte aligned and overlap nothing else. */
+int32_t pk_paged_cache_copy(const int32_t* copies, int32_t count, void* key_cache, void* value_cache,
+                            int64_t page_bytes, int32_t pages, int32_t layers, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

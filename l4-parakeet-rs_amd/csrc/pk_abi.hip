@@ -1134,4 +1134,344 @@ int32_t pk_paged_attention(int32_t kind, const uint16_t* query, int64_t query_st
     return check_launch("paged_attention");
 }
 
+// ---- between projection and cache, and behind the logits, of a step -------------------
+
+int32_t pk_rotary_frequencies(int32_t scaling, int32_t rotary_dim, double base, double factor, double low, double high, int32_t original,
+                              uint64_t* frequencies) {
+    if (scaling < PK_ROTARY_PLAIN || scaling > PK_ROTARY_RAMP) { set_error("rotary scaling must be 0..4, got %d", scaling); return PK_E_ARG; }
+    if (rotary_dim < 16 || rotary_dim > 256 || rotary_dim % 16) {
+        set_error("rotary_dim must be a multiple of 16 up to 256, got %d", rotary_dim);
+        return PK_E_SHAPE;
+    }
+    if (!(base > 1.0 && base <= 1e12)) { set_error("the rotary base must lie in (1, 1e12], got %g", base); return PK_E_ARG; }
+    if (scaling != PK_ROTARY_PLAIN && !(factor >= 1.0 && factor <= 1e6)) {
+        set_error("the rotary factor must lie in [1, 1e6], got %g", factor);
+        return PK_E_ARG;
+    }
+    if (scaling >= PK_ROTARY_BANDS && !(low > 0.0 && low < high && std::isfinite(high) && original > 0)) {
+        set_error("rotary bands need 0 < low < high and original > 0 (low=%g high=%g original=%d)", low, high, original);
+        return PK_E_ARG;
+    }
+    if (!need(frequencies, "frequencies")) return PK_E_ARG;
+    rotary_frequencies(scaling, rotary_dim / 2, base, factor, low, high, original, frequencies);
+    return PK_OK;
+}
+
+// What both forms of the head norm refuse by shape, before any address is looked at; 0 or a status.
+static int32_t head_norm_shape(const RotaryArgs& a) {
+    if (a.tokens < 0 || a.tokens > 1 << 21 || a.heads <= 0 || a.heads > 1024 || a.kv_heads < 0 || a.kv_heads > 1024 || a.head_dim < 32 ||
+        a.head_dim > 256 || a.head_dim % 16 || a.rotary_dim < 0 || a.rotary_dim > a.head_dim || a.rotary_dim % 16) {
+        set_error("head norm needs tokens <= 2^21, 1..1024 heads, up to 1024 kv heads, head_dim %% 16 == 0 from 32 to 256 and rotary_dim %% 16 == 0 "
+                  "up to head_dim (tokens=%d heads=%d kv_heads=%d head_dim=%d rotary_dim=%d)", a.tokens, a.heads, a.kv_heads, a.head_dim, a.rotary_dim);
+        return PK_E_SHAPE;
+    }
+    const int64_t q = (int64_t)a.heads * a.head_dim, k = (int64_t)a.kv_heads * a.head_dim;
+    const int64_t strides[][2] = {{a.query_stride, q}, {a.query_out_stride, q}, {a.key_stride, k}, {a.key_out_stride, k}, {a.value_stride, k}};
+    for (const auto& s : strides)
+        if (s[0] < s[1] || s[0] >= 1ll << 31) {
+            set_error("head norm strides must be at least a row's elements (%lld for queries, %lld for keys and values), got %lld", (long long)q,
+                      (long long)k, (long long)s[0]);
+            return PK_E_SHAPE;
+        }
+    if (!(a.epsilon >= 0.0f) || a.epsilon > 1.0f) { set_error("epsilon must lie in [0, 1], got %g", (double)a.epsilon); return PK_E_ARG; }
+    if (!std::isfinite(a.amplitude)) { set_error("the amplitude must be finite, got %g", (double)a.amplitude); return PK_E_ARG; }
+    return PK_OK;
+}
+
+static RowSet rows_of(const void* base, int64_t stride, int heads, const RotaryArgs& a) {
+    return {base, 2 * stride, 2ll * heads * a.head_dim, heads ? a.tokens : 0};
+}
+
+// Whether a row output meets what the head norm reads, but for the rows (0 queries, 1 keys, -1 none) that it may stand in place of.
+static bool head_norm_meets(const RotaryArgs& a, const RowSet& out, int in_place) {
+    const RowSet q = rows_of(a.query, a.query_stride, a.heads, a), k = rows_of(a.key, a.key_stride, a.kv_heads, a);
+    const RowSet v = rows_of(a.value, a.value_stride, a.value ? a.kv_heads : 0, a);
+    if ((in_place != 0 && overlap(out, q)) || (in_place != 1 && overlap(out, k)) || overlap(out, v)) return true;
+    const int64_t w = 2 * a.head_dim, t = 4ll * a.tokens;
+    return overlap(out, a.query_weight, w) || overlap(out, a.key_weight, w) || overlap(out, a.positions, t) || overlap(out, a.slots, t) ||
+           overlap(out, a.frequencies, 4ll * a.rotary_dim);
+}
+
+static int32_t head_norm_pointers(const RotaryArgs& a) {
+    if (!need(a.query, "query") || !need(a.query_out, "query_out") || (a.kv_heads && !need(a.key, "key")) ||
+        (a.rotary_dim && (!need(a.positions, "positions") || !need(a.frequencies, "frequencies"))))
+        return PK_E_ARG;
+    for (const void* p : {(const void*)a.query, (const void*)a.key, (const void*)a.value, (const void*)a.query_weight, (const void*)a.key_weight,
+                          (const void*)a.query_out, (const void*)a.key_out, (const void*)a.key_cache, (const void*)a.value_cache})
+        if (misaligned(p, 16)) { set_error("head norm rows, weights and caches must be 16-byte aligned"); return PK_E_ALIGN; }
+    if (misaligned(a.positions, 4) || misaligned(a.slots, 4) || misaligned(a.frequencies, 8) || a.query_stride % 8 || a.key_stride % 8 ||
+        a.value_stride % 8 || a.query_out_stride % 8 || a.key_out_stride % 8) {
+        set_error("head norm strides must be multiples of 8, positions and slots 4-byte, frequencies 8-byte aligned");
+        return PK_E_ALIGN;
+    }
+    return PK_OK;
+}
+
+int32_t pk_head_norm_rotary(const uint16_t* query, int64_t query_stride, const uint16_t* key, int64_t key_stride, const uint16_t* query_weight,
+                            const uint16_t* key_weight, const int32_t* positions, const uint64_t* frequencies, uint16_t* query_out,
+                            int64_t query_out_stride, uint16_t* key_out, int64_t key_out_stride, int32_t tokens, int32_t heads, int32_t kv_heads,
+                            int32_t head_dim, int32_t rotary_dim, int32_t interleaved, float amplitude, float epsilon, void* stream) {
+    RotaryArgs a{};
+    a.query = query;
+    a.key = kv_heads ? key : nullptr;
+    a.query_weight = query_weight;
+    a.key_weight = kv_heads ? key_weight : nullptr;
+    a.positions = rotary_dim ? positions : nullptr;
+    a.frequencies = rotary_dim ? (const unsigned long long*)frequencies : nullptr;
+    a.query_out = query_out;
+    a.key_out = kv_heads ? key_out : nullptr;
+    a.query_stride = query_stride;
+    a.query_out_stride = query_out_stride;
+    a.key_stride = kv_heads ? key_stride : 0;
+    a.key_out_stride = kv_heads ? key_out_stride : 0;
+    a.tokens = tokens;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.rotary_dim = rotary_dim;
+    a.interleaved = interleaved != 0;
+    a.amplitude = amplitude;
+    a.epsilon = epsilon;
+    a.value_stride = (int64_t)kv_heads * head_dim;
+    int32_t status = head_norm_shape(a);
+    if (status) return status;
+    if (tokens == 0) return PK_OK;
+    if (kv_heads && !need(key_out, "key_out")) return PK_E_ARG;
+    status = head_norm_pointers(a);
+    if (status) return status;
+    const RowSet qo = rows_of(query_out, query_out_stride, heads, a), ko = rows_of(a.key_out, a.key_out_stride, kv_heads, a);
+    if (head_norm_meets(a, qo, query == query_out && (query_stride == query_out_stride || tokens == 1) ? 0 : -1) ||
+        (kv_heads && (head_norm_meets(a, ko, key == key_out && (key_stride == key_out_stride || tokens == 1) ? 1 : -1) || overlap(qo, ko)))) {
+        set_error("head norm: an output overlaps another array (query_out may be query, key_out key)");
+        return PK_E_ARG;
+    }
+    launch_head_norm_rotary(a, STREAM);
+    return check_launch("head_norm_rotary");
+}
+
+int32_t pk_head_norm_rotary_write(int32_t kind, const uint16_t* query, int64_t query_stride, const uint16_t* key, int64_t key_stride,
+                                  const uint16_t* value, int64_t value_stride, const uint16_t* query_weight, const uint16_t* key_weight,
+                                  const int32_t* positions, const int32_t* slots, const uint64_t* frequencies, uint16_t* query_out,
+                                  int64_t query_out_stride, void* key_cache, void* value_cache, int32_t tokens, int32_t heads, int32_t kv_heads,
+                                  int32_t head_dim, int32_t rotary_dim, int32_t interleaved, float amplitude, float epsilon, int32_t page_size,
+                                  int32_t pages, float key_inverse_scale, float value_inverse_scale, void* stream) {
+    const int32_t shift = cache_shape(kind, kv_heads, head_dim, page_size, pages);
+    if (shift < 0) return shift;
+    RotaryArgs a{};
+    a.query = query;
+    a.key = key;
+    a.value = value;
+    a.query_weight = query_weight;
+    a.key_weight = key_weight;
+    a.positions = rotary_dim ? positions : nullptr;
+    a.slots = slots;
+    a.frequencies = rotary_dim ? (const unsigned long long*)frequencies : nullptr;
+    a.query_out = query_out;
+    a.key_cache = key_cache;
+    a.value_cache = value_cache;
+    a.query_stride = query_stride;
+    a.query_out_stride = query_out_stride;
+    a.key_stride = key_stride;
+    a.value_stride = value_stride;
+    a.key_out_stride = (int64_t)kv_heads * head_dim;
+    a.tokens = tokens;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.rotary_dim = rotary_dim;
+    a.interleaved = interleaved != 0;
+    a.amplitude = amplitude;
+    a.epsilon = epsilon;
+    a.shift = shift;
+    a.slot_count = (long long)pages << shift;
+    a.k_inv = key_inverse_scale;
+    a.v_inv = value_inverse_scale;
+    int32_t status = head_norm_shape(a);
+    if (status) return status;
+    if (tokens == 0) return PK_OK;
+    if (!need(value, "value") || !need(slots, "slots") || !need(key_cache, "key_cache") || !need(value_cache, "value_cache")) return PK_E_ARG;
+    status = head_norm_pointers(a);
+    if (status) return status;
+    const RowSet q = rows_of(query, query_stride, heads, a), qo = rows_of(query_out, query_out_stride, heads, a);
+    const int64_t cache = a.slot_count * kv_heads * head_dim * (kind == PK_CACHE_FP8 ? 1 : 2);
+    bool meet = head_norm_meets(a, qo, query == query_out && (query_stride == query_out_stride || tokens == 1) ? 0 : -1) ||
+                overlap(key_cache, cache, value_cache, cache);
+    const RowSet rows[] = {q, qo, rows_of(key, key_stride, kv_heads, a), rows_of(value, value_stride, kv_heads, a)};
+    for (const void* c : {key_cache, value_cache}) {
+        for (const RowSet& r : rows) meet = meet || overlap(r, c, cache);
+        meet = meet || overlap(c, cache, slots, 4 * (size_t)tokens) || overlap(c, cache, a.positions, 4 * (size_t)tokens) ||
+               overlap(c, cache, a.frequencies, 4 * (size_t)rotary_dim) || overlap(c, cache, query_weight, 2 * (size_t)head_dim) ||
+               overlap(c, cache, key_weight, 2 * (size_t)head_dim);
+    }
+    if (meet) {
+        set_error("head norm: an output or a cache overlaps another array (query_out may be query)");
+        return PK_E_ARG;
+    }
+    launch_head_norm_rotary_write(kind, a, STREAM);
+    return check_launch("head_norm_rotary_write");
+}
+
+static int32_t beam_shape(int32_t sequences, int32_t beams, int32_t vocab, int32_t choices) {
+    if (sequences < 0 || sequences > 4096 || beams <= 0 || beams > 32 || vocab <= 0 || vocab > 1 << 20 || choices <= 0 || choices > 64) {
+        set_error("beam search needs sequences <= 4096, 1..32 beams, 1..2^20 tokens and 1..64 choices (sequences=%d beams=%d vocab=%d choices=%d)",
+                  sequences, beams, vocab, choices);
+        return PK_E_SHAPE;
+    }
+    return PK_OK;
+}
+
+int64_t pk_beam_select_workspace_bytes(int32_t sequences, int32_t beams, int32_t vocab, int32_t choices) {
+    const int32_t status = beam_shape(sequences, beams, vocab, choices);
+    if (status) return status;
+    return (int64_t)beam_workspace(sequences, beams, vocab, choices);
+}
+
+int32_t pk_beam_select(int32_t kind, const void* logits, int64_t logits_stride, const float* scores, const uint8_t* ended, float* out_scores,
+                       int32_t* out_tokens, int32_t* out_parents, uint8_t* out_ended, int32_t sequences, int32_t beams, int32_t vocab,
+                       int32_t choices, int32_t end_token, void* workspace, uint64_t workspace_bytes, void* stream) {
+    if (kind != PK_LOGITS_FP16 && kind != PK_LOGITS_FP32) { set_error("logits kind must be 0 (fp16) or 1 (fp32), got %d", kind); return PK_E_ARG; }
+    const int32_t status = beam_shape(sequences, beams, vocab, choices);
+    if (status) return status;
+    if (logits_stride < vocab || logits_stride >= 1ll << 31) {
+        set_error("logits_stride must be at least vocab = %d, got %lld", vocab, (long long)logits_stride);
+        return PK_E_SHAPE;
+    }
+    if (end_token < -1 || end_token >= vocab || (ended && end_token < 0)) {
+        set_error("end_token must lie in [-1, vocab), and in [0, vocab) with ended beams, got %d", end_token);
+        return PK_E_ARG;
+    }
+    if (sequences == 0) return PK_OK;
+    if (!need(logits, "logits") || !need(scores, "scores") || !need(out_scores, "out_scores") || !need(out_tokens, "out_tokens") ||
+        !need(out_parents, "out_parents"))
+        return PK_E_ARG;
+    if (misaligned(logits, kind == PK_LOGITS_FP16 ? 2 : 4) || misaligned(scores, 4) || misaligned(out_scores, 4) || misaligned(out_tokens, 4) ||
+        misaligned(out_parents, 4) || misaligned(workspace, 16)) {
+        set_error("beam search arrays must be aligned as their types, the workspace to 16 bytes");
+        return PK_E_ALIGN;
+    }
+    const uint64_t wanted = beam_workspace(sequences, beams, vocab, choices);
+    if (wanted > 0 && (!need(workspace, "workspace") || workspace_bytes < wanted)) {
+        if (workspace) set_error("beam search needs %llu bytes of workspace, got %llu", (unsigned long long)wanted, (unsigned long long)workspace_bytes);
+        return PK_E_ARG;
+    }
+    const size_t rows = (size_t)sequences * beams, n = (size_t)sequences * choices, each = kind == PK_LOGITS_FP16 ? 2 : 4;
+    const RowSet x{logits, (int64_t)(logits_stride * each), (int64_t)(vocab * each), (int64_t)rows};
+    const struct { const void* p; size_t bytes; } arrays[] = {{scores, 4 * rows}, {ended, rows},   {out_scores, 4 * n}, {out_tokens, 4 * n},
+                                                              {out_parents, 4 * n}, {out_ended, n}, {workspace, wanted}};
+    for (int i = 2; i < 7; ++i) {
+        bool meet = overlap(x, arrays[i].p, (int64_t)arrays[i].bytes);
+        for (int j = 0; j < i; ++j) meet = meet || overlap(arrays[i].p, arrays[i].bytes, arrays[j].p, arrays[j].bytes);
+        if (meet) { set_error("beam search: an output or the workspace overlaps another array"); return PK_E_ARG; }
+    }
+    const BeamArgs a{logits, scores, ended, out_scores, out_tokens, out_parents, out_ended, workspace, logits_stride, sequences, beams, vocab, choices, end_token};
+    launch_beam_select(kind == PK_LOGITS_FP16, a, STREAM);
+    return check_launch("beam_select");
+}
+
+int32_t pk_beam_reorder(const void* state, const int32_t* parents, void* output, int32_t sequences, int32_t beams, int64_t row_bytes, void* stream) {
+    if (sequences < 0 || sequences > 4096 || beams <= 0 || beams > 32 || row_bytes < 0 || row_bytes > 1ll << 32) {
+        set_error("beam reorder needs sequences <= 4096, 1..32 beams and rows of at most 2^32 bytes (sequences=%d beams=%d row_bytes=%lld)", sequences,
+                  beams, (long long)row_bytes);
+        return PK_E_SHAPE;
+    }
+    if (sequences == 0 || row_bytes == 0) return PK_OK;
+    if (!need(state, "state") || !need(parents, "parents") || !need(output, "output")) return PK_E_ARG;
+    if (misaligned(parents, 4)) { set_error("parents must be 4-byte aligned"); return PK_E_ALIGN; }
+    const size_t rows = (size_t)sequences * beams, bytes = rows * row_bytes;
+    if ((state != output && overlap(state, bytes, output, bytes)) || overlap(parents, 4 * rows, output, bytes)) {
+        set_error("beam reorder: output overlaps another array (it may be state itself)");
+        return PK_E_ARG;
+    }
+    launch_beam_reorder(state, parents, output, sequences, beams, row_bytes, STREAM);
+    return check_launch("beam_reorder");
+}
+
+int64_t pk_page_fork_workspace_bytes(int32_t rows, int32_t max_pages, int32_t pages) {
+    if (rows < 0 || rows > kMostForkRows || max_pages <= 0 || max_pages > 1 << 26 || pages <= 0 || pages >= 1 << 27) {
+        set_error("page_fork needs rows <= %d, max_pages <= 2^26 and pages < 2^27 (rows=%d max_pages=%d pages=%d)", kMostForkRows, rows, max_pages, pages);
+        return PK_E_SHAPE;
+    }
+    return (int64_t)fork_workspace(rows, pages);
+}
+
+int32_t pk_page_fork(const int32_t* parents, const int32_t* block_table, const int32_t* lengths, const int32_t* free_pages,
+                     const int32_t* free_range, int32_t free_capacity, const uint8_t* held, int32_t* new_table, int32_t* new_lengths,
+                     int32_t* copies, int32_t* freed, int32_t* info, int32_t rows, int32_t max_pages, int32_t page_size, int32_t pages,
+                     void* workspace, uint64_t workspace_bytes, void* stream) {
+    const int shift = page_shift(page_size);
+    if (shift < 0) { set_error("page_size must be 16, 32, 64, 128 or 256, got %d", page_size); return PK_E_SHAPE; }
+    const int64_t wanted = pk_page_fork_workspace_bytes(rows, max_pages, pages);
+    if (wanted < 0) return (int32_t)wanted;
+    if (rows == 0 || max_pages > (1 << 30) >> shift || (int64_t)pages << shift > 0x7fffffffll || free_capacity < 0) {
+        set_error("page_fork needs rows >= 1, max_pages * page_size <= 2^30, pages * page_size < 2^31 and free_capacity >= 0 (rows=%d max_pages=%d "
+                  "page_size=%d pages=%d free_capacity=%d)", rows, max_pages, page_size, pages, free_capacity);
+        return PK_E_SHAPE;
+    }
+    if (!need(parents, "parents") || !need(block_table, "block_table") || !need(lengths, "lengths") || !need(free_range, "free_range") ||
+        (free_capacity && !need(free_pages, "free_pages")) || !need(new_table, "new_table") || !need(new_lengths, "new_lengths") ||
+        !need(copies, "copies") || !need(freed, "freed") || !need(info, "info") || !need(workspace, "workspace"))
+        return PK_E_ARG;
+    for (const void* p : {(const void*)parents, (const void*)block_table, (const void*)lengths, (const void*)free_pages, (const void*)free_range,
+                          (const void*)new_table, (const void*)new_lengths, (const void*)copies, (const void*)freed, (const void*)info})
+        if (misaligned(p, 4)) { set_error("page_fork arrays must be 4-byte aligned"); return PK_E_ALIGN; }
+    if (misaligned(workspace, 16)) { set_error("the workspace must be 16-byte aligned"); return PK_E_ALIGN; }
+    if (workspace_bytes < (uint64_t)wanted) {
+        set_error("page_fork needs %lld bytes of workspace, got %llu", (long long)wanted, (unsigned long long)workspace_bytes);
+        return PK_E_ARG;
+    }
+    const size_t r = 4 * (size_t)rows;
+    const struct { const void* p; size_t bytes; } arrays[] = {
+        {parents, r}, {block_table, r * max_pages}, {lengths, r}, {free_pages, 4 * (size_t)free_capacity}, {free_range, 8}, {held, (size_t)pages},
+        {new_table, r * max_pages}, {new_lengths, r}, {copies, 2 * r}, {freed, 4 * (size_t)pages}, {info, 16}, {workspace, (size_t)wanted}};
+    for (int i = 6; i < 12; ++i)
+        for (int j = 0; j < i; ++j)
+            if (overlap(arrays[i].p, arrays[i].bytes, arrays[j].p, arrays[j].bytes)) {
+                set_error("page_fork: an output or the workspace overlaps another array");
+                return PK_E_ARG;
+            }
+    const ForkArgs a{parents, block_table, lengths, free_pages, free_range, held, new_table, new_lengths, copies, freed, info, workspace,
+                     free_capacity, rows, max_pages, shift, pages};
+    launch_page_fork(a, STREAM);
+    return check_launch("page_fork");
+}
+
+int32_t pk_page_keep(const int32_t* info, const int32_t* freed, int32_t* free_pages, int32_t* free_range, int32_t free_capacity, void* stream) {
+    if (free_capacity < 0) { set_error("page_keep needs free_capacity >= 0, got %d", free_capacity); return PK_E_SHAPE; }
+    if (!need(info, "info") || !need(free_range, "free_range") || (free_capacity && !need(free_pages, "free_pages"))) return PK_E_ARG;
+    for (const void* p : {(const void*)info, (const void*)freed, (const void*)free_pages, (const void*)free_range})
+        if (misaligned(p, 4)) { set_error("page_keep arrays must be 4-byte aligned"); return PK_E_ALIGN; }
+    // of freed as many entries as the list holds are read at most
+    const size_t n = 4 * (size_t)free_capacity;
+    if (overlap(free_pages, n, info, 16) || overlap(free_pages, n, freed, n) || overlap(free_pages, n, free_range, 8) || overlap(free_range, 8, info, 16) ||
+        overlap(free_range, 8, freed, n)) {
+        set_error("page_keep: the free list overlaps another array");
+        return PK_E_ARG;
+    }
+    launch_page_keep(info, freed, free_pages, free_range, free_capacity, STREAM);
+    return check_launch("page_keep");
+}
+
+int32_t pk_paged_cache_copy(const int32_t* copies, int32_t count, void* key_cache, void* value_cache, int64_t page_bytes, int32_t pages,
+                            int32_t layers, void* stream) {
+    if (count < 0 || count > 65535 || layers < 0 || layers > 4096 || pages <= 0 || pages >= 1 << 27 || page_bytes <= 0 || page_bytes > 1 << 24 ||
+        page_bytes % 16) {
+        set_error("cache copy needs count <= 65535, layers <= 4096, 1 <= pages < 2^27 and page_bytes %% 16 == 0 up to 2^24 (count=%d layers=%d pages=%d "
+                  "page_bytes=%lld)", count, layers, pages, (long long)page_bytes);
+        return PK_E_SHAPE;
+    }
+    if (count == 0 || layers == 0) return PK_OK;
+    if (!need(copies, "copies") || !need(key_cache, "key_cache") || !need(value_cache, "value_cache")) return PK_E_ARG;
+    if (misaligned(copies, 4) || misaligned(key_cache, 16) || misaligned(value_cache, 16)) {
+        set_error("copies must be 4-byte, caches 16-byte aligned");
+        return PK_E_ALIGN;
+    }
+    const size_t cache = (size_t)layers * pages * page_bytes, pairs = 8 * (size_t)count;
+    if (overlap(key_cache, cache, value_cache, cache) || overlap(key_cache, cache, copies, pairs) || overlap(value_cache, cache, copies, pairs)) {
+        set_error("cache copy: a cache overlaps another array");
+        return PK_E_ARG;
+    }
+    launch_paged_cache_copy(copies, count, key_cache, value_cache, page_bytes, pages, layers, STREAM);
+    return check_launch("paged_cache_copy");
+}
+
 }  // extern "C"

@@ -103,6 +103,65 @@ struct PagedArgs {
 };
 size_t paged_attention_workspace(int head_dim, int page_shift, int max_pages, int max_rows);
 void launch_paged_attention(int kind, const PagedArgs& args, int head_dim, int max_queries, void* workspace, hipStream_t s);
+// frequencies: turns a position in 2^-64; the cache's members in the writing form alone
+struct RotaryArgs {
+    const uint16_t* query;
+    const uint16_t* key;
+    const uint16_t* value;
+    const uint16_t* query_weight;
+    const uint16_t* key_weight;
+    const int* positions;
+    const int* slots;
+    const unsigned long long* frequencies;
+    uint16_t* query_out;
+    uint16_t* key_out;
+    void* key_cache;
+    void* value_cache;
+    long long query_stride, key_stride, value_stride, query_out_stride, key_out_stride, slot_count;
+    int tokens, heads, kv_heads, head_dim, rotary_dim, interleaved, shift;
+    float amplitude, epsilon, k_inv, v_inv;
+};
+void launch_head_norm_rotary(const RotaryArgs& args, hipStream_t s);
+void launch_head_norm_rotary_write(int kind, const RotaryArgs& args, hipStream_t s);
+void rotary_frequencies(int scaling, int pairs, double base, double factor, double low, double high, int original, uint64_t* out);
+
+// Logits [sequences * beams x vocab] fp16 or fp32, rows `stride` elements apart.
+struct BeamArgs {
+    const void* logits;
+    const float* scores;
+    const uint8_t* ended;
+    float* out_scores;
+    int* out_tokens;
+    int* out_parents;
+    uint8_t* out_ended;
+    void* workspace;
+    long long stride;
+    int sequences, beams, vocab, choices, end_token;
+};
+size_t beam_workspace(int sequences, int beams, int vocab, int choices);
+void launch_beam_select(bool fp16, const BeamArgs& args, hipStream_t s);
+void launch_beam_reorder(const void* state, const int* parents, void* out, int sequences, int beams, long long row_bytes, hipStream_t s);
+
+struct ForkArgs {
+    const int* parents;
+    const int* table;
+    const int* lengths;
+    const int* free_pages;
+    const int* free_range;
+    const uint8_t* held;
+    int* new_table;
+    int* new_lengths;
+    int* copies;
+    int* freed;
+    int* info;
+    void* workspace;
+    int free_capacity, rows, max_pages, shift, pages;
+};
+constexpr int kMostForkRows = 4096;  // what a row's children are lies in LDS
+size_t fork_workspace(int rows, int pages);
+void launch_page_fork(const ForkArgs& args, hipStream_t s);
+void launch_page_keep(const int* info, const int* freed, int* free_pages, int* free_range, int free_capacity, hipStream_t s);
+void launch_paged_cache_copy(const int* copies, int count, void* key_cache, void* value_cache, long long page_bytes, int pages, int layers, hipStream_t s);
 void set_error(const char* fmt, ...);
 int cu_count();
 int launch_sparse24_contract(const uint8_t* data, const uint8_t* meta, const uint8_t* w, const float* w_scales, float in_scale,

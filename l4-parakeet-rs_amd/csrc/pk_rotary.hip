@@ -1,0 +1,208 @@
+// Norm of each query and key head and its rotation by the token's position, in one pass:
+//   y = x / sqrt(mean(x^2) + eps) * w   over the features of a head (no weight: y = x),
+//   (u, v) -> a (u cos t - v sin t, v cos t + u sin t),  t = position * frequency,
+// for the pairs (y_i, y_{i + R/2}) or (y_2i, y_2i+1) of the first R features; and the same
+// with keys and values written into the paged cache.
+//
+// Angles: a frequency is held as turns a position in units of 2^-64, so that position *
+// frequency modulo 2^64 is the phase, exact however far the position.  Its upper 32 bits
+// are taken to the nearest quarter turn, and sine and cosine of the rest (within pi / 4)
+// are the Taylor sums to x^9 and x^8, off by less than x^10 / 10! = 2.5e-8.
+//
+// A lane holds 16 features of a head, and in either layout both halves of 8 pairs with the
+// same 8 frequencies; head_dim / 16 lanes make a head.  Everything between the loads and the
+// one rounding at the store is fp32.
+#include <math.h>
+
+#include "pk_paged_write.hpp"
+
+namespace pk {
+
+// amplitude * (cos, sin) of a phase in 2^-64 turns
+__device__ __forceinline__ float2 turned_by(unsigned long long phase, float amplitude) {
+    const uint32_t u = (uint32_t)(phase >> 32), quarter = (u + 0x20000000u) >> 30;
+    const float x = (float)(int)(u - (quarter << 30)) * 1.46291807926715968e-9f;  // 2 pi / 2^32
+    const float z = x * x;
+    const float s = x * __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), 1.0f);
+    const float c = __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 1.0f / 40320, -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
+    const float a = quarter & 1 ? s : c, b = quarter & 1 ? c : s;
+    return float2{(quarter + 1) & 2 ? -a * amplitude : a * amplitude, quarter & 2 ? -b * amplitude : b * amplitude};
+}
+
+__device__ __forceinline__ void unpack(const uint4& raw, float (&y)[8]) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = h2f((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
+}
+
+template <bool kF8> __device__ __forceinline__ void store8(uint8_t* to, const float (&y)[8], float inverse) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (kF8) {
+            const uint32_t pair = e4m3x2(y[2 * j] * inverse, y[2 * j + 1] * inverse);
+            if (j & 1) w[j >> 1] |= pair << 16;
+            else w[j >> 1] = pair;
+        } else {
+            w[j] = (uint32_t)f2h(y[2 * j]) | ((uint32_t)f2h(y[2 * j + 1]) << 16);
+        }
+    }
+    if constexpr (kF8) *(uint2*)to = uint2{w[0], w[1]};
+    else *(uint4*)to = uint4{w[0], w[1], w[2], w[3]};
+}
+
+// kLanes lanes a head (a power of two of at least head_dim / 16).  kCache: -1 rows out, 0 an
+// fp16 cache, 1 an e4m3 one.  A wave takes `sets` times 64 / kLanes heads of a token.
+template <int kLanes, int kCache>
+__global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int parts, int sets, int value_blocks) {
+    constexpr int kSlots = 64 / kLanes;
+    constexpr bool kF8 = kCache == 1;
+    __shared__ float2 angles[4][128];
+    if constexpr (kCache >= 0) {
+        if ((int)blockIdx.x < value_blocks) {  // prompts: the values, turned around in tiles
+            const WriteArgs w{nullptr, a.value, a.slots, nullptr, (uint8_t*)a.value_cache, 0, a.value_stride, a.slot_count, a.tokens, a.kv_heads,
+                              a.shift, 1.0f, a.v_inv};
+            if (a.head_dim == 128) write_tile<128, kF8, false>(w, blockIdx.x % a.kv_heads, blockIdx.x / a.kv_heads);
+            else write_tile<64, kF8, false>(w, blockIdx.x % a.kv_heads, blockIdx.x / a.kv_heads);
+            return;
+        }
+    }
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, p = lane % kLanes;
+    const long long unit = (long long)(blockIdx.x - value_blocks) * 4 + wave;
+    const int t = (int)(unit / parts), first = (int)(unit % parts) * sets * kSlots + lane / kLanes;
+    bool real = t < a.tokens;
+    int slot = 0;
+    if constexpr (kCache >= 0) {
+        slot = real ? a.slots[t] : -1;
+        real = slot >= 0 && slot < a.slot_count;
+    }
+    const long long position = real && a.rotary_dim ? a.positions[t] : 0;  // (no rotation: there may be no positions)
+    for (int i = lane; i < a.rotary_dim / 2; i += 64) angles[wave][i] = turned_by((unsigned long long)position * a.frequencies[i], a.amplitude);
+    __syncthreads();
+    if (!real) return;
+    const bool inside = p * 16 < a.head_dim, turns = p * 16 < a.rotary_dim, halves = turns && !a.interleaved;
+    const int f0 = halves ? 8 * p : 16 * p, f1 = halves ? f0 + a.rotary_dim / 2 : f0 + 8;
+    float2 angle[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) angle[j] = turns ? angles[wave][8 * p + j] : float2{1.0f, 0.0f};
+    const int of_values = kCache >= 0 && value_blocks == 0 ? a.kv_heads : 0, all = a.heads + a.kv_heads + of_values;
+    const int stop = first + sets * kSlots < all ? first + sets * kSlots : all;
+    const int off = slot & ((1 << a.shift) - 1);
+    for (int h = first; h < stop; h += kSlots) {
+        const bool query = h < a.heads, value = h >= a.heads + a.kv_heads;
+        const int kvh = value ? h - a.heads - a.kv_heads : h - a.heads;
+        const uint16_t* row = query ? a.query + (size_t)t * a.query_stride + (size_t)h * a.head_dim
+                                    : (value ? a.value + (size_t)t * a.value_stride : a.key + (size_t)t * a.key_stride) + (size_t)kvh * a.head_dim;
+        uint4 r0{}, r1{};
+        if (inside) {
+            r0 = *(const uint4*)(row + f0);
+            r1 = *(const uint4*)(row + f1);
+        }
+        float u[8], v[8];
+        unpack(r0, u);
+        unpack(r1, v);
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(v[j], v[j], __builtin_fmaf(u[j], u[j], sum));
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) sum = add_level(sum, o);
+        if (!inside) continue;
+        if constexpr (kCache >= 0) {
+            if (value) {  // features lie a page's tokens apart
+                const size_t base = ((size_t)(slot >> a.shift) * a.kv_heads + kvh) * a.head_dim;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const size_t at = ((base + (j < 8 ? f0 + j : f1 + j - 8)) << a.shift) + off;
+                    const float y = j < 8 ? u[j] : v[j - 8];
+                    if constexpr (kF8) ((uint8_t*)a.value_cache)[at] = e4m3(y * a.v_inv);
+                    else ((uint16_t*)a.value_cache)[at] = f2h(y);
+                }
+                continue;
+            }
+        }
+        const uint16_t* weight = query ? a.query_weight : a.key_weight;
+        if (weight) {
+            const float mean = sum / (float)a.head_dim + a.epsilon;
+            const float rstd = mean > 0.0f ? 1.0f / sqrtf(mean) : (mean == 0.0f ? 0.0f : mean);  // NaN stays NaN; all zero with eps 0: zeros
+            float w0[8], w1[8];
+            unpack(*(const uint4*)(weight + f0), w0);
+            unpack(*(const uint4*)(weight + f1), w1);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                u[j] = u[j] * rstd * w0[j];
+                v[j] = v[j] * rstd * w1[j];
+            }
+        }
+        if (turns) {
+            const auto turn = [](float& x, float& y, float2 by) {
+                const float x0 = x;
+                x = __builtin_fmaf(x0, by.x, -(y * by.y));
+                y = __builtin_fmaf(y, by.x, x0 * by.y);
+            };
+            if (a.interleaved) {
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    turn(u[j], u[j + 1], angle[j / 2]);
+                    turn(v[j], v[j + 1], angle[4 + j / 2]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) turn(u[j], v[j], angle[j]);
+            }
+        }
+        if (kCache < 0 || query) {
+            uint16_t* to = query ? a.query_out + (size_t)t * a.query_out_stride + (size_t)h * a.head_dim
+                                 : a.key_out + (size_t)t * a.key_out_stride + (size_t)kvh * a.head_dim;
+            store8<false>((uint8_t*)(to + f0), u, 1.0f);
+            store8<false>((uint8_t*)(to + f1), v, 1.0f);
+        } else {
+            uint8_t* to = (uint8_t*)a.key_cache + (((((size_t)(slot >> a.shift) * a.kv_heads + kvh) << a.shift) + off) * a.head_dim) * (kF8 ? 1 : 2);
+            store8<kF8>(to + f0 * (kF8 ? 1 : 2), u, a.k_inv);
+            store8<kF8>(to + f1 * (kF8 ? 1 : 2), v, a.k_inv);
+        }
+    }
+}
+
+template <int kCache> static void launch_rotary(const RotaryArgs& a, hipStream_t s) {
+    const bool tiles = kCache >= 0 && a.tokens >= kTileTokens;
+    const int value_blocks = tiles ? a.kv_heads * ((a.tokens + kWriteTokens - 1) / kWriteTokens) : 0;
+    const int all = a.heads + a.kv_heads + (kCache >= 0 && !tiles ? a.kv_heads : 0);
+    const auto launch = [&](auto kernel, int lanes) {
+        const int each = 64 / lanes, need = (all + each - 1) / each;
+        const int parts = (long long)a.tokens * need <= 8192 ? need : 1, sets = (need + parts - 1) / parts;
+        const unsigned grid = (unsigned)(((long long)a.tokens * parts + 3) / 4 + value_blocks);
+        kernel<<<grid, 256, 0, s>>>(a, parts, sets, value_blocks);
+    };
+    if (a.head_dim <= 64) launch(head_norm_rotary_kernel<4, kCache>, 4);
+    else if (a.head_dim <= 128) launch(head_norm_rotary_kernel<8, kCache>, 8);
+    else if constexpr (kCache < 0) launch(head_norm_rotary_kernel<16, kCache>, 16);  // (a cache holds heads of 64 or 128)
+}
+
+void launch_head_norm_rotary(const RotaryArgs& a, hipStream_t s) { launch_rotary<-1>(a, s); }
+
+void launch_head_norm_rotary_write(int kind, const RotaryArgs& a, hipStream_t s) {
+    if (kind == 1) launch_rotary<1>(a, s);
+    else launch_rotary<0>(a, s);
+}
+
+// Radians a position, i of `pairs` (frequencies fall from 1 by a constant factor).
+void rotary_frequencies(int scaling, int pairs, double base, double factor, double low, double high, int original, uint64_t* out) {
+    const double pi2 = 6.283185307179586476925286766559, dim = 2.0 * pairs;
+    if (scaling == 2) base *= pow(factor, dim / (dim - 2.0));
+    const auto border = [&](double turns) { return dim * log(original / (pi2 * turns)) / (2.0 * log(base)); };
+    double first = 0.0, last = 0.0;
+    if (scaling == 4) {
+        first = fmax(floor(border(high)), 0.0);
+        last = fmin(ceil(border(low)), dim - 1.0);
+    }
+    for (int i = 0; i < pairs; ++i) {
+        const double f = pow(base, -2.0 * i / dim);
+        double kept = 1.0;
+        if (scaling == 1) kept = 0.0;
+        else if (scaling == 3) kept = fmin(fmax((original * f / pi2 - low) / (high - low), 0.0), 1.0);
+        else if (scaling == 4) kept = 1.0 - fmin(fmax((i - first) / fmax(last - first, 0.001), 0.0), 1.0);
+        out[i] = (uint64_t)llround(ldexp(f * (kept + (1.0 - kept) / factor) / pi2, 64));  // below 2^62
+    }
+}
+
+}  // namespace pk

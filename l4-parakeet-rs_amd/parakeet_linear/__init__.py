@@ -19,6 +19,7 @@ LIB_PATH = os.environ.get("PK_LINEAR_LIB") or os.path.join(os.path.dirname(HERE)
 P = ctypes.c_void_p
 I = ctypes.c_int32
 F = ctypes.c_float
+D = ctypes.c_double
 S = ctypes.c_size_t
 
 U64 = ctypes.c_uint64
@@ -127,6 +128,16 @@ SIGNATURES = {
     "pk_paged_cache_write": (I, [I, P, I64, P, I64, P, P, P, I, I, I, I, I, F, F, P]),
     "pk_paged_attention_workspace_bytes": (I64, [I, I, I, I, I, I, I, I]),
     "pk_paged_attention": (I, [I, P, I64, P, P, P, P, P, P, I64, I, I, I, I, I, I, I, I, I, I, I, F, F, F, P, U64, P]),
+    "pk_rotary_frequencies": (I, [I, I, D, D, D, D, I, P]),
+    "pk_head_norm_rotary": (I, [P, I64, P, I64, P, P, P, P, P, I64, P, I64, I, I, I, I, I, I, F, F, P]),
+    "pk_head_norm_rotary_write": (I, [I, P, I64, P, I64, P, I64, P, P, P, P, P, P, I64, P, P, I, I, I, I, I, I, F, F, I, I, F, F, P]),
+    "pk_beam_select_workspace_bytes": (I64, [I, I, I, I]),
+    "pk_beam_select": (I, [I, P, I64, P, P, P, P, P, P, I, I, I, I, I, P, U64, P]),
+    "pk_beam_reorder": (I, [P, P, P, I, I, I64, P]),
+    "pk_page_fork_workspace_bytes": (I64, [I, I, I]),
+    "pk_page_fork": (I, [P, P, P, P, P, I, P, P, P, P, P, P, I, I, I, I, P, U64, P]),
+    "pk_page_keep": (I, [P, P, P, P, I, P]),
+    "pk_paged_cache_copy": (I, [P, I, P, P, I64, I, I, P]),
 }
 
 
@@ -616,3 +627,245 @@ def paged_attention(query, key_cache, value_cache, block_table, query_starts, ke
         _row_stride("paged_attention", "output", output), tokens, max_queries, sequences, heads, kv_heads, head_dim, page_size, pages, max_pages, left,
         right, head_dim**-0.5 if scale is None else scale, key_scale, value_scale, None if workspace is None else workspace.data_ptr(),
         0 if workspace is None else workspace.numel(), stream))
+
+
+# ---- between projection and cache, and behind the logits, of a step -------------------
+# (checked as the calls above)
+
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BANDS, ROTARY_RAMP = range(5)
+LOGITS_FP16, LOGITS_FP32 = 0, 1
+
+
+def rotary_frequencies(rotary_dim, base=10000.0, scaling=ROTARY_PLAIN, factor=1.0, low=0.0, high=0.0, original=0, device=None):
+    """Frequencies of rotary positions as head_norm_rotary reads them: int64 [rotary_dim / 2] (turns a position in units of
+    2^-64) on `device` (None: the current GPU); the scalings are those of pk_rotary_frequencies in include/pk_linear.h."""
+    torch = _torch or _types()
+    if (rotary_dim | scaling | original) >> 31:
+        raise ValueError("rotary_frequencies: an integer is negative or 2^31 and more")
+    words = torch.empty(max(rotary_dim // 2, 1), dtype=torch.int64)
+    _done("pk_rotary_frequencies", lib.pk_rotary_frequencies(scaling, rotary_dim, base, factor, low, high, original, words.data_ptr()))
+    return words.to("cuda" if device is None else device)
+
+
+def head_norm_rotary(query, key, query_weight, key_weight, positions, frequencies, query_out, key_out, *, interleaved=False, amplitude=1.0,
+                     epsilon=1e-6, stream=None):
+    """Norm of each query and key head (weights None: none) and its rotation by position, fp16 [tokens x heads x head_dim] with
+    a stride between tokens; see pk_head_norm_rotary in include/pk_linear.h.  frequencies (rotary_frequencies) None: no
+    rotation; key and key_out None: queries alone.  The outputs may be query and key themselves."""
+    torch = _torch or _types()
+    device, stream = _device_and_stream(stream)
+    f16, rows = torch.float16, query.shape
+    tokens, heads, head_dim = rows
+    keys = (tokens, 0, head_dim) if key is None else key.shape
+    kv_heads = keys[1]
+    pairs = 0 if frequencies is None else frequencies.numel()
+    if not (query.dtype is f16 and query_out.dtype is f16 and query_out.shape == rows and len(keys) == 3 and keys[0] == tokens and keys[2] == head_dim
+            and (key is None) == (key_out is None) and not (tokens | heads | kv_heads | head_dim | pairs) >> 30
+            and query.get_device() == query_out.get_device() == device
+            and (key is None or (key.dtype is f16 and key_out.dtype is f16 and key_out.shape == keys
+                                 and key.get_device() == key_out.get_device() == device))
+            and all(t is None or (t.dtype is f16 and t.shape == (head_dim,) and t.is_contiguous() and t.get_device() == device)
+                    for t in (query_weight, key_weight))
+            and (pairs == 0 or (frequencies.dtype in (torch.int64, torch.uint64) and frequencies.dim() == 1 and frequencies.is_contiguous()
+                                and positions is not None and positions.dtype is torch.int32 and positions.shape == (tokens,)
+                                and positions.is_contiguous() and frequencies.get_device() == positions.get_device() == device))):
+        if (key is None) != (key_out is None):
+            raise ValueError("head_norm_rotary: key and key_out must both be given, or neither")
+        if pairs and positions is None:
+            raise ValueError("head_norm_rotary: a rotation needs positions")
+        words = (torch.int64, torch.uint64)
+        _refuse("head_norm_rotary", device, ("query", query, (f16,), None, False), ("query_out", query_out, (f16,), (tokens, heads, head_dim), False),
+                ("key", key, (f16,), (tokens, kv_heads, head_dim), False), ("key_out", key_out, (f16,), (tokens, kv_heads, head_dim), False),
+                ("query_weight", query_weight, (f16,), (head_dim,), True), ("key_weight", key_weight, (f16,), (head_dim,), True),
+                ("positions", positions, (torch.int32,), (tokens,), True), ("frequencies", frequencies, words, (pairs,), True))
+    what = "head_norm_rotary"
+    _done("pk_head_norm_rotary", lib.pk_head_norm_rotary(
+        query.data_ptr(), _row_stride(what, "query", query), None if key is None else key.data_ptr(), 0 if key is None else _row_stride(what, "key", key),
+        None if query_weight is None else query_weight.data_ptr(), None if key_weight is None else key_weight.data_ptr(),
+        positions.data_ptr() if pairs else None, frequencies.data_ptr() if pairs else None, query_out.data_ptr(), _row_stride(what, "query_out", query_out),
+        None if key is None else key_out.data_ptr(), 0 if key is None else _row_stride(what, "key_out", key_out), tokens, heads, kv_heads, head_dim,
+        2 * pairs, interleaved, amplitude, epsilon, stream))
+
+
+def head_norm_rotary_write(query, key, value, query_weight, key_weight, positions, slots, frequencies, query_out, key_cache, value_cache,
+                           key_inverse_scale=1.0, value_inverse_scale=1.0, *, interleaved=False, amplitude=1.0, epsilon=1e-6, stream=None):
+    """head_norm_rotary and paged_cache_write in one launch: the keys go into their slots (-1: nothing of that token is
+    written, its query_out included), and the values beside them."""
+    torch = _torch or _types()
+    device, stream = _device_and_stream(stream)
+    f16, i32, kind, kinds = torch.float16, torch.int32, key_cache.dtype, (torch.float16, torch.uint8, torch.float8_e4m3fn)
+    pages, kv_heads, page_size, head_dim = key_cache.shape
+    rows = query.shape
+    tokens, heads, _ = rows
+    new, transposed = (tokens, kv_heads, head_dim), (pages, kv_heads, head_dim, page_size)
+    pairs = 0 if frequencies is None else frequencies.numel()
+    if not (kind in kinds and value_cache.dtype is kind and query.dtype is f16 and query_out.dtype is f16 and key.dtype is f16 and value.dtype is f16
+            and rows[2] == head_dim and query_out.shape == rows and key.shape == new and value.shape == new and value_cache.shape == transposed
+            and slots.dtype is i32 and slots.shape == (tokens,) and slots.is_contiguous() and key_cache.is_contiguous() and value_cache.is_contiguous()
+            and not (tokens | heads | pages | pairs) >> 31 and query.get_device() == query_out.get_device() == key.get_device() == value.get_device()
+            == slots.get_device() == key_cache.get_device() == value_cache.get_device() == device
+            and all(t is None or (t.dtype is f16 and t.shape == (head_dim,) and t.is_contiguous() and t.get_device() == device)
+                    for t in (query_weight, key_weight))
+            and (pairs == 0 or (frequencies.dtype in (torch.int64, torch.uint64) and frequencies.dim() == 1 and frequencies.is_contiguous()
+                                and positions is not None and positions.dtype is i32 and positions.shape == (tokens,) and positions.is_contiguous()
+                                and frequencies.get_device() == positions.get_device() == device))):
+        if pairs and positions is None:
+            raise ValueError("head_norm_rotary_write: a rotation needs positions")
+        words = (torch.int64, torch.uint64)
+        _refuse("head_norm_rotary_write", device, ("key_cache", key_cache, kinds, None, True), ("value_cache", value_cache, (kind,), transposed, True),
+                ("query", query, (f16,), (tokens, heads, head_dim), False), ("query_out", query_out, (f16,), (tokens, heads, head_dim), False),
+                ("key", key, (f16,), new, False), ("value", value, (f16,), new, False), ("slots", slots, (i32,), (tokens,), True),
+                ("query_weight", query_weight, (f16,), (head_dim,), True), ("key_weight", key_weight, (f16,), (head_dim,), True),
+                ("positions", positions, (i32,), (tokens,), True), ("frequencies", frequencies, words, (pairs,), True))
+    what = "head_norm_rotary_write"
+    _done("pk_head_norm_rotary_write", lib.pk_head_norm_rotary_write(
+        CACHE_FP16 if kind is f16 else CACHE_FP8, query.data_ptr(), _row_stride(what, "query", query), key.data_ptr(), _row_stride(what, "key", key),
+        value.data_ptr(), _row_stride(what, "value", value), None if query_weight is None else query_weight.data_ptr(),
+        None if key_weight is None else key_weight.data_ptr(), positions.data_ptr() if pairs else None, slots.data_ptr(),
+        frequencies.data_ptr() if pairs else None, query_out.data_ptr(), _row_stride(what, "query_out", query_out), key_cache.data_ptr(),
+        value_cache.data_ptr(), tokens, heads, kv_heads, head_dim, 2 * pairs, interleaved, amplitude, epsilon, page_size, pages, key_inverse_scale,
+        value_inverse_scale, stream))
+
+
+def beam_select_workspace_bytes(sequences, beams, vocab, choices):
+    """Bytes of workspace that beam_select needs for these sizes (host only)."""
+    if (sequences | beams | vocab | choices) >> 31:
+        raise ValueError("beam_select_workspace_bytes: a size is negative or 2^31 and more")
+    size = lib.pk_beam_select_workspace_bytes(sequences, beams, vocab, choices)
+    _done("pk_beam_select_workspace_bytes", size)
+    return size
+
+
+def beam_select(logits, scores, ended, out_scores, out_tokens, out_parents, out_ended, workspace, *, end_token=-1, stream=None):
+    """The best candidates of a step of beam search, from logits [sequences x beams x vocab] (fp16 or fp32, rows a stride
+    apart) and scores [sequences x beams]; see pk_beam_select in include/pk_linear.h.  ended and out_ended: bool or uint8,
+    or None.  The number of choices is the outputs' width; workspace: a uint8 tensor of beam_select_workspace_bytes, used by
+    one call at a time."""
+    torch = _torch or _types()
+    device, stream = _device_and_stream(stream)
+    sequences, beams, vocab = logits.shape
+    _, choices = out_scores.shape
+    f16, f32, i32, flags = torch.float16, torch.float32, torch.int32, (torch.bool, torch.uint8)
+    kinds, have, found = (f16, f32), (sequences, beams), (sequences, choices)
+    step, row, one = logits.stride()
+    rows = sequences * beams
+    if rows <= 1:
+        row = vocab
+    elif beams == 1:
+        row = step
+    if not (logits.dtype in kinds and (one == 1 or vocab == 1) and (sequences <= 1 or beams == 1 or step == beams * row)
+            and not (rows | vocab | choices | row | end_token + 1) >> 31 and scores.dtype is f32 and scores.shape == have
+            and scores.is_contiguous() and out_scores.dtype is f32 and out_scores.shape == found and out_scores.is_contiguous()
+            and out_tokens.dtype is i32 and out_tokens.shape == found and out_tokens.is_contiguous() and out_parents.dtype is i32
+            and out_parents.shape == found and out_parents.is_contiguous()
+            and logits.get_device() == scores.get_device() == out_scores.get_device() == out_tokens.get_device() == out_parents.get_device() == device
+            and (ended is None or (ended.dtype in flags and ended.shape == have and ended.is_contiguous() and ended.get_device() == device))
+            and (out_ended is None or (out_ended.dtype in flags and out_ended.shape == found and out_ended.is_contiguous()
+                                       and out_ended.get_device() == device))
+            and (workspace is None or (workspace.dtype is torch.uint8 and workspace.is_contiguous() and workspace.get_device() == device))):
+        if not ((one == 1 or vocab == 1) and (sequences <= 1 or beams == 1 or step == beams * row)):
+            raise ValueError("beam_select: the rows of logits must be contiguous and lie equally far apart")
+        _refuse("beam_select", device, ("logits", logits, kinds, None, False), ("scores", scores, (f32,), have, True),
+                ("ended", ended, flags, have, True), ("out_scores", out_scores, (f32,), found, True), ("out_tokens", out_tokens, (i32,), found, True),
+                ("out_parents", out_parents, (i32,), found, True), ("out_ended", out_ended, flags, found, True),
+                ("workspace", workspace, (torch.uint8,), None, True))
+    _done("pk_beam_select", lib.pk_beam_select(
+        LOGITS_FP16 if logits.dtype is f16 else LOGITS_FP32, logits.data_ptr(), row, scores.data_ptr(), None if ended is None else ended.data_ptr(),
+        out_scores.data_ptr(), out_tokens.data_ptr(), out_parents.data_ptr(), None if out_ended is None else out_ended.data_ptr(), sequences, beams,
+        vocab, choices, end_token, None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(), stream))
+
+
+def beam_reorder(state, parents, output, stream=None):
+    """output[s, b] = state[parents[s, b]] for a state [sequences x beams x ...] of any dtype; parents (int32 [sequences x
+    beams], as beam_select gives them) are rows sequence * beams + beam of the same sequence, others leave their row of
+    output as it was.  output may be state itself."""
+    torch = _torch or _types()
+    device, stream = _device_and_stream(stream)
+    shape = state.shape
+    have = shape[:2]
+    if not (len(shape) >= 2 and output.dtype is state.dtype and output.shape == shape and state.is_contiguous() and output.is_contiguous()
+            and parents.dtype is torch.int32 and parents.shape == have and parents.is_contiguous() and not (have[0] | have[1]) >> 31
+            and state.get_device() == output.get_device() == parents.get_device() == device):
+        if len(shape) < 2:
+            raise ValueError("beam_reorder: state must be [sequences x beams x ...]")
+        _refuse("beam_reorder", device, ("state", state, (state.dtype,), None, True), ("output", output, (state.dtype,), shape, True),
+                ("parents", parents, (torch.int32,), have, True))
+    sequences, beams = have
+    rows = sequences * beams
+    _done("pk_beam_reorder", lib.pk_beam_reorder(state.data_ptr(), parents.data_ptr(), output.data_ptr(), sequences, beams,
+                                                 state.numel() // rows * state.element_size() if rows else 0, stream))
+
+
+def page_fork_workspace_bytes(rows, max_pages, pages):
+    """Bytes of workspace that page_fork needs for these sizes (host only)."""
+    if (rows | max_pages | pages) >> 31:
+        raise ValueError("page_fork_workspace_bytes: a size is negative or 2^31 and more")
+    size = lib.pk_page_fork_workspace_bytes(rows, max_pages, pages)
+    _done("pk_page_fork_workspace_bytes", size)
+    return size
+
+
+def page_fork(parents, block_table, lengths, free_pages, free_range, new_table, new_lengths, copies, freed, info, workspace, page_size, held=None,
+              stream=None):
+    """Block tables from the rows' parents, the pages to be copied for them and the pages that no row lists any more, all
+    int32 on the GPU; see pk_page_fork in include/pk_linear.h.  The sizes are the tensors': rows = len(parents), pages =
+    len(freed); held: bool or uint8 [pages], or None.  workspace: a uint8 tensor of page_fork_workspace_bytes, used by one
+    call at a time.  page_keep moves the free list afterwards."""
+    torch = _torch or _types()
+    device, stream = _device_and_stream(stream)
+    i32, flags = torch.int32, (torch.bool, torch.uint8)
+    rows, max_pages = block_table.shape
+    pages, one = freed.numel(), (rows,)
+    arrays = (parents, block_table, lengths, free_pages, free_range, new_table, new_lengths, copies, freed, info)
+    if not (all(t.dtype is i32 and t.get_device() == device and t.is_contiguous() for t in arrays) and parents.shape == one and lengths.shape == one
+            and free_range.shape == (2,) and free_pages.dim() == freed.dim() == 1 and new_table.shape == (rows, max_pages) and new_lengths.shape == one
+            and copies.shape == (rows, 2) and info.shape == (4,) and not (rows | max_pages | pages | free_pages.numel() | page_size) >> 31
+            and (held is None or (held.dtype in flags and held.shape == (pages,) and held.is_contiguous() and held.get_device() == device))
+            and workspace.dtype is torch.uint8 and workspace.is_contiguous() and workspace.get_device() == device):
+        i32 = (i32,)
+        _refuse("page_fork", device, ("parents", parents, i32, one, True), ("block_table", block_table, i32, None, True),
+                ("lengths", lengths, i32, one, True), ("free_pages", free_pages, i32, (free_pages.numel(),), True),
+                ("free_range", free_range, i32, (2,), True), ("new_table", new_table, i32, (rows, max_pages), True),
+                ("new_lengths", new_lengths, i32, one, True), ("copies", copies, i32, (rows, 2), True), ("freed", freed, i32, (pages,), True),
+                ("info", info, i32, (4,), True), ("held", held, flags, (pages,), True), ("workspace", workspace, (torch.uint8,), None, True))
+    _done("pk_page_fork", lib.pk_page_fork(
+        parents.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), free_pages.data_ptr(), free_range.data_ptr(), free_pages.numel(),
+        None if held is None else held.data_ptr(), new_table.data_ptr(), new_lengths.data_ptr(), copies.data_ptr(), freed.data_ptr(), info.data_ptr(),
+        rows, max_pages, page_size, pages, workspace.data_ptr(), workspace.numel(), stream))
+
+
+def page_keep(info, freed, free_pages, free_range, stream=None):
+    """The free list (int32) behind a page_fork, or behind a page_plan (freed None), whose info says status 0: pages taken
+    leave its front, pages given back stand there."""
+    torch = _torch or _types()
+    device, stream = _device_and_stream(stream)
+    i32 = torch.int32
+    if not (all(t is None or (t.dtype is i32 and t.is_contiguous() and t.get_device() == device) for t in (info, freed, free_pages, free_range))
+            and info.shape == (4,) and free_range.shape == (2,) and free_pages.dim() == 1 and (freed is None or freed.dim() == 1)
+            and not free_pages.numel() >> 31):
+        i32 = (i32,)
+        _refuse("page_keep", device, ("info", info, i32, (4,), True), ("freed", freed, i32, None if freed is None else (freed.numel(),), True),
+                ("free_pages", free_pages, i32, (free_pages.numel(),), True), ("free_range", free_range, i32, (2,), True))
+    _done("pk_page_keep", lib.pk_page_keep(info.data_ptr(), None if freed is None else freed.data_ptr(), free_pages.data_ptr(), free_range.data_ptr(),
+                                           free_pages.numel(), stream))
+
+
+def paged_cache_copy(copies, key_cache, value_cache, stream=None):
+    """Pages source -> destination for the pairs of copies (int32 [count x 2], as page_fork gives them; -1: none) in caches
+    of one layer [pages x ...] as paged_cache_write's, or of several [layers x pages x ...]."""
+    torch = _torch or _types()
+    device, stream = _device_and_stream(stream)
+    shape, kinds = key_cache.shape, (torch.float16, torch.uint8, torch.float8_e4m3fn)
+    swapped = shape[:-2] + shape[:-3:-1]
+    if not (4 <= len(shape) <= 5 and key_cache.dtype in kinds and value_cache.dtype is key_cache.dtype and value_cache.shape == swapped
+            and copies.dtype is torch.int32 and copies.dim() == 2 and copies.shape[1] == 2 and copies.is_contiguous() and key_cache.is_contiguous()
+            and value_cache.is_contiguous() and not (copies.shape[0] | shape[-4] | (shape[0] if len(shape) == 5 else 1)) >> 31
+            and key_cache.get_device() == value_cache.get_device() == copies.get_device() == device):
+        if not 4 <= len(shape) <= 5:
+            raise ValueError("paged_cache_copy: caches are [pages x kv_heads x page_size x head_dim], or that for each layer")
+        _refuse("paged_cache_copy", device, ("key_cache", key_cache, kinds, None, True), ("value_cache", value_cache, (key_cache.dtype,), swapped, True),
+                ("copies", copies, (torch.int32,), (copies.numel() // 2, 2), True))
+    pages = shape[-4]
+    _done("pk_paged_cache_copy", lib.pk_paged_cache_copy(
+        copies.data_ptr(), copies.shape[0], key_cache.data_ptr(), value_cache.data_ptr(),
+        shape[-3] * shape[-2] * shape[-1] * key_cache.element_size(), pages, shape[0] if len(shape) == 5 else 1, stream))
