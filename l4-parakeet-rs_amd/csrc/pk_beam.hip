@@ -3,26 +3,31 @@
 //
 //   score(b, t) = scores[b] + (x[b, t] - log sum_t exp x[b, t])
 //
-// Two launches.  The first reads the logits once, in parts of a row that a workgroup
-// holds in registers: the part's maximum, its sum of exponentials, and its best `choices`
-// logits, in order.  The second puts a sequence's parts together.
+// The logits are read once, in parts of a row that a workgroup holds in registers: the part's
+// maximum, its sum of exponentials, and its best `choices` logits, in order.  A second launch puts
+// a sequence's parts together; short rows of few beams are one launch, whose workgroup does both
+// (8 sequences of 4 beams, 1025 fp32 logits: 8.5 us against 4.8 and 5.0).
 //
 // The best of a part: a bound is the choices-th largest of the lanes' maxima of any one
-// wave (as many logits at least reach it), found by bisection over the bits of the value
+// wave (as many logits at least reach it), found by bisection over the upper bits of the value
 // with one ballot a bit; the few logits that reach it are listed in LDS and ranked by
 // counting.  Keys are unique (value, then index), so the order of the list does not matter.
 //
 // The sum's terms are fp32, their sum and the scores 64 bits: beams are compared by
 // differences of sums, and a rounding of 2^-24 of a score of -30 would change places of
 // candidates that 64 bits tell apart.
+//
+// Bound by the reading (4.4 TB/s) in wide rows; a call of few is a chain: loads, a maximum
+// and a bisection over lanes, exponentials, the list, the join.
 #include "pk_kernels.hpp"
 
 namespace pk {
 
-constexpr int kPartElements = 64;                 // a lane's
-constexpr int kPart = 256 * kPartElements;        // a workgroup's
-constexpr int kListed = 1024;                     // candidates that are ranked; more of them are taken out one by one
+constexpr float kLog2e = 1.44269504f;
+constexpr int kMostLoads = 8;  // of 16 bytes a thread
 
+// Of a part: its largest logit m and sum exp2(x log2e - c), c = fp32(m log2e) (fp16 logits), or
+// sum exp2((x - m) log2e) (fp32 ones, whose m log2e may pass fp32's range).
 struct PartSum {
     double sum;
     float most;
@@ -48,231 +53,354 @@ __device__ __forceinline__ uint32_t wave_bound(uint32_t v, int count, int last) 
     uint32_t bound = 0;
     for (int bit = 31; bit >= last; --bit) {
         const uint32_t tried = bound | (1u << bit);
-        if (__popcll(__ballot(v >= tried)) >= count) bound = tried;
+        if (__popcll(__builtin_amdgcn_ballot_w64(v >= tried)) >= count) bound = tried;
     }
     return bound;
 }
 
+// Sums over a wave.
+__device__ __forceinline__ long long wave_sum(long long v) {
+#pragma unroll
+    for (int off = 1; off <= 32; off <<= 1) {
+        const int lo = (int)v, hi = (int)(v >> 32);
+        const auto join = [](int h, int l) { return ((long long)h << 32) | (uint32_t)l; };
+        if (off <= 8) {
+            v += join(partner(hi, off), partner(lo, off));
+        } else {
+            int la, lb, ha, hb;
+            pair_of(lo, off, la, lb);
+            pair_of(hi, off, ha, hb);
+            v = join(ha, la) + join(hb, lb);
+        }
+    }
+    return v;
+}
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+    for (int off = 1; off <= 32; off <<= 1) {
+        const long long bits = __double_as_longlong(v);
+        const int lo = (int)bits, hi = (int)(bits >> 32);
+        const auto join = [](int h, int l) { return __longlong_as_double(((long long)h << 32) | (uint32_t)l); };
+        if (off <= 8) {
+            v += join(partner(hi, off), partner(lo, off));
+        } else {
+            int la, lb, ha, hb;
+            pair_of(lo, off, la, lb);
+            pair_of(hi, off, ha, hb);
+            v = join(ha, la) + join(hb, lb);
+        }
+    }
     return v;
 }
 
-// Eight fp16 or four fp32 logits at the alignment of one.
-struct __attribute__((packed, aligned(2))) Eight { uint32_t w[4]; };
-struct __attribute__((packed, aligned(4))) Four { uint32_t w[4]; };
+template <bool kF16> __device__ __forceinline__ v4i nothing() {  // -infinity
+    constexpr int kNone = kF16 ? (int)0xfc00fc00u : (int)0xff800000u;
+    return v4i{kNone, kNone, kNone, kNone};
+}
+template <bool kF16> __device__ __forceinline__ float logit_of(const v4i& v, int j) {
+    if constexpr (kF16) return h2f((uint16_t)((uint32_t)v[j >> 1] >> (16 * (j & 1))));
+    else return __int_as_float(v[j]);
+}
 
-template <bool kF16>
-__global__ __launch_bounds__(256) void beam_part_kernel(const void* __restrict__ logits, long long stride, const float* __restrict__ scores,
-                                                        const uint8_t* __restrict__ ended, int vocab, int choices, int parts,
-                                                        PartSum* __restrict__ sums, unsigned long long* __restrict__ best) {
-    constexpr int kVec = kF16 ? 8 : 4, kLoads = kPartElements / kVec;
-    __shared__ unsigned long long list[kListed];
-    __shared__ float part_most[4];
-    __shared__ double part_sum[4];
-    __shared__ uint32_t part_bound[4];
-    __shared__ unsigned long long part_key[4];
-    __shared__ int listed;
-    const int row = blockIdx.x / parts, part = blockIdx.x % parts, wave = threadIdx.x >> 6;
-    if ((ended && ended[row]) || !(__builtin_fabsf(scores[row]) < __builtin_inff())) return;  // no candidates from its logits
-    const char* const x = (const char*)logits + (size_t)row * stride * (kF16 ? 2 : 4);
-    const int start = part * kPart;
-    uint32_t raw[kLoads][4];
+// The larger of each of two fp16 (the other one where one is a NaN), without the compiler's quieting of NaNs beforehand.
+__device__ __forceinline__ int pk_max_f16(int a, int b) {
+    int m;
+    asm("v_pk_max_f16 %0, %1, %2" : "=v"(m) : "v"(a), "v"(b));
+    return m;
+}
+
+template <bool kF16> __device__ __forceinline__ float largest_of(const v4i& v) {
+    if constexpr (kF16) {
+        const v2h m = __builtin_bit_cast(v2h, pk_max_f16(pk_max_f16(v[0], v[1]), pk_max_f16(v[2], v[3])));
+        return __builtin_fmaxf((float)m[0], (float)m[1]);
+    } else {
+        return __builtin_fmaxf(__builtin_fmaxf(__int_as_float(v[0]), __int_as_float(v[1])), __builtin_fmaxf(__int_as_float(v[2]), __int_as_float(v[3])));
+    }
+}
+template <int kLoads> __device__ __forceinline__ v4i pick(const v4i (&raw)[kLoads], int l) {  // raw[l] without an indexed register
+    v4i v = raw[0];
+#pragma unroll
+    for (int i = 1; i < kLoads; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = l == i ? raw[i][j] : v[j];
+    return v;
+}
+__device__ __forceinline__ unsigned long long key_of(float v, int i) { return ((unsigned long long)ordered(v) << 32) | (uint32_t)~(uint32_t)i; }
+
+// What the kGroup threads that take a part share.
+template <int kGroup> struct PartShared {
+    static constexpr int kListed = 4 * kGroup;  // candidates that are ranked; more of them are taken out one by one
+    unsigned long long list[kListed];
+    unsigned long long key[kGroup / 64];
+    long long sum[kGroup / 64];
+    float most[kGroup / 64];
+    uint32_t bound[kGroup / 64];
+    int listed;
+};
+
+// The listed candidates in order, by counting those before each.
+template <int kGroup>
+__device__ __forceinline__ void rank_listed(const PartShared<kGroup>& shared, int count, int choices, int tid, unsigned long long* to) {
+    if (tid >= count && tid < choices) to[tid] = 0;
+    for (int i = tid; i < count; i += kGroup) {
+        const unsigned long long key = shared.list[i];
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += shared.list[j] > key;
+        if (rank < choices) to[rank] = key;
+    }
+}
+
+// Part `part` of a row, by kGroup threads of a workgroup all of whose threads are here: its sum, and
+// `choices` keys, best first, 0 where there are none (`to` null: neither is wanted).  `real` says, behind
+// the loads, whether the row's logits are candidates.
+//
+// Logits are read 16 bytes at once at multiples of 16 (512 rows of 131071 fp16 logits: 30.6 us, 4.4
+// TB/s; 33.4 with loads that straddle lines); those before the first and behind the last go to single threads.
+// So a logit's thread depends on where its row lies, and the sum must not depend on the threads:
+// equal rows have equal sums, and their candidates are ties.  It is therefore exact: a lane adds its
+// terms (at most 1 each, 65 of them) to 384 in fp64, where a step is 2^-44 from 256 to 512, so that
+// each term is rounded alike wherever it is added, and whole steps are added from there.  A term
+// times 1 + 2^-52 is never half way between two steps, whose rounding would go by the sum before it:
+// its lowest bit is 2^-52 of an fp32 term's, and half a step such a term's only from 128 on.
+template <bool kF16, int kLoads, int kGroup, typename Real>
+__device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab, int part, int choices, int tid, PartShared<kGroup>& shared,
+                                             PartSum* sum_out, unsigned long long* to) {
+    constexpr int kVec = kF16 ? 8 : 4, kWaves = kGroup / 64, kListed = PartShared<kGroup>::kListed;
+    constexpr int kPart = kGroup * kLoads * kVec, kBytes = kF16 ? 2 : 4;
+    const int wave = tid >> 6, first = part * kPart, count_here = vocab - first < kPart ? vocab - first : kPart;
+    const char* const here_x = x + (size_t)first * kBytes;
+    const int gap = (int)(-(uintptr_t)here_x & 15) / kBytes, lead = gap < count_here ? gap : count_here;
+    const int vectors = (count_here - lead) / kVec, tail = count_here - lead - vectors * kVec;
+    v4i raw[kLoads];
 #pragma unroll
     for (int l = 0; l < kLoads; ++l) {
-        const int i = start + (l * 256 + (int)threadIdx.x) * kVec;
-        if (i + kVec <= vocab) {
-            if constexpr (kF16) {
-                const Eight e = *(const Eight*)(x + (size_t)i * 2);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) raw[l][j] = e.w[j];
-            } else {
-                const Four e = *(const Four*)(x + (size_t)i * 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) raw[l][j] = e.w[j];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (kF16) {
-                    const uint32_t a = i + 2 * j < vocab ? ((const uint16_t*)x)[i + 2 * j] : 0xfc00u;
-                    const uint32_t b = i + 2 * j + 1 < vocab ? ((const uint16_t*)x)[i + 2 * j + 1] : 0xfc00u;
-                    raw[l][j] = a | (b << 16);
-                } else {
-                    raw[l][j] = i + j < vocab ? ((const uint32_t*)x)[i + j] : 0xff800000u;
-                }
-            }
-        }
+        const int i = l * kGroup + tid;
+        raw[l] = i < vectors ? *(const v4i*)(here_x + lead * kBytes + (size_t)i * 16) : nothing<kF16>();
     }
-    const auto at = [&](int l, int j) {
-        if constexpr (kF16) return h2f((uint16_t)(raw[l][j >> 1] >> (16 * (j & 1))));
-        else return __uint_as_float(raw[l][j]);
-    };
-    float mine = -__builtin_inff();
+    const int extra_at = tid < lead ? first + tid : (tid >= 8 && tid < 8 + tail ? first + count_here - tail + tid - 8 : -1);
+    float extra = -__builtin_inff();
+    if (extra_at >= 0) extra = kF16 ? h2f(((const uint16_t*)x)[extra_at]) : ((const float*)x)[extra_at];
+    const bool candidates = real();
+    const auto place = [&](int l, int j) { return first + lead + (l * kGroup + tid) * kVec + j; };
+    float top[kLoads], mine = extra;  // of 16 bytes, of all
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l)
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) mine = __builtin_fmaxf(mine, at(l, j));
+    for (int l = 0; l < kLoads; ++l) {
+        top[l] = largest_of<kF16>(raw[l]);
+        mine = __builtin_fmaxf(mine, top[l]);
+    }
     const float wave_most = wave_max(mine);
-    const bool any = mine > -__builtin_inff();
-    const uint32_t bound_here = wave_bound(any ? ordered(mine) : 0, choices, kF16 ? 13 : 0);  // fp16 values end 13 bits earlier
-    if ((threadIdx.x & 63) == 0) {
-        part_most[wave] = wave_most;
-        part_bound[wave] = bound_here;
+    // (seven bits of the mantissa tell enough logits apart); 0: fewer than `choices` lanes have a candidate
+    const uint32_t here = wave_bound(candidates && mine > -__builtin_inff() ? ordered(mine) : 0, choices, 16);
+    if ((tid & 63) == 0) {
+        shared.most[wave] = wave_most;
+        shared.bound[wave] = here;
     }
-    if (threadIdx.x == 0) listed = 0;
+    if (tid == 0) shared.listed = 0;
     __syncthreads();
-    const float most = __builtin_fmaxf(__builtin_fmaxf(part_most[0], part_most[1]), __builtin_fmaxf(part_most[2], part_most[3]));
-    uint32_t bound = part_bound[0];
+    uint32_t found = shared.bound[0];
+    float most = shared.most[0];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) bound = part_bound[w] > bound ? part_bound[w] : bound;
-    const float base = most > -__builtin_inff() ? most : 0.0f;
-    double total = 0.0;
+    for (int w = 1; w < kWaves; ++w) {
+        found = shared.bound[w] > found ? shared.bound[w] : found;
+        most = __builtin_fmaxf(most, shared.most[w]);
+    }
+    const float bound = !candidates ? __builtin_nanf("") : (found ? unordered(found) : -3.402823466e38f);
+    const float base = most > -__builtin_inff() ? most : 0.0f, c = base * kLog2e;
+    const auto term = [&](float v) { return __builtin_amdgcn_exp2f(kF16 ? __builtin_fmaf(v, kLog2e, -c) : (v - base) * kLog2e); };
+    const auto note = [&](float v, int i) {
+        if (v >= bound) {
+            const int k = atomicAdd(&shared.listed, 1);
+            if (k < kListed) shared.list[k] = key_of(v, i);
+        }
+    };
+    constexpr double kNudge = 1.0 + 0x1p-52;
+    double total = __builtin_fma((double)term(extra), kNudge, 384.0);
+    uint32_t hits = 0;
 #pragma unroll
     for (int l = 0; l < kLoads; ++l) {
-        float sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) sum += __builtin_amdgcn_exp2f((at(l, j) - base) * 1.44269504088896341f);
-        total += (double)sum;
+        for (int j = 0; j < kVec; ++j) total = __builtin_fma((double)term(logit_of<kF16>(raw[l], j)), kNudge, total);
+        hits |= top[l] >= bound ? 1u << l : 0u;
     }
-    if (any && ordered(mine) >= bound) {
+    note(extra, extra_at);
+    const uint32_t loads = hits;
+    while (hits) {
+        const int l = __ffs(hits) - 1;
+        hits &= hits - 1;
+        const v4i v = pick<kLoads>(raw, l);
 #pragma unroll
-        for (int l = 0; l < kLoads; ++l)
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-                const float v = at(l, j);
-                if (v > -__builtin_inff() && ordered(v) >= bound) {
-                    const int k = atomicAdd(&listed, 1);
-                    if (k < kListed)
-                        list[k] = ((unsigned long long)ordered(v) << 32) | (uint32_t)~(uint32_t)(start + (l * 256 + (int)threadIdx.x) * kVec + j);
-                }
-            }
+        for (int j = 0; j < kVec; ++j) note(logit_of<kF16>(v, j), place(l, j));
     }
-    total = wave_sum(total);
-    if ((threadIdx.x & 63) == 0) part_sum[wave] = total;
+    const bool odd = __builtin_amdgcn_ballot_w64(total != total) != 0;
+    const long long steps = wave_sum(__double_as_longlong(total) - __double_as_longlong(384.0));
+    if ((tid & 63) == 0) shared.sum[wave] = odd ? -1 : steps;  // a NaN among the logits
     __syncthreads();
-    const size_t out = (size_t)row * parts + part;
-    if (threadIdx.x == 0) sums[out] = PartSum{(part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]), most, 0};
-    unsigned long long* to = best + out * choices;
-    const int count = listed;
-    if (count <= kListed) {
-        for (int i = threadIdx.x; i < choices; i += 256)
-            if (i >= count) to[i] = 0;
-        for (int i = threadIdx.x; i < count; i += 256) {
-            const unsigned long long key = list[i];
-            int rank = 0;
-            for (int j = 0; j < count; ++j) rank += list[j] > key;
-            if (rank < choices) to[rank] = key;
+    if (tid == 0 && to) {
+        long long sum = 0;
+        bool some = false;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            some = some || shared.sum[w] < 0;
+            sum += shared.sum[w];
         }
+        *sum_out = PartSum{some ? __builtin_nan("") : (double)sum * 0x1p-44, most, 0};
+    }
+    const int count = shared.listed;
+    if (!__syncthreads_or(count > kListed)) {
+        if (to) rank_listed(shared, count, choices, tid, to);
         return;
     }
     // Many equal logits: the largest key below the last one, `choices` times.
     unsigned long long last = ~0ull;
-    for (int c = 0; c < choices; ++c) {
+    for (int n = 0; n < choices; ++n) {
         unsigned long long key = 0;
+        const auto look = [&](float v, int i) {
+            const unsigned long long k = key_of(v, i);
+            if (v > -__builtin_inff() && k < last && k > key) key = k;
+        };
+        for (uint32_t left = loads; left; left &= left - 1) {
+            const int l = __ffs(left) - 1;
+            const v4i v = pick<kLoads>(raw, l);
 #pragma unroll
-        for (int l = 0; l < kLoads; ++l)
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-                const float v = at(l, j);
-                const unsigned long long k =
-                    ((unsigned long long)ordered(v) << 32) | (uint32_t)~(uint32_t)(start + (l * 256 + (int)threadIdx.x) * kVec + j);
-                if (v > -__builtin_inff() && k < last && k > key) key = k;
-            }
+            for (int j = 0; j < kVec; ++j) look(logit_of<kF16>(v, j), place(l, j));
+        }
+        look(extra, extra_at);
 #pragma unroll
         for (int off = 1; off <= 32; off <<= 1) key = max_level(key, off);
-        if ((threadIdx.x & 63) == 0) part_key[wave] = key;
+        if ((tid & 63) == 0) shared.key[wave] = key;
         __syncthreads();
-        key = part_key[0];
+        key = shared.key[0];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) key = part_key[w] > key ? part_key[w] : key;
-        if (threadIdx.x == 0) to[c] = key;
+        for (int w = 1; w < kWaves; ++w) key = shared.key[w] > key ? shared.key[w] : key;
+        if (tid == 0 && to) to[n] = key;
         last = key;
         __syncthreads();
     }
 }
 
+// A beam's candidates: 0 none, 1 of its logits, 2 ended.
+__device__ __forceinline__ int beam_state(float score, const uint8_t* ended, size_t row) {
+    return !(__builtin_fabsf(score) < __builtin_inff()) ? 0 : (ended && ended[row] ? 2 : 1);
+}
+
+template <bool kF16, int kLoads>
+__global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a, int parts, PartSum* __restrict__ sums, unsigned long long* __restrict__ best) {
+    __shared__ PartShared<256> shared;
+    const int row = blockIdx.x / parts, part = blockIdx.x % parts;
+    if (beam_state(a.scores[row], a.ended, row) != 1) return;
+    const size_t out = (size_t)row * parts + part;
+    best_of_part<kF16, kLoads, 256>((const char*)a.logits + (size_t)row * a.stride * (kF16 ? 2 : 4), [] { return true; }, a.vocab, part, a.choices, threadIdx.x, shared,
+                               sums + out, best + out * a.choices);
+}
+
 struct Candidate {
-    unsigned long long score;  // ordered
+    unsigned long long score;  // ordered; 0 (a NaN's): none
     uint32_t place;            // beam * vocab + token
     __device__ __forceinline__ bool before(const Candidate& o) const { return score > o.score || (score == o.score && place < o.place); }
 };
 
-// A workgroup a sequence.  A thread has the lists (beam, part) it, it + 256, ...; each is in
-// order, so that a list's first candidate is its best.
-constexpr int kMostBeams = 32;
+constexpr int kMostBeams = 32, kJoinListed = 1024;
 
-__global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs a, int parts, const PartSum* __restrict__ sums,
-                                                        const unsigned long long* __restrict__ best) {
-    __shared__ double whole[kMostBeams];  // log of a beam's sum
-    __shared__ int state[kMostBeams];     // 0 no candidates, 1 its logits, 2 ended
-    __shared__ unsigned long long list_score[kListed];
-    __shared__ uint32_t list_place[kListed];
-    __shared__ uint32_t wave_part[4];
-    __shared__ unsigned long long wave_score[4];
-    __shared__ uint32_t wave_place[4];
-    __shared__ int listed;
-    const int seq = blockIdx.x, wave = threadIdx.x >> 6, lists = a.beams * parts;
+template <int kThreads> struct JoinShared {
+    unsigned long long list_score[kJoinListed];
+    double whole[kMostBeams], have[kMostBeams];  // log of a beam's sum, its score
+    unsigned long long wave_score[kThreads / 64];
+    uint32_t list_place[kJoinListed];
+    uint32_t wave_place[kThreads / 64], wave_bound[kThreads / 64];
+    int state[kMostBeams];
+    int listed;
+};
+
+// A sequence's answer, by a workgroup: the logarithms of the beams' sums, a wave a beam, then the
+// best of all parts' candidates by the same bound, over the upper bits of their scores.  sums and keys are
+// the sequence's, and need not be set for beams without candidates.
+template <int kThreads, bool kF16>
+__device__ __forceinline__ void join_parts(const BeamArgs& a, int seq, int parts, const PartSum* sums, const unsigned long long* keys,
+                                           JoinShared<kThreads>& shared) {
+    constexpr int kWaves = kThreads / 64, kKept = 2;  // candidates a thread keeps between its two looks at them
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const size_t row0 = (size_t)seq * a.beams;
-    if (threadIdx.x == 0) listed = 0;
-    if ((int)threadIdx.x < a.beams) {
-        const size_t row = row0 + threadIdx.x;
-        const float score = a.scores[row];
-        int s = 0;
-        double log_sum = 0.0;
-        if (__builtin_fabsf(score) < __builtin_inff()) {
-            if (a.ended && a.ended[row]) {
-                s = 2;
-            } else {
-                float most = -__builtin_inff();
-                for (int p = 0; p < parts; ++p) most = __builtin_fmaxf(most, sums[row * parts + p].most);
-                if (most > -__builtin_inff() && most < __builtin_inff()) {
-                    double sum = 0.0;
-                    for (int p = 0; p < parts; ++p) {
-                        const PartSum& one = sums[row * parts + p];
-                        if (one.most > -__builtin_inff()) sum += one.sum * exp((double)one.most - (double)most);
-                        else if (one.sum != one.sum) sum = one.sum;
-                    }
-                    log_sum = (double)most + log(sum);
-                    s = log_sum == log_sum ? 1 : 0;  // a NaN among the logits: no candidates
-                }
-            }
-        }
-        whole[threadIdx.x] = log_sum;
-        state[threadIdx.x] = s;
-    }
-    __syncthreads();
-    // candidate c of list i; score 0 stands for none (that of a NaN's bits)
-    const auto candidate = [&](int i, int c) {
-        const int b = i / parts, s = state[b];
-        if (s == 2) return i % parts == 0 && c == 0 ? Candidate{ordered((double)a.scores[row0 + b]), (uint32_t)b * a.vocab + a.end_token} : Candidate{0, 0};
-        const unsigned long long key = s ? best[(row0 * parts + i) * a.choices + c] : 0;
-        if (!key) return Candidate{0, 0};
-        const double x = (double)unordered((uint32_t)(key >> 32));
-        return Candidate{ordered((x - whole[b]) + (double)a.scores[row0 + b]), (uint32_t)b * a.vocab + ~(uint32_t)key};
-    };
-    uint32_t mine = 0;
-    for (int i = threadIdx.x; i < lists; i += 256) {
-        const uint32_t top = (uint32_t)(candidate(i, 0).score >> 32);
-        mine = top > mine ? top : mine;
-    }
-    const uint32_t here = wave_bound(mine, a.choices, 0);
-    if ((threadIdx.x & 63) == 0) wave_part[wave] = here;
-    __syncthreads();
-    uint32_t bound = wave_part[0];
+    // the first `depth` of each part: all threads have some to set the bound by; behind them a part goes on while it reaches it
+    const int lists = a.beams * parts, enough = (kThreads + lists - 1) / lists, depth = enough < a.choices ? enough : a.choices, front = lists * depth;
+    unsigned long long raw[kKept];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) bound = wave_part[w] > bound ? wave_part[w] : bound;
-    for (int i = threadIdx.x; i < lists; i += 256)
-        for (int c = 0; c < a.choices; ++c) {
-            const Candidate one = candidate(i, c);
-            if (!one.score || (uint32_t)(one.score >> 32) < bound) break;
-            const int k = atomicAdd(&listed, 1);
-            if (k < kListed) {
-                list_score[k] = one.score;
-                list_place[k] = one.place;
+    for (int n = 0; n < kKept; ++n) {
+        const int i = tid + n * kThreads;
+        raw[n] = i < front ? keys[(size_t)(i / depth) * a.choices + i % depth] : 0;
+    }
+    if (tid == 0) shared.listed = 0;
+    for (int b = wave; b < a.beams; b += kWaves) {
+        const PartSum none{0.0, -__builtin_inff(), 0};
+        const PartSum* const own = sums + (size_t)b * parts;
+        const PartSum mine_of = lane < parts ? own[lane] : none;
+        const float score = a.scores[row0 + b];
+        int s = beam_state(score, a.ended, row0 + b);
+        double log_sum = 0.0;
+        if (s == 1) {
+            float most = mine_of.most;
+            for (int p = lane + 64; p < parts; p += 64) most = __builtin_fmaxf(most, own[p].most);
+            most = wave_max(most);
+            double mine = 0.0;
+            for (int p = lane; p < parts; p += 64) {
+                const PartSum one = p == lane ? mine_of : own[p];
+                const bool some = one.most > -__builtin_inff() && one.most < __builtin_inff();
+                // what c lacks of m log2e, in powers of 2
+                const double lost = kF16 && some ? (double)(one.most * kLog2e) - (double)one.most * (double)kLog2e : 0.0;
+                mine += some ? one.sum * exp(((double)one.most - (double)most) + lost * 0.69314718055994530942) : one.sum;
             }
+            log_sum = (double)most + log(wave_sum(mine));
+            s = most > -__builtin_inff() && most < __builtin_inff() && log_sum == log_sum;  // a NaN or an infinity: no candidates
         }
+        if (lane == 0) {
+            shared.whole[b] = log_sum;
+            shared.have[b] = (double)score;
+            shared.state[b] = s;
+        }
+    }
+    __syncthreads();
+    const auto candidate_of = [&](int list, int c, unsigned long long key) {
+        const int b = list / parts, s = shared.state[b];
+        if (s == 2) return list == b * parts && c == 0 ? Candidate{ordered(shared.have[b]), (uint32_t)b * a.vocab + a.end_token} : Candidate{0, 0};
+        if (!s || !key) return Candidate{0, 0};
+        const double x = (double)unordered((uint32_t)(key >> 32));
+        return Candidate{ordered((x - shared.whole[b]) + shared.have[b]), (uint32_t)b * a.vocab + ~(uint32_t)key};
+    };
+    const auto candidate = [&](int list, int c) { return candidate_of(list, c, keys[(size_t)list * a.choices + c]); };
+    Candidate kept[kKept];
+    uint32_t mine = 0;
+    const auto larger = [&](const Candidate& one) {
+        const uint32_t top = (uint32_t)(one.score >> 32);
+        mine = top > mine ? top : mine;
+    };
+#pragma unroll
+    for (int n = 0; n < kKept; ++n) {
+        const int i = tid + n * kThreads;
+        kept[n] = i < front ? candidate_of(i / depth, i % depth, raw[n]) : Candidate{0, 0};
+        larger(kept[n]);
+    }
+    for (int i = tid + kKept * kThreads; i < front; i += kThreads) larger(candidate(i / depth, i % depth));
+    const uint32_t here = wave_bound(mine, a.choices, 12);  // eight bits of the mantissa
+    if (lane == 0) shared.wave_bound[wave] = here;
+    __syncthreads();
+    uint32_t bound = shared.wave_bound[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) bound = shared.wave_bound[w] > bound ? shared.wave_bound[w] : bound;
+    const auto reaches = [&](const Candidate& one) {
+        if (!one.score || (uint32_t)(one.score >> 32) < bound) return false;
+        const int k = atomicAdd(&shared.listed, 1);
+        if (k < kJoinListed) {
+            shared.list_score[k] = one.score;
+            shared.list_place[k] = one.place;
+        }
+        return true;
+    };
+    const auto note = [&](int i, const Candidate& one) {
+        if (reaches(one) && i % depth == depth - 1)
+            for (int c = depth; c < a.choices && reaches(candidate(i / depth, c)); ++c) {}
+    };
+#pragma unroll
+    for (int n = 0; n < kKept; ++n) note(tid + n * kThreads, kept[n]);
+    for (int i = tid + kKept * kThreads; i < front; i += kThreads) note(i, candidate(i / depth, i % depth));
     __syncthreads();
     const auto answer = [&](int c, const Candidate& one) {
         const size_t to = (size_t)seq * a.choices + c;
@@ -280,16 +408,15 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs a, int parts, c
         a.out_scores[to] = one.score ? (float)unordered(one.score) : -__builtin_inff();
         a.out_tokens[to] = token;
         a.out_parents[to] = one.score ? (int)(row0 + b) : -1;
-        if (a.out_ended) a.out_ended[to] = one.score && (state[b] == 2 || token == a.end_token);
+        if (a.out_ended) a.out_ended[to] = one.score && (shared.state[b] == 2 || token == a.end_token);
     };
-    const int count = listed;
-    if (count <= kListed) {
-        for (int c = threadIdx.x; c < a.choices; c += 256)
-            if (c >= count) answer(c, Candidate{0, 0});
-        for (int i = threadIdx.x; i < count; i += 256) {
-            const Candidate one{list_score[i], list_place[i]};
+    const int count = shared.listed;
+    if (count <= kJoinListed) {
+        if (tid >= count && tid < a.choices) answer(tid, Candidate{0, 0});
+        for (int i = tid; i < count; i += kThreads) {
+            const Candidate one{shared.list_score[i], shared.list_place[i]};
             int rank = 0;
-            for (int j = 0; j < count; ++j) rank += Candidate{list_score[j], list_place[j]}.before(one);
+            for (int j = 0; j < count; ++j) rank += Candidate{shared.list_score[j], shared.list_place[j]}.before(one);
             if (rank < a.choices) answer(rank, one);
         }
         return;
@@ -298,51 +425,102 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs a, int parts, c
     Candidate last{~0ull, 0};
     for (int c = 0; c < a.choices; ++c) {
         Candidate top{0, 0};
-        for (int i = threadIdx.x; i < lists; i += 256)
-            for (int k = 0; k < a.choices; ++k) {
-                const Candidate one = candidate(i, k);
-                if (!one.score) break;
-                if (last.before(one)) {  // the list's first that is left
-                    if (!top.score || one.before(top)) top = one;
-                    break;
-                }
-            }
+        for (int i = tid; i < lists * a.choices; i += kThreads) {
+            const Candidate one = candidate(i / a.choices, i % a.choices);
+            if (one.score && last.before(one) && (!top.score || one.before(top))) top = one;
+        }
 #pragma unroll
         for (int off = 1; off <= 32; off <<= 1) {
             const Candidate other{(unsigned long long)__shfl_xor((long long)top.score, off, 64), (uint32_t)__shfl_xor((int)top.place, off, 64)};
             if (other.score && (!top.score || other.before(top))) top = other;
         }
-        if ((threadIdx.x & 63) == 0) {
-            wave_score[wave] = top.score;
-            wave_place[wave] = top.place;
+        if (lane == 0) {
+            shared.wave_score[wave] = top.score;
+            shared.wave_place[wave] = top.place;
         }
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const Candidate other{wave_score[w], wave_place[w]};
+        for (int w = 0; w < kWaves; ++w) {
+            const Candidate other{shared.wave_score[w], shared.wave_place[w]};
             if (other.score && (!top.score || other.before(top))) top = other;
         }
-        if (threadIdx.x == 0) answer(c, top);
-        last = top;
+        if (tid == 0) answer(c, top);
+        last = top.score ? top : Candidate{0, 0xffffffffu};
         __syncthreads();
-        if (!top.score) last = Candidate{0, 0xffffffffu};
     }
 }
 
-static int beam_parts(int vocab) { return (vocab + kPart - 1) / kPart; }
+constexpr int kJoinThreads = 512;
 
-size_t beam_workspace(int sequences, int beams, int vocab, int choices) {
-    return (size_t)sequences * beams * beam_parts(vocab) * (sizeof(PartSum) + 8 * (size_t)choices);
+template <bool kF16>
+__global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int parts, const PartSum* __restrict__ sums,
+                                                                 const unsigned long long* __restrict__ best) {
+    __shared__ JoinShared<kJoinThreads> shared;
+    const size_t first = (size_t)blockIdx.x * a.beams;
+    join_parts<kJoinThreads, kF16>(a, blockIdx.x, parts, sums + first * parts, best + first * parts * a.choices, shared);
 }
 
-void launch_beam_select(bool fp16, const BeamArgs& a, hipStream_t s) {
-    const int parts = beam_parts(a.vocab), rows = a.sequences * a.beams;
+// Both in one launch where the rows are short and a sequence has few beams: kGroup threads a beam.
+constexpr int kWholeThreads = 1024, kWholeBeams = 16, kWholeVectors = 512;  // 16-byte loads a row
+
+template <bool kF16, int kGroup> __global__ __launch_bounds__(kWholeThreads) void beam_whole_kernel(BeamArgs a) {
+    constexpr int kGroups = kWholeThreads / kGroup;
+    __shared__ PartShared<kGroup> part[kGroups];
+    __shared__ JoinShared<kWholeThreads> shared;
+    __shared__ PartSum sums[kGroups];
+    __shared__ unsigned long long keys[kGroups * 64];
+    const int seq = blockIdx.x, b = threadIdx.x / kGroup;
+    const size_t row = (size_t)seq * a.beams + (b < a.beams ? b : 0);
+    const float score = a.scores[row];
+    const uint8_t over = a.ended ? a.ended[row] : 0;
+    const auto real = [&] { return b < a.beams && !over && __builtin_fabsf(score) < __builtin_inff(); };
+    best_of_part<kF16, kWholeVectors / kGroup, kGroup>((const char*)a.logits + row * a.stride * (kF16 ? 2 : 4), real, a.vocab, 0, a.choices,
+                                                       threadIdx.x % kGroup, part[b], sums + b, b < a.beams ? keys + b * a.choices : nullptr);
+    __syncthreads();
+    join_parts<kWholeThreads, kF16>(a, seq, 1, sums, keys, shared);
+}
+
+// Loads a thread, and with them the parts: many workgroups where rows are few or short, else many
+// loads, which hide what a part begins and ends with (512 rows of 131072 fp16 logits 28.6 us with 8 loads,
+// 32.9 with 4; 32 rows of 131071 8.5 with 2 loads, 64 rows 9.1 with 8).
+constexpr long long kManyVectors = 1 << 20;  // of 16 bytes, of a call
+
+template <bool kF16> static int beam_loads(int rows, int vocab) {
+    const long long vectors = (vocab + (kF16 ? 7 : 3)) / (kF16 ? 8 : 4);
+    return vectors <= 256 ? 1 : (vectors <= 512 || rows * vectors < kManyVectors ? 2 : kMostLoads);
+}
+template <bool kF16> static int beam_parts(int loads, int vocab) {
+    const int part = 256 * loads * (kF16 ? 8 : 4);
+    return (vocab + part - 1) / part;
+}
+
+// Enough for both kinds, and for fewer of everything: parts of the most loads, and those of two in a small call.
+size_t beam_workspace(int sequences, int beams, int vocab, int choices) {
+    const long long rows = (long long)sequences * beams, vectors = (vocab + 3) / 4, all = rows * vectors;
+    const long long small = (all < kManyVectors ? all : kManyVectors) / 512, large = rows * (vectors / (256 * kMostLoads));
+    return (size_t)(2 * rows + (small > large ? small : large)) * (sizeof(PartSum) + 8 * (size_t)choices);
+}
+
+template <bool kF16> static void select(const BeamArgs& a, hipStream_t s) {
+    const int rows = a.sequences * a.beams, loads = beam_loads<kF16>(rows, a.vocab), parts = beam_parts<kF16>(loads, a.vocab);
+    if (parts == 1 && loads <= 2 && a.beams <= kWholeBeams) {
+        if (a.beams <= 4) beam_whole_kernel<kF16, 256><<<(unsigned)a.sequences, kWholeThreads, 0, s>>>(a);
+        else if (a.beams <= 8) beam_whole_kernel<kF16, 128><<<(unsigned)a.sequences, kWholeThreads, 0, s>>>(a);
+        else beam_whole_kernel<kF16, 64><<<(unsigned)a.sequences, kWholeThreads, 0, s>>>(a);
+        return;
+    }
     PartSum* sums = (PartSum*)a.workspace;
     unsigned long long* best = (unsigned long long*)(sums + (size_t)rows * parts);
     const unsigned grid = (unsigned)rows * parts;
-    if (fp16) beam_part_kernel<true><<<grid, 256, 0, s>>>(a.logits, a.stride, a.scores, a.ended, a.vocab, a.choices, parts, sums, best);
-    else beam_part_kernel<false><<<grid, 256, 0, s>>>(a.logits, a.stride, a.scores, a.ended, a.vocab, a.choices, parts, sums, best);
-    beam_join_kernel<<<(unsigned)a.sequences, 256, 0, s>>>(a, parts, sums, best);
+    if (loads == 1) beam_part_kernel<kF16, 1><<<grid, 256, 0, s>>>(a, parts, sums, best);  // more beams than the one launch takes
+    else if (loads == 2) beam_part_kernel<kF16, 2><<<grid, 256, 0, s>>>(a, parts, sums, best);
+    else beam_part_kernel<kF16, kMostLoads><<<grid, 256, 0, s>>>(a, parts, sums, best);
+    beam_join_kernel<kF16><<<(unsigned)a.sequences, kJoinThreads, 0, s>>>(a, parts, sums, best);
+}
+
+void launch_beam_select(bool fp16, const BeamArgs& a, hipStream_t s) {
+    if (fp16) select<true>(a, s);
+    else select<false>(a, s);
 }
 
 // Rows in their beams' new order.  A thread owns a column of a sequence's rows, reads what

@@ -102,6 +102,28 @@ def test_ties_go_to_the_lowest(pk, vocab, fp16, choices):  # noqa: F811
     s.go()
 
 
+@pytest.mark.parametrize("vocab", [33000, 131071])
+@pytest.mark.parametrize("fp16", [False, True])
+def test_equal_rows_at_all_alignments(pk, vocab, fp16):  # noqa: F811
+    """Many wide rows (they are read in aligned blocks), each at another offset: equal ones tie, and a row's first and last
+    logits and those at the borders of waves and parts are found at their places."""
+    n, beams, per = 20, 16, 16 if fp16 else 8
+    g = gen(vocab)
+    row = torch.randn(vocab, generator=g, device="cuda")
+    part = 2048 * (8 if fp16 else 4)
+    spots = [0, 1, 7, 8, vocab - 1, vocab - 2, vocab - 9, 511, 512, 4095, 4096, part - 1, part, part + 1, 2 * part - 1]
+    wide = torch.full((n, beams, vocab + 2 * per + 3), 30.0, device="cuda")
+    for i in range(n):
+        row2 = row.clone()
+        row2[spots[i % len(spots)]] = 9.0
+        wide[i, :, per:per + vocab] = row2
+    wide = wide.half() if fp16 else wide
+    s = Search(pk, n, beams, vocab, 20, fp16)  # strides are odd: every row lies at another alignment
+    s.logits = wide[..., per:per + vocab]
+    s.scores[:] = -1.0
+    s.go()
+
+
 def test_rows_a_stride_apart(pk):  # noqa: F811
     for fp16 in (False, True):
         s = Search(pk, 3, 4, 1031, 4, fp16)
