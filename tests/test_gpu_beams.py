@@ -212,6 +212,22 @@ def test_reorder_of_unaligned_states(pk, shift):  # noqa: F811
     assert torch.equal(whole[:shift], before[:shift]) and torch.equal(whole[shift + 3 * 4 * 96:], before[shift + 3 * 4 * 96:])
 
 
+def test_reorder_of_many_chunks_a_row(pk):  # noqa: F811
+    """More columns than one launch has workgroups for, in bytes and out of place."""
+    row = (1 << 26) + 12345
+    g = gen(9)
+    state = torch.randint(0, 256, (1, 3, row), generator=g, device="cuda", dtype=torch.uint8)
+    out = torch.zeros_like(state)
+    parents = torch.tensor([[2, 0, 2]], dtype=torch.int32, device="cuda")
+    pk.beam_reorder(state, parents, out)
+    for b, p in enumerate((2, 0, 2)):
+        assert torch.equal(out[0, b], state[0, p])
+    before = state[0, :, :].clone()
+    pk.beam_reorder(state, parents, state)
+    for b, p in enumerate((2, 0, 2)):
+        assert torch.equal(state[0, b], before[p])
+
+
 def test_reorder_of_rows_of_more_than_32_bits(pk):  # noqa: F811
     row = (1 << 32) - 16
     state = torch.empty((1, 2, row // 8), dtype=torch.int64, device="cuda")
