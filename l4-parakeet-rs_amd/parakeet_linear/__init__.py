@@ -427,14 +427,16 @@ def launch_decode(encoder_projection, frames, lstm, projection, joint, tokens, r
 NORM_FP8, NORM_INT8 = 0, 1
 CACHE_FP16, CACHE_FP8 = 0, 1
 
-_torch = None
+_torch = _CACHED = _WORDS = None
 
 
 def _types():
     global _torch
+    global _CACHED, _WORDS
     import torch
 
     _torch = torch
+    _CACHED, _WORDS = (torch.float16, torch.uint8, torch.float8_e4m3fn), (torch.int64, torch.uint64)
     return torch
 
 
@@ -636,6 +638,14 @@ ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BANDS, ROTARY_RAMP = range(5)
 LOGITS_FP16, LOGITS_FP32 = 0, 1
 
 
+def _token_stride(what, name, t, tokens, heads, head_dim):
+    """_row_stride of a tensor whose shape is known."""
+    step, head, one = t.stride()
+    if one == 1 and (head == head_dim or heads == 1):
+        return step if tokens > 1 else heads * head_dim
+    return _row_stride(what, name, t)
+
+
 def rotary_frequencies(rotary_dim, base=10000.0, scaling=ROTARY_PLAIN, factor=1.0, low=0.0, high=0.0, original=0, device=None):
     """Frequencies of rotary positions as head_norm_rotary reads them: int64 [rotary_dim / 2] (turns a position in units of
     2^-64) on `device` (None: the current GPU); the scalings are those of pk_rotary_frequencies in include/pk_linear.h."""
@@ -656,35 +666,37 @@ def head_norm_rotary(query, key, query_weight, key_weight, positions, frequencie
     device, stream = _device_and_stream(stream)
     f16, rows = torch.float16, query.shape
     tokens, heads, head_dim = rows
+    one, what = (head_dim,), "head_norm_rotary"
     keys = (tokens, 0, head_dim) if key is None else key.shape
-    kv_heads = keys[1]
+    _, kv_heads, _ = keys
     pairs = 0 if frequencies is None else frequencies.numel()
-    if not (query.dtype is f16 and query_out.dtype is f16 and query_out.shape == rows and len(keys) == 3 and keys[0] == tokens and keys[2] == head_dim
-            and (key is None) == (key_out is None) and not (tokens | heads | kv_heads | head_dim | pairs) >> 30
+    if not (query.dtype is f16 and query_out.dtype is f16 and query_out.shape == rows and not (tokens | heads | kv_heads | head_dim | pairs) >> 30
             and query.get_device() == query_out.get_device() == device
-            and (key is None or (key.dtype is f16 and key_out.dtype is f16 and key_out.shape == keys
-                                 and key.get_device() == key_out.get_device() == device))
-            and all(t is None or (t.dtype is f16 and t.shape == (head_dim,) and t.is_contiguous() and t.get_device() == device)
-                    for t in (query_weight, key_weight))
-            and (pairs == 0 or (frequencies.dtype in (torch.int64, torch.uint64) and frequencies.dim() == 1 and frequencies.is_contiguous()
+            and (key_out is None if key is None else
+                 key_out is not None and key.dtype is f16 and key_out.dtype is f16 and keys == (tokens, kv_heads, head_dim) and key_out.shape == keys
+                 and key.get_device() == key_out.get_device() == device)
+            and (query_weight is None or (query_weight.dtype is f16 and query_weight.shape == one and query_weight.get_device() == device
+                                          and query_weight.is_contiguous()))
+            and (key_weight is None or (key_weight.dtype is f16 and key_weight.shape == one and key_weight.get_device() == device
+                                        and key_weight.is_contiguous()))
+            and (pairs == 0 or (frequencies.dtype in _WORDS and frequencies.get_device() == device and frequencies.is_contiguous()
                                 and positions is not None and positions.dtype is torch.int32 and positions.shape == (tokens,)
-                                and positions.is_contiguous() and frequencies.get_device() == positions.get_device() == device))):
+                                and positions.get_device() == device and positions.is_contiguous()))):
         if (key is None) != (key_out is None):
             raise ValueError("head_norm_rotary: key and key_out must both be given, or neither")
         if pairs and positions is None:
             raise ValueError("head_norm_rotary: a rotation needs positions")
-        words = (torch.int64, torch.uint64)
-        _refuse("head_norm_rotary", device, ("query", query, (f16,), None, False), ("query_out", query_out, (f16,), (tokens, heads, head_dim), False),
+        _refuse(what, device, ("query", query, (f16,), None, False), ("query_out", query_out, (f16,), (tokens, heads, head_dim), False),
                 ("key", key, (f16,), (tokens, kv_heads, head_dim), False), ("key_out", key_out, (f16,), (tokens, kv_heads, head_dim), False),
-                ("query_weight", query_weight, (f16,), (head_dim,), True), ("key_weight", key_weight, (f16,), (head_dim,), True),
-                ("positions", positions, (torch.int32,), (tokens,), True), ("frequencies", frequencies, words, (pairs,), True))
-    what = "head_norm_rotary"
+                ("query_weight", query_weight, (f16,), one, True), ("key_weight", key_weight, (f16,), one, True),
+                ("positions", positions, (torch.int32,), (tokens,), True), ("frequencies", frequencies, _WORDS, None, True))
     _done("pk_head_norm_rotary", lib.pk_head_norm_rotary(
-        query.data_ptr(), _row_stride(what, "query", query), None if key is None else key.data_ptr(), 0 if key is None else _row_stride(what, "key", key),
-        None if query_weight is None else query_weight.data_ptr(), None if key_weight is None else key_weight.data_ptr(),
-        positions.data_ptr() if pairs else None, frequencies.data_ptr() if pairs else None, query_out.data_ptr(), _row_stride(what, "query_out", query_out),
-        None if key is None else key_out.data_ptr(), 0 if key is None else _row_stride(what, "key_out", key_out), tokens, heads, kv_heads, head_dim,
-        2 * pairs, interleaved, amplitude, epsilon, stream))
+        query.data_ptr(), _token_stride(what, "query", query, tokens, heads, head_dim), None if key is None else key.data_ptr(),
+        0 if key is None else _token_stride(what, "key", key, tokens, kv_heads, head_dim), None if query_weight is None else query_weight.data_ptr(),
+        None if key_weight is None else key_weight.data_ptr(), positions.data_ptr() if pairs else None, frequencies.data_ptr() if pairs else None,
+        query_out.data_ptr(), _token_stride(what, "query_out", query_out, tokens, heads, head_dim), None if key is None else key_out.data_ptr(),
+        0 if key is None else _token_stride(what, "key_out", key_out, tokens, kv_heads, head_dim), tokens, heads, kv_heads, head_dim, 2 * pairs,
+        interleaved, amplitude, epsilon, stream))
 
 
 def head_norm_rotary_write(query, key, value, query_weight, key_weight, positions, slots, frequencies, query_out, key_cache, value_cache,
@@ -693,38 +705,39 @@ def head_norm_rotary_write(query, key, value, query_weight, key_weight, position
     written, its query_out included), and the values beside them."""
     torch = _torch or _types()
     device, stream = _device_and_stream(stream)
-    f16, i32, kind, kinds = torch.float16, torch.int32, key_cache.dtype, (torch.float16, torch.uint8, torch.float8_e4m3fn)
+    f16, i32, kind, what = torch.float16, torch.int32, key_cache.dtype, "head_norm_rotary_write"
     pages, kv_heads, page_size, head_dim = key_cache.shape
     rows = query.shape
-    tokens, heads, _ = rows
-    new, transposed = (tokens, kv_heads, head_dim), (pages, kv_heads, head_dim, page_size)
+    tokens, heads, width = rows
+    new, one, each = (tokens, kv_heads, head_dim), (head_dim,), (tokens,)
     pairs = 0 if frequencies is None else frequencies.numel()
-    if not (kind in kinds and value_cache.dtype is kind and query.dtype is f16 and query_out.dtype is f16 and key.dtype is f16 and value.dtype is f16
-            and rows[2] == head_dim and query_out.shape == rows and key.shape == new and value.shape == new and value_cache.shape == transposed
-            and slots.dtype is i32 and slots.shape == (tokens,) and slots.is_contiguous() and key_cache.is_contiguous() and value_cache.is_contiguous()
-            and not (tokens | heads | pages | pairs) >> 31 and query.get_device() == query_out.get_device() == key.get_device() == value.get_device()
-            == slots.get_device() == key_cache.get_device() == value_cache.get_device() == device
-            and all(t is None or (t.dtype is f16 and t.shape == (head_dim,) and t.is_contiguous() and t.get_device() == device)
-                    for t in (query_weight, key_weight))
-            and (pairs == 0 or (frequencies.dtype in (torch.int64, torch.uint64) and frequencies.dim() == 1 and frequencies.is_contiguous()
-                                and positions is not None and positions.dtype is i32 and positions.shape == (tokens,) and positions.is_contiguous()
-                                and frequencies.get_device() == positions.get_device() == device))):
+    if not (kind in _CACHED and value_cache.dtype is kind and query.dtype is f16 and query_out.dtype is f16 and key.dtype is f16 and value.dtype is f16
+            and width == head_dim and query_out.shape == rows and key.shape == new and value.shape == new
+            and value_cache.shape == (pages, kv_heads, head_dim, page_size) and slots.dtype is i32 and slots.shape == each and slots.is_contiguous()
+            and key_cache.is_contiguous() and value_cache.is_contiguous() and not (tokens | heads | pages | pairs) >> 30
+            and query.get_device() == query_out.get_device() == key.get_device() == value.get_device() == slots.get_device()
+            == key_cache.get_device() == value_cache.get_device() == device
+            and (query_weight is None or (query_weight.dtype is f16 and query_weight.shape == one and query_weight.get_device() == device
+                                          and query_weight.is_contiguous()))
+            and (key_weight is None or (key_weight.dtype is f16 and key_weight.shape == one and key_weight.get_device() == device
+                                        and key_weight.is_contiguous()))
+            and (pairs == 0 or (frequencies.dtype in _WORDS and frequencies.get_device() == device and frequencies.is_contiguous()
+                                and positions is not None and positions.dtype is i32 and positions.shape == each
+                                and positions.get_device() == device and positions.is_contiguous()))):
         if pairs and positions is None:
             raise ValueError("head_norm_rotary_write: a rotation needs positions")
-        words = (torch.int64, torch.uint64)
-        _refuse("head_norm_rotary_write", device, ("key_cache", key_cache, kinds, None, True), ("value_cache", value_cache, (kind,), transposed, True),
-                ("query", query, (f16,), (tokens, heads, head_dim), False), ("query_out", query_out, (f16,), (tokens, heads, head_dim), False),
-                ("key", key, (f16,), new, False), ("value", value, (f16,), new, False), ("slots", slots, (i32,), (tokens,), True),
-                ("query_weight", query_weight, (f16,), (head_dim,), True), ("key_weight", key_weight, (f16,), (head_dim,), True),
-                ("positions", positions, (i32,), (tokens,), True), ("frequencies", frequencies, words, (pairs,), True))
-    what = "head_norm_rotary_write"
+        _refuse(what, device, ("key_cache", key_cache, _CACHED, None, True),
+                ("value_cache", value_cache, (kind,), (pages, kv_heads, head_dim, page_size), True), ("query", query, (f16,), (tokens, heads, head_dim), False),
+                ("query_out", query_out, (f16,), (tokens, heads, head_dim), False), ("key", key, (f16,), new, False), ("value", value, (f16,), new, False),
+                ("slots", slots, (i32,), each, True), ("query_weight", query_weight, (f16,), one, True), ("key_weight", key_weight, (f16,), one, True),
+                ("positions", positions, (i32,), each, True), ("frequencies", frequencies, _WORDS, None, True))
     _done("pk_head_norm_rotary_write", lib.pk_head_norm_rotary_write(
-        CACHE_FP16 if kind is f16 else CACHE_FP8, query.data_ptr(), _row_stride(what, "query", query), key.data_ptr(), _row_stride(what, "key", key),
-        value.data_ptr(), _row_stride(what, "value", value), None if query_weight is None else query_weight.data_ptr(),
-        None if key_weight is None else key_weight.data_ptr(), positions.data_ptr() if pairs else None, slots.data_ptr(),
-        frequencies.data_ptr() if pairs else None, query_out.data_ptr(), _row_stride(what, "query_out", query_out), key_cache.data_ptr(),
-        value_cache.data_ptr(), tokens, heads, kv_heads, head_dim, 2 * pairs, interleaved, amplitude, epsilon, page_size, pages, key_inverse_scale,
-        value_inverse_scale, stream))
+        CACHE_FP16 if kind is f16 else CACHE_FP8, query.data_ptr(), _token_stride(what, "query", query, tokens, heads, head_dim), key.data_ptr(),
+        _token_stride(what, "key", key, tokens, kv_heads, head_dim), value.data_ptr(), _token_stride(what, "value", value, tokens, kv_heads, head_dim),
+        None if query_weight is None else query_weight.data_ptr(), None if key_weight is None else key_weight.data_ptr(),
+        positions.data_ptr() if pairs else None, slots.data_ptr(), frequencies.data_ptr() if pairs else None, query_out.data_ptr(),
+        _token_stride(what, "query_out", query_out, tokens, heads, head_dim), key_cache.data_ptr(), value_cache.data_ptr(), tokens, heads, kv_heads,
+        head_dim, 2 * pairs, interleaved, amplitude, epsilon, page_size, pages, key_inverse_scale, value_inverse_scale, stream))
 
 
 def beam_select_workspace_bytes(sequences, beams, vocab, choices):
@@ -745,32 +758,33 @@ def beam_select(logits, scores, ended, out_scores, out_tokens, out_parents, out_
     device, stream = _device_and_stream(stream)
     sequences, beams, vocab = logits.shape
     _, choices = out_scores.shape
-    f16, f32, i32, flags = torch.float16, torch.float32, torch.int32, (torch.bool, torch.uint8)
-    kinds, have, found = (f16, f32), (sequences, beams), (sequences, choices)
+    f16, f32, i32, flag, byte = torch.float16, torch.float32, torch.int32, torch.bool, torch.uint8
+    kind, have, found = logits.dtype, (sequences, beams), (sequences, choices)
     step, row, one = logits.stride()
-    rows = sequences * beams
-    if rows <= 1:
+    if sequences * beams <= 1:
         row = vocab
     elif beams == 1:
         row = step
-    if not (logits.dtype in kinds and (one == 1 or vocab == 1) and (sequences <= 1 or beams == 1 or step == beams * row)
-            and not (rows | vocab | choices | row | end_token + 1) >> 31 and scores.dtype is f32 and scores.shape == have
-            and scores.is_contiguous() and out_scores.dtype is f32 and out_scores.shape == found and out_scores.is_contiguous()
+    if not ((kind is f16 or kind is f32) and (one == 1 or vocab == 1) and (sequences <= 1 or beams == 1 or step == beams * row)
+            and not (sequences | beams | vocab | choices | row | end_token + 1) >> 31 and scores.dtype is f32 and scores.shape == have
+            and scores.is_contiguous() and out_scores.dtype is f32 and out_scores.is_contiguous()
             and out_tokens.dtype is i32 and out_tokens.shape == found and out_tokens.is_contiguous() and out_parents.dtype is i32
             and out_parents.shape == found and out_parents.is_contiguous()
             and logits.get_device() == scores.get_device() == out_scores.get_device() == out_tokens.get_device() == out_parents.get_device() == device
-            and (ended is None or (ended.dtype in flags and ended.shape == have and ended.is_contiguous() and ended.get_device() == device))
-            and (out_ended is None or (out_ended.dtype in flags and out_ended.shape == found and out_ended.is_contiguous()
+            and (ended is None or ((ended.dtype is flag or ended.dtype is byte) and ended.shape == have and ended.is_contiguous()
+                                   and ended.get_device() == device))
+            and (out_ended is None or ((out_ended.dtype is flag or out_ended.dtype is byte) and out_ended.shape == found and out_ended.is_contiguous()
                                        and out_ended.get_device() == device))
-            and (workspace is None or (workspace.dtype is torch.uint8 and workspace.is_contiguous() and workspace.get_device() == device))):
+            and out_scores.shape == found
+            and (workspace is None or (workspace.dtype is byte and workspace.is_contiguous() and workspace.get_device() == device))):
         if not ((one == 1 or vocab == 1) and (sequences <= 1 or beams == 1 or step == beams * row)):
             raise ValueError("beam_select: the rows of logits must be contiguous and lie equally far apart")
-        _refuse("beam_select", device, ("logits", logits, kinds, None, False), ("scores", scores, (f32,), have, True),
-                ("ended", ended, flags, have, True), ("out_scores", out_scores, (f32,), found, True), ("out_tokens", out_tokens, (i32,), found, True),
-                ("out_parents", out_parents, (i32,), found, True), ("out_ended", out_ended, flags, found, True),
-                ("workspace", workspace, (torch.uint8,), None, True))
+        _refuse("beam_select", device, ("logits", logits, (f16, f32), None, False), ("scores", scores, (f32,), have, True),
+                ("ended", ended, (flag, byte), have, True), ("out_scores", out_scores, (f32,), found, True), ("out_tokens", out_tokens, (i32,), found, True),
+                ("out_parents", out_parents, (i32,), found, True), ("out_ended", out_ended, (flag, byte), found, True),
+                ("workspace", workspace, (byte,), None, True))
     _done("pk_beam_select", lib.pk_beam_select(
-        LOGITS_FP16 if logits.dtype is f16 else LOGITS_FP32, logits.data_ptr(), row, scores.data_ptr(), None if ended is None else ended.data_ptr(),
+        LOGITS_FP16 if kind is f16 else LOGITS_FP32, logits.data_ptr(), row, scores.data_ptr(), None if ended is None else ended.data_ptr(),
         out_scores.data_ptr(), out_tokens.data_ptr(), out_parents.data_ptr(), None if out_ended is None else out_ended.data_ptr(), sequences, beams,
         vocab, choices, end_token, None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(), stream))
 
@@ -816,10 +830,16 @@ def page_fork(parents, block_table, lengths, free_pages, free_range, new_table, 
     i32, flags = torch.int32, (torch.bool, torch.uint8)
     rows, max_pages = block_table.shape
     pages, one = freed.numel(), (rows,)
-    arrays = (parents, block_table, lengths, free_pages, free_range, new_table, new_lengths, copies, freed, info)
-    if not (all(t.dtype is i32 and t.get_device() == device and t.is_contiguous() for t in arrays) and parents.shape == one and lengths.shape == one
-            and free_range.shape == (2,) and free_pages.dim() == freed.dim() == 1 and new_table.shape == (rows, max_pages) and new_lengths.shape == one
-            and copies.shape == (rows, 2) and info.shape == (4,) and not (rows | max_pages | pages | free_pages.numel() | page_size) >> 31
+    both, four = (rows, max_pages), (4,)
+    if not (parents.dtype is i32 and block_table.dtype is i32 and lengths.dtype is i32 and free_pages.dtype is i32 and free_range.dtype is i32
+            and new_table.dtype is i32 and new_lengths.dtype is i32 and copies.dtype is i32 and freed.dtype is i32 and info.dtype is i32
+            and parents.get_device() == block_table.get_device() == lengths.get_device() == free_pages.get_device() == free_range.get_device()
+            == new_table.get_device() == new_lengths.get_device() == copies.get_device() == freed.get_device() == info.get_device() == device
+            and parents.is_contiguous() and block_table.is_contiguous() and lengths.is_contiguous() and free_pages.is_contiguous()
+            and free_range.is_contiguous() and new_table.is_contiguous() and new_lengths.is_contiguous() and copies.is_contiguous()
+            and freed.is_contiguous() and info.is_contiguous() and parents.shape == one and lengths.shape == one and free_range.shape == (2,)
+            and free_pages.dim() == freed.dim() == 1 and new_table.shape == both and new_lengths.shape == one
+            and copies.shape == (rows, 2) and info.shape == four and not (rows | max_pages | pages | free_pages.numel() | page_size) >> 31
             and (held is None or (held.dtype in flags and held.shape == (pages,) and held.is_contiguous() and held.get_device() == device))
             and workspace.dtype is torch.uint8 and workspace.is_contiguous() and workspace.get_device() == device):
         i32 = (i32,)
@@ -855,7 +875,7 @@ def paged_cache_copy(copies, key_cache, value_cache, stream=None):
     of one layer [pages x ...] as paged_cache_write's, or of several [layers x pages x ...]."""
     torch = _torch or _types()
     device, stream = _device_and_stream(stream)
-    shape, kinds = key_cache.shape, (torch.float16, torch.uint8, torch.float8_e4m3fn)
+    shape, kinds = key_cache.shape, _CACHED
     swapped = shape[:-2] + shape[:-3:-1]
     if not (4 <= len(shape) <= 5 and key_cache.dtype in kinds and value_cache.dtype is key_cache.dtype and value_cache.shape == swapped
             and copies.dtype is torch.int32 and copies.dim() == 2 and copies.shape[1] == 2 and copies.is_contiguous() and key_cache.is_contiguous()
