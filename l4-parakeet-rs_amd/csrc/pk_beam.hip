@@ -528,7 +528,6 @@ void launch_beam_select(bool fp16, const BeamArgs& a, hipStream_t s) {
 // rows of 2 MB: 74 us, 80 without; a copy of all of them 99).  Stores past the caches where the
 // state is larger than they are (74 us against 80).
 constexpr int kRowLoads = 2;
-constexpr long long kCached = 32ll << 20;  // bytes of the L2 caches
 
 template <typename Unit, bool kPast>
 __global__ __launch_bounds__(256) void beam_rows_kernel(const Unit* __restrict__ in, const int* __restrict__ parents, Unit* __restrict__ out, int beams,

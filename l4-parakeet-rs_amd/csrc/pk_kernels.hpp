@@ -103,6 +103,8 @@ struct PagedArgs {
 };
 size_t paged_attention_workspace(int head_dim, int page_shift, int max_pages, int max_rows);
 void launch_paged_attention(int kind, const PagedArgs& args, int head_dim, int max_queries, void* workspace, hipStream_t s);
+constexpr long long kCached = 32ll << 20;  // bytes of the L2 caches of all XCDs
+
 // frequencies: turns a position in 2^-64; the cache's members in the writing form alone
 struct RotaryArgs {
     const uint16_t* query;

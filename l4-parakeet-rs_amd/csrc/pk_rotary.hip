@@ -35,7 +35,8 @@ __device__ __forceinline__ void unpack(const uint4& raw, float (&y)[8]) {
     for (int j = 0; j < 8; ++j) y[j] = h2f((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
 }
 
-template <bool kF8> __device__ __forceinline__ void store8(uint8_t* to, const float (&y)[8], float inverse) {
+// kPast: past the caches, for results larger than they are (16000 tokens of 32 / 8 heads of 128 64 us, else 68).
+template <bool kF8, bool kPast> __device__ __forceinline__ void store8(uint8_t* to, const float (&y)[8], float inverse) {
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -47,13 +48,21 @@ template <bool kF8> __device__ __forceinline__ void store8(uint8_t* to, const fl
             w[j] = (uint32_t)f2h(y[2 * j]) | ((uint32_t)f2h(y[2 * j + 1]) << 16);
         }
     }
-    if constexpr (kF8) *(uint2*)to = uint2{w[0], w[1]};
-    else *(uint4*)to = uint4{w[0], w[1], w[2], w[3]};
+    if constexpr (kF8) {
+        const v2i v{(int)w[0], (int)w[1]};
+        if constexpr (kPast) __builtin_nontemporal_store(v, (v2i*)to);
+        else *(v2i*)to = v;
+    } else {
+        const v4i v{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+        if constexpr (kPast) __builtin_nontemporal_store(v, (v4i*)to);
+        else *(v4i*)to = v;
+    }
 }
 
-// kLanes lanes a head (a power of two of at least head_dim / 16).  kCache: -1 rows out, 0 an
-// fp16 cache, 1 an e4m3 one.  A wave takes `sets` times 64 / kLanes heads of a token.
-template <int kLanes, int kCache>
+// kLanes lanes a head (a power of two of at least head_dim / 16), 64 / kLanes heads a set: query sets,
+// then key sets, then (few tokens into a cache) value sets.  kCache: -1 rows out, 0 an fp16 cache, 1 an
+// e4m3 one.  A wave takes `sets` sets of a token, the next one's loads in flight.
+template <int kLanes, int kCache, bool kPast>
 __global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int parts, int sets, int value_blocks) {
     constexpr int kSlots = 64 / kLanes;
     constexpr bool kF8 = kCache == 1;
@@ -67,66 +76,95 @@ __global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int
             return;
         }
     }
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, p = lane % kLanes;
-    const long long unit = (long long)(blockIdx.x - value_blocks) * 4 + wave;
-    const int t = (int)(unit / parts), first = (int)(unit % parts) * sets * kSlots + lane / kLanes;
-    bool real = t < a.tokens;
-    int slot = 0;
-    if constexpr (kCache >= 0) {
-        slot = real ? a.slots[t] : -1;
-        real = slot >= 0 && slot < a.slot_count;
-    }
-    const long long position = real && a.rotary_dim ? a.positions[t] : 0;  // (no rotation: there may be no positions)
-    for (int i = lane; i < a.rotary_dim / 2; i += 64) angles[wave][i] = turned_by((unsigned long long)position * a.frequencies[i], a.amplitude);
-    __syncthreads();
-    if (!real) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, p = lane % kLanes, place = lane / kLanes;
+    const int unit = (int)(blockIdx.x - value_blocks) * 4 + wave, t = unit / parts;  // (below 2^31: at most 2^21 tokens of 8192 / tokens parts)
+    const int query_sets = (a.heads + kSlots - 1) / kSlots, kv_sets = (a.kv_heads + kSlots - 1) / kSlots;
+    const int all = query_sets + kv_sets + (kCache >= 0 && value_blocks == 0 ? kv_sets : 0);
+    const int first = unit % parts * sets, stop = first + sets < all ? first + sets : all;
+    const bool there = t < a.tokens && first < stop, rotates = there && a.rotary_dim && first < query_sets + kv_sets;
     const bool inside = p * 16 < a.head_dim, turns = p * 16 < a.rotary_dim, halves = turns && !a.interleaved;
     const int f0 = halves ? 8 * p : 16 * p, f1 = halves ? f0 + a.rotary_dim / 2 : f0 + 8;
+    struct Raw {
+        uint4 u, v;
+    };
+    const auto ask = [&](int set) {
+        const bool query = set < query_sets, value = set >= query_sets + kv_sets;
+        const int h = (query ? set : value ? set - query_sets - kv_sets : set - query_sets) * kSlots + place;
+        const uint16_t* row = query ? a.query + (size_t)t * a.query_stride : value ? a.value + (size_t)t * a.value_stride : a.key + (size_t)t * a.key_stride;
+        Raw raw{};
+        if (inside && h < (query ? a.heads : a.kv_heads)) {
+            raw.u = *(const uint4*)(row + h * a.head_dim + f0);
+            raw.v = *(const uint4*)(row + h * a.head_dim + f1);
+        }
+        return raw;
+    };
+    // all that can be asked for at once: a chain of one load, the angles and the store is left
+    Raw now{};
+    if (there) now = ask(first);
+    int slot = 0;
+    if constexpr (kCache >= 0) slot = there ? a.slots[t] : -1;
+    const long long position = rotates ? a.positions[t] : 0;  // (no rotation: there may be no positions)
+    const uint16_t* weight = nullptr;
+    uint4 raw0{}, raw1{};
+    const auto ask_weight = [&](int set) {
+        weight = set < query_sets ? a.query_weight : a.key_weight;
+        if (weight && inside) {
+            raw0 = *(const uint4*)(weight + f0);
+            raw1 = *(const uint4*)(weight + f1);
+        }
+    };
+    if (there) ask_weight(first);
+    if (rotates)
+        for (int i = lane; i < a.rotary_dim / 2; i += 64) angles[wave][i] = turned_by((unsigned long long)position * a.frequencies[i], a.amplitude);
+    __syncthreads();
+    if (!there || slot < 0 || (kCache >= 0 && slot >= a.slot_count)) return;
     float2 angle[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) angle[j] = turns ? angles[wave][8 * p + j] : float2{1.0f, 0.0f};
-    const int of_values = kCache >= 0 && value_blocks == 0 ? a.kv_heads : 0, all = a.heads + a.kv_heads + of_values;
-    const int stop = first + sets * kSlots < all ? first + sets * kSlots : all;
     const int off = slot & ((1 << a.shift) - 1);
-    for (int h = first; h < stop; h += kSlots) {
-        const bool query = h < a.heads, value = h >= a.heads + a.kv_heads;
-        const int kvh = value ? h - a.heads - a.kv_heads : h - a.heads;
-        const uint16_t* row = query ? a.query + (size_t)t * a.query_stride + (size_t)h * a.head_dim
-                                    : (value ? a.value + (size_t)t * a.value_stride : a.key + (size_t)t * a.key_stride) + (size_t)kvh * a.head_dim;
-        uint4 r0{}, r1{};
-        if (inside) {
-            r0 = *(const uint4*)(row + f0);
-            r1 = *(const uint4*)(row + f1);
-        }
+    float w0[8], w1[8];
+    unpack(raw0, w0);
+    unpack(raw1, w1);
+    for (int set = first; set < stop; ++set) {
+        const bool query = set < query_sets, value = set >= query_sets + kv_sets;
+        const int h = (query ? set : value ? set - query_sets - kv_sets : set - query_sets) * kSlots + place;
+        const bool mine = inside && h < (query ? a.heads : a.kv_heads);
         float u[8], v[8];
-        unpack(r0, u);
-        unpack(r1, v);
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(v[j], v[j], __builtin_fmaf(u[j], u[j], sum));
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) sum = add_level(sum, o);
-        if (!inside) continue;
+        unpack(now.u, u);
+        unpack(now.v, v);
+        if (set + 1 < stop) now = ask(set + 1);
         if constexpr (kCache >= 0) {
             if (value) {  // features lie a page's tokens apart
-                const size_t base = ((size_t)(slot >> a.shift) * a.kv_heads + kvh) * a.head_dim;
+                if (mine) {
+                    const size_t base = ((size_t)(slot >> a.shift) * a.kv_heads + h) * a.head_dim;
+                    const size_t at0 = ((base + f0) << a.shift) + off, at1 = ((base + f1) << a.shift) + off;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const size_t at = ((base + (j < 8 ? f0 + j : f1 + j - 8)) << a.shift) + off;
-                    const float y = j < 8 ? u[j] : v[j - 8];
-                    if constexpr (kF8) ((uint8_t*)a.value_cache)[at] = e4m3(y * a.v_inv);
-                    else ((uint16_t*)a.value_cache)[at] = f2h(y);
+                    for (int j = 0; j < 8; ++j) {
+                        if constexpr (kF8) {
+                            ((uint8_t*)a.value_cache)[at0 + ((size_t)j << a.shift)] = e4m3(u[j] * a.v_inv);
+                            ((uint8_t*)a.value_cache)[at1 + ((size_t)j << a.shift)] = e4m3(v[j] * a.v_inv);
+                        } else {
+                            ((uint16_t*)a.value_cache)[at0 + ((size_t)j << a.shift)] = f2h(u[j]);
+                            ((uint16_t*)a.value_cache)[at1 + ((size_t)j << a.shift)] = f2h(v[j]);
+                        }
+                    }
                 }
                 continue;
             }
         }
-        const uint16_t* weight = query ? a.query_weight : a.key_weight;
+        if (set == query_sets && set > first) {
+            ask_weight(set);
+            unpack(raw0, w0);
+            unpack(raw1, w1);
+        }
         if (weight) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(v[j], v[j], __builtin_fmaf(u[j], u[j], sum));
+#pragma unroll
+            for (int o = 1; o < kLanes; o <<= 1) sum = add_level(sum, o);
             const float mean = sum / (float)a.head_dim + a.epsilon;
             const float rstd = mean > 0.0f ? 1.0f / sqrtf(mean) : (mean == 0.0f ? 0.0f : mean);  // NaN stays NaN; all zero with eps 0: zeros
-            float w0[8], w1[8];
-            unpack(*(const uint4*)(weight + f0), w0);
-            unpack(*(const uint4*)(weight + f1), w1);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 u[j] = u[j] * rstd * w0[j];
@@ -150,39 +188,44 @@ __global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int
                 for (int j = 0; j < 8; ++j) turn(u[j], v[j], angle[j]);
             }
         }
+        if (!mine) continue;
         if (kCache < 0 || query) {
-            uint16_t* to = query ? a.query_out + (size_t)t * a.query_out_stride + (size_t)h * a.head_dim
-                                 : a.key_out + (size_t)t * a.key_out_stride + (size_t)kvh * a.head_dim;
-            store8<false>((uint8_t*)(to + f0), u, 1.0f);
-            store8<false>((uint8_t*)(to + f1), v, 1.0f);
+            uint16_t* to = (query ? a.query_out + (size_t)t * a.query_out_stride : a.key_out + (size_t)t * a.key_out_stride) + h * a.head_dim;
+            store8<false, kPast>((uint8_t*)(to + f0), u, 1.0f);
+            store8<false, kPast>((uint8_t*)(to + f1), v, 1.0f);
         } else {
-            uint8_t* to = (uint8_t*)a.key_cache + (((((size_t)(slot >> a.shift) * a.kv_heads + kvh) << a.shift) + off) * a.head_dim) * (kF8 ? 1 : 2);
-            store8<kF8>(to + f0 * (kF8 ? 1 : 2), u, a.k_inv);
-            store8<kF8>(to + f1 * (kF8 ? 1 : 2), v, a.k_inv);
+            uint8_t* to = (uint8_t*)a.key_cache + (((((size_t)(slot >> a.shift) * a.kv_heads + h) << a.shift) + off) * a.head_dim) * (kF8 ? 1 : 2);
+            store8<kF8, kPast>(to + f0 * (kF8 ? 1 : 2), u, a.k_inv);
+            store8<kF8, kPast>(to + f1 * (kF8 ? 1 : 2), v, a.k_inv);
         }
     }
 }
 
-template <int kCache> static void launch_rotary(const RotaryArgs& a, hipStream_t s) {
+template <int kCache, bool kPast> static void launch_rotary(const RotaryArgs& a, hipStream_t s) {
     const bool tiles = kCache >= 0 && a.tokens >= kTileTokens;
     const int value_blocks = tiles ? a.kv_heads * ((a.tokens + kWriteTokens - 1) / kWriteTokens) : 0;
-    const int all = a.heads + a.kv_heads + (kCache >= 0 && !tiles ? a.kv_heads : 0);
     const auto launch = [&](auto kernel, int lanes) {
-        const int each = 64 / lanes, need = (all + each - 1) / each;
-        const int parts = (long long)a.tokens * need <= 8192 ? need : 1, sets = (need + parts - 1) / parts;
+        const int each = 64 / lanes, kv_sets = (a.kv_heads + each - 1) / each;
+        const int all = (a.heads + each - 1) / each + kv_sets + (kCache >= 0 && !tiles ? kv_sets : 0);
+        const int parts = (long long)a.tokens * all <= 8192 ? all : 1, sets = (all + parts - 1) / parts;
         const unsigned grid = (unsigned)(((long long)a.tokens * parts + 3) / 4 + value_blocks);
         kernel<<<grid, 256, 0, s>>>(a, parts, sets, value_blocks);
     };
-    if (a.head_dim <= 64) launch(head_norm_rotary_kernel<4, kCache>, 4);
-    else if (a.head_dim <= 128) launch(head_norm_rotary_kernel<8, kCache>, 8);
-    else if constexpr (kCache < 0) launch(head_norm_rotary_kernel<16, kCache>, 16);  // (a cache holds heads of 64 or 128)
+    if (a.head_dim <= 64) launch(head_norm_rotary_kernel<4, kCache, kPast>, 4);
+    else if (a.head_dim <= 128) launch(head_norm_rotary_kernel<8, kCache, kPast>, 8);
+    else if constexpr (kCache < 0) launch(head_norm_rotary_kernel<16, kCache, kPast>, 16);  // (a cache holds heads of 64 or 128)
 }
 
-void launch_head_norm_rotary(const RotaryArgs& a, hipStream_t s) { launch_rotary<-1>(a, s); }
+template <int kCache> static void rotary(const RotaryArgs& a, hipStream_t s) {
+    if ((long long)a.tokens * (a.heads + a.kv_heads) * a.head_dim * 2 > kCached) launch_rotary<kCache, true>(a, s);
+    else launch_rotary<kCache, false>(a, s);
+}
+
+void launch_head_norm_rotary(const RotaryArgs& a, hipStream_t s) { rotary<-1>(a, s); }
 
 void launch_head_norm_rotary_write(int kind, const RotaryArgs& a, hipStream_t s) {
-    if (kind == 1) launch_rotary<1>(a, s);
-    else launch_rotary<0>(a, s);
+    if (kind == 1) rotary<1>(a, s);
+    else rotary<0>(a, s);
 }
 
 // Radians a position, i of `pairs` (frequencies fall from 1 by a constant factor).
