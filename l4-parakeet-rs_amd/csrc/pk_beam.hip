@@ -164,7 +164,7 @@ __device__ __forceinline__ void rank_listed(const PartShared<kGroup>& shared, in
 // its lowest bit is 2^-52 of an fp32 term's, and half a step such a term's only from 128 on.
 template <bool kF16, int kLoads, int kGroup, typename Real>
 __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab, int part, int choices, int tid, PartShared<kGroup>& shared,
-                                             PartSum* sum_out, unsigned long long* to) {
+                                             int& over, PartSum* sum_out, unsigned long long* to) {
     constexpr int kVec = kF16 ? 8 : 4, kWaves = kGroup / 64, kListed = PartShared<kGroup>::kListed;
     constexpr int kPart = kGroup * kLoads * kVec, kBytes = kF16 ? 2 : 4;
     const int wave = tid >> 6, first = part * kPart, count_here = vocab - first < kPart ? vocab - first : kPart;
@@ -195,7 +195,10 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
         shared.most[wave] = wave_most;
         shared.bound[wave] = here;
     }
-    if (tid == 0) shared.listed = 0;
+    if (tid == 0) {
+        shared.listed = 0;
+        over = 0;  // (of all that are here)
+    }
     __syncthreads();
     uint32_t found = shared.bound[0];
     float most = shared.most[0];
@@ -211,6 +214,7 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
         if (v >= bound) {
             const int k = atomicAdd(&shared.listed, 1);
             if (k < kListed) shared.list[k] = key_of(v, i);
+            else over = 1;
         }
     };
     constexpr double kNudge = 1.0 + 0x1p-52;
@@ -245,9 +249,8 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
         }
         *sum_out = PartSum{some ? __builtin_nan("") : (double)sum * 0x1p-44, most, 0};
     }
-    const int count = shared.listed;
-    if (!__syncthreads_or(count > kListed)) {
-        if (to) rank_listed(shared, count, choices, tid, to);
+    if (!over) {
+        if (to) rank_listed(shared, shared.listed, choices, tid, to);
         return;
     }
     // Many equal logits: the largest key below the last one, `choices` times.
@@ -286,10 +289,11 @@ __device__ __forceinline__ int beam_state(float score, const uint8_t* ended, siz
 template <bool kF16, int kLoads>
 __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a, int parts, PartSum* __restrict__ sums, unsigned long long* __restrict__ best) {
     __shared__ PartShared<256> shared;
+    __shared__ int over;
     const int row = blockIdx.x / parts, part = blockIdx.x % parts;
     if (beam_state(a.scores[row], a.ended, row) != 1) return;
     const size_t out = (size_t)row * parts + part;
-    best_of_part<kF16, kLoads, 256>((const char*)a.logits + (size_t)row * a.stride * (kF16 ? 2 : 4), [] { return true; }, a.vocab, part, a.choices, threadIdx.x, shared,
+    best_of_part<kF16, kLoads, 256>((const char*)a.logits + (size_t)row * a.stride * (kF16 ? 2 : 4), [] { return true; }, a.vocab, part, a.choices, threadIdx.x, shared, over,
                                sums + out, best + out * a.choices);
 }
 
@@ -314,7 +318,7 @@ template <int kThreads> struct JoinShared {
 // A sequence's answer, by a workgroup: the logarithms of the beams' sums, a wave a beam, then the
 // best of all parts' candidates by the same bound, over the upper bits of their scores.  sums and keys are
 // the sequence's, and need not be set for beams without candidates.
-template <int kThreads, bool kF16>
+template <int kThreads, bool kF16, bool kOnePart>
 __device__ __forceinline__ void join_parts(const BeamArgs& a, int seq, int parts, const PartSum* sums, const unsigned long long* keys,
                                            JoinShared<kThreads>& shared) {
     constexpr int kWaves = kThreads / 64, kKept = 2;  // candidates a thread keeps between its two looks at them
@@ -346,7 +350,9 @@ __device__ __forceinline__ void join_parts(const BeamArgs& a, int seq, int parts
                 const bool some = one.most > -__builtin_inff() && one.most < __builtin_inff();
                 // what c lacks of m log2e, in powers of 2
                 const double lost = kF16 && some ? (double)(one.most * kLog2e) - (double)one.most * (double)kLog2e : 0.0;
-                mine += some ? one.sum * exp(((double)one.most - (double)most) + lost * 0.69314718055994530942) : one.sum;
+                const double z = lost * 0.69314718055994530942;  // at most 94504 2^-24 ln 2 = 4e-3 off 0
+                const double factor = kOnePart ? 1.0 + z * (1.0 + z * (0.5 + z * (1.0 / 6))) : exp(((double)one.most - (double)most) + z);
+                mine += some ? one.sum * factor : one.sum;
             }
             log_sum = (double)most + log(wave_sum(mine));
             s = most > -__builtin_inff() && most < __builtin_inff() && log_sum == log_sum;  // a NaN or an infinity: no candidates
@@ -379,12 +385,14 @@ __device__ __forceinline__ void join_parts(const BeamArgs& a, int seq, int parts
         larger(kept[n]);
     }
     for (int i = tid + kKept * kThreads; i < front; i += kThreads) larger(candidate(i / depth, i % depth));
-    const uint32_t here = wave_bound(mine, a.choices, 12);  // eight bits of the mantissa
-    if (lane == 0) shared.wave_bound[wave] = here;
-    __syncthreads();
-    uint32_t bound = shared.wave_bound[0];
+    uint32_t bound = 0;
+    if (front > 128 || depth < a.choices) {  // else all of them are ranked
+        const uint32_t here = wave_bound(mine, a.choices, 12);  // eight bits of the mantissa
+        if (lane == 0) shared.wave_bound[wave] = here;
+        __syncthreads();
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) bound = shared.wave_bound[w] > bound ? shared.wave_bound[w] : bound;
+        for (int w = 0; w < kWaves; ++w) bound = shared.wave_bound[w] > bound ? shared.wave_bound[w] : bound;
+    }
     const auto reaches = [&](const Candidate& one) {
         if (!one.score || (uint32_t)(one.score >> 32) < bound) return false;
         const int k = atomicAdd(&shared.listed, 1);
@@ -457,7 +465,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
                                                                  const unsigned long long* __restrict__ best) {
     __shared__ JoinShared<kJoinThreads> shared;
     const size_t first = (size_t)blockIdx.x * a.beams;
-    join_parts<kJoinThreads, kF16>(a, blockIdx.x, parts, sums + first * parts, best + first * parts * a.choices, shared);
+    join_parts<kJoinThreads, kF16, false>(a, blockIdx.x, parts, sums + first * parts, best + first * parts * a.choices, shared);
 }
 
 // Both in one launch where the rows are short and a sequence has few beams: kGroup threads a beam.
@@ -466,18 +474,19 @@ constexpr int kWholeThreads = 1024, kWholeBeams = 16, kWholeVectors = 512;  // 1
 template <bool kF16, int kGroup> __global__ __launch_bounds__(kWholeThreads) void beam_whole_kernel(BeamArgs a) {
     constexpr int kGroups = kWholeThreads / kGroup;
     __shared__ PartShared<kGroup> part[kGroups];
+    __shared__ int over;
     __shared__ JoinShared<kWholeThreads> shared;
     __shared__ PartSum sums[kGroups];
     __shared__ unsigned long long keys[kGroups * 64];
     const int seq = blockIdx.x, b = threadIdx.x / kGroup;
     const size_t row = (size_t)seq * a.beams + (b < a.beams ? b : 0);
     const float score = a.scores[row];
-    const uint8_t over = a.ended ? a.ended[row] : 0;
-    const auto real = [&] { return b < a.beams && !over && __builtin_fabsf(score) < __builtin_inff(); };
+    const uint8_t done = a.ended ? a.ended[row] : 0;
+    const auto real = [&] { return b < a.beams && !done && __builtin_fabsf(score) < __builtin_inff(); };
     best_of_part<kF16, kWholeVectors / kGroup, kGroup>((const char*)a.logits + row * a.stride * (kF16 ? 2 : 4), real, a.vocab, 0, a.choices,
-                                                       threadIdx.x % kGroup, part[b], sums + b, b < a.beams ? keys + b * a.choices : nullptr);
+                                                       threadIdx.x % kGroup, part[b], over, sums + b, b < a.beams ? keys + b * a.choices : nullptr);
     __syncthreads();
-    join_parts<kWholeThreads, kF16>(a, seq, 1, sums, keys, shared);
+    join_parts<kWholeThreads, kF16, true>(a, seq, 1, sums, keys, shared);
 }
 
 // Loads a thread, and with them the parts: many workgroups where rows are few or short, else many

@@ -342,22 +342,31 @@ void launch_page_keep(const int* info, const int* freed, int* free_pages, int* f
     page_keep_kernel<<<1, 256, 0, s>>>(info, freed, free_pages, free_range, free_capacity);
 }
 
-// Pairs (source, destination) of pages in all layers' keys and values.
-__global__ __launch_bounds__(256) void paged_cache_copy_kernel(const int* __restrict__ copies, uint4* key_cache, uint4* value_cache, long long units,
+// Pairs (source, destination) of pages in all layers' keys and values.  Bound by HBM: 1434 pages of
+// 16 KB in 12 layers' keys and values (1.13 GB read and written) 214 us, 5.3 TB/s, with stores past the
+// caches; 223 without.
+template <bool kPast>
+__global__ __launch_bounds__(256) void paged_cache_copy_kernel(const int* __restrict__ copies, v4i* key_cache, v4i* value_cache, long long units,
                                                                int pages, int layers) {
     const int from = copies[2 * blockIdx.y], to = copies[2 * blockIdx.y + 1];
     if (from < 0 || from >= pages || to < 0 || to >= pages || from == to) return;
     const int layer = blockIdx.z % layers;
-    uint4* cache = (int)blockIdx.z < layers ? key_cache : value_cache;
-    const uint4* src = cache + ((long long)layer * pages + from) * units;
-    uint4* dst = cache + ((long long)layer * pages + to) * units;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < units; i += (long long)gridDim.x * 256) dst[i] = src[i];
+    v4i* cache = (int)blockIdx.z < layers ? key_cache : value_cache;
+    const v4i* src = cache + ((long long)layer * pages + from) * units;
+    v4i* dst = cache + ((long long)layer * pages + to) * units;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < units; i += (long long)gridDim.x * 256) {
+        const v4i v = src[i];
+        if constexpr (kPast) __builtin_nontemporal_store(v, dst + i);
+        else dst[i] = v;
+    }
 }
 
 void launch_paged_cache_copy(const int* copies, int count, void* key_cache, void* value_cache, long long page_bytes, int pages, int layers, hipStream_t s) {
     const long long units = page_bytes / 16;
     const dim3 grid((unsigned)((units + 255) / 256 > 64 ? 64 : (units + 255) / 256), (unsigned)count, (unsigned)(2 * layers));
-    paged_cache_copy_kernel<<<grid, 256, 0, s>>>(copies, (uint4*)key_cache, (uint4*)value_cache, units, pages, layers);
+    const auto launch = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(copies, (v4i*)key_cache, (v4i*)value_cache, units, pages, layers); };
+    if (2 * page_bytes * layers * count > kCached) launch(paged_cache_copy_kernel<true>);
+    else launch(paged_cache_copy_kernel<false>);
 }
 
 }  // namespace pk
