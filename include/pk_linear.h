@@ -837,8 +837,9 @@ int32_t pk_head_norm_rotary_write(int32_t kind, const uint16_t* query, int64_t q
  * beams + b) and out_ended (the parent had ended, or the token is end_token; may be
  * NULL); where candidates run out score -infinity, token -1, parent -1, ended 0.
  * end_token in [0, vocab), or -1: none (ended is NULL then).  Sums and scores are compared in 64
- * bits, terms of the sums are fp32.  sequences <= 4096, beams <= 32, choices <= 64,
- * vocab <= 2^20.  logits as their type aligned, workspace (16-byte aligned) of
+ * bits, terms of the sums are fp32; equal rows of one call have equal sums, wherever they
+ * lie (a row's sum is cut into parts by the call's sizes).  sequences <= 4096, beams <= 32,
+ * choices <= 64, vocab <= 2^20, at most 2^36 logits.  logits as their type aligned, workspace (16-byte aligned) of
  * pk_beam_select_workspace_bytes (enough also for fewer sequences, beams, tokens and
  * choices), used by one call at a time, need not be kept; outputs and workspace
  * overlap nothing else. */

@@ -1336,6 +1336,10 @@ int32_t pk_beam_select(int32_t kind, const void* logits, int64_t logits_stride, 
         set_error("logits_stride must be at least vocab = %d, got %lld", vocab, (long long)logits_stride);
         return PK_E_SHAPE;
     }
+    if ((int64_t)sequences * beams * vocab > 1ll << 36) {  // a launch has fewer than 2^32 threads
+        set_error("beam search takes at most 2^36 logits (sequences=%d beams=%d vocab=%d)", sequences, beams, vocab);
+        return PK_E_SHAPE;
+    }
     if (end_token < -1 || end_token >= vocab || (ended && end_token < 0)) {
         set_error("end_token must lie in [-1, vocab), and in [0, vocab) with ended beams, got %d", end_token);
         return PK_E_ARG;

@@ -80,6 +80,11 @@ def test_beam_select(want, kw):
     call("pk_beam_select", SELECT, kw, want)
 
 
+@pytest.mark.parametrize("sequences,want", [(4096, SHAPE), (2049, SHAPE), (2048, ARG)])  # the last: only its missing outputs
+def test_beam_select_threads_of_one_launch(sequences, want):
+    call("pk_beam_select", SELECT, dict(sequences=sequences, beams=32, vocab=1 << 20, stride=1 << 20, out_scores=None), want)
+
+
 @pytest.mark.parametrize("want,kw", [
     (SHAPE, {"sequences": 4097}), (SHAPE, {"sequences": -1}), (SHAPE, {"beams": 0}), (SHAPE, {"beams": 33}), (SHAPE, {"row": -1}),
     (SHAPE, {"row": (1 << 32) + 1}), (ARG, {"state": None}), (ARG, {"parents": None}), (ARG, {"output": None}), (ALIGN, {"parents": at(1) + 1}),
