@@ -192,6 +192,8 @@ template <int kD, bool kF8> __global__ __launch_bounds__(256) void paged_cache_w
 // 15.8 against 11.2 / 10.2, 16000 117 / 130 against 28 / 38, 3.5 TB/s).  What tiles are short of
 // a copy's rate is a chain: a border's slot, then the rows, then the stores, in workgroups that
 // the GPU holds hardly more than once over, so that reading and writing barely overlap.
+constexpr int kTileTokens = 1536;
+
 template <int kD, bool kF8> static void launch_write(const WriteArgs& a, hipStream_t s) {
     if (a.tokens < kTileTokens) {
         const unsigned grid = (unsigned)(((long long)a.tokens * a.kv_heads * (kD / 8) + 255) / 256);

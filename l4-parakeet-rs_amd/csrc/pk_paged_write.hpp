@@ -128,7 +128,4 @@ template <int kD, bool kF8, bool kKeys> __device__ __forceinline__ void write_ti
     }
 }
 
-// From this many tokens on a call is taken to be prompts, written in tiles (figures in pk_paged.hip).
-constexpr int kTileTokens = 1536;
-
 }  // namespace pk

@@ -103,12 +103,17 @@ template <int kPer> __device__ __forceinline__ int plan_rows(const ForkArgs& a, 
         if (lane == 0) wave_total[j * 16 + wave] = __popcll(takes) | (__popcll(real) << 16);
     }
     __syncthreads();
-    int all = 0;
+    static_assert(kPer <= 4);  // a lane a wave's total
+    const int mine = lane < 16 * kPer ? wave_total[lane] : 0;
+    int sums = mine;
 #pragma unroll
-    for (int i = 0; i < 16 * kPer; ++i) {
-        if (i % 16 == wave) before[i / 16] += all & 0xffff;
-        all += wave_total[i];
+    for (int off = 1; off < 64; off <<= 1) {
+        const int up = __shfl_up(sums, off, 64);
+        if (lane >= off) sums += up;
     }
+    const int all = __builtin_amdgcn_readlane(sums, 63);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) before[j] += __builtin_amdgcn_readlane(sums - mine, __builtin_amdgcn_readfirstlane(j * 16 + wave)) & 0xffff;
     const int taken = all & 0xffff, forked = all >> 16;
     if (!status && taken > 0 && taken > (long long)end - begin) status = 1;
     const int failed = status ? -1 : 0;

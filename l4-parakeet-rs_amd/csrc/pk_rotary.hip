@@ -12,6 +12,10 @@
 // A lane holds 16 features of a head, and in either layout both halves of 8 pairs with the
 // same 8 frequencies; head_dim / 16 lanes make a head.  Everything between the loads and the
 // one rounding at the store is fp32.
+//
+// Bound by HBM: 16000 tokens, 32 / 8 heads of 128, rows to rows (328 MB) 61.6 us, 5.3 TB/s; with keys
+// and values into an fp16 cache (393 MB) 77 us, 5.1 TB/s.  One token 2.9 us, about a launch; 61 into an
+// e4m3 cache 4.7 us: a load, the angles, and values that lie in as many rows of a page as they are.
 #include <math.h>
 
 #include "pk_paged_write.hpp"
@@ -77,7 +81,7 @@ __global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int
         }
     }
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, p = lane % kLanes, place = lane / kLanes;
-    const int unit = (int)(blockIdx.x - value_blocks) * 4 + wave, t = unit / parts;  // (below 2^31: at most 2^21 tokens of 8192 / tokens parts)
+    const int unit = (int)(blockIdx.x - value_blocks) * 4 + wave, t = unit / parts;  // (at most 2^21 tokens, or kMostSetWaves)
     const int query_sets = (a.heads + kSlots - 1) / kSlots, kv_sets = (a.kv_heads + kSlots - 1) / kSlots;
     const int all = query_sets + kv_sets + (kCache >= 0 && value_blocks == 0 ? kv_sets : 0);
     const int first = unit % parts * sets, stop = first + sets < all ? first + sets : all;
@@ -201,13 +205,21 @@ __global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int
     }
 }
 
+// From this many tokens on the values of a call go in tiles (32 / 8 heads of 128, one prompt, fp16: 600
+// tokens 10.1 us without and 9.4 with, 1000 14.3 and 10.6, 1400 20.3 and 11.7; as many single tokens 10.7
+// and 15.8, 15.0 and 15.9, 22.8 and 17.9; e4m3 like these).
+constexpr int kValueTiles = 768;
+// Up to this many waves a wave takes one set of heads, else all of its token's (rows of fp16: 1500 tokens
+// 10.1 us in 7500 waves and 10.5 in 1500, 3000 14.9 and 13.1).
+constexpr int kMostSetWaves = 8192;
+
 template <int kCache, bool kPast> static void launch_rotary(const RotaryArgs& a, hipStream_t s) {
-    const bool tiles = kCache >= 0 && a.tokens >= kTileTokens;
+    const bool tiles = kCache >= 0 && a.tokens >= kValueTiles;
     const int value_blocks = tiles ? a.kv_heads * ((a.tokens + kWriteTokens - 1) / kWriteTokens) : 0;
     const auto launch = [&](auto kernel, int lanes) {
         const int each = 64 / lanes, kv_sets = (a.kv_heads + each - 1) / each;
         const int all = (a.heads + each - 1) / each + kv_sets + (kCache >= 0 && !tiles ? kv_sets : 0);
-        const int parts = (long long)a.tokens * all <= 8192 ? all : 1, sets = (all + parts - 1) / parts;
+        const int parts = (long long)a.tokens * all <= kMostSetWaves ? all : 1, sets = (all + parts - 1) / parts;
         const unsigned grid = (unsigned)(((long long)a.tokens * parts + 3) / 4 + value_blocks);
         kernel<<<grid, 256, 0, s>>>(a, parts, sets, value_blocks);
     };

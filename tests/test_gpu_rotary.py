@@ -146,7 +146,7 @@ def slots_for(g, tokens, page, pages, how):
 
 @pytest.mark.parametrize("tokens,heads,kv,d,r,page,how", [
     (1, 8, 8, 128, 128, 16, "scattered"), (5, 4, 2, 64, 32, 16, "scattered"), (61, 32, 8, 128, 64, 64, "scattered"), (200, 6, 3, 64, 64, 256, "runs"),
-    (1535, 4, 2, 128, 128, 32, "runs"), (1536, 4, 2, 128, 128, 32, "runs"), (1700, 5, 1, 64, 48, 16, "scattered"), (2500, 4, 4, 64, 64, 128, "runs"),
+    (767, 4, 2, 128, 128, 32, "runs"), (768, 4, 2, 128, 128, 32, "runs"), (800, 3, 2, 64, 32, 16, "scattered"), (1535, 4, 2, 128, 128, 32, "runs"), (1536, 4, 2, 128, 128, 32, "runs"), (1700, 5, 1, 64, 48, 16, "scattered"), (2500, 4, 4, 64, 64, 128, "runs"),
     (3001, 3, 1, 128, 0, 64, "runs"), (9001, 4, 2, 64, 64, 64, "runs")])
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("interleaved", [False, True])
