@@ -17,8 +17,9 @@
 // differences of sums, and a rounding of 2^-24 of a score of -30 would change places of
 // candidates that 64 bits tell apart.
 //
-// Bound by the reading (4.4 TB/s) in wide rows; a call of few is a chain: loads, a maximum
-// and a bisection over lanes, exponentials, the list, the join.
+// Wide rows are bound by vector instructions (some 660 a wave for 64 logits a lane, which keep the SIMDs
+// busy for four fifths of the time) at 4.5 TB/s; a call of few is a chain: loads, a maximum and a
+// bisection over lanes, exponentials, the list, the join.
 #include "pk_kernels.hpp"
 
 namespace pk {
@@ -154,7 +155,7 @@ __device__ __forceinline__ void rank_listed(const PartShared<kGroup>& shared, in
 // `choices` keys, best first, 0 where there are none (`to` null: neither is wanted).  `real` says, behind
 // the loads, whether the row's logits are candidates.
 //
-// Logits are read 16 bytes at once at multiples of 16 (512 rows of 131071 fp16 logits: 30.6 us, 4.4
+// Logits are read 16 bytes at once at multiples of 16 (512 rows of 131071 fp16 logits: 29.4 us, 4.5
 // TB/s; 33.4 with loads that straddle lines); those before the first and behind the last go to single threads.
 // So a logit's thread depends on where its row lies, and the sum must not depend on the threads:
 // equal rows have equal sums, and their candidates are ties.  It is therefore exact: a lane adds its
@@ -218,6 +219,7 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
         }
     };
     constexpr double kNudge = 1.0 + 0x1p-52;
+    static_assert(kLoads * kVec + 1 < 128);  // terms: the sum stays below 512
     double total = __builtin_fma((double)term(extra), kNudge, 384.0);
     uint32_t hits = 0;
 #pragma unroll
@@ -228,12 +230,21 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
     }
     note(extra, extra_at);
     const uint32_t loads = hits;
-    while (hits) {
+    while (hits) {  // most often one logit of a lane
         const int l = __ffs(hits) - 1;
         hits &= hits - 1;
         const v4i v = pick<kLoads>(raw, l);
+        uint32_t which = 0;
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) note(logit_of<kF16>(v, j), place(l, j));
+        for (int j = 0; j < kVec; ++j) which |= logit_of<kF16>(v, j) >= bound ? 1u << j : 0u;
+        int k = atomicAdd(&shared.listed, __popc(which));
+        for (; which; which &= which - 1, ++k) {
+            const int j = __ffs(which) - 1, w = kF16 ? j >> 1 : j;
+            const int word = w & 2 ? (w & 1 ? v[3] : v[2]) : (w & 1 ? v[1] : v[0]);
+            const float one = kF16 ? h2f((uint16_t)((uint32_t)word >> (16 * (j & 1)))) : __int_as_float(word);
+            if (k < kListed) shared.list[k] = key_of(one, place(l, j));
+            else over = 1;
+        }
     }
     const bool odd = __builtin_amdgcn_ballot_w64(total != total) != 0;
     const long long steps = wave_sum(__double_as_longlong(total) - __double_as_longlong(384.0));

@@ -236,7 +236,8 @@ __global__ __launch_bounds__(1024) void fork_plan_kernel(ForkArgs a, RowPlan* __
 // A wave a row and task: as a new one its pages, as an old one its marks, but for those that the row
 // before it (often another beam of the same request) sets.
 __global__ __launch_bounds__(256) void fork_table_kernel(ForkArgs a, const RowPlan* __restrict__ plan, uint8_t* __restrict__ kept, uint8_t* __restrict__ gone) {
-    const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    // neighbouring rows, which list the same pages, on one XCD: workgroups go to the eight in turn
+    const int r = (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (r >= a.rows) return;
     const RowPlan one = plan[r];
     if (blockIdx.y == 0) {
@@ -323,7 +324,7 @@ void launch_page_fork(const ForkArgs& a, hipStream_t s) {
     int* counts = (int*)(plan + a.rows);
     const long long units = mark_bytes(a.pages) / 8, blocks = (units + 1023) / 1024;
     fork_plan_kernel<<<1 + (unsigned)(blocks < 255 ? blocks : 255), 1024, 0, s>>>(a, plan, (uint4*)kept, units);
-    fork_table_kernel<<<dim3((unsigned)(a.rows + 3) / 4, 2), 256, 0, s>>>(a, plan, kept, gone);
+    fork_table_kernel<<<dim3((unsigned)(a.rows + 31) / 32 * 8, 2), 256, 0, s>>>(a, plan, kept, gone);
     fork_count_kernel<<<(unsigned)segments(a.pages), 256, 0, s>>>(a, kept, gone, counts);
     fork_list_kernel<<<(unsigned)segments(a.pages), 256, 0, s>>>(a, kept, gone, counts);
 }
