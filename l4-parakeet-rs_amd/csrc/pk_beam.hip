@@ -6,7 +6,8 @@
 // The logits are read once, in parts of a row that a workgroup holds in registers: the part's
 // maximum, its sum of exponentials, and its best `choices` logits, in order.  A second launch puts
 // a sequence's parts together; short rows of few beams are one launch, whose workgroup does both
-// (8 sequences of 4 beams, 1025 fp32 logits: 8.5 us against 4.8 and 5.0).
+// (8 sequences of 4 beams, 1025 fp32 logits: 7.6 us against 4.8 and 4.5 in two launches; 510 of 16 beams
+// 18.6 against 22.4 and 8.7).
 //
 // The best of a part: a bound is the choices-th largest of the lanes' maxima of any one
 // wave (as many logits at least reach it), found by bisection over the upper bits of the value
@@ -502,7 +503,7 @@ template <bool kF16, int kGroup> __global__ __launch_bounds__(kWholeThreads) voi
 
 // Loads a thread, and with them the parts: many workgroups where rows are few or short, else many
 // loads, which hide what a part begins and ends with (512 rows of 131072 fp16 logits 28.6 us with 8 loads,
-// 32.9 with 4; 32 rows of 131071 8.5 with 2 loads, 64 rows 9.1 with 8).
+// 32.9 with 4, 31 with 16; 32 rows of 131071 7.3 with 2 loads, 64 rows 7.9 with 8).
 constexpr long long kManyVectors = 1 << 20;  // of 16 bytes, of a call
 
 template <bool kF16> static int beam_loads(int rows, int vocab) {
