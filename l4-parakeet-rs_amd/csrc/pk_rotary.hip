@@ -13,9 +13,9 @@
 // same 8 frequencies; head_dim / 16 lanes make a head.  Everything between the loads and the
 // one rounding at the store is fp32.
 //
-// Bound by HBM: 16000 tokens, 32 / 8 heads of 128, rows to rows (328 MB) 61.6 us, 5.3 TB/s; with keys
-// and values into an fp16 cache (393 MB) 77 us, 5.1 TB/s.  One token 2.9 us, about a launch; 61 into an
-// e4m3 cache 4.7 us: a load, the angles, and values that lie in as many rows of a page as they are.
+// Bound by HBM: 16000 tokens, 32 / 8 heads of 128, rows to rows (328 MB) 60 us, 5.5 TB/s; with keys
+// and values into an fp16 cache (393 MB) 76 us, 5.2 TB/s.  One token 2.7 us, about a launch; 61 into an
+// e4m3 cache 4.6 us: a load, the angles, and values that lie in as many rows of a page as they are.
 #include <math.h>
 
 #include "pk_paged_write.hpp"
@@ -33,34 +33,56 @@ __device__ __forceinline__ float2 turned_by(unsigned long long phase, float ampl
     return float2{(quarter + 1) & 2 ? -a * amplitude : a * amplitude, quarter & 2 ? -b * amplitude : b * amplitude};
 }
 
-__device__ __forceinline__ void unpack(const uint4& raw, float (&y)[8]) {
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = h2f((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
-}
+typedef float v2f __attribute__((ext_vector_type(2)));
 
-// kPast: past the caches, for results larger than they are (16000 tokens of 32 / 8 heads of 128 64 us, else 68).
-template <bool kF8, bool kPast> __device__ __forceinline__ void store8(uint8_t* to, const float (&y)[8], float inverse) {
-    uint32_t w[4];
+// A lane's 16 features: u and v of 8 pairs.
+struct Pairs {
+    v4i u, v;
+};
+
+// Neighbours (u0 v0 u1 v1 ..) to (u0 u1 ..), (v0 v1 ..).
+__device__ __forceinline__ void apart(Pairs& x) {
+    const uint32_t w[8] = {(uint32_t)x.u[0], (uint32_t)x.u[1], (uint32_t)x.u[2], (uint32_t)x.u[3],
+                           (uint32_t)x.v[0], (uint32_t)x.v[1], (uint32_t)x.v[2], (uint32_t)x.v[3]};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        if constexpr (kF8) {
-            const uint32_t pair = e4m3x2(y[2 * j] * inverse, y[2 * j + 1] * inverse);
-            if (j & 1) w[j >> 1] |= pair << 16;
-            else w[j >> 1] = pair;
-        } else {
-            w[j] = (uint32_t)f2h(y[2 * j]) | ((uint32_t)f2h(y[2 * j + 1]) << 16);
-        }
+        x.u[j] = (int)__builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100u);
+        x.v[j] = (int)__builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302u);
     }
-    if constexpr (kF8) {
-        const v2i v{(int)w[0], (int)w[1]};
-        if constexpr (kPast) __builtin_nontemporal_store(v, (v2i*)to);
-        else *(v2i*)to = v;
-    } else {
-        const v4i v{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
-        if constexpr (kPast) __builtin_nontemporal_store(v, (v4i*)to);
-        else *(v4i*)to = v;
+}
+// And back.
+__device__ __forceinline__ void together(Pairs& x) {
+    const v4i u = x.u, v = x.v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t a = __builtin_amdgcn_perm((uint32_t)v[j], (uint32_t)u[j], 0x05040100u),
+                       b = __builtin_amdgcn_perm((uint32_t)v[j], (uint32_t)u[j], 0x07060302u);
+        (j < 2 ? x.u : x.v)[2 * (j & 1)] = (int)a;
+        (j < 2 ? x.u : x.v)[2 * (j & 1) + 1] = (int)b;
     }
+}
+
+__device__ __forceinline__ void unpack(const v4i& raw, float (&y)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = h2f((uint16_t)((uint32_t)raw[j >> 1] >> (16 * (j & 1))));
+}
+__device__ __forceinline__ v4i pack(const float (&y)[8]) {
+    v4i w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = __builtin_bit_cast(int, __builtin_convertvector(v2f{y[2 * j], y[2 * j + 1]}, v2h));  // to nearest even, both at once
+    return w;
+}
+
+// kPast: past the caches, for results larger than they are (16000 tokens of 32 / 8 heads of 128 60 us; kept in them 4 us more).
+template <bool kPast, typename T> __device__ __forceinline__ void store(void* to, T v) {
+    if constexpr (kPast) __builtin_nontemporal_store(v, (T*)to);
+    else *(T*)to = v;
+}
+__device__ __forceinline__ v2i e4m3x8(const float (&y)[8], float inverse) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = e4m3x2(y[2 * j] * inverse, y[2 * j + 1] * inverse);
+    return v2i{(int)(w[0] | (w[1] << 16)), (int)(w[2] | (w[3] << 16))};
 }
 
 // kLanes lanes a head (a power of two of at least head_dim / 16), 64 / kLanes heads a set: query sets,
@@ -88,34 +110,27 @@ __global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int
     const bool there = t < a.tokens && first < stop, rotates = there && a.rotary_dim && first < query_sets + kv_sets;
     const bool inside = p * 16 < a.head_dim, turns = p * 16 < a.rotary_dim, halves = turns && !a.interleaved;
     const int f0 = halves ? 8 * p : 16 * p, f1 = halves ? f0 + a.rotary_dim / 2 : f0 + 8;
-    struct Raw {
-        uint4 u, v;
-    };
+    // lanes without a feature or a head read those of the first
+    const int r0 = inside ? f0 : 0, r1 = inside ? f1 : 0;
     const auto ask = [&](int set) {
         const bool query = set < query_sets, value = set >= query_sets + kv_sets;
-        const int h = (query ? set : value ? set - query_sets - kv_sets : set - query_sets) * kSlots + place;
-        const uint16_t* row = query ? a.query + (size_t)t * a.query_stride : value ? a.value + (size_t)t * a.value_stride : a.key + (size_t)t * a.key_stride;
-        Raw raw{};
-        if (inside && h < (query ? a.heads : a.kv_heads)) {
-            raw.u = *(const uint4*)(row + h * a.head_dim + f0);
-            raw.v = *(const uint4*)(row + h * a.head_dim + f1);
-        }
-        return raw;
+        const int h = (query ? set : value ? set - query_sets - kv_sets : set - query_sets) * kSlots + place, n = query ? a.heads : a.kv_heads;
+        const uint16_t* row = (query ? a.query + (size_t)t * a.query_stride : value ? a.value + (size_t)t * a.value_stride : a.key + (size_t)t * a.key_stride) +
+                              (h < n ? h : 0) * a.head_dim;
+        return Pairs{*(const v4i*)(row + r0), *(const v4i*)(row + r1)};
     };
     // all that can be asked for at once: a chain of one load, the angles and the store is left
-    Raw now{};
+    Pairs now{};
     if (there) now = ask(first);
     int slot = 0;
     if constexpr (kCache >= 0) slot = there ? a.slots[t] : -1;
     const long long position = rotates ? a.positions[t] : 0;  // (no rotation: there may be no positions)
     const uint16_t* weight = nullptr;
-    uint4 raw0{}, raw1{};
+    Pairs weights{};
     const auto ask_weight = [&](int set) {
         weight = set < query_sets ? a.query_weight : a.key_weight;
-        if (weight && inside) {
-            raw0 = *(const uint4*)(weight + f0);
-            raw1 = *(const uint4*)(weight + f1);
-        }
+        if (weight) weights = Pairs{*(const v4i*)(weight + r0), *(const v4i*)(weight + r1)};
+        if (a.interleaved) apart(weights);
     };
     if (there) ask_weight(first);
     if (rotates)
@@ -126,13 +141,15 @@ __global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int
 #pragma unroll
     for (int j = 0; j < 8; ++j) angle[j] = turns ? angles[wave][8 * p + j] : float2{1.0f, 0.0f};
     const int off = slot & ((1 << a.shift) - 1);
+    const float per_feature = 1.0f / (float)a.head_dim;
     float w0[8], w1[8];
-    unpack(raw0, w0);
-    unpack(raw1, w1);
+    unpack(weights.u, w0);
+    unpack(weights.v, w1);
     for (int set = first; set < stop; ++set) {
         const bool query = set < query_sets, value = set >= query_sets + kv_sets;
         const int h = (query ? set : value ? set - query_sets - kv_sets : set - query_sets) * kSlots + place;
         const bool mine = inside && h < (query ? a.heads : a.kv_heads);
+        if (a.interleaved && !value) apart(now);
         float u[8], v[8];
         unpack(now.u, u);
         unpack(now.v, v);
@@ -158,17 +175,20 @@ __global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int
         }
         if (set == query_sets && set > first) {
             ask_weight(set);
-            unpack(raw0, w0);
-            unpack(raw1, w1);
+            unpack(weights.u, w0);
+            unpack(weights.v, w1);
         }
         if (weight) {
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(v[j], v[j], __builtin_fmaf(u[j], u[j], sum));
+            sum = inside ? sum : 0.0f;
 #pragma unroll
             for (int o = 1; o < kLanes; o <<= 1) sum = add_level(sum, o);
-            const float mean = sum / (float)a.head_dim + a.epsilon;
-            const float rstd = mean > 0.0f ? 1.0f / sqrtf(mean) : (mean == 0.0f ? 0.0f : mean);  // NaN stays NaN; all zero with eps 0: zeros
+            const float mean = __builtin_fmaf(sum, per_feature, a.epsilon);
+            // the instruction's reciprocal root (1 ulp) for normal numbers; NaN stays NaN; all zero with eps 0: zeros
+            float rstd = __builtin_amdgcn_rsqf(mean);
+            if (!(mean >= 1.17549435e-38f)) rstd = mean > 0.0f ? 1.0f / sqrtf(mean) : (mean == 0.0f ? 0.0f : mean);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 u[j] = u[j] * rstd * w0[j];
@@ -176,31 +196,32 @@ __global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int
             }
         }
         if (turns) {
-            const auto turn = [](float& x, float& y, float2 by) {
-                const float x0 = x;
-                x = __builtin_fmaf(x0, by.x, -(y * by.y));
-                y = __builtin_fmaf(y, by.x, x0 * by.y);
-            };
-            if (a.interleaved) {
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    turn(u[j], u[j + 1], angle[j / 2]);
-                    turn(v[j], v[j + 1], angle[4 + j / 2]);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) turn(u[j], v[j], angle[j]);
+            for (int j = 0; j < 8; ++j) {
+                const float x = u[j];
+                u[j] = __builtin_fmaf(x, angle[j].x, -(v[j] * angle[j].y));
+                v[j] = __builtin_fmaf(v[j], angle[j].x, x * angle[j].y);
             }
         }
         if (!mine) continue;
-        if (kCache < 0 || query) {
-            uint16_t* to = (query ? a.query_out + (size_t)t * a.query_out_stride : a.key_out + (size_t)t * a.key_out_stride) + h * a.head_dim;
-            store8<false, kPast>((uint8_t*)(to + f0), u, 1.0f);
-            store8<false, kPast>((uint8_t*)(to + f1), v, 1.0f);
+        if (kF8 && !query) {  // neighbours: the unrounded features in their order
+            float x[8], y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = a.interleaved ? (j & 1 ? v : u)[j >> 1] : u[j];
+                y[j] = a.interleaved ? (j & 1 ? v : u)[4 + (j >> 1)] : v[j];
+            }
+            uint8_t* to = (uint8_t*)a.key_cache + ((((size_t)(slot >> a.shift) * a.kv_heads + h) << a.shift) + off) * a.head_dim;
+            store<kPast>(to + f0, e4m3x8(x, a.k_inv));
+            store<kPast>(to + f1, e4m3x8(y, a.k_inv));
         } else {
-            uint8_t* to = (uint8_t*)a.key_cache + (((((size_t)(slot >> a.shift) * a.kv_heads + h) << a.shift) + off) * a.head_dim) * (kF8 ? 1 : 2);
-            store8<kF8, kPast>(to + f0 * (kF8 ? 1 : 2), u, a.k_inv);
-            store8<kF8, kPast>(to + f1 * (kF8 ? 1 : 2), v, a.k_inv);
+            Pairs out{pack(u), pack(v)};
+            if (a.interleaved) together(out);
+            uint16_t* to = query        ? a.query_out + (size_t)t * a.query_out_stride + h * a.head_dim
+                           : kCache < 0 ? a.key_out + (size_t)t * a.key_out_stride + h * a.head_dim
+                                        : (uint16_t*)a.key_cache + ((((size_t)(slot >> a.shift) * a.kv_heads + h) << a.shift) + off) * a.head_dim;
+            store<kPast>(to + f0, out.u);
+            store<kPast>(to + f1, out.v);
         }
     }
 }

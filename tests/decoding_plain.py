@@ -41,7 +41,7 @@ def head_norm_rotary(x, weight, positions, words, interleaved, amplitude, eps):
     if weight is not None:
         mean = y.square().mean(2, keepdim=True) + eps
         y = torch.where(mean > 0, y / mean.sqrt(), torch.zeros_like(y)) * weight.double()
-        # a sum of d squares, of which the root keeps half; quotient, root, reciprocal, two products
+        # a sum of d squares over d, of which the root keeps half; reciprocal root within a step (2), two products; at most 6
         rel = ((d + 2) / 2 + 6) * U32
     bound = rel * y.abs()
     if words is None:
