@@ -874,7 +874,8 @@ int32_t pk_beam_reorder(const void* state, const int32_t* parents, void* output,
  * max_pages pages, or a negative free_range[0]); if it is not 0, the new tables and
  * lengths are the old ones, and nothing is taken, copied or given back.
  * pk_page_keep moves the free list behind a fork, or behind a plan, that is kept.
- * Nothing that is read is changed; what is written overlaps nothing else.  rows <=
+ * Rows of the old tables share full pages alone (as this call leaves them).
+ * Nothing that is read is changed; what is written overlaps nothing else.  1 <= rows <=
  * 4096, max_pages * page_size <= 2^30, pages * page_size < 2^31.  workspace (16-byte
  * aligned) of pk_page_fork_workspace_bytes (enough also for fewer rows, columns and
  * pages), used by one call at a time, need not be kept. */
@@ -887,11 +888,11 @@ int32_t pk_page_fork(const int32_t* parents, const int32_t* block_table, const i
 
 /* The free list behind a step that is kept: free_range[0] += info[1] - info[3], and the
  * info[3] pages of freed stand in front of the list, free_pages[free_range[0] ..).
- * info as pk_page_fork or (freed NULL) pk_page_plan wrote it; nothing happens where its status is
- * not 0.  A list in front of which there is no room for all (its pages never came from
- * it) takes the first ones. */
+ * info as pk_page_fork or (freed NULL) pk_page_plan wrote it, freed with room for `pages`; nothing
+ * happens where the status is not 0.  A list in front of which there is no room for all
+ * (its pages never came from it) takes the first ones, as do more than `pages`. */
 int32_t pk_page_keep(const int32_t* info, const int32_t* freed, int32_t* free_pages, int32_t* free_range,
-                     int32_t free_capacity, void* stream);
+                     int32_t free_capacity, int32_t pages, void* stream);
 
 /* Copies of pages: for each pair {source, destination} of copies [count x 2], the keys
  * and values of page source into page destination, in each of `layers` layers

@@ -1439,19 +1439,22 @@ int32_t pk_page_fork(const int32_t* parents, const int32_t* block_table, const i
     return check_launch("page_fork");
 }
 
-int32_t pk_page_keep(const int32_t* info, const int32_t* freed, int32_t* free_pages, int32_t* free_range, int32_t free_capacity, void* stream) {
-    if (free_capacity < 0) { set_error("page_keep needs free_capacity >= 0, got %d", free_capacity); return PK_E_SHAPE; }
+int32_t pk_page_keep(const int32_t* info, const int32_t* freed, int32_t* free_pages, int32_t* free_range, int32_t free_capacity, int32_t pages,
+                     void* stream) {
+    if (free_capacity < 0 || (freed && pages < 0)) {
+        set_error("page_keep needs free_capacity and pages >= 0 (free_capacity=%d pages=%d)", free_capacity, pages);
+        return PK_E_SHAPE;
+    }
     if (!need(info, "info") || !need(free_range, "free_range") || (free_capacity && !need(free_pages, "free_pages"))) return PK_E_ARG;
     for (const void* p : {(const void*)info, (const void*)freed, (const void*)free_pages, (const void*)free_range})
         if (misaligned(p, 4)) { set_error("page_keep arrays must be 4-byte aligned"); return PK_E_ALIGN; }
-    // of freed as many entries as the list holds are read at most
-    const size_t n = 4 * (size_t)free_capacity;
-    if (overlap(free_pages, n, info, 16) || overlap(free_pages, n, freed, n) || overlap(free_pages, n, free_range, 8) || overlap(free_range, 8, info, 16) ||
-        overlap(free_range, 8, freed, n)) {
+    const size_t n = 4 * (size_t)free_capacity, m = freed ? 4 * (size_t)pages : 0;
+    if (overlap(free_pages, n, info, 16) || overlap(free_pages, n, freed, m) || overlap(free_pages, n, free_range, 8) || overlap(free_range, 8, info, 16) ||
+        overlap(free_range, 8, freed, m)) {
         set_error("page_keep: the free list overlaps another array");
         return PK_E_ARG;
     }
-    launch_page_keep(info, freed, free_pages, free_range, free_capacity, STREAM);
+    launch_page_keep(info, freed, free_pages, free_range, free_capacity, pages, STREAM);
     return check_launch("page_keep");
 }
 

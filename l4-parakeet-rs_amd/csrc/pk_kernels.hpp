@@ -162,7 +162,7 @@ struct ForkArgs {
 constexpr int kMostForkRows = 4096;  // what a row's children are lies in LDS
 size_t fork_workspace(int rows, int pages);
 void launch_page_fork(const ForkArgs& args, hipStream_t s);
-void launch_page_keep(const int* info, const int* freed, int* free_pages, int* free_range, int free_capacity, hipStream_t s);
+void launch_page_keep(const int* info, const int* freed, int* free_pages, int* free_range, int free_capacity, int pages, hipStream_t s);
 void launch_paged_cache_copy(const int* copies, int count, void* key_cache, void* value_cache, long long page_bytes, int pages, int layers, hipStream_t s);
 void set_error(const char* fmt, ...);
 int cu_count();

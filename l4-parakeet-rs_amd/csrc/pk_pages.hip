@@ -332,11 +332,12 @@ void launch_page_fork(const ForkArgs& a, hipStream_t s) {
 // The free list behind a plan or a fork that is kept: pages taken leave its front, pages that
 // went back stand there.
 __global__ __launch_bounds__(256) void page_keep_kernel(const int* __restrict__ info, const int* __restrict__ freed, int* __restrict__ free_pages,
-                                                        int* free_range, int free_capacity) {
+                                                        int* free_range, int free_capacity, int pages) {
     if (info[2]) return;
     const int begin = free_range[0] + info[1];
     if (begin < 0) return;
     int back = freed ? info[3] : 0;
+    back = back < 0 ? 0 : back < pages ? back : pages;
     back = back < begin ? back : begin;  // a list that gave out what the tables hold has room for all
     __syncthreads();
     for (int i = threadIdx.x; i < back; i += 256)
@@ -344,8 +345,8 @@ __global__ __launch_bounds__(256) void page_keep_kernel(const int* __restrict__ 
     if (threadIdx.x == 0) free_range[0] = begin - back;
 }
 
-void launch_page_keep(const int* info, const int* freed, int* free_pages, int* free_range, int free_capacity, hipStream_t s) {
-    page_keep_kernel<<<1, 256, 0, s>>>(info, freed, free_pages, free_range, free_capacity);
+void launch_page_keep(const int* info, const int* freed, int* free_pages, int* free_range, int free_capacity, int pages, hipStream_t s) {
+    page_keep_kernel<<<1, 256, 0, s>>>(info, freed, free_pages, free_range, free_capacity, pages);
 }
 
 // Pairs (source, destination) of pages in all layers' keys and values.  Bound by HBM: 1434 pages of

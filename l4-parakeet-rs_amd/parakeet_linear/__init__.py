@@ -136,7 +136,7 @@ SIGNATURES = {
     "pk_beam_reorder": (I, [P, P, P, I, I, I64, P]),
     "pk_page_fork_workspace_bytes": (I64, [I, I, I]),
     "pk_page_fork": (I, [P, P, P, P, P, I, P, P, P, P, P, P, I, I, I, I, P, U64, P]),
-    "pk_page_keep": (I, [P, P, P, P, I, P]),
+    "pk_page_keep": (I, [P, P, P, P, I, I, P]),
     "pk_paged_cache_copy": (I, [P, I, P, P, I64, I, I, P]),
 }
 
@@ -862,12 +862,12 @@ def page_keep(info, freed, free_pages, free_range, stream=None):
     i32 = torch.int32
     if not (all(t is None or (t.dtype is i32 and t.is_contiguous() and t.get_device() == device) for t in (info, freed, free_pages, free_range))
             and info.shape == (4,) and free_range.shape == (2,) and free_pages.dim() == 1 and (freed is None or freed.dim() == 1)
-            and not free_pages.numel() >> 31):
+            and not (free_pages.numel() | (0 if freed is None else freed.numel())) >> 31):
         i32 = (i32,)
         _refuse("page_keep", device, ("info", info, i32, (4,), True), ("freed", freed, i32, None if freed is None else (freed.numel(),), True),
                 ("free_pages", free_pages, i32, (free_pages.numel(),), True), ("free_range", free_range, i32, (2,), True))
     _done("pk_page_keep", lib.pk_page_keep(info.data_ptr(), None if freed is None else freed.data_ptr(), free_pages.data_ptr(), free_range.data_ptr(),
-                                           free_pages.numel(), stream))
+                                           free_pages.numel(), 0 if freed is None else freed.numel(), stream))
 
 
 def paged_cache_copy(copies, key_cache, value_cache, stream=None):

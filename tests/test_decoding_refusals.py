@@ -110,10 +110,10 @@ def test_page_fork(want, kw):
 
 
 @pytest.mark.parametrize("want,kw", [
-    (SHAPE, {"capacity": -1}), (ARG, {"info": None}), (ARG, {"free": None}), (ARG, {"range": None}), (ALIGN, {"freed": at(1) + 2}),
+    (SHAPE, {"capacity": -1}), (SHAPE, {"pages": -1}), (ARG, {"info": None}), (ARG, {"free": None}), (ARG, {"range": None}), (ALIGN, {"freed": at(1) + 2}),
     (ARG, {"free": at(0) - 4}), (ARG, {"freed": at(2) + 396}), (ARG, {"range": at(0) + 12}), (ARG, {"range": at(2)})])
 def test_page_keep(want, kw):
-    call("pk_page_keep", dict(info=at(0), freed=at(1), free=at(2), range=at(3), capacity=100), kw, want)
+    call("pk_page_keep", dict(info=at(0), freed=at(1), free=at(2), range=at(3), capacity=100, pages=100), kw, want)
 
 
 @pytest.mark.parametrize("want,kw", [

@@ -160,6 +160,9 @@ def test_keep(pk):  # noqa: F811
     assert run([0, 1, 0, 3], 10) == (base[:8] + [7, 8, 9] + base[11:], [8, 30])
     assert run([0, 5, 0, 5], 0) == ([7, 8, 9, 50, 51] + base[5:], [0, 30])
     assert run([0, 1, 0, 5], 1) == ([7, 8] + base[2:], [0, 30])  # room for two
+    assert run([0, 1, 0, 9], 10) == (base[:6] + [7, 8, 9, 50, 51] + base[11:], [6, 30])  # more than freed holds
+    assert run([0, 1, 0, -2], 10) == (base, [11, 30])
+    assert run([0, 1, 0, 3], 10, freed[:0]) == (base, [11, 30])
 
 
 def test_keep_many(pk):  # noqa: F811
