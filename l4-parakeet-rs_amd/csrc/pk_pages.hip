@@ -6,15 +6,18 @@
 // its own from the free list and a pair (page, new page) to be copied.
 //
 // A page goes back if a row without children listed it and no row with children does: marks
-// are bytes that any number of rows set to 1, so their order does not matter, and the pages
-// that go back are listed in ascending order.
+// are bits that any number of rows set, and then any number clear, so their order does not
+// matter, and the pages that go back are listed in ascending order.
+#include <type_traits>
+
 #include "pk_kernels.hpp"
 
 namespace pk {
 
-// Small tables are one workgroup's, with the marks as bits in LDS.  Large ones take four launches:
-// children, copies and lengths (and the marks cleared); tables and marks; how many pages of each
-// 4096 go back; their list.  Bound by latency: each launch is a chain of a few dependent loads.
+// Small tables are one workgroup's, with the marks in LDS.  Large ones take four launches: marks cleared;
+// children, copies and lengths, and marks of what rows without children list; tables, and marks cleared of
+// what rows with children list; the list.  Bound by latency: each launch is a chain of a few dependent loads
+// (4096 rows of 501 entries over 1.29 M pages 2.1 + 8.8 + 5.5 + 4.8 us).
 struct RowPlan {
     int parent;     // the row whose pages it takes; -1: none
     int last;       // the page in the last column if it is not the parent's; -1
@@ -26,15 +29,21 @@ __device__ __forceinline__ int pages_of(const ForkArgs& a, int length) {
     return n < a.max_pages ? n : a.max_pages;  // (a length that is refused)
 }
 
-// Inclusive scan over 1024 threads; `all` is the total.
-__device__ __forceinline__ int scan_1024(int v, int* wave_total, int& all) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Inclusive sum over a wave's lanes.
+__device__ __forceinline__ int wave_scan(int v) {
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
         const int up = __shfl_up(v, off, 64);
-        if (lane >= off) v += up;
+        if ((int)(threadIdx.x & 63) >= off) v += up;
     }
-    if (lane == 63) wave_total[wave] = v;
+    return v;
+}
+
+// Inclusive scan over 1024 threads; `all` is the total.
+__device__ __forceinline__ int scan_1024(int v, int* wave_total, int& all) {
+    const int wave = threadIdx.x >> 6;
+    v = wave_scan(v);
+    if ((threadIdx.x & 63) == 63) wave_total[wave] = v;
     __syncthreads();
     all = 0;
 #pragma unroll
@@ -82,17 +91,15 @@ template <int kPer> __device__ __forceinline__ int plan_rows(const ForkArgs& a, 
     if (bad) atomicOr(flags, bad);
     __syncthreads();
     int status = *flags | (begin < 0 ? 8 : 0);
+    bool copied[kPer];
     if (!status) {
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-            const int c = length[j] >> a.shift;  // (of lengths that are all right)
-            source[j] = a.table[(size_t)(parent[j] >= 0 ? parent[j] : 0) * a.max_pages + (c < a.max_pages ? c : 0)];
+            copied[j] = parent[j] >= 0 && length[j] & (page - 1) && eldest[parent[j] >= 0 ? parent[j] : 0] != j * 1024 + tid;
+            source[j] = a.table[copied[j] ? (size_t)parent[j] * a.max_pages + (length[j] >> a.shift) : 0];  // (lengths are all right)
         }
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const bool copied = parent[j] >= 0 && length[j] & (page - 1) && eldest[parent[j] >= 0 ? parent[j] : 0] != j * 1024 + tid;
-            source[j] = copied && source[j] >= 0 && source[j] < a.pages ? source[j] : -1;
-        }
+        for (int j = 0; j < kPer; ++j) source[j] = copied[j] && source[j] >= 0 && source[j] < a.pages ? source[j] : -1;
     }
     // rows before this one that take a page: in its wave, and in the waves of lower rows; both counts are at most 4096
     int before[kPer];
@@ -105,12 +112,7 @@ template <int kPer> __device__ __forceinline__ int plan_rows(const ForkArgs& a, 
     __syncthreads();
     static_assert(kPer <= 4);  // a lane a wave's total
     const int mine = lane < 16 * kPer ? wave_total[lane] : 0;
-    int sums = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int up = __shfl_up(sums, off, 64);
-        if (lane >= off) sums += up;
-    }
+    const int sums = wave_scan(mine);
     const int all = __builtin_amdgcn_readlane(sums, 63);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) before[j] += __builtin_amdgcn_readlane(sums - mine, __builtin_amdgcn_readfirstlane(j * 16 + wave)) & 0xffff;
@@ -128,12 +130,12 @@ template <int kPer> __device__ __forceinline__ int plan_rows(const ForkArgs& a, 
     for (int j = 0; j < kPer; ++j) {
         const int r = j * 1024 + tid;
         if (there(j)) {
-            const bool copied = !status && source[j] >= 0;
+            const bool new_page = !status && source[j] >= 0;
             plan[r].parent = status ? r : parent[j];
-            plan[r].last = copied ? to[j] : -1;
+            plan[r].last = new_page ? to[j] : -1;
             plan[r].has_child = status || eldest[r] < a.rows;
-            a.copies[2 * r] = copied ? source[j] : -1;
-            a.copies[2 * r + 1] = copied ? to[j] : -1;
+            a.copies[2 * r] = new_page ? source[j] : -1;
+            a.copies[2 * r + 1] = new_page ? to[j] : -1;
             a.new_lengths[r] = (own[j] & failed) | (length[j] & ~failed);
         }
     }
@@ -146,27 +148,31 @@ template <int kPer> __device__ __forceinline__ int plan_rows(const ForkArgs& a, 
     return status;
 }
 
-// A row's entries by a wave; of long rows eight a lane at once, all asked for before the first is used
-// (`other`: a second row that is read beside it up to `others`).
-template <typename Use> __device__ __forceinline__ void each_entry(const int* row, const int* other, int others, int count, int lane, Use use) {
-    if (count <= 256) {
-        for (int c = lane; c < count; c += 64) {
-            const int id = row[c];
-            use(c, id, c < others ? other[c] : -1);
-        }
-        return;
-    }
-    for (int first = lane; first < count; first += 512) {
-        int id[8], beside[8];
+// A row's entries by a wave; of long rows eight a lane at once, all asked for before the first is used, beside
+// those of two other rows up to their counts (else -1).
+struct Beside {
+    const int* row;
+    int count;
+};
+template <typename Use> __device__ __forceinline__ void each_entry(const int* row, int count, Beside x, Beside y, int lane, Use use) {
+    const auto some = [&](int first, auto per) {
+        constexpr int kPer = decltype(per)::value;
+        int id[kPer], ix[kPer], iy[kPer];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
+        for (int n = 0; n < kPer; ++n) {
             const int c = first + 64 * n < count ? first + 64 * n : first;
             id[n] = row[c];
-            beside[n] = c < others ? other[c] : -1;
+            ix[n] = c < x.count ? x.row[c] : -1;
+            iy[n] = c < y.count ? y.row[c] : -1;
         }
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
-            if (first + 64 * n < count) use(first + 64 * n, id[n], beside[n]);
+        for (int n = 0; n < kPer; ++n)
+            if (first + 64 * n < count) use(first + 64 * n, id[n], ix[n], iy[n]);
+    };
+    if (count <= 256) {
+        for (int c = lane; c < count; c += 64) some(c, std::integral_constant<int, 1>{});
+    } else {
+        for (int c = lane; c < count; c += 512) some(c, std::integral_constant<int, 8>{});
     }
 }
 
@@ -175,8 +181,8 @@ __device__ __forceinline__ void new_row(const ForkArgs& a, int r, const RowPlan&
     if (one.parent < 0) return;
     const int count = pages_of(a, length);
     int* to = a.new_table + (size_t)r * a.max_pages;
-    each_entry(a.table + (size_t)one.parent * a.max_pages, nullptr, 0, count, lane,
-               [&](int c, int id, int) { to[c] = c == count - 1 && one.last >= 0 ? one.last : id; });
+    each_entry(a.table + (size_t)one.parent * a.max_pages, count, Beside{}, Beside{}, lane,
+               [&](int c, int id, int, int) { to[c] = c == count - 1 && one.last >= 0 ? one.last : id; });
 }
 
 constexpr int kSmallRows = 1024, kSmallEntries = 1 << 14, kSmallPages = 1 << 17;
@@ -197,7 +203,7 @@ __global__ __launch_bounds__(1024) void fork_small_kernel(ForkArgs a) {
         new_row(a, r, one, a.lengths[one.parent >= 0 ? one.parent : r], lane);
         if (status) continue;  // nothing goes back
         uint32_t* mark = one.has_child ? kept : gone;
-        each_entry(a.table + (size_t)r * a.max_pages, nullptr, 0, pages_of(a, own), lane, [&](int, int id, int) {
+        each_entry(a.table + (size_t)r * a.max_pages, pages_of(a, own), Beside{}, Beside{}, lane, [&](int, int id, int, int) {
             if (id >= 0 && id < a.pages) atomicOr(&mark[id >> 5], 1u << (id & 31));
         });
     }
@@ -222,20 +228,50 @@ __global__ __launch_bounds__(1024) void fork_small_kernel(ForkArgs a) {
     if (threadIdx.x == 0) a.info[3] = all;
 }
 
-// Workgroup 0 plans the rows; the others clear the marks.
-__global__ __launch_bounds__(1024) void fork_plan_kernel(ForkArgs a, RowPlan* __restrict__ plan, uint4* __restrict__ marks, long long mark_units) {
+__global__ __launch_bounds__(256) void fork_clear_kernel(v4i* gone, int units) {
+    const int i = (int)blockIdx.x * 256 + threadIdx.x;
+    if (i < units) gone[i] = v4i{};
+}
+
+// Workgroup 0 plans the rows; the others mark what rows without children list, a wave a row.  Most of that
+// is also in the next row with children, of another beam of the same request, above or below it: those
+// entries are passed over (marked, they would be cleared again).  The rest, pages of a beam of its own, are
+// 3 of the 9 us of 4096 rows of 501 entries: an atomic each, as the bits of a word are many rows'.
+__global__ __launch_bounds__(1024) void fork_plan_kernel(ForkArgs a, RowPlan* __restrict__ plan, uint32_t* __restrict__ gone) {
     __shared__ int eldest[kMostForkRows];
     __shared__ int wave_total[kMostForkRows / 64], flags;
     if (blockIdx.x == 0) {
         plan_rows<kMostForkRows / 1024>(a, eldest, wave_total, &flags, plan);
-    } else {
-        for (long long i = (long long)(blockIdx.x - 1) * 1024 + threadIdx.x; i < mark_units; i += (long long)(gridDim.x - 1) * 1024) marks[i] = uint4{};
+        return;
     }
+    uint8_t* has_child = (uint8_t*)eldest;
+    const int r = __builtin_amdgcn_readfirstlane((int)(blockIdx.x - 1) * 16 + (int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    int parent[kMostForkRows / 1024];
+#pragma unroll
+    for (int j = 0; j < kMostForkRows / 1024; ++j) {
+        const int i = j * 1024 + threadIdx.x;
+        parent[j] = i < a.rows ? a.parents[i] : -1;
+        eldest[j * 256 + (threadIdx.x >> 2)] = 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kMostForkRows / 1024; ++j)
+        if (parent[j] >= 0 && parent[j] < a.rows) has_child[parent[j]] = 1;
+    __syncthreads();
+    if (r >= a.rows || has_child[r]) return;
+    const int near = r - 32 + lane;
+    const unsigned long long with = __builtin_amdgcn_ballot_w64(near >= 0 && near < a.rows && has_child[near >= 0 && near < a.rows ? near : 0]);
+    const uint32_t lower = (uint32_t)with, upper = (uint32_t)(with >> 32);
+    const int above = lower ? r - 1 - __clz(lower) : r, below = upper ? r - 1 + __ffs(upper) : r;
+    const auto beside = [&](int other) { return Beside{a.table + (size_t)other * a.max_pages, other == r ? 0 : pages_of(a, a.lengths[other])}; };
+    each_entry(a.table + (size_t)r * a.max_pages, pages_of(a, a.lengths[r]), beside(above), beside(below), lane, [&](int, int id, int x, int y) {
+        if (id >= 0 && id < a.pages && id != x && id != y && !(a.held && a.held[id])) atomicOr(&gone[id >> 5], 1u << (id & 31));
+    });
 }
 
-// A wave a row and task: as a new one its pages, as an old one its marks, but for those that the row
-// before it (often another beam of the same request) sets.
-__global__ __launch_bounds__(256) void fork_table_kernel(ForkArgs a, const RowPlan* __restrict__ plan, uint8_t* __restrict__ kept, uint8_t* __restrict__ gone) {
+// A wave a row and task: as a new one its pages, as an old one with children their marks cleared, but for
+// those that the row above clears.
+__global__ __launch_bounds__(256) void fork_table_kernel(ForkArgs a, const RowPlan* __restrict__ plan, uint32_t* gone) {
     // neighbouring rows, which list the same pages, on one XCD: workgroups go to the eight in turn
     const int r = (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (r >= a.rows) return;
@@ -244,73 +280,60 @@ __global__ __launch_bounds__(256) void fork_table_kernel(ForkArgs a, const RowPl
         new_row(a, r, one, a.new_lengths[r], lane);
         return;
     }
-    const int own = a.lengths[r], above = r > 0 ? a.lengths[r - 1] : 0, failed = a.info[2];
-    if (failed) return;  // nothing goes back
-    const int before = r > 0 && plan[r - 1].has_child == one.has_child ? pages_of(a, above) : 0;
-    const int* mine = a.table + (size_t)r * a.max_pages;
-    uint8_t* mark = one.has_child ? kept : gone;
-    each_entry(mine, mine - a.max_pages, before, pages_of(a, own), lane, [&](int, int id, int beside) {
-        if (id >= 0 && id < a.pages && id != beside) mark[id] = 1;
+    if (!one.has_child) return;
+    const int own = a.lengths[r], up = r > 0 ? r - 1 : 0, up_length = a.lengths[up];
+    const Beside above{a.table + (size_t)up * a.max_pages, r > 0 && plan[up].has_child ? pages_of(a, up_length) : 0};
+    each_entry(a.table + (size_t)r * a.max_pages, pages_of(a, own), above, Beside{}, lane, [&](int, int id, int x, int) {
+        if (id >= 0 && id < a.pages && id != x && gone[id >> 5] >> (id & 31) & 1) atomicAnd(&gone[id >> 5], ~(1u << (id & 31)));
     });
 }
 
-constexpr int kPageSegment = 4096;  // pages a workgroup of the last two launches, 16 a thread
+constexpr int kListWords = 1024;  // a workgroup of the list: a word of 32 pages a thread
+// Up to this many workgroups each counts what goes back before its words by itself, else a launch counts first
+// (1.3 M pages 4.8 us by themselves and 2.3 + 4.0 with a launch, 2.9 M 5.5 and 3.9 + 4.1, 4.5 M 7.2 and 4.6 + 4.0).
+constexpr int kMostCounting = 128;
 
-// A thread's 16 pages as bytes: 1 for those that go back.  (Marks reach to a multiple of 16 pages.)
-__device__ __forceinline__ uint4 going(const ForkArgs& a, const uint8_t* kept, const uint8_t* gone, long long page0) {
-    if (page0 >= a.pages) return uint4{};
-    const uint4 k = *(const uint4*)(kept + page0), g = *(const uint4*)(gone + page0);
-    uint32_t w[4] = {g.x & ~k.x, g.y & ~k.y, g.z & ~k.z, g.w & ~k.w};
-    if (a.held && (w[0] | w[1] | w[2] | w[3]))
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (w[i >> 2] >> (8 * (i & 3)) & 1u && a.held[page0 + i]) w[i >> 2] &= ~(1u << (8 * (i & 3)));
-    return uint4{w[0], w[1], w[2], w[3]};
-}
-__device__ __forceinline__ int count_of(const uint4& w) { return __popc(w.x) + __popc(w.y) + __popc(w.z) + __popc(w.w); }
-
-__global__ __launch_bounds__(256) void fork_count_kernel(ForkArgs a, const uint8_t* __restrict__ kept, const uint8_t* __restrict__ gone, int* __restrict__ counts) {
-    __shared__ int sum;
-    if (threadIdx.x == 0) sum = 0;
-    __syncthreads();
-    const int n = count_of(going(a, kept, gone, ((long long)blockIdx.x * 256 + threadIdx.x) * 16));
-    if (n) atomicAdd(&sum, n);
-    __syncthreads();
-    if (threadIdx.x == 0) counts[blockIdx.x] = sum;
+__global__ __launch_bounds__(kListWords) void fork_count_kernel(const uint32_t* __restrict__ gone, int words, int* __restrict__ counts) {
+    __shared__ int wave_total[16];
+    const int i = (int)blockIdx.x * kListWords + threadIdx.x;
+    int all;
+    scan_1024(i < words ? __popc(gone[i]) : 0, wave_total, all);
+    if (threadIdx.x == 0) counts[blockIdx.x] = all;
 }
 
-__global__ __launch_bounds__(256) void fork_list_kernel(ForkArgs a, const uint8_t* __restrict__ kept, const uint8_t* __restrict__ gone, const int* __restrict__ counts) {
-    __shared__ int before, wave_total[4];
-    const long long page0 = ((long long)blockIdx.x * 256 + threadIdx.x) * 16;
-    const uint4 back = going(a, kept, gone, page0);
-    if (threadIdx.x == 0) before = 0;
-    __syncthreads();
+__global__ __launch_bounds__(kListWords) void fork_list_kernel(ForkArgs a, const uint32_t* __restrict__ gone, int words, const int* __restrict__ counts) {
+    __shared__ int wave_total[16], wave_before[16];
+    const int i = (int)blockIdx.x * kListWords + threadIdx.x;
+    uint32_t back = i < words ? gone[i] : 0;
+    const int failed = a.info[2];  // nothing goes back
     int n = 0;
-    for (int i = threadIdx.x; i < (int)blockIdx.x; i += 256) n += counts[i];
-    if (n) atomicAdd(&before, n);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = count_of(back);
-    int v = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int up = __shfl_up(v, off, 64);
-        if (lane >= off) v += up;
+    if (counts) {
+        for (int k = threadIdx.x; k < (int)blockIdx.x; k += kListWords) n += counts[k];
+    } else {
+        const int units = (int)blockIdx.x * (kListWords / 4);
+#pragma unroll 4
+        for (int k = threadIdx.x; k < units; k += kListWords) {
+            const uint4 x = ((const uint4*)gone)[k];
+            n += __popc(x.x) + __popc(x.y) + __popc(x.z) + __popc(x.w);
+        }
     }
-    if (lane == 63) wave_total[wave] = v;
-    __syncthreads();
-    int at = before + v - mine;
-    for (int w = 0; w < wave; ++w) at += wave_total[w];
-    const uint32_t words[4] = {back.x, back.y, back.z, back.w};
+    if (failed) return;
+    n = wave_scan(n);
+    if ((threadIdx.x & 63) == 63) wave_before[threadIdx.x >> 6] = n;
+    const int mine = __popc(back);
+    int all, before = 0;
+    int at = scan_1024(mine, wave_total, all) - mine;  // (its barrier is also wave_before's)
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
-        for (uint32_t left = words[w]; left; left &= left - 1) a.freed[at++] = (int)page0 + 4 * w + (__ffs(left) - 1) / 8;
-    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) a.info[3] = before + wave_total[0] + wave_total[1] + wave_total[2] + wave_total[3];
+    for (int w = 0; w < 16; ++w) before += wave_before[w];
+    for (at += before; back; back &= back - 1) a.freed[at++] = i * 32 + __ffs(back) - 1;
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) a.info[3] = before + all;
 }
 
-static long long mark_bytes(int pages) { return ((long long)pages + 15) / 16 * 16; }  // of one of the two
-static int segments(int pages) { return (int)(((long long)pages + kPageSegment - 1) / kPageSegment); }
+static int mark_words(int pages) { return (int)(((long long)pages + 127) / 128 * 4); }
+static int segments(int pages) { return (mark_words(pages) + kListWords - 1) / kListWords; }
 
 size_t fork_workspace(int rows, int pages) {
-    return (size_t)mark_bytes(pages) * 2 + (size_t)rows * sizeof(RowPlan) + (size_t)segments(pages) * 4;
+    return (size_t)mark_words(pages) * 4 + (size_t)rows * sizeof(RowPlan) + (size_t)segments(pages) * 4;
 }
 
 void launch_page_fork(const ForkArgs& a, hipStream_t s) {
@@ -318,15 +341,16 @@ void launch_page_fork(const ForkArgs& a, hipStream_t s) {
         fork_small_kernel<<<1, 1024, (size_t)(a.pages + 31) / 32 * 8, s>>>(a);
         return;
     }
-    uint8_t* kept = (uint8_t*)a.workspace;
-    uint8_t* gone = kept + mark_bytes(a.pages);
-    RowPlan* plan = (RowPlan*)(gone + mark_bytes(a.pages));
+    const int words = mark_words(a.pages), blocks = segments(a.pages);
+    uint32_t* gone = (uint32_t*)a.workspace;
+    RowPlan* plan = (RowPlan*)(gone + words);
     int* counts = (int*)(plan + a.rows);
-    const long long units = mark_bytes(a.pages) / 8, blocks = (units + 1023) / 1024;
-    fork_plan_kernel<<<1 + (unsigned)(blocks < 255 ? blocks : 255), 1024, 0, s>>>(a, plan, (uint4*)kept, units);
-    fork_table_kernel<<<dim3((unsigned)(a.rows + 31) / 32 * 8, 2), 256, 0, s>>>(a, plan, kept, gone);
-    fork_count_kernel<<<(unsigned)segments(a.pages), 256, 0, s>>>(a, kept, gone, counts);
-    fork_list_kernel<<<(unsigned)segments(a.pages), 256, 0, s>>>(a, kept, gone, counts);
+    fork_clear_kernel<<<(unsigned)(words / 4 + 255) / 256, 256, 0, s>>>((v4i*)gone, words / 4);
+    fork_plan_kernel<<<1 + (unsigned)(a.rows + 15) / 16, 1024, 0, s>>>(a, plan, gone);
+    fork_table_kernel<<<dim3((unsigned)(a.rows + 31) / 32 * 8, 2), 256, 0, s>>>(a, plan, gone);
+    if (blocks > kMostCounting) fork_count_kernel<<<blocks, kListWords, 0, s>>>(gone, words, counts);
+    else counts = nullptr;
+    fork_list_kernel<<<blocks, kListWords, 0, s>>>(a, gone, words, counts);
 }
 
 // The free list behind a plan or a fork that is kept: pages taken leave its front, pages that

@@ -125,6 +125,25 @@ def test_fork_of_large_pools(pk, pages):  # noqa: F811
     pool.go(pk, [-1, -1, -1])
 
 
+@pytest.mark.parametrize("pages", [(1 << 17) + 1, 200003, (1 << 21) - 31, 1 << 21, (1 << 21) + 1])
+def test_fork_of_pools_listed_by_several_workgroups(pk, pages):  # noqa: F811
+    rng = random.Random(pages)
+    rows, columns, page = 24, 90, 32
+    pool = Pool(rng, rows, columns, page)
+    some = sorted({0, 31, 32, 127, 32767, 32768, 65535, 65536, 98304, pages - 1, pages - 2} | set(rng.sample(range(pages), rows * columns)))
+    ids = some[:11] + some[-11:] + some[11:-11]
+    pool.table = [[ids[(r * columns + c) % len(ids)] if c < -(-n // page) else -7 for c in range(columns)] for r, n in enumerate(pool.lengths)]
+    pool.free, pool.begin, pool.end, pool.pages = [i for i in range(50000, 50100)], 2, 100, pages
+    pool.go(pk, [-1] * rows)
+    for _ in range(2):
+        parents = [-1 if rng.random() < 0.3 else rng.randrange(rows) for _ in range(rows)]
+        pool.go(pk, parents)
+        held = bytearray(pages)
+        for i in rng.sample(ids, len(ids) // 3):
+            held[i] = 1 + i % 255
+        pool.go(pk, parents, list(held))
+
+
 def test_fork_with_a_larger_workspace_and_replays(pk):  # noqa: F811
     rng = random.Random(8)
     pool = Pool(rng, 12, 9, 16)
