@@ -168,6 +168,36 @@ def test_fork_with_a_larger_workspace_and_replays(pk):  # noqa: F811
         pool.check(parents)
 
 
+def test_fork_of_a_large_table_replays(pk):  # noqa: F811
+    """The several launches of one call, and two calls that share a workspace one behind the other."""
+    rng = random.Random(21)
+    pools = [Pool(rng, rows, 7, 16, spare=rows) for rows in (1100, 1300)]
+    space = torch.full((pk.page_fork_workspace_bytes(1300, 7, max(p.pages for p in pools)),), 0xFF, dtype=torch.uint8, device="cuda")
+    parents, given = [], []
+    for p in pools:
+        ids = [rng.randrange(-1, p.rows) for _ in range(p.rows)]
+        p.run(pk, ids, workspace=space)
+        p.check(ids)
+        given.append([dev(ids), dev(p.table), dev(p.lengths), dev(p.free), p.range])
+    call = lambda: [pk.page_fork(*g, p.new_table, p.new_lengths, p.copies, p.freed, p.info, space, p.page) for g, p in zip(given, pools)]  # noqa: E731
+    graph = torch.cuda.CUDAGraph()
+    call()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        call()
+    for _ in range(3):
+        parents = [[rng.randrange(-1, p.rows) for _ in range(p.rows)] for p in pools]
+        for g, p, ids in zip(given, pools, parents):
+            g[0].copy_(dev(ids))
+            for t in (p.new_table, p.copies, p.freed):
+                t.fill_(-3)
+        space.fill_(0xFF)
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, ids in zip(pools, parents):
+            p.check(ids)
+
+
 def test_keep(pk):  # noqa: F811
     free, freed = dev(list(range(100, 140))), dev([7, 8, 9, 50, 51])
     run = lambda info, begin, freed=freed: (  # noqa: E731
