@@ -227,11 +227,11 @@ __global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int
 }
 
 // From this many tokens on the values of a call go in tiles (32 / 8 heads of 128, one prompt, fp16: 600
-// tokens 10.1 us without and 9.4 with, 1000 14.3 and 10.6, 1400 20.3 and 11.7; as many single tokens 10.7
-// and 15.8, 15.0 and 15.9, 22.8 and 17.9; e4m3 like these).
+// tokens 11.0 us without and 9.4 with, 1000 14.3 and 10.3, 1400 18.8 and 11.5; as many single tokens 11.6
+// and 15.4, 14.9 and 15.6, 21.1 and 18.1; e4m3 like these).
 constexpr int kValueTiles = 768;
-// Up to this many waves a wave takes one set of heads, else all of its token's (rows of fp16: 1500 tokens
-// 10.1 us in 7500 waves and 10.5 in 1500, 3000 14.9 and 13.1).
+// Up to this many waves a wave takes one set of heads, else all of its token's (rows of fp16: 1000 tokens
+// 7.2 us in 5000 waves and 7.6 in 1000, 1500 9.2 and 9.1, 3000 15.0 and 12.0).
 constexpr int kMostSetWaves = 8192;
 
 template <int kCache, bool kPast> static void launch_rotary(const RotaryArgs& a, hipStream_t s) {
