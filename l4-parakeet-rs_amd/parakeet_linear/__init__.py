@@ -639,7 +639,7 @@ LOGITS_FP16, LOGITS_FP32 = 0, 1
 
 
 def _token_stride(what, name, t, tokens, heads, head_dim):
-    """_row_stride of a tensor whose shape is known."""
+    """_row_stride of a tensor whose shape is known and that is not contiguous."""
     step, head, one = t.stride()
     if one == 1 and (head == head_dim or heads == 1):
         return step if tokens > 1 else heads * head_dim
@@ -690,13 +690,17 @@ def head_norm_rotary(query, key, query_weight, key_weight, positions, frequencie
                 ("key", key, (f16,), (tokens, kv_heads, head_dim), False), ("key_out", key_out, (f16,), (tokens, kv_heads, head_dim), False),
                 ("query_weight", query_weight, (f16,), one, True), ("key_weight", key_weight, (f16,), one, True),
                 ("positions", positions, (torch.int32,), (tokens,), True), ("frequencies", frequencies, _WORDS, None, True))
+    row, key_row, key_stride, key_out_stride = heads * head_dim, kv_heads * head_dim, 0, 0
+    if key is not None:
+        key_stride = key_row if key.is_contiguous() else _token_stride(what, "key", key, tokens, kv_heads, head_dim)
+        key_out_stride = key_row if key_out.is_contiguous() else _token_stride(what, "key_out", key_out, tokens, kv_heads, head_dim)
     _done("pk_head_norm_rotary", lib.pk_head_norm_rotary(
-        query.data_ptr(), _token_stride(what, "query", query, tokens, heads, head_dim), None if key is None else key.data_ptr(),
-        0 if key is None else _token_stride(what, "key", key, tokens, kv_heads, head_dim), None if query_weight is None else query_weight.data_ptr(),
+        query.data_ptr(), row if query.is_contiguous() else _token_stride(what, "query", query, tokens, heads, head_dim),
+        None if key is None else key.data_ptr(), key_stride, None if query_weight is None else query_weight.data_ptr(),
         None if key_weight is None else key_weight.data_ptr(), positions.data_ptr() if pairs else None, frequencies.data_ptr() if pairs else None,
-        query_out.data_ptr(), _token_stride(what, "query_out", query_out, tokens, heads, head_dim), None if key is None else key_out.data_ptr(),
-        0 if key is None else _token_stride(what, "key_out", key_out, tokens, kv_heads, head_dim), tokens, heads, kv_heads, head_dim, 2 * pairs,
-        interleaved, amplitude, epsilon, stream))
+        query_out.data_ptr(), row if query_out.is_contiguous() else _token_stride(what, "query_out", query_out, tokens, heads, head_dim),
+        None if key is None else key_out.data_ptr(), key_out_stride, tokens, heads, kv_heads, head_dim, 2 * pairs, interleaved, amplitude, epsilon,
+        stream))
 
 
 def head_norm_rotary_write(query, key, value, query_weight, key_weight, positions, slots, frequencies, query_out, key_cache, value_cache,
@@ -731,13 +735,17 @@ def head_norm_rotary_write(query, key, value, query_weight, key_weight, position
                 ("query_out", query_out, (f16,), (tokens, heads, head_dim), False), ("key", key, (f16,), new, False), ("value", value, (f16,), new, False),
                 ("slots", slots, (i32,), each, True), ("query_weight", query_weight, (f16,), one, True), ("key_weight", key_weight, (f16,), one, True),
                 ("positions", positions, (i32,), each, True), ("frequencies", frequencies, _WORDS, None, True))
+    row, key_row = heads * head_dim, kv_heads * head_dim
     _done("pk_head_norm_rotary_write", lib.pk_head_norm_rotary_write(
-        CACHE_FP16 if kind is f16 else CACHE_FP8, query.data_ptr(), _token_stride(what, "query", query, tokens, heads, head_dim), key.data_ptr(),
-        _token_stride(what, "key", key, tokens, kv_heads, head_dim), value.data_ptr(), _token_stride(what, "value", value, tokens, kv_heads, head_dim),
+        CACHE_FP16 if kind is f16 else CACHE_FP8, query.data_ptr(),
+        row if query.is_contiguous() else _token_stride(what, "query", query, tokens, heads, head_dim), key.data_ptr(),
+        key_row if key.is_contiguous() else _token_stride(what, "key", key, tokens, kv_heads, head_dim), value.data_ptr(),
+        key_row if value.is_contiguous() else _token_stride(what, "value", value, tokens, kv_heads, head_dim),
         None if query_weight is None else query_weight.data_ptr(), None if key_weight is None else key_weight.data_ptr(),
         positions.data_ptr() if pairs else None, slots.data_ptr(), frequencies.data_ptr() if pairs else None, query_out.data_ptr(),
-        _token_stride(what, "query_out", query_out, tokens, heads, head_dim), key_cache.data_ptr(), value_cache.data_ptr(), tokens, heads, kv_heads,
-        head_dim, 2 * pairs, interleaved, amplitude, epsilon, page_size, pages, key_inverse_scale, value_inverse_scale, stream))
+        row if query_out.is_contiguous() else _token_stride(what, "query_out", query_out, tokens, heads, head_dim), key_cache.data_ptr(),
+        value_cache.data_ptr(), tokens, heads, kv_heads, head_dim, 2 * pairs, interleaved, amplitude, epsilon, page_size, pages, key_inverse_scale,
+        value_inverse_scale, stream))
 
 
 def beam_select_workspace_bytes(sequences, beams, vocab, choices):
