@@ -6,8 +6,8 @@
 // The logits are read once, in parts of a row that a workgroup holds in registers: the part's
 // maximum, its sum of exponentials, and its best `choices` logits, in order.  A second launch puts
 // a sequence's parts together; short rows of few beams are one launch, whose workgroup does both
-// (8 sequences of 4 beams, 1025 fp32 logits: 7.6 us against 4.8 and 4.5 in two launches; 510 of 16 beams
-// 18.6 against 22.4 and 8.7).
+// (8 sequences of 4 beams, 1025 fp32 logits: 7.7 us against 4.6 and 4.8 in two launches; 510 of 16 beams
+// 19.5 against 22.9 and 7.7).
 //
 // The best of a part: a bound is the choices-th largest of the lanes' maxima of any one
 // wave (as many logits at least reach it), found by bisection over the upper bits of the value
@@ -398,7 +398,9 @@ __device__ __forceinline__ void join_parts(const BeamArgs& a, int seq, int parts
     }
     for (int i = tid + kKept * kThreads; i < front; i += kThreads) larger(candidate(i / depth, i % depth));
     uint32_t bound = 0;
-    if (front > 128 || depth < a.choices) {  // else all of them are ranked
+    // a few are all ranked (16 of them 7.6 us of a call of one launch, 8.0 with a bound; 32 8.3 and 8.2; 128 7.9 us
+    // of the join, 5.0 with a bound)
+    if (front > 16 || depth < a.choices) {
         const uint32_t here = wave_bound(mine, a.choices, 12);  // eight bits of the mantissa
         if (lane == 0) shared.wave_bound[wave] = here;
         __syncthreads();
