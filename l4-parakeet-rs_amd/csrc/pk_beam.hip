@@ -10,9 +10,10 @@
 // 19.5 against 22.9 and 7.7).
 //
 // The best of a part: a bound is the choices-th largest of the lanes' maxima of any one
-// wave (as many logits at least reach it), found by bisection over the upper bits of the value
-// with one ballot a bit; the few logits that reach it are listed in LDS and ranked by
-// counting.  Keys are unique (value, then index), so the order of the list does not matter.
+// wave (as many logits at least reach it) or, for many choices, of all threads' maxima, found by
+// bisection over the upper bits of the value with ballots; the few logits that reach it are listed
+// in LDS and ranked by counting.  Keys are unique (value, then index), so the order of the list does
+// not matter.
 //
 // The sum's terms are fp32, their sum and the scores 64 bits: beams are compared by
 // differences of sums, and a rounding of 2^-24 of a score of -30 would change places of
@@ -27,6 +28,10 @@ namespace pk {
 
 constexpr float kLog2e = 1.44269504f;
 constexpr int kMostLoads = 8;  // of 16 bytes a thread
+// Up to as many choices a bound of one wave is near enough, in one launch and in two (64 sequences of 8 beams,
+// 1025 logits: 14.9 us with it and 15.4 with that of all threads for 32 choices, 26 and 18.4 for 48; 131071 fp16
+// logits: 40.5 and 39.6 for 16, 47 and 40.5 for 24, and 897 and 50 for 64, where it is the lowest of its lanes).
+constexpr int kFewWhole = 32, kFewChoices = 16;
 
 // Of a part: its largest logit m and sum exp2(x log2e - c), c = fp32(m log2e) (fp16 logits), or
 // sum exp2((x - m) log2e) (fp32 ones, whose m log2e may pass fp32's range).
@@ -56,6 +61,24 @@ __device__ __forceinline__ uint32_t wave_bound(uint32_t v, int count, int last) 
     for (int bit = 31; bit >= last; --bit) {
         const uint32_t tried = bound | (1u << bit);
         if (__popcll(__builtin_amdgcn_ballot_w64(v >= tried)) >= count) bound = tried;
+    }
+    return bound;
+}
+// The same of the first `waves` times 64 values in LDS; each wave finds it by itself, lane l by values l, l + 64, ..
+template <int kWaves> __device__ __forceinline__ uint32_t bound_of(const uint32_t* values, int waves, int lane, int count, int last) {
+    uint32_t v[kWaves], bound = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) v[w] = w < waves ? values[w * 64 + lane] : 0;
+    for (int bit = 31; bit >= last; --bit) {
+        const uint32_t tried = bound | (1u << bit);
+        int reach = 0;
+#pragma unroll
+        for (int first = 0; first < kWaves; first += 4)
+            if (first < waves)
+#pragma unroll
+                for (int w = first; w < first + 4 && w < kWaves; ++w) reach += __popcll(__builtin_amdgcn_ballot_w64(v[w] >= tried));
+        if (reach >= count) bound = tried;
+        if (reach == count) break;
     }
     return bound;
 }
@@ -137,6 +160,8 @@ template <int kGroup> struct PartShared {
     long long sum[kGroup / 64];
     float most[kGroup / 64];
     uint32_t bound[kGroup / 64];
+    static constexpr int kTops = kGroup == 64 ? 2 : 1;  // more values than the most choices
+    uint32_t top[kTops * kGroup];  // the threads' largest logits, ordered; 0: none
     int listed;
 };
 
@@ -164,10 +189,10 @@ __device__ __forceinline__ void rank_listed(const PartShared<kGroup>& shared, in
 // each term is rounded alike wherever it is added, and whole steps are added from there.  A term
 // times 1 + 2^-52 is never half way between two steps, whose rounding would go by the sum before it:
 // its lowest bit is 2^-52 of an fp32 term's, and half a step such a term's only from 128 on.
-template <bool kF16, int kLoads, int kGroup, typename Real>
+template <bool kF16, int kLoads, int kGroup, int kFew, typename Real>
 __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab, int part, int choices, int tid, PartShared<kGroup>& shared,
                                              int& over, PartSum* sum_out, unsigned long long* to) {
-    constexpr int kVec = kF16 ? 8 : 4, kWaves = kGroup / 64, kListed = PartShared<kGroup>::kListed;
+    constexpr int kVec = kF16 ? 8 : 4, kWaves = kGroup / 64, kListed = PartShared<kGroup>::kListed, kTops = PartShared<kGroup>::kTops;
     constexpr int kPart = kGroup * kLoads * kVec, kBytes = kF16 ? 2 : 4;
     const int wave = tid >> 6, first = part * kPart, count_here = vocab - first < kPart ? vocab - first : kPart;
     const char* const here_x = x + (size_t)first * kBytes;
@@ -191,8 +216,19 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
         mine = __builtin_fmaxf(mine, top[l]);
     }
     const float wave_most = wave_max(mine);
-    // (seven bits of the mantissa tell enough logits apart); 0: fewer than `choices` lanes have a candidate
-    const uint32_t here = wave_bound(candidates && mine > -__builtin_inff() ? ordered(mine) : 0, choices, 16);
+    // (seven bits of the mantissa tell enough logits apart); 0: fewer than `choices` have a candidate
+    const auto rated = [&](float v) { return candidates && v > -__builtin_inff() ? ordered(v) : 0; };
+    const bool few = choices <= kFew;
+    const uint32_t here = few ? wave_bound(rated(mine), choices, 16) : 0;
+    if (!few) {
+        float half[kTops];  // of every second 16 bytes, or of all
+#pragma unroll
+        for (int i = 0; i < kTops; ++i) half[i] = i ? -__builtin_inff() : extra;
+#pragma unroll
+        for (int l = 0; l < kLoads; ++l) half[l % kTops] = __builtin_fmaxf(half[l % kTops], top[l]);
+#pragma unroll
+        for (int i = 0; i < kTops; ++i) shared.top[i * kGroup + tid] = rated(half[i]);
+    }
     if ((tid & 63) == 0) {
         shared.most[wave] = wave_most;
         shared.bound[wave] = here;
@@ -209,6 +245,7 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
         found = shared.bound[w] > found ? shared.bound[w] : found;
         most = __builtin_fmaxf(most, shared.most[w]);
     }
+    if (!few) found = bound_of<kWaves * kTops>(shared.top, kWaves * kTops, tid & 63, choices, 16);
     const float bound = !candidates ? __builtin_nanf("") : (found ? unordered(found) : -3.402823466e38f);
     const float base = most > -__builtin_inff() ? most : 0.0f, c = base * kLog2e;
     const auto term = [&](float v) { return __builtin_amdgcn_exp2f(kF16 ? __builtin_fmaf(v, kLog2e, -c) : (v - base) * kLog2e); };
@@ -305,7 +342,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a, int parts, P
     const int row = blockIdx.x / parts, part = blockIdx.x % parts;
     if (beam_state(a.scores[row], a.ended, row) != 1) return;
     const size_t out = (size_t)row * parts + part;
-    best_of_part<kF16, kLoads, 256>((const char*)a.logits + (size_t)row * a.stride * (kF16 ? 2 : 4), [] { return true; }, a.vocab, part, a.choices, threadIdx.x, shared, over,
+    best_of_part<kF16, kLoads, 256, kFewChoices>((const char*)a.logits + (size_t)row * a.stride * (kF16 ? 2 : 4), [] { return true; }, a.vocab, part, a.choices, threadIdx.x, shared, over,
                                sums + out, best + out * a.choices);
 }
 
@@ -323,6 +360,7 @@ template <int kThreads> struct JoinShared {
     unsigned long long wave_score[kThreads / 64];
     uint32_t list_place[kJoinListed];
     uint32_t wave_place[kThreads / 64], wave_bound[kThreads / 64];
+    uint32_t top[kThreads];  // upper bits of the threads' best scores
     int state[kMostBeams];
     int listed;
 };
@@ -401,11 +439,17 @@ __device__ __forceinline__ void join_parts(const BeamArgs& a, int seq, int parts
     // a few are all ranked (16 of them 7.6 us of a call of one launch, 8.0 with a bound; 32 8.3 and 8.2; 128 7.9 us
     // of the join, 5.0 with a bound)
     if (front > 16 || depth < a.choices) {
-        const uint32_t here = wave_bound(mine, a.choices, 12);  // eight bits of the mantissa
-        if (lane == 0) shared.wave_bound[wave] = here;
+        const bool few = a.choices <= (kOnePart ? kFewWhole : kFewChoices);
+        const uint32_t here = few ? wave_bound(mine, a.choices, 12) : 0;  // eight bits of the mantissa
+        if (few && lane == 0) shared.wave_bound[wave] = here;
+        if (!few) shared.top[tid] = mine;
         __syncthreads();
+        if (few) {
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) bound = shared.wave_bound[w] > bound ? shared.wave_bound[w] : bound;
+            for (int w = 0; w < kWaves; ++w) bound = shared.wave_bound[w] > bound ? shared.wave_bound[w] : bound;
+        } else {
+            bound = bound_of<kWaves>(shared.top, (front + 63) / 64, lane, a.choices, 12);
+        }
     }
     const auto reaches = [&](const Candidate& one) {
         if (!one.score || (uint32_t)(one.score >> 32) < bound) return false;
@@ -497,7 +541,7 @@ template <bool kF16, int kGroup> __global__ __launch_bounds__(kWholeThreads) voi
     const float score = a.scores[row];
     const uint8_t done = a.ended ? a.ended[row] : 0;
     const auto real = [&] { return b < a.beams && !done && __builtin_fabsf(score) < __builtin_inff(); };
-    best_of_part<kF16, kWholeVectors / kGroup, kGroup>((const char*)a.logits + row * a.stride * (kF16 ? 2 : 4), real, a.vocab, 0, a.choices,
+    best_of_part<kF16, kWholeVectors / kGroup, kGroup, kFewWhole>((const char*)a.logits + row * a.stride * (kF16 ? 2 : 4), real, a.vocab, 0, a.choices,
                                                        threadIdx.x % kGroup, part[b], over, sums + b, b < a.beams ? keys + b * a.choices : nullptr);
     __syncthreads();
     join_parts<kWholeThreads, kF16, true>(a, seq, 1, sums, keys, shared);

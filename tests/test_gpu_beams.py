@@ -235,3 +235,29 @@ def test_reorder_of_rows_of_more_than_32_bits(pk):  # noqa: F811
     state[0, 0, -1], state[0, 1, -1] = 7, 8
     pk.beam_reorder(state, torch.tensor([[1, 0]], dtype=torch.int32, device="cuda"), state)
     assert state[0, 0, 0] == 6 and state[0, 0, -1] == 8 and state[0, 1, 0] == 5 and state[0, 1, -1] == 7 and state[0, 0, row // 16] == 6
+
+
+@pytest.mark.parametrize("n,beams,vocab", [(3, 4, 1025), (2, 8, 1027), (3, 16, 1030), (2, 16, 600), (2, 3, 30001), (1, 20, 9000), (2, 2, 70000)])
+@pytest.mark.parametrize("choices", [16, 17, 32, 33, 64])
+@pytest.mark.parametrize("fp16", [False, True])
+def test_many_choices(pk, n, beams, vocab, choices, fp16):  # noqa: F811
+    """Borders between the bounds of one wave and of all threads; then rows of which most is masked."""
+    s = Search(pk, n, beams, vocab, choices, fp16, seed=5)
+    s.go()
+    g = gen(vocab)
+    hidden = torch.rand(s.logits.shape, generator=g, device="cuda") < 0.97
+    hidden[:, :, vocab // 3:] |= torch.rand((n, beams, 1), generator=g, device="cuda") < 0.5
+    s.logits.masked_fill_(hidden, -math.inf)
+    s.go()
+
+
+@pytest.mark.parametrize("n,beams,vocab,choices", [(2, 4, 1025, 8), (2, 16, 1025, 4), (1, 2, 20000, 8), (1, 1, 70001, 64), (1, 20, 3000, 33)])
+@pytest.mark.parametrize("fp16", [False, True])
+def test_rows_masked_by_the_lowest_value(pk, n, beams, vocab, choices, fp16):  # noqa: F811
+    """Fewer allowed tokens than choices: the rest are candidates all the same, the lowest indices first."""
+    s = Search(pk, n, beams, vocab, choices, fp16, seed=9)
+    allowed = torch.rand(s.logits.shape, generator=gen(choices), device="cuda") < 2.0 / vocab
+    s.logits.masked_fill_(~allowed, torch.finfo(s.logits.dtype).min)
+    if not fp16:
+        s.scores[:, 1:] = -math.inf  # (scores near fp32's lowest value are all alike)
+    s.go()
