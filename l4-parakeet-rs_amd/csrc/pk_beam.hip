@@ -154,9 +154,8 @@ __device__ __forceinline__ unsigned long long key_of(float v, int i) { return ((
 
 // What the kGroup threads that take a part share.
 template <int kGroup> struct PartShared {
-    static constexpr int kListed = 4 * kGroup;  // candidates that are ranked; more of them are taken out one by one
+    static constexpr int kListed = 4 * kGroup, kRanked = kGroup > 128 ? kGroup : 128;  // candidates that are listed, and ranked as they are
     unsigned long long list[kListed];
-    unsigned long long key[kGroup / 64];
     long long sum[kGroup / 64];
     float most[kGroup / 64];
     uint32_t bound[kGroup / 64];
@@ -164,6 +163,32 @@ template <int kGroup> struct PartShared {
     uint32_t top[kTops * kGroup];  // the threads' largest logits, ordered; 0: none
     int listed;
 };
+
+// The count-th largest of `size` different keys in LDS, or one below it that no more of them reach, by bisection of
+// the bits in which they differ; each wave finds it by itself.  More than `count` keys: not all reach it.
+template <int kMost> __device__ __forceinline__ unsigned long long bound_of_keys(const unsigned long long* list, int size, int count, int lane) {
+    constexpr int kKeys = kMost / 64;
+    const unsigned long long one = list[0];
+    unsigned long long key[kKeys], differ = 0;
+#pragma unroll
+    for (int n = 0; n < kKeys; ++n) {
+        key[n] = n * 64 + lane < size ? list[n * 64 + lane] : 0;
+        differ |= n * 64 + lane < size ? key[n] ^ one : 0;
+    }
+#pragma unroll
+    for (int off = 1; off <= 32; off <<= 1) differ |= (unsigned long long)__shfl_xor((long long)differ, off, 64);
+    const int highest = 63 - __clzll((long long)differ);
+    unsigned long long bound = one >> highest >> 1 << highest << 1;
+    for (int bit = highest; bit >= 0; --bit) {
+        const unsigned long long tried = bound | (1ull << bit);
+        int reach = 0;
+#pragma unroll
+        for (int n = 0; n < kKeys; ++n) reach += __popcll(__builtin_amdgcn_ballot_w64(key[n] >= tried));
+        if (reach >= count) bound = tried;
+        if (reach == count) break;
+    }
+    return bound;
+}
 
 // The listed candidates in order, by counting those before each.
 template <int kGroup>
@@ -192,7 +217,7 @@ __device__ __forceinline__ void rank_listed(const PartShared<kGroup>& shared, in
 template <bool kF16, int kLoads, int kGroup, int kFew, typename Real>
 __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab, int part, int choices, int tid, PartShared<kGroup>& shared,
                                              int& over, PartSum* sum_out, unsigned long long* to) {
-    constexpr int kVec = kF16 ? 8 : 4, kWaves = kGroup / 64, kListed = PartShared<kGroup>::kListed, kTops = PartShared<kGroup>::kTops;
+    constexpr int kVec = kF16 ? 8 : 4, kWaves = kGroup / 64, kListed = PartShared<kGroup>::kListed, kRanked = PartShared<kGroup>::kRanked, kTops = PartShared<kGroup>::kTops;
     constexpr int kPart = kGroup * kLoads * kVec, kBytes = kF16 ? 2 : 4;
     const int wave = tid >> 6, first = part * kPart, count_here = vocab - first < kPart ? vocab - first : kPart;
     const char* const here_x = x + (size_t)first * kBytes;
@@ -253,7 +278,7 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
         if (v >= bound) {
             const int k = atomicAdd(&shared.listed, 1);
             if (k < kListed) shared.list[k] = key_of(v, i);
-            else over = 1;
+            if (k >= kRanked) over = 1;
         }
     };
     constexpr double kNudge = 1.0 + 0x1p-52;
@@ -281,7 +306,7 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
             const int word = w & 2 ? (w & 1 ? v[3] : v[2]) : (w & 1 ? v[1] : v[0]);
             const float one = kF16 ? h2f((uint16_t)((uint32_t)word >> (16 * (j & 1)))) : __int_as_float(word);
             if (k < kListed) shared.list[k] = key_of(one, place(l, j));
-            else over = 1;
+            if (k >= kRanked) over = 1;
         }
     }
     const bool odd = __builtin_amdgcn_ballot_w64(total != total) != 0;
@@ -302,32 +327,55 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
         if (to) rank_listed(shared, shared.listed, choices, tid, to);
         return;
     }
-    // Many equal logits: the largest key below the last one, `choices` times.
-    unsigned long long last = ~0ull;
-    for (int n = 0; n < choices; ++n) {
-        unsigned long long key = 0;
-        const auto look = [&](float v, int i) {
-            const unsigned long long k = key_of(v, i);
-            if (v > -__builtin_inff() && k < last && k > key) key = k;
-        };
-        for (uint32_t left = loads; left; left &= left - 1) {
-            const int l = __ffs(left) - 1;
-            const v4i v = pick<kLoads>(raw, l);
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) look(logit_of<kF16>(v, j), place(l, j));
-        }
-        look(extra, extra_at);
-#pragma unroll
-        for (int off = 1; off <= 32; off <<= 1) key = max_level(key, off);
-        if ((tid & 63) == 0) shared.key[wave] = key;
+    // More than the list holds, often equal logits: 256 of those listed give a new bound, by value and index, and the
+    // list is made again, until all fit: a few passes, each of which leaves about choices / 256 of those that are
+    // equal (all logits of 64 sequences of 8 beams equal, 8 choices: 1025 of them 18.5 us, 131071 fp16 195).
+    while (true) {
+        const bool wide = shared.listed > kListed;
         __syncthreads();
-        key = shared.key[0];
+        if (tid == 0) over = 0;
+        __syncthreads();
+        if (wide) over = 1;
+        __syncthreads();
+        if (!over) break;
+        const unsigned long long at_least = wide ? bound_of_keys<256>(shared.list, 256, choices, tid & 63) : 0;
+        __syncthreads();
+        if (tid == 0 && wide) shared.listed = 0;
+        __syncthreads();
+        if (wide) {
+            const auto reach = [&](float v, int i) {
+                const unsigned long long key = key_of(v, i);
+                if (v > -__builtin_inff() && key >= at_least) {
+                    const int k = atomicAdd(&shared.listed, 1);
+                    if (k < kListed) shared.list[k] = key;
+                }
+            };
+            for (uint32_t left = loads; left; left &= left - 1) {
+                const int l = __ffs(left) - 1;
+                const v4i v = pick<kLoads>(raw, l);
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) key = shared.key[w] > key ? shared.key[w] : key;
-        if (tid == 0 && to) to[n] = key;
-        last = key;
+                for (int j = 0; j < kVec; ++j) reach(logit_of<kF16>(v, j), place(l, j));
+            }
+            if (extra_at >= 0) reach(extra, extra_at);
+        }
         __syncthreads();
     }
+    // Still more than are ranked soon: the choices best of them alone.
+    const int count = shared.listed;
+    const bool narrow = count > kRanked;
+    const unsigned long long at_least = narrow ? bound_of_keys<kListed>(shared.list, count, choices, tid & 63) : 0;
+    unsigned long long key[kListed / kGroup];
+#pragma unroll
+    for (int n = 0; n < kListed / kGroup; ++n) key[n] = n * kGroup + tid < count ? shared.list[n * kGroup + tid] : 0;
+    __syncthreads();
+    if (tid == 0 && narrow) shared.listed = 0;
+    __syncthreads();
+    if (narrow)
+#pragma unroll
+        for (int n = 0; n < kListed / kGroup; ++n)
+            if (n * kGroup + tid < count && key[n] >= at_least) shared.list[atomicAdd(&shared.listed, 1)] = key[n];
+    __syncthreads();
+    if (to) rank_listed(shared, shared.listed, choices, tid, to);
 }
 
 // A beam's candidates: 0 none, 1 of its logits, 2 ended.
