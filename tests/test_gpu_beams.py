@@ -200,6 +200,21 @@ def test_reorder(pk, n, beams, row, kind, in_place):  # noqa: F811
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("row", [1, 2, 255, 256, 257, 1023, 1024, 1028, 4080, 4096, 4112])
+def test_reorder_of_short_rows(pk, row):  # noqa: F811
+    """Rows of bytes at the border of the two ways, and parents that are no rows of their sequence."""
+    g = gen(row)
+    n, beams = 301, 6
+    state = torch.randint(0, 256, (n, beams, row), generator=g, device="cuda", dtype=torch.uint8)
+    parents = torch.randint(0, beams, (n, beams), generator=g, device="cuda") + beams * torch.arange(n, device="cuda")[:, None]
+    wrong = torch.tensor([-1, -beams, -2**31, n * beams, 2**31 - 1, 0], device="cuda")[torch.randint(0, 6, (n, beams), generator=g, device="cuda")]
+    parents = torch.where(torch.rand((n, beams), generator=g, device="cuda") < 0.3, wrong, parents).int()
+    out = torch.randint(0, 256, (n, beams, row), generator=g, device="cuda", dtype=torch.uint8)
+    want = reordered(state, parents, out)
+    pk.beam_reorder(state, parents, out)
+    assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("shift", [1, 2, 4, 8])
 def test_reorder_of_unaligned_states(pk, shift):  # noqa: F811
     whole = torch.randint(0, 256, (shift + 3 * 4 * 96 + 64,), device="cuda").to(torch.uint8)
