@@ -9,9 +9,8 @@
 // are taken to the nearest quarter turn, and sine and cosine of the rest (within pi / 4)
 // are the Taylor sums to x^9 and x^8, off by less than x^10 / 10! = 2.5e-8.
 //
-// A lane holds 16 features of a head, and in either layout both halves of 8 pairs with the
-// same 8 frequencies; head_dim / 16 lanes make a head.  Everything between the loads and the
-// one rounding at the store is fp32.
+// A lane holds twice 8 features of a head, in either layout both members of 8 pairs; head_dim / 16
+// lanes make a head.  Everything between the loads and the one rounding at the store is fp32.
 //
 // Bound by HBM: 16000 tokens, 32 / 8 heads of 128, rows to rows (328 MB) 60 us, 5.5 TB/s; with keys
 // and values into an fp16 cache (393 MB) 76 us, 5.2 TB/s.  One token 2.7 us, about a launch; 61 into an
@@ -108,8 +107,11 @@ __global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int
     const int all = query_sets + kv_sets + (kCache >= 0 && value_blocks == 0 ? kv_sets : 0);
     const int first = unit % parts * sets, stop = first + sets < all ? first + sets : all;
     const bool there = t < a.tokens && first < stop, rotates = there && a.rotary_dim && first < query_sets + kv_sets;
-    const bool inside = p * 16 < a.head_dim, turns = p * 16 < a.rotary_dim, halves = turns && !a.interleaved;
-    const int f0 = halves ? 8 * p : 16 * p, f1 = halves ? f0 + a.rotary_dim / 2 : f0 + 8;
+    const bool inside = p * 16 < a.head_dim, turning = p * 16 < a.rotary_dim && !a.interleaved;
+    // 8 features each, those of neighbouring lanes behind one another (where lanes held 16 in a row, stores past
+    // the caches were halves of lines: 16000 tokens of 32 / 8 heads of 128, neighbours, 82 us instead of 60)
+    const int f0 = 8 * p + (turning || a.interleaved ? 0 : a.rotary_dim / 2), f1 = 8 * p + (turning ? a.rotary_dim : a.head_dim) / 2;
+    const bool turn0 = a.interleaved ? f0 < a.rotary_dim : turning, turn1 = a.interleaved ? f1 < a.rotary_dim : turning;
     // lanes without a feature or a head read those of the first
     const int r0 = inside ? f0 : 0, r1 = inside ? f1 : 0;
     const auto ask = [&](int set) {
@@ -139,7 +141,10 @@ __global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int
     if (!there || slot < 0 || (kCache >= 0 && slot >= a.slot_count)) return;
     float2 angle[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) angle[j] = turns ? angles[wave][8 * p + j] : float2{1.0f, 0.0f};
+    for (int j = 0; j < 4; ++j) {
+        angle[j] = turn0 ? angles[wave][(a.interleaved ? f0 / 2 : 8 * p) + j] : float2{};
+        angle[4 + j] = turn1 ? angles[wave][(a.interleaved ? f1 / 2 : 8 * p + 4) + j] : float2{};
+    }
     const int off = slot & ((1 << a.shift) - 1);
     const float per_feature = 1.0f / (float)a.head_dim;
     float w0[8], w1[8];
@@ -195,14 +200,17 @@ __global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int
                 v[j] = v[j] * rstd * w1[j];
             }
         }
-        if (turns) {
+        const auto turn = [&](int j) {
+            const float x = u[j];
+            u[j] = __builtin_fmaf(x, angle[j].x, -(v[j] * angle[j].y));
+            v[j] = __builtin_fmaf(v[j], angle[j].x, x * angle[j].y);
+        };
+        if (turn0)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = u[j];
-                u[j] = __builtin_fmaf(x, angle[j].x, -(v[j] * angle[j].y));
-                v[j] = __builtin_fmaf(v[j], angle[j].x, x * angle[j].y);
-            }
-        }
+            for (int j = 0; j < 4; ++j) turn(j);
+        if (turn1)
+#pragma unroll
+            for (int j = 4; j < 8; ++j) turn(j);
         if (!mine) continue;
         if (kF8 && !query) {  // neighbours: the unrounded features in their order
             float x[8], y[8];
@@ -249,8 +257,13 @@ template <int kCache, bool kPast> static void launch_rotary(const RotaryArgs& a,
     else if constexpr (kCache < 0) launch(head_norm_rotary_kernel<16, kCache, kPast>, 16);  // (a cache holds heads of 64 or 128)
 }
 
+// Bytes that neighbouring lanes store behind one another at the least; of less than 64 the caches put lines
+// together (16000 tokens of 32 / 8 heads of 128 of which 32 turn by halves 65 us, past the caches 76; 64 both 64.5).
+constexpr int kShortPiece = 64;
+
 template <int kCache> static void rotary(const RotaryArgs& a, hipStream_t s) {
-    if ((long long)a.tokens * (a.heads + a.kv_heads) * a.head_dim * 2 > kCached) launch_rotary<kCache, true>(a, s);
+    const int rest = a.head_dim - a.rotary_dim, piece = a.interleaved || !rest || rest == a.head_dim ? a.head_dim : (rest < a.rotary_dim ? rest : a.rotary_dim);
+    if ((long long)a.tokens * (a.heads + a.kv_heads) * a.head_dim * 2 > kCached && piece >= kShortPiece) launch_rotary<kCache, true>(a, s);
     else launch_rotary<kCache, false>(a, s);
 }
 
