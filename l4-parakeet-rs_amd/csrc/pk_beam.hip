@@ -28,6 +28,9 @@ namespace pk {
 
 constexpr float kLog2e = 1.44269504f;
 constexpr int kMostLoads = 8;  // of 16 bytes a thread
+// With more, a SIMD holds fewer than 8 waves, and a CU one workgroup of 1024 threads instead of two (2048 sequences
+// of 4 of 1025 logits 47 us instead of 34).
+constexpr int kSgprs = 80;
 // Up to as many choices a bound of one wave is near enough, in one launch and in two (64 sequences of 8 beams,
 // 1025 logits: 14.9 us with it and 15.4 with that of all threads for 32 choices, 26 and 18.4 for 48; 131071 fp16
 // logits: 40.5 and 39.6 for 16, 47 and 40.5 for 24, and 897 and 50 for 64, where it is the lowest of its lanes).
@@ -218,6 +221,7 @@ template <bool kF16, int kLoads, int kGroup, int kFew, typename Real>
 __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab, int part, int choices, int tid, PartShared<kGroup>& shared,
                                              int& over, PartSum* sum_out, unsigned long long* to) {
     constexpr int kVec = kF16 ? 8 : 4, kWaves = kGroup / 64, kListed = PartShared<kGroup>::kListed, kRanked = PartShared<kGroup>::kRanked, kTops = PartShared<kGroup>::kTops;
+    constexpr bool kShort = kFew == kFewWhole;  // rows are short, and loads without logits worth a branch
     constexpr int kPart = kGroup * kLoads * kVec, kBytes = kF16 ? 2 : 4;
     const int wave = tid >> 6, first = part * kPart, count_here = vocab - first < kPart ? vocab - first : kPart;
     const char* const here_x = x + (size_t)first * kBytes;
@@ -232,6 +236,7 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
     const int extra_at = tid < lead ? first + tid : (tid >= 8 && tid < 8 + tail ? first + count_here - tail + tid - 8 : -1);
     float extra = -__builtin_inff();
     if (extra_at >= 0) extra = kF16 ? h2f(((const uint16_t*)x)[extra_at]) : ((const float*)x)[extra_at];
+    const int filled = __builtin_amdgcn_readfirstlane(vectors);  // (of a wave: all its lanes are at one row)
     const bool candidates = real();
     const auto place = [&](int l, int j) { return first + lead + (l * kGroup + tid) * kVec + j; };
     float top[kLoads], mine = extra;  // of 16 bytes, of all
@@ -287,12 +292,12 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
     uint32_t hits = 0;
 #pragma unroll
     for (int l = 0; l < kLoads; ++l) {
+        if (kShort && l * kGroup >= filled) break;
 #pragma unroll
         for (int j = 0; j < kVec; ++j) total = __builtin_fma((double)term(logit_of<kF16>(raw[l], j)), kNudge, total);
         hits |= top[l] >= bound ? 1u << l : 0u;
     }
     note(extra, extra_at);
-    const uint32_t loads = hits;
     while (hits) {  // most often one logit of a lane
         const int l = __ffs(hits) - 1;
         hits &= hits - 1;
@@ -350,9 +355,9 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
                     if (k < kListed) shared.list[k] = key;
                 }
             };
-            for (uint32_t left = loads; left; left &= left - 1) {
-                const int l = __ffs(left) - 1;
-                const v4i v = pick<kLoads>(raw, l);
+#pragma unroll 1
+            for (int l = 0; l * kGroup + tid < vectors; ++l) {  // (read again: little code that calls without it carry)
+                const v4i v = *(const v4i*)(here_x + lead * kBytes + (size_t)(l * kGroup + tid) * 16);
 #pragma unroll
                 for (int j = 0; j < kVec; ++j) reach(logit_of<kF16>(v, j), place(l, j));
             }
@@ -384,7 +389,7 @@ __device__ __forceinline__ int beam_state(float score, const uint8_t* ended, siz
 }
 
 template <bool kF16, int kLoads>
-__global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a, int parts, PartSum* __restrict__ sums, unsigned long long* __restrict__ best) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_num_sgpr(kSgprs))) void beam_part_kernel(BeamArgs a, int parts, PartSum* __restrict__ sums, unsigned long long* __restrict__ best) {
     __shared__ PartShared<256> shared;
     __shared__ int over;
     const int row = blockIdx.x / parts, part = blockIdx.x % parts;
@@ -577,7 +582,8 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
 // Both in one launch where the rows are short and a sequence has few beams: kGroup threads a beam.
 constexpr int kWholeThreads = 1024, kWholeBeams = 16, kWholeVectors = 512;  // 16-byte loads a row
 
-template <bool kF16, int kGroup> __global__ __launch_bounds__(kWholeThreads) void beam_whole_kernel(BeamArgs a) {
+template <bool kF16, int kGroup>
+__global__ __launch_bounds__(kWholeThreads) __attribute__((amdgpu_num_sgpr(kSgprs))) void beam_whole_kernel(BeamArgs a) {
     constexpr int kGroups = kWholeThreads / kGroup;
     __shared__ PartShared<kGroup> part[kGroups];
     __shared__ int over;
