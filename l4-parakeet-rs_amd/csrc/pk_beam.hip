@@ -6,8 +6,8 @@
 // The logits are read once, in parts of a row that a workgroup holds in registers: the part's
 // maximum, its sum of exponentials, and its best `choices` logits, in order.  A second launch puts
 // a sequence's parts together; short rows of few beams are one launch, whose workgroup does both
-// (8 sequences of 4 beams, 1025 fp32 logits: 7.7 us against 4.6 and 4.8 in two launches; 510 of 16 beams
-// 19.5 against 22.9 and 7.7).
+// (8 sequences of 4 beams, 1025 fp32 logits: 7.5 us against 8.9 in two launches; 512 of 16 beams 19 against
+// 37; 8 of 16 beams of 2048 11.9 and 11.3).
 //
 // The best of a part: a bound is the choices-th largest of the lanes' maxima of any one
 // wave (as many logits at least reach it) or, for many choices, of all threads' maxima, found by
@@ -28,12 +28,13 @@ namespace pk {
 
 constexpr float kLog2e = 1.44269504f;
 constexpr int kMostLoads = 8;  // of 16 bytes a thread
-// With more, a SIMD holds fewer than 8 waves, and a CU one workgroup of 1024 threads instead of two (2048 sequences
-// of 4 of 1025 logits 47 us instead of 34).
+// Scalar registers: with more a SIMD holds fewer than 8 waves, and a CU one workgroup of 16 waves instead of two (a
+// call of thousands of them 47 us instead of 34).
 constexpr int kSgprs = 80;
-// Up to as many choices a bound of one wave is near enough, in one launch and in two (64 sequences of 8 beams,
-// 1025 logits: 14.9 us with it and 15.4 with that of all threads for 32 choices, 26 and 18.4 for 48; 131071 fp16
-// logits: 40.5 and 39.6 for 16, 47 and 40.5 for 24, and 897 and 50 for 64, where it is the lowest of its lanes).
+// Up to as many choices a bound of one wave is near enough, in one launch and in two (64 sequences of 16 beams,
+// 1025 logits: 15.7 us with it and 18.6 with the other for 24 choices, 17.9 and 19.3 for 32, 23.2 and 21.8 for 40;
+// of 8 beams, 131071 fp16 logits: 40.5 and 39.6 for 16, 47 and 40.5 for 24, and 897 and 50 for 64, where it is the
+// lowest of its lanes).
 constexpr int kFewWhole = 32, kFewChoices = 16;
 
 // Of a part: its largest logit m and sum exp2(x log2e - c), c = fp32(m log2e) (fp16 logits), or
@@ -334,7 +335,7 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
     }
     // More than the list holds, often equal logits: 256 of those listed give a new bound, by value and index, and the
     // list is made again, until all fit: a few passes, each of which leaves about choices / 256 of those that are
-    // equal (all logits of 64 sequences of 8 beams equal, 8 choices: 1025 of them 18.5 us, 131071 fp16 195).
+    // equal (all logits of 64 sequences of 8 beams equal, 8 choices: 1025 of them 14 us, 131071 fp16 182).
     while (true) {
         const bool wide = shared.listed > kListed;
         __syncthreads();
@@ -405,9 +406,9 @@ struct Candidate {
     __device__ __forceinline__ bool before(const Candidate& o) const { return score > o.score || (score == o.score && place < o.place); }
 };
 
-constexpr int kMostBeams = 32, kJoinListed = 1024;
+constexpr int kMostBeams = 32;
 
-template <int kThreads> struct JoinShared {
+template <int kThreads, int kJoinListed> struct JoinShared {
     unsigned long long list_score[kJoinListed];
     double whole[kMostBeams], have[kMostBeams];  // log of a beam's sum, its score
     unsigned long long wave_score[kThreads / 64];
@@ -421,9 +422,9 @@ template <int kThreads> struct JoinShared {
 // A sequence's answer, by a workgroup: the logarithms of the beams' sums, a wave a beam, then the
 // best of all parts' candidates by the same bound, over the upper bits of their scores.  sums and keys are
 // the sequence's, and need not be set for beams without candidates.
-template <int kThreads, bool kF16, bool kOnePart>
+template <int kThreads, bool kF16, bool kOnePart, int kJoinListed>
 __device__ __forceinline__ void join_parts(const BeamArgs& a, int seq, int parts, const PartSum* sums, const unsigned long long* keys,
-                                           JoinShared<kThreads>& shared) {
+                                           JoinShared<kThreads, kJoinListed>& shared) {
     constexpr int kWaves = kThreads / 64, kKept = 2;  // candidates a thread keeps between its two looks at them
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const size_t row0 = (size_t)seq * a.beams;
@@ -489,7 +490,7 @@ __device__ __forceinline__ void join_parts(const BeamArgs& a, int seq, int parts
     }
     for (int i = tid + kKept * kThreads; i < front; i += kThreads) larger(candidate(i / depth, i % depth));
     uint32_t bound = 0;
-    // a few are all ranked (16 of them 7.6 us of a call of one launch, 8.0 with a bound; 32 8.3 and 8.2; 128 7.9 us
+    // a few are all ranked (16 of them 7.6 us of a call of one launch, 8.0 with a bound; 32 8.3 and 7.9; 128 7.9 us
     // of the join, 5.0 with a bound)
     if (front > 16 || depth < a.choices) {
         const bool few = a.choices <= (kOnePart ? kFewWhole : kFewChoices);
@@ -574,20 +575,23 @@ constexpr int kJoinThreads = 512;
 template <bool kF16>
 __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int parts, const PartSum* __restrict__ sums,
                                                                  const unsigned long long* __restrict__ best) {
-    __shared__ JoinShared<kJoinThreads> shared;
+    __shared__ JoinShared<kJoinThreads, 1024> shared;
     const size_t first = (size_t)blockIdx.x * a.beams;
     join_parts<kJoinThreads, kF16, false>(a, blockIdx.x, parts, sums + first * parts, best + first * parts * a.choices, shared);
 }
 
-// Both in one launch where the rows are short and a sequence has few beams: kGroup threads a beam.
-constexpr int kWholeThreads = 1024, kWholeBeams = 16, kWholeVectors = 512;  // 16-byte loads a row
+// Both in one launch where the rows are short and a sequence has few beams: a wave a beam (4 waves a beam: 8
+// sequences of 4 of 1025 logits 7.9 us instead of 7.6, 2048 of them 34 instead of 17, as fewer fit a CU at once).
+constexpr int kWholeBeams = 16, kWholeVectors = 512;  // 16-byte loads a row
 
-template <bool kF16, int kGroup>
-__global__ __launch_bounds__(kWholeThreads) __attribute__((amdgpu_num_sgpr(kSgprs))) void beam_whole_kernel(BeamArgs a) {
-    constexpr int kGroups = kWholeThreads / kGroup;
+// (of 16 waves two workgroups a CU: 4096 sequences of 16 of 600 fp16 logits 105 us instead of 141)
+template <bool kF16, int kThreads>
+__global__ __launch_bounds__(kThreads, kThreads == 1024 ? 8 : 1) __attribute__((amdgpu_num_sgpr(kSgprs))) void beam_whole_kernel(BeamArgs a) {
+    constexpr int kGroup = 64;
+    constexpr int kGroups = kThreads / kGroup;
     __shared__ PartShared<kGroup> part[kGroups];
     __shared__ int over;
-    __shared__ JoinShared<kWholeThreads> shared;
+    __shared__ JoinShared<kThreads, kGroups * 64> shared;  // (has room for all choices of all beams)
     __shared__ PartSum sums[kGroups];
     __shared__ unsigned long long keys[kGroups * 64];
     const int seq = blockIdx.x, b = threadIdx.x / kGroup;
@@ -596,9 +600,9 @@ __global__ __launch_bounds__(kWholeThreads) __attribute__((amdgpu_num_sgpr(kSgpr
     const uint8_t done = a.ended ? a.ended[row] : 0;
     const auto real = [&] { return b < a.beams && !done && __builtin_fabsf(score) < __builtin_inff(); };
     best_of_part<kF16, kWholeVectors / kGroup, kGroup, kFewWhole>((const char*)a.logits + row * a.stride * (kF16 ? 2 : 4), real, a.vocab, 0, a.choices,
-                                                       threadIdx.x % kGroup, part[b], over, sums + b, b < a.beams ? keys + b * a.choices : nullptr);
+                                                                  threadIdx.x % kGroup, part[b], over, sums + b, b < a.beams ? keys + b * a.choices : nullptr);
     __syncthreads();
-    join_parts<kWholeThreads, kF16, true>(a, seq, 1, sums, keys, shared);
+    join_parts<kThreads, kF16, true>(a, seq, 1, sums, keys, shared);
 }
 
 // Loads a thread, and with them the parts: many workgroups where rows are few or short, else many
@@ -625,9 +629,10 @@ size_t beam_workspace(int sequences, int beams, int vocab, int choices) {
 template <bool kF16> static void select(const BeamArgs& a, hipStream_t s) {
     const int rows = a.sequences * a.beams, loads = beam_loads<kF16>(rows, a.vocab), parts = beam_parts<kF16>(loads, a.vocab);
     if (parts == 1 && loads <= 2 && a.beams <= kWholeBeams) {
-        if (a.beams <= 4) beam_whole_kernel<kF16, 256><<<(unsigned)a.sequences, kWholeThreads, 0, s>>>(a);
-        else if (a.beams <= 8) beam_whole_kernel<kF16, 128><<<(unsigned)a.sequences, kWholeThreads, 0, s>>>(a);
-        else beam_whole_kernel<kF16, 64><<<(unsigned)a.sequences, kWholeThreads, 0, s>>>(a);
+        const auto whole = [&](auto kernel, int threads) { kernel<<<(unsigned)a.sequences, threads, 0, s>>>(a); };
+        if (a.beams <= 4) whole(beam_whole_kernel<kF16, 256>, 256);
+        else if (a.beams <= 8) whole(beam_whole_kernel<kF16, 512>, 512);
+        else whole(beam_whole_kernel<kF16, 1024>, 1024);
         return;
     }
     PartSum* sums = (PartSum*)a.workspace;
