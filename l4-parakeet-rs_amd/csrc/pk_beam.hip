@@ -649,104 +649,135 @@ void launch_beam_select(bool fp16, const BeamArgs& a, hipStream_t s) {
     else select<false>(a, s);
 }
 
-// Rows in their beams' new order, into another array: a workgroup copies a chunk of a row.  Chunks of
-// the same columns lie on one XCD, whose L2 then reads a parent's once for all its children (16 x 8
-// rows of 2 MB: 74 us, 80 without; a copy of all of them 99).  Stores past the caches where the
-// state is larger than they are (74 us against 80).
+// Rows in their beams' new order.  They go in units of 16 bytes, and where addresses or the row's bytes are no
+// multiples of 16 the units lie at any address, which costs no more than lines touched twice (4096 x 8 rows of
+// 4099 bytes 36 us, in single bytes 343; of 20004 183 us, in words of 4 511).  The last unit of a row ends where the
+// row ends, and writes some bytes a second time.
+typedef int AnyAddress __attribute__((ext_vector_type(4), aligned(1)));
+struct Wide {
+    static constexpr int kBytes = 16;
+    v4i v;
+    __device__ __forceinline__ void load(const char* p) { v = *(const AnyAddress*)p; }
+    __device__ __forceinline__ void store(char* p) const { *(AnyAddress*)p = v; }
+    __device__ __forceinline__ void store_past(char* p) const { __builtin_nontemporal_store(v, (AnyAddress*)p); }
+};
+struct Byte {
+    static constexpr int kBytes = 1;
+    uint8_t v;
+    __device__ __forceinline__ void load(const char* p) { v = *(const uint8_t*)p; }
+    __device__ __forceinline__ void store(char* p) const { *(uint8_t*)p = v; }
+};
+
+template <typename Unit> __device__ __forceinline__ long long unit_at(long long unit, long long row_bytes) {
+    const long long at = unit * Unit::kBytes, last = row_bytes - Unit::kBytes;
+    return at < last ? at : last;
+}
+
+// Into another array: a workgroup copies a chunk of a row.  Chunks of the same columns lie on one
+// XCD, whose L2 then reads a parent's once for all its children (16 x 8 rows of 2 MB: 74 us, 80
+// without; a copy of all of them 99).  Stores past the caches where the state is larger than they
+// are (74 us against 80).
 constexpr int kRowLoads = 2;
 
-template <typename Unit, bool kPast>
-__global__ __launch_bounds__(256) void beam_rows_kernel(const Unit* __restrict__ in, const int* __restrict__ parents, Unit* __restrict__ out, int beams,
-                                                        long long units, int chunks, int step) {
+template <bool kPast>
+__global__ __launch_bounds__(256) void beam_rows_kernel(const char* __restrict__ in, const int* __restrict__ parents, char* __restrict__ out, int beams,
+                                                        long long row_bytes, long long units, int chunks, int step) {
     const long long row0 = (long long)blockIdx.y * beams;
     const int t = step >= 8 ? blockIdx.x >> 3 : blockIdx.x, b = t % beams;  // XCDs take workgroups in turn
     const long long p = (long long)parents[row0 + b] - row0;
     if (p < 0 || p >= beams) return;
-    const Unit* const from = in + (row0 + p) * units;
-    Unit* const to = out + (row0 + b) * units;
+    const char* const from = in + (row0 + p) * row_bytes;
+    char* const to = out + (row0 + b) * row_bytes;
     for (int chunk = step >= 8 ? t / beams * 8 + (blockIdx.x & 7) : t / beams; chunk < chunks; chunk += step) {
         const long long first = (long long)chunk * 256 * kRowLoads + threadIdx.x;
-        Unit held[kRowLoads];
+        Wide held[kRowLoads];
 #pragma unroll
         for (int n = 0; n < kRowLoads; ++n)
-            if (first + n * 256 < units) held[n] = from[first + n * 256];
+            if (first + n * 256 < units) held[n].load(from + unit_at<Wide>(first + n * 256, row_bytes));
 #pragma unroll
         for (int n = 0; n < kRowLoads; ++n)
             if (first + n * 256 < units) {
-                if constexpr (kPast) __builtin_nontemporal_store(held[n], to + first + n * 256);
-                else to[first + n * 256] = held[n];
+                char* const at = to + unit_at<Wide>(first + n * 256, row_bytes);
+                if constexpr (kPast) held[n].store_past(at);
+                else held[n].store(at);
             }
     }
 }
 
 // Short rows: a thread a unit of all rows, one behind the other.
 template <typename Unit>
-__global__ __launch_bounds__(256) void beam_units_kernel(const Unit* __restrict__ in, const int* __restrict__ parents, Unit* __restrict__ out, uint32_t beams,
-                                                         uint32_t units, uint32_t all) {
+__global__ __launch_bounds__(256) void beam_units_kernel(const char* __restrict__ in, const int* __restrict__ parents, char* __restrict__ out, uint32_t beams,
+                                                         uint32_t row_bytes, uint32_t units, uint32_t all) {
     const uint32_t at = blockIdx.x * 256 + threadIdx.x;
     if (at >= all) return;
     const uint32_t row = at / units, parent = (uint32_t)parents[row];
-    if (parent / beams == row / beams) out[at] = in[parent * units + (at - row * units)];
+    const long long in_row = unit_at<Unit>(at - row * units, row_bytes);
+    if (parent / beams != row / beams) return;
+    Unit one;
+    one.load(in + (size_t)parent * row_bytes + in_row);
+    one.store(out + (size_t)row * row_bytes + in_row);
 }
-// Of 16, 4 or 1 bytes a row (32768 rows of 80 of 16 bytes 12.4 us, 25.2 with a workgroup a row; 250 33.2 and 34.0;
-// 400 65 and 51).
+// Units a row (32768 rows of 80 units 12.4 us, 25.2 with a workgroup a row; 250 33.2 and 34.0; 400 65 and 51).
 constexpr long long kShortUnits = 256;
 
-// In place: a thread owns a column of a sequence's rows, reads what they will hold and writes
-// those that change then (the rows above: 66 us, for fewer of them are written).
+// In place: a thread owns a column of a sequence's rows, a unit wide, reads what they will hold and writes those that
+// change then (the rows above: 66 us, for fewer of them are written).
 template <typename Unit, int kBeams>
-__global__ __launch_bounds__(256) void beam_columns_kernel(Unit* state, const int* __restrict__ parents, int beams, long long units) {
+__global__ __launch_bounds__(256) void beam_columns_kernel(char* state, const int* __restrict__ parents, int beams, long long row_bytes, long long units) {
     const long long row0 = (long long)blockIdx.y * beams;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < units; i += (long long)gridDim.x * 256) {
+        char* const column = state + row0 * row_bytes + i * Unit::kBytes;
         Unit held[kBeams];
 #pragma unroll
         for (int b = 0; b < kBeams; ++b) {
             const int at = b < beams ? b : 0;
             const long long p = (long long)parents[row0 + at] - row0;
-            held[b] = state[(row0 + (p >= 0 && p < beams ? p : at)) * units + i];
+            held[b].load(column + (p >= 0 && p < beams ? p : at) * row_bytes);
         }
 #pragma unroll
         for (int b = 0; b < kBeams; ++b) {
             const long long p = b < beams ? (long long)parents[row0 + b] - row0 : -1;
-            if (p >= 0 && p < beams && p != b) state[(row0 + b) * units + i] = held[b];
+            if (p >= 0 && p < beams && p != b) held[b].store(column + b * row_bytes);
         }
     }
 }
 
 constexpr int kMostChunks = 1 << 16;  // of a row, in a launch: its threads in a dimension stay far below 2^32
 
-template <typename Unit, bool kPast>
-static void reorder_rows(const void* in, const int* parents, void* out, int sequences, int beams, long long units, hipStream_t s) {
+template <bool kPast> static void reorder_rows(const char* in, const int* parents, char* out, int sequences, int beams, long long row_bytes, long long units, hipStream_t s) {
     const int chunks = (int)((units + 256 * kRowLoads - 1) / (256 * kRowLoads)), once = chunks < kMostChunks ? chunks : kMostChunks;
     const int step = once >= 8 ? (once + 7) / 8 * 8 : once;
-    beam_rows_kernel<Unit, kPast><<<dim3((unsigned)(step * beams), (unsigned)sequences), 256, 0, s>>>((const Unit*)in, parents, (Unit*)out, beams, units,
-                                                                                                      chunks, step);
+    beam_rows_kernel<kPast><<<dim3((unsigned)(step * beams), (unsigned)sequences), 256, 0, s>>>(in, parents, out, beams, row_bytes, units, chunks, step);
 }
 
-template <typename Unit>
-static void reorder(const void* in, const int* parents, void* out, int sequences, int beams, long long row_bytes, hipStream_t s) {
-    const long long units = row_bytes / (long long)sizeof(Unit);
-    const long long all = units * sequences * beams;
-    if (in != out && units <= kShortUnits && all < 1ll << 31) {
-        beam_units_kernel<Unit><<<(unsigned)((all + 255) / 256), 256, 0, s>>>((const Unit*)in, parents, (Unit*)out, beams, (uint32_t)units, (uint32_t)all);
-        return;
-    }
-    if (in != out) {
-        if (row_bytes * sequences * beams > kCached) reorder_rows<Unit, true>(in, parents, out, sequences, beams, units, s);
-        else reorder_rows<Unit, false>(in, parents, out, sequences, beams, units, s);
-        return;
-    }
+template <typename Unit> static void reorder_units(const char* in, const int* parents, char* out, int sequences, int beams, int row_bytes, hipStream_t s) {
+    const uint32_t units = (row_bytes + Unit::kBytes - 1) / Unit::kBytes, all = units * sequences * beams;  // at most 2^25
+    beam_units_kernel<Unit><<<(all + 255) / 256, 256, 0, s>>>(in, parents, out, beams, row_bytes, units, all);
+}
+
+template <typename Unit> static void reorder_columns(char* state, const int* parents, int sequences, int beams, long long row_bytes, long long units, hipStream_t s) {
     const long long blocks = (units + 255) / 256;
     const dim3 grid((unsigned)(blocks < kMostChunks ? blocks : kMostChunks), (unsigned)sequences);
-    if (beams <= 8) beam_columns_kernel<Unit, 8><<<grid, 256, 0, s>>>((Unit*)out, parents, beams, units);
-    else beam_columns_kernel<Unit, 32><<<grid, 256, 0, s>>>((Unit*)out, parents, beams, units);
+    if (beams <= 8) beam_columns_kernel<Unit, 8><<<grid, 256, 0, s>>>(state, parents, beams, row_bytes, units);
+    else beam_columns_kernel<Unit, 32><<<grid, 256, 0, s>>>(state, parents, beams, row_bytes, units);
 }
 
 void launch_beam_reorder(const void* state, const int* parents, void* out, int sequences, int beams, long long row_bytes, hipStream_t s) {
-    const uintptr_t all = (uintptr_t)state | (uintptr_t)out | (uintptr_t)row_bytes;
-    if (all % 16 == 0) reorder<v4i>(state, parents, out, sequences, beams, row_bytes, s);
-    else if (all % 4 == 0) reorder<uint32_t>(state, parents, out, sequences, beams, row_bytes, s);
-    else reorder<uint8_t>(state, parents, out, sequences, beams, row_bytes, s);
+    const char* in = (const char*)state;
+    char* to = (char*)out;
+    if (in != to) {
+        const long long units = (row_bytes + Wide::kBytes - 1) / Wide::kBytes;
+        if (row_bytes < Wide::kBytes) reorder_units<Byte>(in, parents, to, sequences, beams, (int)row_bytes, s);
+        else if (units <= kShortUnits) reorder_units<Wide>(in, parents, to, sequences, beams, (int)row_bytes, s);
+        else if (row_bytes * sequences * beams > kCached) reorder_rows<true>(in, parents, to, sequences, beams, row_bytes, units, s);
+        else reorder_rows<false>(in, parents, to, sequences, beams, row_bytes, units, s);
+        return;
+    }
+    // no unit of a column may reach into another's: the last bytes are columns of their own (a second launch; 16 x 8
+    // rows of 1 MB + 1 33 us, all in single bytes 134)
+    const long long units = row_bytes / Wide::kBytes, rest = row_bytes % Wide::kBytes;
+    if (units) reorder_columns<Wide>(to, parents, sequences, beams, row_bytes, units, s);
+    if (rest) reorder_columns<Byte>(to + units * Wide::kBytes, parents, sequences, beams, row_bytes, rest, s);
 }
 
 }  // namespace pk
