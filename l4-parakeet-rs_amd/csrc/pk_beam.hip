@@ -221,7 +221,8 @@ __device__ __forceinline__ void rank_listed(const PartShared<kGroup>& shared, in
 template <bool kF16, int kLoads, int kGroup, int kFew, typename Real>
 __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab, int part, int choices, int tid, PartShared<kGroup>& shared,
                                              int& over, PartSum* sum_out, unsigned long long* to) {
-    constexpr int kVec = kF16 ? 8 : 4, kWaves = kGroup / 64, kListed = PartShared<kGroup>::kListed, kRanked = PartShared<kGroup>::kRanked, kTops = PartShared<kGroup>::kTops;
+    constexpr int kVec = kF16 ? 8 : 4, kWaves = kGroup / 64, kListed = PartShared<kGroup>::kListed, kRanked = PartShared<kGroup>::kRanked;
+    constexpr int kTops = PartShared<kGroup>::kTops;
     constexpr bool kShort = kFew == kFewWhole;  // rows are short, and loads without logits worth a branch
     constexpr int kPart = kGroup * kLoads * kVec, kBytes = kF16 ? 2 : 4;
     const int wave = tid >> 6, first = part * kPart, count_here = vocab - first < kPart ? vocab - first : kPart;
@@ -390,14 +391,16 @@ __device__ __forceinline__ int beam_state(float score, const uint8_t* ended, siz
 }
 
 template <bool kF16, int kLoads>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_num_sgpr(kSgprs))) void beam_part_kernel(BeamArgs a, int parts, PartSum* __restrict__ sums, unsigned long long* __restrict__ best) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_num_sgpr(kSgprs))) void beam_part_kernel(BeamArgs a, int parts, PartSum* __restrict__ sums,
+                                                                                                unsigned long long* __restrict__ best) {
     __shared__ PartShared<256> shared;
     __shared__ int over;
     const int row = blockIdx.x / parts, part = blockIdx.x % parts;
     if (beam_state(a.scores[row], a.ended, row) != 1) return;
     const size_t out = (size_t)row * parts + part;
-    best_of_part<kF16, kLoads, 256, kFewChoices>((const char*)a.logits + (size_t)row * a.stride * (kF16 ? 2 : 4), [] { return true; }, a.vocab, part, a.choices, threadIdx.x, shared, over,
-                               sums + out, best + out * a.choices);
+    best_of_part<kF16, kLoads, 256, kFewChoices>((const char*)a.logits + (size_t)row * a.stride * (kF16 ? 2 : 4), [] { return true; },
+                                                 a.vocab, part, a.choices, threadIdx.x, shared, over,
+                                                 sums + out, best + out * a.choices);
 }
 
 struct Candidate {
@@ -744,7 +747,8 @@ __global__ __launch_bounds__(256) void beam_columns_kernel(char* state, const in
 
 constexpr int kMostChunks = 1 << 16;  // of a row, in a launch: its threads in a dimension stay far below 2^32
 
-template <bool kPast> static void reorder_rows(const char* in, const int* parents, char* out, int sequences, int beams, long long row_bytes, long long units, hipStream_t s) {
+template <bool kPast>
+static void reorder_rows(const char* in, const int* parents, char* out, int sequences, int beams, long long row_bytes, long long units, hipStream_t s) {
     const int chunks = (int)((units + 256 * kRowLoads - 1) / (256 * kRowLoads)), once = chunks < kMostChunks ? chunks : kMostChunks;
     const int step = once >= 8 ? (once + 7) / 8 * 8 : once;
     beam_rows_kernel<kPast><<<dim3((unsigned)(step * beams), (unsigned)sequences), 256, 0, s>>>(in, parents, out, beams, row_bytes, units, chunks, step);
@@ -755,7 +759,8 @@ template <typename Unit> static void reorder_units(const char* in, const int* pa
     beam_units_kernel<Unit><<<(all + 255) / 256, 256, 0, s>>>(in, parents, out, beams, row_bytes, units, all);
 }
 
-template <typename Unit> static void reorder_columns(char* state, const int* parents, int sequences, int beams, long long row_bytes, long long units, hipStream_t s) {
+template <typename Unit>
+static void reorder_columns(char* state, const int* parents, int sequences, int beams, long long row_bytes, long long units, hipStream_t s) {
     const long long blocks = (units + 255) / 256;
     const dim3 grid((unsigned)(blocks < kMostChunks ? blocks : kMostChunks), (unsigned)sequences);
     if (beams <= 8) beam_columns_kernel<Unit, 8><<<grid, 256, 0, s>>>(state, parents, beams, row_bytes, units);
