@@ -413,7 +413,7 @@ constexpr int kMostBeams = 32;
 
 template <int kThreads, int kJoinListed> struct JoinShared {
     unsigned long long list_score[kJoinListed];
-    double whole[kMostBeams], have[kMostBeams];  // log of a beam's sum, its score
+    double most[kMostBeams], rest[kMostBeams], have[kMostBeams];  // a beam's largest logit, log sum exp(x - most), its score
     unsigned long long wave_score[kThreads / 64];
     uint32_t list_place[kJoinListed];
     uint32_t wave_place[kThreads / 64], wave_bound[kThreads / 64];
@@ -446,9 +446,10 @@ __device__ __forceinline__ void join_parts(const BeamArgs& a, int seq, int parts
         const PartSum mine_of = lane < parts ? own[lane] : none;
         const float score = a.scores[row0 + b];
         int s = beam_state(score, a.ended, row0 + b);
-        double log_sum = 0.0;
+        double rest = 0.0;
+        float most = 0.0f;
         if (s == 1) {
-            float most = mine_of.most;
+            most = mine_of.most;
             for (int p = lane + 64; p < parts; p += 64) most = __builtin_fmaxf(most, own[p].most);
             most = wave_max(most);
             double mine = 0.0;
@@ -461,11 +462,13 @@ __device__ __forceinline__ void join_parts(const BeamArgs& a, int seq, int parts
                 const double factor = kOnePart ? 1.0 + z * (1.0 + z * (0.5 + z * (1.0 / 6))) : exp(((double)one.most - (double)most) + z);
                 mine += some ? one.sum * factor : one.sum;
             }
-            log_sum = (double)most + log(wave_sum(mine));
-            s = most > -__builtin_inff() && most < __builtin_inff() && log_sum == log_sum;  // a NaN or an infinity: no candidates
+            // (kept apart from the maximum: beside one of 2^53 and more, an fp32 mask's lowest value, nothing of it would be left)
+            rest = log(wave_sum(mine));
+            s = most > -__builtin_inff() && most < __builtin_inff() && rest == rest;  // a NaN or an infinity: no candidates
         }
         if (lane == 0) {
-            shared.whole[b] = log_sum;
+            shared.most[b] = (double)most;
+            shared.rest[b] = rest;
             shared.have[b] = (double)score;
             shared.state[b] = s;
         }
@@ -476,7 +479,7 @@ __device__ __forceinline__ void join_parts(const BeamArgs& a, int seq, int parts
         if (s == 2) return list == b * parts && c == 0 ? Candidate{ordered(shared.have[b]), (uint32_t)b * a.vocab + a.end_token} : Candidate{0, 0};
         if (!s || !key) return Candidate{0, 0};
         const double x = (double)unordered((uint32_t)(key >> 32));
-        return Candidate{ordered((x - shared.whole[b]) + shared.have[b]), (uint32_t)b * a.vocab + ~(uint32_t)key};
+        return Candidate{ordered(((x - shared.most[b]) - shared.rest[b]) + shared.have[b]), (uint32_t)b * a.vocab + ~(uint32_t)key};
     };
     const auto candidate = [&](int list, int c) { return candidate_of(list, c, keys[(size_t)list * a.choices + c]); };
     Candidate kept[kKept];

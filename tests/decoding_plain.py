@@ -87,8 +87,7 @@ def select(logits, scores, ended, end, choices):
             top = x.max()
             if not torch.isfinite(top):  # NaN, infinity, or nothing that is allowed
                 continue
-            total = top + (x - top).exp().sum().log()
-            value = (x - total) + have
+            value = ((x - top) - (x - top).exp().sum().log()) + have  # (the logarithm beside a maximum of 2^53 and more would be lost)
             order = torch.argsort(x, descending=True, stable=True)[:choices]
             every += [(-float(value[t]), b * vocab + t, t == end) for t in order.tolist() if float(x[t]) > -math.inf]
         every.sort()
