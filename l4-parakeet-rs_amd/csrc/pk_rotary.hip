@@ -277,6 +277,7 @@ void launch_head_norm_rotary_write(int kind, const RotaryArgs& a, hipStream_t s)
 // Radians a position, i of `pairs` (frequencies fall from 1 by a constant factor).
 void rotary_frequencies(int scaling, int pairs, double base, double factor, double low, double high, int original, uint64_t* out) {
     const double pi2 = 6.283185307179586476925286766559, dim = 2.0 * pairs;
+    if (scaling == 0) factor = 1.0;  // not looked at, and 0 or a NaN would be left of (1 - kept) / factor
     if (scaling == 2) base *= pow(factor, dim / (dim - 2.0));
     const auto border = [&](double turns) { return dim * log(original / (pi2 * turns)) / (2.0 * log(base)); };
     double first = 0.0, last = 0.0;
