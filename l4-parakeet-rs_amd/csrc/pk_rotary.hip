@@ -234,16 +234,18 @@ __global__ __launch_bounds__(256) void head_norm_rotary_kernel(RotaryArgs a, int
     }
 }
 
-// From this many tokens on the values of a call go in tiles (32 / 8 heads of 128, one prompt, fp16: 600
-// tokens 11.0 us without and 9.4 with, 1000 14.3 and 10.3, 1400 18.8 and 11.5; as many single tokens 11.6
-// and 15.4, 14.9 and 15.6, 21.1 and 18.1; e4m3 like these).
-constexpr int kValueTiles = 768;
+// From this many tokens on, and this many rows of values (tokens times kv heads), the values go in tiles: a tile's chain is
+// as long for one head as for many, and a lane's scattered stores are hidden while they are few (one prompt, fp16, heads of
+// 128, us without and with tiles: 8 kv heads 400 tokens 7.7 and 9.9, 800 13.2 and 11.1; 4 800 7.5 and 9.1, 2000 14.2 and
+// 9.3; 2 2000 9.3 and 9.9, 4000 14.6 and 10.9; 1 2000 7.8 and 9.8, 8000 17.5 and 13.6; as many single tokens, 8 kv heads,
+// 400 10.0 and 16.5, 800 16.1 and 18.1, 4000 206 and 212; e4m3 like these).
+constexpr int kTileTokens = 768, kTileRows = 6144;
 // Up to this many waves a wave takes one set of heads, else all of its token's (rows of fp16: 1000 tokens
 // 7.2 us in 5000 waves and 7.6 in 1000, 1500 9.2 and 9.1, 3000 15.0 and 12.0).
 constexpr int kMostSetWaves = 8192;
 
 template <int kCache, bool kPast> static void launch_rotary(const RotaryArgs& a, hipStream_t s) {
-    const bool tiles = kCache >= 0 && a.tokens >= kValueTiles;
+    const bool tiles = kCache >= 0 && a.tokens >= kTileTokens && a.tokens * a.kv_heads >= kTileRows;  // (at most 2^29)
     const int value_blocks = tiles ? a.kv_heads * ((a.tokens + kWriteTokens - 1) / kWriteTokens) : 0;
     const auto launch = [&](auto kernel, int lanes) {
         const int each = 64 / lanes, kv_sets = (a.kv_heads + each - 1) / each;
