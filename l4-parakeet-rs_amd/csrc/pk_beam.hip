@@ -729,23 +729,36 @@ constexpr long long kShortUnits = 256;
 // In place: a thread owns a column of a sequence's rows, a unit wide, reads what they will hold and writes those that
 // change then (the rows above: 66 us, for fewer of them are written).
 template <typename Unit, int kBeams>
-__global__ __launch_bounds__(256) void beam_columns_kernel(char* state, const int* __restrict__ parents, int beams, long long row_bytes, long long units) {
-    const long long row0 = (long long)blockIdx.y * beams;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < units; i += (long long)gridDim.x * 256) {
-        char* const column = state + row0 * row_bytes + i * Unit::kBytes;
-        Unit held[kBeams];
+__device__ __forceinline__ void turn_column(char* column, const int* __restrict__ parents, long long row0, int beams, long long row_bytes) {
+    Unit held[kBeams];
 #pragma unroll
-        for (int b = 0; b < kBeams; ++b) {
-            const int at = b < beams ? b : 0;
-            const long long p = (long long)parents[row0 + at] - row0;
-            held[b].load(column + (p >= 0 && p < beams ? p : at) * row_bytes);
-        }
-#pragma unroll
-        for (int b = 0; b < kBeams; ++b) {
-            const long long p = b < beams ? (long long)parents[row0 + b] - row0 : -1;
-            if (p >= 0 && p < beams && p != b) held[b].store(column + b * row_bytes);
-        }
+    for (int b = 0; b < kBeams; ++b) {
+        const int at = b < beams ? b : 0;
+        const long long p = (long long)parents[row0 + at] - row0;
+        held[b].load(column + (p >= 0 && p < beams ? p : at) * row_bytes);
     }
+#pragma unroll
+    for (int b = 0; b < kBeams; ++b) {
+        const long long p = b < beams ? (long long)parents[row0 + b] - row0 : -1;
+        if (p >= 0 && p < beams && p != b) held[b].store(column + b * row_bytes);
+    }
+}
+
+// No unit of a column may reach into another's: the `rest` bytes behind the last unit are columns of their own, which the
+// last workgroup has (16 x 8 rows of 1 MB + 1 30 us, all in single bytes 134; 2 beams of 100 bytes 3.1 us, 5.2 with a launch
+// for them, 64 x 16 of 100 9.1 and 15.0).
+template <int kBeams>
+__global__ __launch_bounds__(256) void beam_columns_kernel(char* state, const int* __restrict__ parents, int beams, long long row_bytes, long long units,
+                                                           int rest) {
+    const long long row0 = (long long)blockIdx.y * beams;
+    char* const rows = state + row0 * row_bytes;
+    const long long blocks = (long long)gridDim.x - (rest != 0);
+    if (blockIdx.x >= blocks) {
+        if ((int)threadIdx.x < rest) turn_column<Byte, kBeams>(rows + units * Wide::kBytes + threadIdx.x, parents, row0, beams, row_bytes);
+        return;
+    }
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < units; i += blocks * 256)
+        turn_column<Wide, kBeams>(rows + i * Wide::kBytes, parents, row0, beams, row_bytes);
 }
 
 constexpr int kMostChunks = 1 << 16;  // of a row, in a launch: its threads in a dimension stay far below 2^32
@@ -762,12 +775,12 @@ template <typename Unit> static void reorder_units(const char* in, const int* pa
     beam_units_kernel<Unit><<<(all + 255) / 256, 256, 0, s>>>(in, parents, out, beams, row_bytes, units, all);
 }
 
-template <typename Unit>
-static void reorder_columns(char* state, const int* parents, int sequences, int beams, long long row_bytes, long long units, hipStream_t s) {
-    const long long blocks = (units + 255) / 256;
-    const dim3 grid((unsigned)(blocks < kMostChunks ? blocks : kMostChunks), (unsigned)sequences);
-    if (beams <= 8) beam_columns_kernel<Unit, 8><<<grid, 256, 0, s>>>(state, parents, beams, row_bytes, units);
-    else beam_columns_kernel<Unit, 32><<<grid, 256, 0, s>>>(state, parents, beams, row_bytes, units);
+static void reorder_columns(char* state, const int* parents, int sequences, int beams, long long row_bytes, hipStream_t s) {
+    const long long units = row_bytes / Wide::kBytes, blocks = (units + 255) / 256;
+    const int rest = (int)(row_bytes % Wide::kBytes);
+    const dim3 grid((unsigned)((blocks < kMostChunks ? blocks : kMostChunks) + (rest != 0)), (unsigned)sequences);
+    if (beams <= 8) beam_columns_kernel<8><<<grid, 256, 0, s>>>(state, parents, beams, row_bytes, units, rest);
+    else beam_columns_kernel<32><<<grid, 256, 0, s>>>(state, parents, beams, row_bytes, units, rest);
 }
 
 void launch_beam_reorder(const void* state, const int* parents, void* out, int sequences, int beams, long long row_bytes, hipStream_t s) {
@@ -781,11 +794,7 @@ void launch_beam_reorder(const void* state, const int* parents, void* out, int s
         else reorder_rows<false>(in, parents, to, sequences, beams, row_bytes, units, s);
         return;
     }
-    // no unit of a column may reach into another's: the last bytes are columns of their own (a second launch; 16 x 8
-    // rows of 1 MB + 1 33 us, all in single bytes 134)
-    const long long units = row_bytes / Wide::kBytes, rest = row_bytes % Wide::kBytes;
-    if (units) reorder_columns<Wide>(to, parents, sequences, beams, row_bytes, units, s);
-    if (rest) reorder_columns<Byte>(to + units * Wide::kBytes, parents, sequences, beams, row_bytes, rest, s);
+    reorder_columns(to, parents, sequences, beams, row_bytes, s);
 }
 
 }  // namespace pk

@@ -7,8 +7,10 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import test_gpu_rotary as rotary  # noqa: E402
+from test_gpu_beams import reordered  # noqa: E402
 from test_gpu_pages import Pool  # noqa: E402
 from test_gpu_parity import pk  # noqa: E402, F401
+from test_gpu_serving import gen  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +34,20 @@ def test_fork_in_one_launch_and_in_several(pk, rows, columns, spare):  # noqa: F
 @pytest.mark.parametrize("fp8", [False, True])
 def test_write_of_values_in_tiles_and_without(pk, tokens, heads, kv, d, r, page, how, fp8):  # noqa: F811
     rotary.test_write(pk, tokens, heads, kv, d, r, page, how, fp8, tokens % 2 == 0)
+
+
+@pytest.mark.parametrize("row", [1, 15, 16, 17, 31, 4095, 4096, 4097, 4111, 8207])
+@pytest.mark.parametrize("beams", [1, 2, 8, 9, 32])
+def test_reorder_in_place_of_units_and_single_bytes(pk, row, beams):  # noqa: F811
+    """Rows of no unit, of units alone and with bytes behind them, in the first and last workgroup of a sequence; an unaligned
+    state whose neighbours stay as they are."""
+    n, g = 7, gen(row + beams)
+    whole = torch.randint(0, 256, (n * beams * row + 32,), generator=g, device="cuda", dtype=torch.uint8)
+    parents = torch.randint(0, beams, (n, beams), generator=g, device="cuda") + beams * torch.arange(n, device="cuda")[:, None]
+    parents = torch.where(torch.rand((n, beams), generator=g, device="cuda") < 0.2, -1, parents).int()
+    for shift in (0, 5):
+        state = whole[16 + shift:16 + shift + n * beams * row].view(n, beams, row)
+        before, want = whole.clone(), reordered(state, parents, state)
+        pk.beam_reorder(state, parents, state)
+        assert torch.equal(state, want)
+        assert torch.equal(whole[:16 + shift], before[:16 + shift]) and torch.equal(whole[16 + shift + n * beams * row:], before[16 + shift + n * beams * row:])
