@@ -31,10 +31,11 @@ constexpr int kMostLoads = 8;  // of 16 bytes a thread
 // Scalar registers: with more a SIMD holds fewer than 8 waves, and a CU one workgroup of 16 waves instead of two (a
 // call of thousands of them 47 us instead of 34).
 constexpr int kSgprs = 80;
-// Up to as many choices a bound of one wave is near enough, in one launch and in two (64 sequences of 16 beams,
-// 1025 logits: 15.7 us with it and 18.6 with the other for 24 choices, 17.9 and 19.3 for 32, 23.2 and 21.8 for 40;
-// of 8 beams, 131071 fp16 logits: 40.5 and 39.6 for 16, 47 and 40.5 for 24, and 897 and 50 for 64, where it is the
-// lowest of its lanes).
+// Up to as many choices a bound of one wave is near enough, in one launch (and in parts of one load a thread) and in two
+// (64 sequences of 16 beams, 1025 logits: 15.7 us with it and 18.6 with the other for 24 choices, 17.9 and 19.3 for 32,
+// 23.2 and 21.8 for 40; 1000 of 20 beams, 300 fp32 logits: 68 and 84 for 20, 76 and 91 for 32; of parts of two loads 8 of
+// 16 beams, 20000 logits: 18.8 and 18.4 for 20, 23.2 and 20.3 for 32; of eight 64 of 8 beams, 131071 fp16 logits: 40.5 and
+// 39.6 for 16, 47 and 40.5 for 24, and 897 and 50 for 64, where it is the lowest of its lanes).
 constexpr int kFewWhole = 32, kFewChoices = 16;
 
 // Of a part: its largest logit m and sum exp2(x log2e - c), c = fp32(m log2e) (fp16 logits), or
@@ -223,7 +224,7 @@ __device__ __forceinline__ void best_of_part(const char* x, Real real, int vocab
                                              int& over, PartSum* sum_out, unsigned long long* to) {
     constexpr int kVec = kF16 ? 8 : 4, kWaves = kGroup / 64, kListed = PartShared<kGroup>::kListed, kRanked = PartShared<kGroup>::kRanked;
     constexpr int kTops = PartShared<kGroup>::kTops;
-    constexpr bool kShort = kFew == kFewWhole;  // rows are short, and loads without logits worth a branch
+    constexpr bool kShort = kGroup == 64;  // rows are short, and loads without logits worth a branch
     constexpr int kPart = kGroup * kLoads * kVec, kBytes = kF16 ? 2 : 4;
     const int wave = tid >> 6, first = part * kPart, count_here = vocab - first < kPart ? vocab - first : kPart;
     const char* const here_x = x + (size_t)first * kBytes;
@@ -398,9 +399,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_num_sgpr(kSgprs))) void 
     const int row = blockIdx.x / parts, part = blockIdx.x % parts;
     if (beam_state(a.scores[row], a.ended, row) != 1) return;
     const size_t out = (size_t)row * parts + part;
-    best_of_part<kF16, kLoads, 256, kFewChoices>((const char*)a.logits + (size_t)row * a.stride * (kF16 ? 2 : 4), [] { return true; },
-                                                 a.vocab, part, a.choices, threadIdx.x, shared, over,
-                                                 sums + out, best + out * a.choices);
+    constexpr int kFew = kLoads == 1 ? kFewWhole : kFewChoices;
+    best_of_part<kF16, kLoads, 256, kFew>((const char*)a.logits + (size_t)row * a.stride * (kF16 ? 2 : 4), [] { return true; }, a.vocab, part, a.choices,
+                                          threadIdx.x, shared, over, sums + out, best + out * a.choices);
 }
 
 struct Candidate {

@@ -1,5 +1,6 @@
 """Sizes at which the calls around a decoding step's cache go from one form of a kernel to another: both sides, against the
 plain forms."""
+import math
 import random
 
 import pytest
@@ -7,7 +8,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import test_gpu_rotary as rotary  # noqa: E402
-from test_gpu_beams import reordered  # noqa: E402
+from test_gpu_beams import Search, reordered  # noqa: E402
 from test_gpu_pages import Pool  # noqa: E402
 from test_gpu_parity import pk  # noqa: E402, F401
 from test_gpu_serving import gen  # noqa: E402
@@ -51,3 +52,16 @@ def test_reorder_in_place_of_units_and_single_bytes(pk, row, beams):  # noqa: F8
         pk.beam_reorder(state, parents, state)
         assert torch.equal(state, want)
         assert torch.equal(whole[:16 + shift], before[:16 + shift]) and torch.equal(whole[16 + shift + n * beams * row:], before[16 + shift + n * beams * row:])
+
+
+@pytest.mark.parametrize("beams,vocab", [(17, 300), (20, 64), (32, 1024), (20, 1028)])
+@pytest.mark.parametrize("choices", [16, 17, 32, 33])
+@pytest.mark.parametrize("fp16", [False, True])
+def test_select_of_short_rows_of_many_beams(pk, beams, vocab, choices, fp16):  # noqa: F811
+    """More beams than the one launch takes, rows of up to a load a thread and of more: bounds of one wave and of all threads."""
+    s = Search(pk, 3, beams, vocab, choices, fp16, seed=17)
+    s.go()
+    s.logits[0] = 0.25                      # equal logits, more than a list holds
+    s.logits[1, :, choices // 2:] = -math.inf  # fewer candidates a row than choices
+    s.logits[2] = s.logits[2].round()
+    s.go()
