@@ -838,7 +838,9 @@ int32_t pk_head_norm_rotary_write(int32_t kind, const uint16_t* query, int64_t q
  * NULL); where candidates run out score -infinity, token -1, parent -1, ended 0.
  * end_token in [0, vocab), or -1: none (ended is NULL then).  Sums and scores are compared in 64
  * bits, terms of the sums are fp32; equal rows of one call have equal sums, wherever they
- * lie (a row's sum is cut into parts by the call's sizes).  sequences <= 4096, beams <= 32,
+ * lie (a row's sum is cut into parts by the call's sizes); sums of rows that differ are off by
+ * their terms' roundings (2^-24), so that scores equal by the formula alone may be told apart.
+ * A score below fp32's range is written as -infinity.  sequences <= 4096, beams <= 32,
  * choices <= 64, vocab <= 2^20, at most 2^36 logits.  logits as their type aligned, workspace (16-byte aligned) of
  * pk_beam_select_workspace_bytes (enough also for fewer sequences, beams, tokens and
  * choices), used by one call at a time, need not be kept; outputs and workspace

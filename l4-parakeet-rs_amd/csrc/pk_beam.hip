@@ -20,8 +20,9 @@
 // candidates that 64 bits tell apart.
 //
 // Wide rows are bound by vector instructions (some 660 a wave for 64 logits a lane, which keep the SIMDs
-// busy for four fifths of the time) at 4.5 TB/s; a call of few is a chain: loads, a maximum and a
-// bisection over lanes, exponentials, the list, the join.
+// busy for four fifths of the time) at 4.5 TB/s; so are short rows of many sequences, a wave a row (850 a wave for 600
+// fp16 logits, of which the wave has places for 4096: 4096 sequences of 8 beams 56 us, SIMDs busy 95 % of the time); a
+// call of few is a chain: loads, a maximum and a bisection over lanes, exponentials, the list, the join.
 #include "pk_kernels.hpp"
 
 namespace pk {
@@ -591,7 +592,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
 // sequences of 4 of 1025 logits 7.9 us instead of 7.6, 2048 of them 34 instead of 17, as fewer fit a CU at once).
 constexpr int kWholeBeams = 16, kWholeVectors = 512;  // 16-byte loads a row
 
-// (of 16 waves two workgroups a CU: 4096 sequences of 16 of 600 fp16 logits 105 us instead of 141)
+// (of 16 waves two workgroups a CU: 4096 sequences of 16 of 600 fp16 logits, 8 choices, 105 us instead of 141)
 template <bool kF16, int kThreads>
 __global__ __launch_bounds__(kThreads, kThreads == 1024 ? 8 : 1) __attribute__((amdgpu_num_sgpr(kSgprs))) void beam_whole_kernel(BeamArgs a) {
     constexpr int kGroup = 64;
@@ -728,7 +729,8 @@ __global__ __launch_bounds__(256) void beam_units_kernel(const char* __restrict_
 constexpr long long kShortUnits = 256;
 
 // In place: a thread owns a column of a sequence's rows, a unit wide, reads what they will hold and writes those that
-// change then (the rows above: 66 us, for fewer of them are written).
+// change then (the rows above: 66 us, for fewer of them are written).  From 9 beams on the places of 32 are read, those
+// behind the last beam as its first row's (64 sequences, rows of 64 KB: 8 beams 7.3 us, 9 20.4, 16 22.7, 32 34.2).
 template <typename Unit, int kBeams>
 __device__ __forceinline__ void turn_column(char* column, const int* __restrict__ parents, long long row0, int beams, long long row_bytes) {
     Unit held[kBeams];
