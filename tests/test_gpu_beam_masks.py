@@ -57,3 +57,22 @@ def test_few_of_the_largest_value(pk, vocab):  # noqa: F811
     s.scores[:] = torch.tensor([-2.0, -1.0, -0.5])
     s.run()
     check(s)
+
+
+@pytest.mark.parametrize("beams", [2, 20])
+def test_a_score_below_the_range_is_written_as_infinity(pk, beams):  # noqa: F811
+    """Its token and parent are written all the same, in the order of the scores in 64 bits; as a beam it has no candidates then."""
+    s = Search(pk, 1, beams, 9, 18, False, seed=33)
+    s.scores[:] = -math.inf
+    s.scores[0, 0], s.scores[0, 1] = -3e38, -1.0
+    s.logits[0, 0] = -3e38
+    s.logits[0, 0, 4] = 0.0
+    s.logits[0, 1] = 1.0
+    s.run()
+    score = s.out.tolist()[0]
+    assert score[:9] == [score[0]] * 9 and abs(score[0] + 1 + math.log(9)) < 1e-5 and score[9] == float(torch.tensor(-3e38))
+    assert score[10:] == [-math.inf] * 8 and s.tokens.tolist()[0] == [*range(9), 4, 0, 1, 2, 3, 5, 6, 7, 8] and s.parents.tolist()[0] == [1] * 9 + [0] * 9
+    s.scores[0, 1] = -math.inf
+    s.scores[0, 0] = s.out[0, 12]
+    s.run()
+    assert s.tokens.tolist()[0] == [-1] * 18
