@@ -187,9 +187,9 @@ __device__ __forceinline__ void new_row(const ForkArgs& a, int r, const RowPlan&
 
 // Up to here one workgroup: its 16 waves take rows in turn, so rows tell most (rows of 60 entries, calls of a captured graph:
 // 32 of them 5.8 us and 10.4 in four launches, 64 7.2 and 10.6, 128 10.1 and 10.4, 160 11.6 and 10.4, 256 16.0 and 10.6;
-// 1024 of 16 48.4 and 10.8), then a row's length (64 rows of 256 entries 9.1 and 11.0,
-// of 512 10.1 and 11.7, 96 of 256 11.4 and 11.0, 128 of 512 15.7 and 12.6), then the words of marks that are cleared and
-// counted (32 rows of 30 in 673 pages 5.4 and 9.9, in 2^17 6.9 and 10.3).
+// 1024 of 16 48.4 and 10.8), then a row's length (64 rows of 256 entries 9.1 and 11.0, of 512 10.1 and 11.7, 96 of 256
+// 11.4 and 11.0, 128 of 512 15.7 and 12.6), then the words of marks that are cleared and counted (32 rows of 30 in 673
+// pages 5.4 and 9.9, in 2^17 6.9 and 10.3).
 constexpr int kSmallRows = 128, kSmallEntries = 1 << 14, kSmallPages = 1 << 17;
 
 __global__ __launch_bounds__(1024) void fork_small_kernel(ForkArgs a) {

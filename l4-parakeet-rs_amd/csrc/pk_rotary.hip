@@ -13,8 +13,9 @@
 // lanes make a head.  Everything between the loads and the one rounding at the store is fp32.
 //
 // Bound by HBM: 16000 tokens, 32 / 8 heads of 128, rows to rows (328 MB) 60 us, 5.5 TB/s; with keys
-// and values into an fp16 cache (393 MB) 76 us, 5.2 TB/s, into an e4m3 one (360 MB) 74 us, 4.9 TB/s.  One token 2.7 us, about a launch; 61 into an
-// e4m3 cache 4.6 us: a load, the angles, and values that lie in as many rows of a page as they are.
+// and values into an fp16 cache (393 MB) 76 us, 5.2 TB/s, into an e4m3 one (360 MB) 74 us, 4.9 TB/s.
+// One token 2.7 us, about a launch; 61 into an e4m3 cache 4.6 us: a load, the angles, and values that
+// lie in as many rows of a page as they are.
 #include <math.h>
 
 #include "pk_paged_write.hpp"
